@@ -354,6 +354,91 @@ int mcamd_residual_rmsnorm(const void *x, const float *part, int64_t splits, con
                            void *x_out, void *h_out, int64_t m, int64_t n, float eps,
                            void *stream);
 
+/*
+ * The paged KV cache: K and V in pools of n_pages pages, (n_pages, page_size, H_kv, D) per slot, each
+ * page contiguous and pages `page_stride` elements apart, and per row a line of a block table,
+ * (n_rows, max_pages) int32 with lines `table_stride` numbers apart: position t of row b is token
+ * t % page_size of page block_table[b][t / page_size]. page_size is a power of two, at least 16
+ * (MCAMD_EINVAL otherwise). Entries of pages a row does not hold are not read; a page number outside
+ * [0, n_pages) that is needed is never followed. It has no counterpart in the reference, whose cache
+ * reserves T_max positions per row (modelcore/cache.py:22-23).
+ */
+
+/*
+ * Pages, slots and positions of a forward's new tokens, on the device. Row b holds cache_seqlens[b]
+ * tokens and gets new_lens[b] more; the rows in order take the pages they lack off the top of the
+ * stack of free pages, free_pages[0 .. *free_count), and *free_count goes down:
+ *   block_table[b][have + i] = free_pages[*free_count - 1 - taken before b - i].
+ * cu_seqlens (n_rows + 1) becomes the running sum of new_lens. Token i of it, i < total, gets its
+ * position cache_seqlens[b] + i - cu_seqlens[b] and its slot, page * page_size + position % page_size.
+ * A row whose pages the stack does not hold, or that would outgrow the table, or with a negative
+ * length, takes none and its tokens get position and slot -1, as do tokens past the last row's;
+ * *refused becomes the number of such rows. Tokens past `total` are not planned and get no pages.
+ * row_scratch: n_rows int32, the call's own until it ends on the stream. cache_seqlens is only read:
+ * the caller advances it after the forward, as with the contiguous cache.
+ */
+int mcamd_paged_reserve(int32_t *block_table, int64_t table_stride, const int32_t *cache_seqlens,
+                        const int32_t *new_lens, const int32_t *free_pages, int32_t *free_count,
+                        int32_t *row_scratch, int32_t *cu_seqlens, int64_t *slots,
+                        int32_t *positions, int32_t *refused, int64_t n_rows, int64_t max_pages,
+                        int64_t n_pages, int64_t page_size, int64_t total, void *stream);
+
+/*
+ * Rows rows[0 .. n_release) end: their pages go onto the stack of free pages, in the order of `rows`
+ * and of their tables, their table entries become -1 and their cache_seqlens 0. A row named twice
+ * gives its pages once; numbers outside [0, n_rows) are passed over.
+ */
+int mcamd_paged_release(int32_t *block_table, int64_t table_stride, int32_t *cache_seqlens,
+                        const int32_t *rows, int64_t n_release, int64_t n_rows,
+                        int32_t *free_pages, int32_t *free_count, int64_t max_pages,
+                        int64_t n_pages, int64_t page_size, void *stream);
+
+/*
+ * mcamd_qk_rope_norm_append over a paged cache: token i of `total` is at positions[i], for the rotary
+ * tables, and its k and v go to slots[i] (as mcamd_paged_reserve gives both). q_out is (total,
+ * n_head, head_dim) contiguous. Arithmetic is fp32 throughout and each result is rounded once; v is
+ * copied bit for bit. A position outside [0, n_pos) makes q_out NaN and writes nothing, a slot outside
+ * the pool writes nothing. k = v = NULL transforms q only (slots and pages unused).
+ */
+int mcamd_qk_rope_norm_append_paged(const void *q, int64_t q_token_stride, const void *k,
+                                    int64_t k_token_stride, const void *v, int64_t v_token_stride,
+                                    const void *cos, const void *sin, int64_t n_pos,
+                                    const int32_t *positions, const int64_t *slots, void *k_pages,
+                                    void *v_pages, void *q_out, int64_t total, int64_t n_head,
+                                    int64_t n_kv_head, int64_t head_dim, int64_t n_pages,
+                                    int64_t page_size, int64_t page_stride, float eps, float scale,
+                                    int dtype, void *stream);
+
+/*
+ * Bytes of scratch with which mcamd_flash_attn_paged_with_kvcache() runs these sizes best: room for
+ * the fp32 partials of rows whose keys are cut into ranges. With less (NULL and 0 included) no keys
+ * are cut. 0 where none is of use.
+ */
+size_t mcamd_paged_scratch_bytes(int64_t n_rows, int64_t total, int64_t max_seqlen, int64_t n_head,
+                                 int64_t n_kv_head, int64_t head_dim, int64_t max_pages,
+                                 int64_t page_size, int64_t window, int dtype);
+
+/*
+ * The cached-attention operator over a paged cache, for any mixture of rows with one new token and
+ * with many. q and out are (total, n_head, head_dim), k and v (both NULL = no append) (total,
+ * n_kv_head, head_dim). Row b's tokens are [cu_seqlens[b], cu_seqlens[b + 1]) of them, at most
+ * max_seqlen each, at positions cache_seqlens[b] + t; without cu_seqlens every row has max_seqlen
+ * tokens and total = n_rows * max_seqlen. k and v are written to their pages bit for bit, then each
+ * query attends the keys of its row that the rules at the top of this file name. head_dim is at most
+ * 256, at most 64 query heads share a KV head. cache_seqlens is only read.
+ * A row whose positions fall outside [0, max_pages * page_size) gets NaN output and appends nothing; a
+ * query that sees a key in a page outside the pool is NaN, and nothing is appended there. Tokens past the
+ * last row's are not read, and their outputs not written. The scratch (16-byte aligned) belongs to the
+ * call until it ends on the stream. No two rows may append to one page.
+ */
+int mcamd_flash_attn_paged_with_kvcache(
+    const void *q, const void *k, const void *v, void *k_pages, void *v_pages,
+    const int32_t *block_table, int64_t table_stride, const int32_t *cache_seqlens,
+    const int32_t *cu_seqlens, void *out, int64_t n_rows, int64_t total, int64_t max_seqlen,
+    int64_t n_head, int64_t n_kv_head, int64_t head_dim, int64_t n_pages, int64_t page_size,
+    int64_t page_stride, int64_t max_pages, int64_t window, int causal, int dtype, void *scratch,
+    size_t scratch_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

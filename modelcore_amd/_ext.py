@@ -9,6 +9,7 @@ raises it through :func:`lib`; there is no other implementation to fall back to.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -77,6 +78,20 @@ SIGNATURES = {
     "mcamd_linear_bf16_partials": (_int, [_ptr, _i64, _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr]),
     "mcamd_residual_rmsnorm": (_int, [_ptr, _ptr, _i64, _ptr, _ptr, _ptr, _i64, _i64,
                                       ctypes.c_float, _ptr]),
+    "mcamd_paged_reserve": (_int, [_ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
+                                   _i64, _i64, _i64, _i64, _i64, _ptr]),
+    "mcamd_paged_release": (_int, [_ptr, _i64, _ptr, _ptr, _i64, _i64, _ptr, _ptr, _i64, _i64, _i64,
+                                   _ptr]),
+    "mcamd_qk_rope_norm_append_paged": (_int, [_ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr, _i64,
+                                               _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64,
+                                               _i64, _i64, _i64, ctypes.c_float, ctypes.c_float,
+                                               _int, _ptr]),
+    "mcamd_paged_scratch_bytes": (_size, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                          _int]),
+    "mcamd_flash_attn_paged_with_kvcache": (_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr,
+                                                   _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64,
+                                                   _i64, _i64, _i64, _i64, _i64, _int, _int, _ptr,
+                                                   _size, _ptr]),
 }
 
 _LIB = None
@@ -167,6 +182,20 @@ def workspace(device, nbytes: int):
     ws = torch.empty(size, dtype=torch.uint8, device=device)
     _WORKSPACES[idx] = ws
     return ws
+
+
+def same_device(device, **tensors):
+    """Every given tensor must be on `device`: the kernels follow pointers as they are."""
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
+
+
+def on_device(device):
+    """A context in which `device` is the current one, as a launch on its streams needs."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def require_rocm(*tensors, what: str):

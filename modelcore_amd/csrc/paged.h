@@ -1,0 +1,148 @@
+// The paged KV cache as the kernels see it: a pool of pages and, per row, a line of a block table.
+//
+// Position t of row b lies in page table[b][t >> shift] at token t & (page_size - 1) of it; a page
+// holds page_size tokens of (H_kv, D) and pages are page_stride elements apart, so an address is 64
+// bits wide in any pool. Page sizes are powers of two from 16 on: a group of 16 keys aligned to 16
+// lies in one page, which is what lets a wave take a page per load instead of one per lane.
+//
+// A number in the table that is no page of the pool (-1 where no page was given) is never followed:
+// its keys are read from page 0 and the outputs that see them become NaN.
+#pragma once
+
+#include "kernels.h"
+
+namespace mcamd {
+
+constexpr int64_t kMinPageSize = 16;
+
+struct PagedKv {
+  const int32_t *table;
+  int64_t table_stride;  // numbers between rows of the table
+  int64_t page_stride;   // elements between pages
+  int shift, n_pages, max_pages;
+
+  __device__ __forceinline__ bool is_page(int id) const {
+    return uint32_t(id) < uint32_t(n_pages);
+  }
+  // Elements from the pool's start to token `at` (of page_size) of a page, tok elements a token.
+  __device__ __forceinline__ int64_t offset(int id, int at, int64_t tok) const {
+    return int64_t(is_page(id) ? id : 0) * page_stride + at * tok;
+  }
+  __device__ __forceinline__ int in_page(int t) const { return t & ((1 << shift) - 1); }
+};
+
+struct PagedArgs {
+  const void *q, *k_new, *v_new;  // k_new, v_new: appended (NULL = they are in the pages)
+  void *k_pages, *v_pages;
+  PagedKv kv;
+  const int32_t *seqlens, *cu;  // cu: packed rows of their own lengths; NULL = t_new tokens each
+  void *out;
+  int64_t n_rows, t_new, total, n_head, n_kv_head, head_dim, window;
+  int dtype;
+  void *scratch;
+  size_t scratch_bytes;
+  hipStream_t stream;
+};
+
+// The new tokens of row b: [tok0, tok0 + T) of q, whatever cu holds.
+__device__ __forceinline__ void row_tokens(const int32_t *cu, int t_new, int total, int b, int &tok0,
+                                           int &T) {
+  tok0 = cu ? max(cu[b], 0) : b * t_new;
+  T = cu ? max(min(cu[b + 1], total) - tok0, 0) : t_new;
+}
+
+// A block of queries of a row: its block qt, the row's tokens and its position.
+struct PagedBlock {
+  int b, qt, tok0, T, s0;
+  int n_blocks;    // of the whole call, its KV heads counted
+  int part, most;  // which key range of the block, of how many at most
+};
+
+// Block i of a call, blocks with the most keys first: by their number within their row, last first,
+// and rows in order within a number, so that long rows do not fall to one XCD. `pairs` (position,
+// head) pairs make a block; rows of at most `skip` pairs have none. Each wave does this by itself:
+// the rows' counts, four a lane, stay in registers (rows past 256 are read again), and the number is
+// found by bisection over how many blocks there are from it on.
+//
+// Where the partials of `slots` blocks have room, fewer blocks than half of that may be cut into key
+// ranges: the first ranges of all blocks come first, then the second ones, and so on.
+constexpr int kMaxPagedSplits = 32;
+__device__ __forceinline__ bool find_paged_block(const int32_t *cu, const int32_t *seqlens,
+                                                 int n_rows, int t_new, int total, int G, int H_kv,
+                                                 int pairs, int skip, int slots, int i, int lane,
+                                                 PagedBlock &v) {
+  auto range_of = [&](int blocks) {
+    v.n_blocks = blocks * H_kv;
+    v.most = blocks > 0 ? max(1, min(slots / v.n_blocks, kMaxPagedSplits)) : 1;
+    v.part = blocks > 0 ? i / blocks : 0;
+    i -= v.part * blocks;
+    return v.part < v.most && blocks > 0;
+  };
+  if (!cu) {
+    const int64_t n_pairs = int64_t(t_new) * G;
+    const int each = n_pairs > skip ? int((n_pairs + pairs - 1) / pairs) : 0;
+    if (!range_of(each * n_rows)) return false;
+    v.qt = each - 1 - i / n_rows;
+    v.b = i % n_rows;
+  } else {
+    auto blocks = [&](int b) {
+      if (b >= n_rows) return 0;
+      int tok0, T;
+      row_tokens(cu, t_new, total, b, tok0, T);
+      const int64_t n = int64_t(T) * G;
+      return n > skip ? int((n + pairs - 1) / pairs) : 0;
+    };
+    int mine[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) mine[u] = blocks(64 * u + lane);
+    // Blocks numbered k or more.
+    auto from = [&](int k) {
+      int n = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) n += max(mine[u] - k, 0);
+      for (int b = 256 + lane; b < n_rows; b += 64) n += max(blocks(b) - k, 0);
+      return wave_total(n);
+    };
+    if (!range_of(from(0))) return false;
+    int lo = 0, hi = int((int64_t(total) * G + pairs - 1) / pairs);  // more than i from lo on
+    while (hi - lo > 1) {
+      const int k = (lo + hi) >> 1;
+      if (from(k) > i)
+        lo = k;
+      else
+        hi = k;
+    }
+    v.qt = lo;
+    int nth = i - from(lo + 1);  // among the rows that have a block lo
+    v.b = -1;
+    auto look = [&](int b0, int n) {
+      uint64_t has = __builtin_amdgcn_ballot_w64(n > lo);
+      const int c = __builtin_popcountll(has);
+      if (v.b < 0 && nth < c) {
+        for (; nth > 0; --nth) has &= has - 1;
+        v.b = b0 + __builtin_ctzll(has);
+      }
+      nth -= c;
+    };
+#pragma unroll
+    for (int u = 0; u < 4; ++u) look(64 * u, mine[u]);
+    for (int b0 = 256; b0 < n_rows && v.b < 0; b0 += 64) look(b0, blocks(b0 + lane));
+    if (v.b < 0) return false;
+  }
+  v.b = __builtin_amdgcn_readfirstlane(v.b);
+  row_tokens(cu, t_new, total, v.b, v.tok0, v.T);
+  v.s0 = seqlens[v.b];
+  return true;
+}
+
+// At most so many blocks of `pairs` pairs in a call.
+inline int64_t paged_blocks_bound(const PagedArgs &a, int64_t pairs) {
+  const int64_t G = a.n_head / a.n_kv_head;
+  if (!a.cu) return a.n_rows * ((a.t_new * G + pairs - 1) / pairs);
+  return a.total * G / pairs + (a.n_rows < a.total ? a.n_rows : a.total);
+}
+
+int launch_paged_append(const PagedArgs &a);
+int launch_paged_tiled(const PagedArgs &a);
+
+}  // namespace mcamd

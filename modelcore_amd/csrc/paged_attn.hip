@@ -1,0 +1,190 @@
+// The attention operator over a paged cache: its argument checks, the append of new tokens into
+// their pages, and which kernels a call takes.
+#include "paged.h"
+
+#include <cmath>
+
+namespace mcamd {
+namespace {
+
+constexpr int kThreads = 256;
+
+// New tokens' K and V into their pages, bit for bit: kTokens tokens a workgroup, whose places its
+// first threads find, then 16-byte pieces by all of them. A row that does not fit its line of the
+// table, and a token whose page is outside the pool, are passed over.
+constexpr int kTokens = 8;
+
+struct PagedAppend {
+  const uint4 *k, *v;
+  uint4 *k_pages, *v_pages;
+  PagedKv kv;  // page_stride in pieces
+  const int32_t *seqlens, *cu;
+  int n_rows, t_new, total, units;
+};
+
+__global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedAppend A) {
+  __shared__ int64_t s_at[kTokens];
+  const int t0 = blockIdx.x * kTokens;
+  if (threadIdx.x < kTokens) {
+    const int t = t0 + threadIdx.x;
+    int64_t at = -1;
+    if (t < A.total) {
+      int b, tok0, T;
+      if (A.cu) {
+        int lo = 0, hi = A.n_rows;  // the last row that begins at or before t
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (A.cu[mid] <= t)
+            lo = mid;
+          else
+            hi = mid;
+        }
+        b = lo;
+      } else {
+        b = t / A.t_new;
+      }
+      row_tokens(A.cu, A.t_new, A.total, b, tok0, T);
+      const int64_t s0 = A.seqlens[b], pos = s0 + (t - tok0);
+      if (t >= tok0 && t < tok0 + T && s0 >= 0 && s0 + T <= int64_t(A.kv.max_pages) << A.kv.shift) {
+        const int id = A.kv.table[b * A.kv.table_stride + (pos >> A.kv.shift)];
+        if (A.kv.is_page(id)) at = A.kv.offset(id, A.kv.in_page(int(pos)), A.units);
+      }
+    }
+    s_at[threadIdx.x] = at;
+  }
+  __syncthreads();
+  const int n = min(kTokens, A.total - t0) * A.units;
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const int t = i / A.units, u = i - t * A.units;
+    const int64_t at = s_at[t], from = (int64_t(t0) + t) * A.units + u;
+    if (at < 0) continue;
+    const uint4 x = A.k[from], y = A.v[from];
+    A.k_pages[at + u] = x;
+    A.v_pages[at + u] = y;
+  }
+}
+
+int check(const PagedArgs &a) {
+  if (a.dtype != MCAMD_F32 && a.dtype != MCAMD_BF16)
+    return fail(MCAMD_EINVAL, "paged attention: dtype must be MCAMD_F32 or MCAMD_BF16");
+  if (a.n_rows < 0 || a.t_new < 0 || a.total < 0 || a.n_head <= 0 || a.n_kv_head <= 0 ||
+      a.head_dim <= 0)
+    return fail(MCAMD_EINVAL, "paged attention: sizes must be positive (rows and tokens may be 0)");
+  if (a.n_kv_head > a.n_head || a.n_head % a.n_kv_head != 0)
+    return fail(MCAMD_EINVAL, "paged attention: n_head must be a multiple of n_kv_head");
+  const int64_t elem = a.dtype == MCAMD_F32 ? 4 : 2;
+  if (a.head_dim > 256 || a.head_dim * elem % 16 != 0)
+    return fail(MCAMD_EUNSUPPORTED,
+                "paged attention: head_dim must be at most 256, its bytes a multiple of 16");
+  if (a.n_head / a.n_kv_head > 64)
+    return fail(MCAMD_EUNSUPPORTED, "paged attention: more than 64 query heads per KV head");
+  if (!a.q || !a.out || !a.k_pages || !a.v_pages || !a.kv.table || !a.seqlens)
+    return a.n_rows > 0 && a.total > 0 ? fail(MCAMD_EINVAL, "paged attention: null pointer") : MCAMD_OK;
+  if (!aligned(a.q, 16) || !aligned(a.out, 16) || !aligned(a.k_pages, 16) ||
+      !aligned(a.v_pages, 16) || (a.k_new && !aligned(a.k_new, 16)) ||
+      (a.v_new && !aligned(a.v_new, 16)) || a.kv.page_stride * elem % 16 != 0 ||
+      !aligned(a.scratch, 16))
+    return fail(MCAMD_EINVAL, "paged attention: tensors must be 16-byte aligned");
+  return MCAMD_OK;
+}
+
+int launch(const PagedArgs &a) {
+  if (a.k_new) {
+    int st = launch_paged_append(a);
+    if (st != MCAMD_OK) return st;
+  }
+  return launch_paged_tiled(a);
+}
+
+}  // namespace
+
+int launch_paged_append(const PagedArgs &a) {
+  const int64_t elem = a.dtype == MCAMD_F32 ? 4 : 2;
+  PagedAppend A;
+  A.k = static_cast<const uint4 *>(a.k_new);
+  A.v = static_cast<const uint4 *>(a.v_new);
+  A.k_pages = static_cast<uint4 *>(a.k_pages);
+  A.v_pages = static_cast<uint4 *>(a.v_pages);
+  A.kv = a.kv;
+  A.kv.page_stride = a.kv.page_stride * elem / 16;
+  A.seqlens = a.seqlens;
+  A.cu = a.cu;
+  A.n_rows = int(a.n_rows);
+  A.t_new = int(a.t_new);
+  A.total = int(a.total);
+  A.units = int(a.n_kv_head * a.head_dim * elem / 16);
+  const int64_t blocks = (a.total + kTokens - 1) / kTokens;
+  hipLaunchKernelGGL(paged_append_kernel, dim3(unsigned(blocks)), dim3(kThreads), 0, a.stream, A);
+  return launch_status("paged_append");
+}
+
+}  // namespace mcamd
+
+using namespace mcamd;
+
+extern "C" size_t mcamd_paged_scratch_bytes(int64_t n_rows, int64_t total, int64_t max_seqlen,
+                                            int64_t n_head, int64_t n_kv_head, int64_t head_dim,
+                                            int64_t max_pages, int64_t page_size, int64_t window,
+                                            int dtype) {
+  (void)n_rows, (void)total, (void)max_seqlen, (void)n_head, (void)n_kv_head, (void)head_dim;
+  (void)max_pages, (void)page_size, (void)window, (void)dtype;
+  return 0;
+}
+
+extern "C" int mcamd_flash_attn_paged_with_kvcache(
+    const void *q, const void *k, const void *v, void *k_pages, void *v_pages,
+    const int32_t *block_table, int64_t table_stride, const int32_t *cache_seqlens,
+    const int32_t *cu_seqlens, void *out, int64_t n_rows, int64_t total, int64_t max_seqlen,
+    int64_t n_head, int64_t n_kv_head, int64_t head_dim, int64_t n_pages, int64_t page_size,
+    int64_t page_stride, int64_t max_pages, int64_t window, int causal, int dtype, void *scratch,
+    size_t scratch_bytes, void *stream) {
+  (void)causal;
+  if ((k == nullptr) != (v == nullptr))
+    return fail(MCAMD_EINVAL, "flash_attn_paged_with_kvcache: pass both k and v, or neither");
+  PagedArgs a{};
+  while ((int64_t(1) << a.kv.shift) < page_size) ++a.kv.shift;
+  if (page_size < kMinPageSize || (int64_t(1) << a.kv.shift) != page_size)
+    return fail(MCAMD_EINVAL, "paged attention: page_size must be a power of two, at least 16");
+  if (n_pages <= 0 || max_pages <= 0 || max_seqlen < 0)
+    return fail(MCAMD_EINVAL, "paged attention: empty pool or block table, or negative max_seqlen");
+  if (page_stride < page_size * n_kv_head * head_dim)
+    return fail(MCAMD_EINVAL, "paged attention: page_stride smaller than page_size*H_kv*D");
+  if (table_stride < max_pages)
+    return fail(MCAMD_EINVAL, "paged attention: table_stride smaller than max_pages");
+  if (n_pages * page_size > 0x7fffffff || max_pages > (int64_t(1) << 30) / page_size ||
+      n_rows > 65535 || n_head > 65535 || total > (int64_t(1) << 30) / (n_head > 0 ? n_head : 1))
+    return fail(MCAMD_EUNSUPPORTED, "paged attention: sizes beyond the 32-bit index range of the kernels");
+  if (!cu_seqlens && total != n_rows * max_seqlen)
+    return fail(MCAMD_EINVAL, "paged attention: without cu_seqlens every row has max_seqlen tokens");
+  a.q = q;
+  a.k_new = k;
+  a.v_new = v;
+  a.k_pages = k_pages;
+  a.v_pages = v_pages;
+  a.kv.table = block_table;
+  a.kv.table_stride = table_stride;
+  a.kv.page_stride = page_stride;
+  a.kv.n_pages = int(n_pages);
+  a.kv.max_pages = int(max_pages);
+  a.seqlens = cache_seqlens;
+  a.cu = cu_seqlens;
+  a.out = out;
+  a.n_rows = n_rows;
+  a.t_new = max_seqlen;
+  a.total = total;
+  a.n_head = n_head;
+  a.n_kv_head = n_kv_head;
+  a.head_dim = head_dim;
+  a.window = window;
+  a.dtype = dtype;
+  a.scratch = scratch;
+  a.scratch_bytes = scratch_bytes;
+  a.stream = as_stream(stream);
+  const int st = check(a);
+  if (st != MCAMD_OK) return st;
+  if (n_rows == 0 || total == 0 || max_seqlen == 0) {
+    clear_error();
+    return MCAMD_OK;
+  }
+  return launch(a);
+}

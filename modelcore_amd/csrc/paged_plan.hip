@@ -1,0 +1,282 @@
+// Pages, slots and positions of a forward's new tokens, and pages given back: the bookkeeping of a
+// paged KV cache on the device, so that a step needs no host read and can be captured.
+//
+// The free pages are a stack: free_pages[0 .. free_count). Row b holds have = ceil(len / P) pages
+// (P = page_size) and needs need = ceil((len + new) / P), so it takes need - have off the stack, the
+// rows in order: with upto the inclusive sum of the takes,
+//   table[b][have + i] = free_pages[free_count - 1 - (upto_b - take_b) - i].
+// A row whose pages the stack no longer holds, or that would outgrow the table, or whose lengths are
+// negative, takes none and its tokens get slot and position -1 (`refused` counts such rows). Token i
+// of row b is at position len + i, slot table[b][position / P] * P + position % P; tokens past the
+// last row's get -1.
+//
+// reserve: one workgroup sums over the rows (integer sums: the same pages whatever the timing), then
+// tokens are dealt to threads. A page that is taken begins at its first new token, which writes its
+// number into the table. Up to kOneLaunchTokens tokens the same workgroup does both; more take a
+// second launch, bound by the slots and positions it writes.
+#include "paged.h"
+
+namespace mcamd {
+namespace {
+
+constexpr int kThreads = 1024;
+constexpr int kWaves = kThreads / 64;
+constexpr int kOneLaunchTokens = 4096;
+constexpr int kTokens = 4;  // consecutive tokens of a thread
+
+struct PlanParams {
+  int32_t *table;
+  const int32_t *seqlens, *new_lens;
+  const int32_t *free_pages;
+  int32_t *free_count, *refused, *cu;
+  int32_t *first;  // per row: the stack index of its first page, or -1 (refused)
+  int64_t *slots;
+  int32_t *positions;
+  int64_t table_stride;
+  int n_rows, max_pages, n_pages, shift, total;
+};
+
+// Inclusive sum over the wave.
+__device__ __forceinline__ int64_t wave_scan(int64_t x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+
+// Inclusive sum of x over the workgroup, after `carry`; carry becomes the whole sum.
+__device__ __forceinline__ int64_t group_scan(int64_t x, int64_t &carry, int64_t *s_sum) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t y = wave_scan(x, lane);
+  __syncthreads();  // the sums of the scan before have been read
+  if (lane == 63) s_sum[wave] = y;
+  __syncthreads();
+  int64_t all = 0, before = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) before += s_sum[w];
+    all += s_sum[w];
+  }
+  y += carry + before;
+  carry += all;
+  return y;
+}
+
+__device__ __forceinline__ void write_tokens(const PlanParams &P, int t0) {
+  if (t0 >= P.total) return;
+  // The row of token t0: the last one that begins at or before it, past any empty ones.
+  int lo = 0, hi = P.n_rows;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (P.cu[mid] <= t0)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  int b = lo, end = P.cu[b + 1];
+  const int page_mask = (1 << P.shift) - 1;
+#pragma unroll
+  for (int u = 0; u < kTokens; ++u) {
+    const int t = t0 + u;
+    if (t >= P.total) return;
+    while (t >= end && b + 1 < P.n_rows) end = P.cu[++b + 1];
+    int64_t slot = -1;
+    int pos = -1;
+    const int first = P.first[b];
+    if (t < end && first >= 0) {
+      const int len = P.seqlens[b];
+      pos = len + t - P.cu[b];
+      const int have = int((int64_t(len) + page_mask) >> P.shift), page = pos >> P.shift;
+      int id;
+      if (page < have) {
+        id = P.table[b * P.table_stride + page];
+      } else {
+        id = P.free_pages[first - (page - have)];
+        if ((pos & page_mask) == 0) P.table[b * P.table_stride + page] = id;
+      }
+      slot = id < 0 ? -1 : (int64_t(id) << P.shift) + (pos & page_mask);
+    }
+    P.slots[t] = slot;
+    P.positions[t] = pos;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void reserve_kernel(PlanParams P, int with_tokens) {
+  __shared__ int64_t s_sum[kWaves];
+  __shared__ int s_refused;
+  const int tid = threadIdx.x;
+  if (tid == 0) s_refused = 0;
+  const int64_t stack = min(max(P.free_count[0], 0), P.n_pages);
+  const int64_t page = int64_t(1) << P.shift;
+  int64_t taken = 0, tokens = 0, kept = 0;  // pages asked for, tokens, pages given so far
+  int64_t given = 0;                        // of this thread's rows
+  for (int b0 = 0; b0 < P.n_rows; b0 += kThreads) {
+    const int b = b0 + tid;
+    const bool here = b < P.n_rows;
+    const int64_t len = here ? P.seqlens[b] : 0;
+    const int64_t asked = here ? P.new_lens[b] : 0;
+    // Tokens past `total` are not planned, and get no pages.
+    const int64_t all = group_scan(max(asked, int64_t(0)), tokens, s_sum);
+    const int64_t end = min(all, int64_t(P.total));
+    const int64_t fresh = end - min(all - max(asked, int64_t(0)), int64_t(P.total));
+    const int64_t have = (max(len, int64_t(0)) + page - 1) >> P.shift;
+    const int64_t need = (max(len, int64_t(0)) + fresh + page - 1) >> P.shift;
+    const bool fits = len >= 0 && asked >= 0 && need <= P.max_pages;
+    const int64_t take = fits ? need - have : 0;
+    const int64_t upto = group_scan(take, taken, s_sum);
+    const bool ok = fits && (take == 0 || upto <= stack);
+    if (here) {
+      // A row that takes none has no first page; any index but -1 will do.
+      P.first[b] = !ok ? -1 : take == 0 ? 0 : int(stack - 1 - (upto - take));
+      P.cu[b + 1] = int(end);
+      if (!ok) atomicAdd(&s_refused, 1);
+      given += ok ? take : 0;
+    }
+  }
+  group_scan(given, kept, s_sum);
+  if (tid == 0) {
+    P.cu[0] = 0;
+    P.free_count[0] = int(stack - kept);
+    P.refused[0] = s_refused;
+  }
+  if (!with_tokens) return;
+  __syncthreads();  // the rows' numbers are written
+  for (int t = tid * kTokens; t < P.total; t += kThreads * kTokens) write_tokens(P, t);
+}
+
+__global__ __launch_bounds__(256) void tokens_kernel(PlanParams P) {
+  write_tokens(P, (int(blockIdx.x) * 256 + int(threadIdx.x)) * kTokens);
+}
+
+// Rows rows[0 .. n) give their pages back, in order, and are empty then. A row that is named twice
+// gives them once; a row outside the batch, or a page outside the pool, is passed over.
+__global__ __launch_bounds__(kThreads) void release_kernel(int32_t *table, int64_t table_stride,
+                                                           int32_t *seqlens, const int32_t *rows,
+                                                           int n, int n_rows, int32_t *free_pages,
+                                                           int32_t *free_count, int max_pages,
+                                                           int n_pages, int shift) {
+  __shared__ int64_t s_sum[kWaves];
+  __shared__ int s_row[kThreads], s_end[kThreads];
+  const int tid = threadIdx.x;
+  int64_t top = min(max(free_count[0], 0), n_pages);
+  for (int i0 = 0; i0 < n; i0 += kThreads) {
+    const int i = i0 + tid;
+    int row = i < n ? rows[i] : -1;
+    if (row >= n_rows) row = -1;
+    const int len = row >= 0 ? atomicExch(&seqlens[row], 0) : 0;
+    const int64_t held =
+        min((max(int64_t(len), int64_t(0)) + (1 << shift) - 1) >> shift, int64_t(max_pages));
+    const int64_t base = top;
+    const int64_t end = group_scan(held, top, s_sum) - base;
+    s_row[tid] = row;
+    s_end[tid] = int(end);
+    __syncthreads();
+    const int64_t all = top - base;
+    for (int64_t p = tid; p < all; p += kThreads) {
+      int lo = 0, hi = kThreads - 1;  // the first row whose pages end past p
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (s_end[mid] > p)
+          hi = mid;
+        else
+          lo = mid + 1;
+      }
+      const int64_t at = s_row[lo] * table_stride + p - (lo ? s_end[lo - 1] : 0);
+      const int id = table[at];
+      table[at] = -1;
+      if (base + p < n_pages) free_pages[base + p] = id;
+    }
+    __syncthreads();  // s_row and s_end have been read
+  }
+  if (tid == 0) free_count[0] = int(min(top, int64_t(n_pages)));
+}
+
+bool page_size_ok(int64_t page_size, int &shift) {
+  shift = 0;
+  while ((int64_t(1) << shift) < page_size) ++shift;
+  return page_size >= kMinPageSize && (int64_t(1) << shift) == page_size;
+}
+
+constexpr int64_t kMax31 = 0x7fffffff;
+
+}  // namespace
+}  // namespace mcamd
+
+using namespace mcamd;
+
+extern "C" int mcamd_paged_reserve(int32_t *block_table, int64_t table_stride,
+                                   const int32_t *cache_seqlens, const int32_t *new_lens,
+                                   const int32_t *free_pages, int32_t *free_count,
+                                   int32_t *row_scratch, int32_t *cu_seqlens, int64_t *slots,
+                                   int32_t *positions, int32_t *refused, int64_t n_rows,
+                                   int64_t max_pages, int64_t n_pages, int64_t page_size,
+                                   int64_t total, void *stream) {
+  PlanParams P{};
+  if (n_rows < 0 || total < 0 || max_pages <= 0 || n_pages <= 0)
+    return fail(MCAMD_EINVAL, "paged_reserve: sizes must be positive (n_rows, total may be 0)");
+  if (!page_size_ok(page_size, P.shift))
+    return fail(MCAMD_EINVAL, "paged_reserve: page_size must be a power of two, at least 16");
+  if (table_stride < max_pages)
+    return fail(MCAMD_EINVAL, "paged_reserve: table_stride smaller than max_pages");
+  if (n_rows >= kMax31 - kThreads || total > kMax31 - kThreads * kTokens ||
+      n_pages * page_size > kMax31 || max_pages * page_size > kMax31)
+    return fail(MCAMD_EUNSUPPORTED, "paged_reserve: sizes beyond 31 bits");
+  if (!free_count || !cu_seqlens || !refused ||
+      (n_rows > 0 && (!block_table || !cache_seqlens || !new_lens || !free_pages || !row_scratch)) ||
+      (total > 0 && (!slots || !positions)))
+    return fail(MCAMD_EINVAL, "paged_reserve: null pointer");
+  if (n_rows == 0 && total > 0)
+    return fail(MCAMD_EINVAL, "paged_reserve: tokens without a row");
+  P.table = block_table;
+  P.table_stride = table_stride;
+  P.seqlens = cache_seqlens;
+  P.new_lens = new_lens;
+  P.free_pages = free_pages;
+  P.free_count = free_count;
+  P.refused = refused;
+  P.cu = cu_seqlens;
+  P.first = row_scratch;
+  P.slots = slots;
+  P.positions = positions;
+  P.n_rows = int(n_rows);
+  P.max_pages = int(max_pages);
+  P.n_pages = int(n_pages);
+  P.total = int(total);
+  const bool one = total <= kOneLaunchTokens;
+  hipLaunchKernelGGL(reserve_kernel, dim3(1), dim3(kThreads), 0, as_stream(stream), P, int(one));
+  const int st = launch_status("paged_reserve");
+  if (st != MCAMD_OK || one) return st;
+  const int64_t threads = (total + kTokens - 1) / kTokens;
+  hipLaunchKernelGGL(tokens_kernel, dim3(unsigned((threads + 255) / 256)), dim3(256), 0,
+                     as_stream(stream), P);
+  return launch_status("paged_reserve");
+}
+
+extern "C" int mcamd_paged_release(int32_t *block_table, int64_t table_stride,
+                                   int32_t *cache_seqlens, const int32_t *rows, int64_t n_release,
+                                   int64_t n_rows, int32_t *free_pages, int32_t *free_count,
+                                   int64_t max_pages, int64_t n_pages, int64_t page_size,
+                                   void *stream) {
+  int shift = 0;
+  if (n_rows < 0 || n_release < 0 || max_pages <= 0 || n_pages <= 0)
+    return fail(MCAMD_EINVAL, "paged_release: sizes must be positive (n_rows, n_release may be 0)");
+  if (!page_size_ok(page_size, shift))
+    return fail(MCAMD_EINVAL, "paged_release: page_size must be a power of two, at least 16");
+  if (table_stride < max_pages)
+    return fail(MCAMD_EINVAL, "paged_release: table_stride smaller than max_pages");
+  if (n_rows >= kMax31 - kThreads || n_release >= kMax31 - kThreads ||
+      n_pages * page_size > kMax31 || max_pages * page_size > kMax31)
+    return fail(MCAMD_EUNSUPPORTED, "paged_release: sizes beyond 31 bits");
+  if (n_release == 0 || n_rows == 0) {
+    clear_error();
+    return MCAMD_OK;
+  }
+  if (!block_table || !cache_seqlens || !rows || !free_pages || !free_count)
+    return fail(MCAMD_EINVAL, "paged_release: null pointer");
+  hipLaunchKernelGGL(release_kernel, dim3(1), dim3(kThreads), 0, as_stream(stream), block_table,
+                     table_stride, cache_seqlens, rows, int(n_release), int(n_rows), free_pages,
+                     free_count, int(max_pages), int(n_pages), shift);
+  return launch_status("paged_release");
+}

@@ -313,6 +313,142 @@ def flash_attn_varlen_with_kvcache(q, k_cache, v_cache, k=None, v=None, cache_se
     return out
 
 
+@functools.lru_cache(maxsize=1024)
+def _paged_scratch_bytes(device_index, *sizes):
+    """mcamd_paged_scratch_bytes, a function of the sizes and the device alone."""
+    return _ext.lib().mcamd_paged_scratch_bytes(*sizes)
+
+
+def _check_paged_positions(block_table, seqlens, lens, n_pages, page, window):
+    """Checked mode over a paged cache: every position within its row's line of the table, every page
+    that is read or written a page of the pool."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("flash_attn_paged_with_kvcache: checked mode reads the block table on the "
+                           "host and cannot run under graph capture; call set_checked(False) first")
+    table, room = block_table.tolist(), block_table.shape[1] * page
+    for b, (s0, n) in enumerate(zip(seqlens.tolist(), lens)):
+        if n == 0:
+            continue
+        if s0 < 0 or s0 + n > room:
+            raise IndexError(f"flash_attn_paged_with_kvcache: positions [{s0}, {s0 + n}) of row {b} "
+                             f"fall outside the {room} of its line of the block table")
+        first = max(0, s0 - window) if window >= 0 else 0
+        for i in range(first // page, (s0 + n - 1) // page + 1):
+            if not 0 <= table[b][i] < n_pages:
+                raise IndexError(f"flash_attn_paged_with_kvcache: page {table[b][i]} of row {b} is "
+                                 f"not one of the pool's {n_pages}")
+
+
+def flash_attn_paged_with_kvcache(q, k_pages, v_pages, k=None, v=None, *, block_table=None,
+                                  cache_seqlens=None, cu_seqlens=None, max_seqlen=None,
+                                  causal=False, window_size=(-1, -1)):
+    """Cached attention over a paged cache, for single tokens, chunks, and both in one call. Extension
+    with no counterpart in the reference, whose cache reserves T_max positions per row.
+
+    Args:
+        q: queries (B, T_new, H, D), every row with T_new new tokens; or, with cu_seqlens, packed
+            (total, H, D), row b's tokens [cu_seqlens[b], cu_seqlens[b + 1])
+        k_pages, v_pages: (n_pages, page_size, H_kv, D) pools, updated in place; page_size a power of
+            two, at least 16
+        k, v: new keys/values, of q's layout with H_kv heads, written to their pages, or both None
+            (they are there: ``rope_norm_scale_append_paged`` wrote them)
+        block_table: (B, max_pages) int32; position t of row b is token t % page_size of page
+            block_table[b, t // page_size]. Rows may read the same pages; no two rows may write one.
+        cache_seqlens: (B,) int32 position of each row before the new tokens (read only)
+        cu_seqlens: (B + 1,) int32 on the device, ascending from 0 (``PagedPlan.cu_seqlens``); a row
+            may have no tokens, and tokens past the last row's are left out (their outputs are not
+            written)
+        max_seqlen: with cu_seqlens, at least the longest row's new tokens (host int)
+        causal: accepted for signature parity; attention is always causal
+        window_size: (left, right); left = -1 means unlimited
+
+    Returns:
+        A tensor of q's shape and dtype. A row whose positions fall outside its line of the table is
+        NaN and appends nothing, and a query that sees a key in a page outside the pool is NaN; in
+        checked mode (``set_checked``) such a call raises IndexError instead.
+    """
+    what = "flash_attn_paged_with_kvcache"
+    _ext.require_rocm(q, k_pages, v_pages, k, v, block_table, cache_seqlens, cu_seqlens, what=what)
+    packed = cu_seqlens is not None
+    if q.dim() != (3 if packed else 4):
+        raise ValueError(f"q must be {'(total, H, D)' if packed else '(B, T_new, H, D)'}; got "
+                         f"{tuple(q.shape)}")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v)):
+        raise NotImplementedError(f"{what} is forward-only (no autograd)")
+    H, D = q.shape[-2:]
+    dt, dev = q.dtype, q.device
+    code = _ext.dtype_code(dt)
+    if block_table is None or block_table.dtype != torch.int32 or block_table.dim() != 2 \
+            or block_table.shape[1] < 1 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError("block_table is required: (B, max_pages) int32 with contiguous lines")
+    B, max_pages = block_table.shape
+    if packed:
+        if cu_seqlens.dtype != torch.int32 or tuple(cu_seqlens.shape) != (B + 1,):
+            raise ValueError(f"cu_seqlens must be ({B + 1},) int32; got {tuple(cu_seqlens.shape)} "
+                             f"{cu_seqlens.dtype}")
+        if max_seqlen is None or int(max_seqlen) < 0:
+            raise ValueError("max_seqlen (at least the longest row's new tokens) is required with "
+                             "cu_seqlens")
+        total, longest = q.shape[0], min(int(max_seqlen), q.shape[0])
+        cu_seqlens = cu_seqlens.contiguous()
+    else:
+        if q.shape[0] != B:
+            raise ValueError(f"q has {q.shape[0]} rows, block_table {B}")
+        longest = q.shape[1]
+        if max_seqlen is not None and int(max_seqlen) < longest:
+            raise ValueError(f"max_seqlen {max_seqlen} is less than q's {longest} tokens")
+        total = B * longest
+    if (k is None) != (v is None):
+        raise ValueError("pass both k and v, or neither")
+    H_kv = None
+    if k is not None:
+        if k.shape != v.shape or k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] \
+                or k.shape[-1] != D:
+            raise ValueError(f"k/v must be of q's layout {tuple(q.shape)} with H_kv heads; got "
+                             f"{tuple(k.shape)} and {tuple(v.shape)}")
+        for name, t in (("k", k), ("v", v)):
+            if t.dtype != dt:
+                raise TypeError(f"{name} is {t.dtype}, q is {dt}")
+        H_kv = k.shape[-2]
+    from modelcore_amd.kernels.qk_epilogue import check_pages
+    n_pages, page, stride = check_pages(k_pages, v_pages, H_kv, D, dt, dev)
+    H_kv = k_pages.shape[2]
+    if H_kv == 0 or H % H_kv:
+        raise ValueError(f"n_head {H} is not a multiple of n_kv_head {H_kv}")
+    _ext.same_device(dev, k=k, v=v, block_table=block_table, cu_seqlens=cu_seqlens)
+    seqlens = _check_seqlens(cache_seqlens, B, dev)
+    w = _window(window_size)
+    if CHECK_POSITIONS and B > 0:
+        lens = [longest] * B
+        if packed:
+            at = cu_seqlens.tolist()
+            if at[0] != 0 or at[-1] > total or any(y - x < 0 or y - x > longest
+                                                   for x, y in zip(at, at[1:])):
+                raise IndexError(f"{what}: cu_seqlens must ascend from 0 to at most {total} in "
+                                 f"steps of at most max_seqlen {longest}")
+            lens = [y - x for x, y in zip(at, at[1:])]
+        _check_paged_positions(block_table, seqlens, lens, n_pages, page, w)
+    q = q.contiguous()
+    if k is not None:
+        k, v = k.contiguous(), v.contiguous()
+    out = torch.empty(q.shape, dtype=dt, device=dev)
+    with _ext.on_device(dev):
+        nbytes = _paged_scratch_bytes(dev.index, B, total, longest, H, H_kv, D, max_pages, page, w,
+                                      code)
+        # Scratch of the call's own: calls on several streams, and captured graphs, share nothing.
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        st = _ext.lib().mcamd_flash_attn_paged_with_kvcache(
+            q.data_ptr(), k.data_ptr() if k is not None else None,
+            v.data_ptr() if v is not None else None, k_pages.data_ptr(), v_pages.data_ptr(),
+            block_table.data_ptr(), max(block_table.stride(0), max_pages) if B <= 1
+            else block_table.stride(0), seqlens.data_ptr(),
+            cu_seqlens.data_ptr() if packed else None, out.data_ptr(), B, total, longest, H, H_kv, D,
+            n_pages, page, stride, max_pages, w, int(bool(causal)), code,
+            ws.data_ptr() if ws is not None else None, nbytes, _ext.stream_handle(dev))
+    _ext.check(st, what)
+    return out
+
+
 def flash_attn_func(q, k, v, causal=False, window_size=(-1, -1), doc_args=None):
     """No-cache attention (modelcore/kernels/flash_attn.py:270-303), inference only.
 
@@ -354,6 +490,7 @@ flash_attn = SimpleNamespace(
     flash_attn_func=flash_attn_func,
     flash_attn_with_kvcache=flash_attn_with_kvcache,
     flash_attn_varlen_with_kvcache=flash_attn_varlen_with_kvcache,
+    flash_attn_paged_with_kvcache=flash_attn_paged_with_kvcache,
     # Keyword arguments of flash_attn_with_kvcache beyond the reference's (callers check this
     # before passing them, so that an operator without them can stand in).
     EXTENSIONS=frozenset({"advance", "shared_prefix"}),

@@ -1,0 +1,123 @@
+"""Block tables and slot maps of a paged KV cache, built on the GPU from request lengths.
+
+A paged cache keeps K and V in a pool of pages of ``page_size`` tokens and, per row, a line of a block
+table that names the row's pages. Before a forward ``paged_reserve`` gives every row the pages its new
+tokens need and returns where each token goes: its slot (page * page_size + token of the page), which
+``rope_norm_scale_append_paged`` writes to, its position, which it rotates by, and the rows' offsets
+``cu_seqlens``, which ``flash_attn_paged_with_kvcache`` takes. ``paged_release`` returns the pages of
+rows that have ended. Neither reads anything on the host, so both can sit in a captured graph; the
+same inputs always give the same pages. ``modelcore_amd.cache.PagedKVCache`` keeps the tables and calls
+both.
+
+There is no counterpart in the reference, whose cache reserves T_max positions for every row
+(modelcore/cache.py:22-23).
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from modelcore_amd import _ext
+
+__all__ = ["PagedPlan", "paged_reserve", "paged_release", "check_page_size"]
+
+
+class PagedPlan(NamedTuple):
+    """Where a forward's new tokens go (``paged_reserve``)."""
+    slots: torch.Tensor       # (total,) int64: page * page_size + token of the page, or -1
+    positions: torch.Tensor   # (total,) int32: position within the row, or -1
+    cu_seqlens: torch.Tensor  # (rows + 1,) int32: the rows' offsets
+    refused: torch.Tensor     # (1,) int32: rows that got no pages
+
+
+def check_page_size(page_size) -> int:
+    page_size = int(page_size)
+    if page_size < 16 or page_size & (page_size - 1):
+        raise ValueError(f"page_size must be a power of two, at least 16; got {page_size}")
+    return page_size
+
+
+def _check_tables(block_table, cache_seqlens, free_pages, free_count, what):
+    _ext.require_rocm(block_table, cache_seqlens, free_pages, free_count, what=what)
+    dev = block_table.device
+    _ext.same_device(dev, cache_seqlens=cache_seqlens, free_pages=free_pages, free_count=free_count)
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[1] < 1 \
+            or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
+        raise ValueError("block_table must be (rows, max_pages) int32 with contiguous lines; got "
+                         f"{tuple(block_table.shape)} {block_table.dtype}")
+    n = block_table.shape[0]
+    for name, t, shape in (("cache_seqlens", cache_seqlens, (n,)),
+                           ("free_pages", free_pages, tuple(free_pages.shape[:1])),
+                           ("free_count", free_count, (1,))):
+        if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{name} must be {shape} int32, contiguous; got {tuple(t.shape)} "
+                             f"{t.dtype}")
+    if free_pages.numel() < 1:
+        raise ValueError("free_pages must have room for every page of the pool")
+    return n, block_table.shape[1], _line_stride(block_table), dev
+
+
+def _line_stride(block_table):
+    """Numbers between lines of a block table (a single line has none of its own)."""
+    return max(block_table.stride(0), block_table.shape[1]) if block_table.shape[0] <= 1 \
+        else block_table.stride(0)
+
+
+def paged_reserve(block_table, cache_seqlens, new_lens, free_pages, free_count, *, total,
+                  page_size) -> PagedPlan:
+    """Pages, slots and positions of a forward's new tokens.
+
+    Args:
+        block_table: (rows, max_pages) int32, updated in place; -1 where a row holds no page
+        cache_seqlens: (rows,) int32, each row's tokens so far (read only)
+        new_lens: (rows,) int32, each row's new tokens (0 for a row that has none)
+        free_pages: (n_pages,) int32, the stack of free pages, its first free_count numbers
+        free_count: (1,) int32, updated in place
+        total: the sum of new_lens, known to the host (the forward's token count). Tokens past it
+            are not planned; where it is larger, the tokens past the last row's get -1.
+        page_size: tokens per page, a power of two, at least 16
+
+    Returns:
+        PagedPlan. A row whose pages the stack does not hold, or that would outgrow its line of the
+        table, takes none; its tokens get slot and position -1 and ``refused`` counts it.
+    """
+    n, max_pages, stride, dev = _check_tables(block_table, cache_seqlens, free_pages, free_count,
+                                              "paged_reserve")
+    _ext.same_device(dev, new_lens=new_lens)
+    if new_lens.dtype != torch.int32 or tuple(new_lens.shape) != (n,):
+        raise ValueError(f"new_lens must be ({n},) int32; got {tuple(new_lens.shape)} "
+                         f"{new_lens.dtype}")
+    new_lens = new_lens.contiguous()
+    total, page_size = int(total), check_page_size(page_size)
+    if total < 0:
+        raise ValueError(f"total must not be negative; got {total}")
+    ints = torch.empty(2 * n + 2 + total, dtype=torch.int32, device=dev)
+    cu, refused, scratch, positions = ints.split([n + 1, 1, n, total])
+    slots = torch.empty(total, dtype=torch.int64, device=dev)
+    with _ext.on_device(dev):
+        st = _ext.lib().mcamd_paged_reserve(
+            block_table.data_ptr(), stride, cache_seqlens.data_ptr(), new_lens.data_ptr(),
+            free_pages.data_ptr(), free_count.data_ptr(), scratch.data_ptr(), cu.data_ptr(),
+            slots.data_ptr(), positions.data_ptr(), refused.data_ptr(), n, max_pages,
+            free_pages.numel(), page_size, total, _ext.stream_handle(dev))
+    _ext.check(st, "paged_reserve")
+    return PagedPlan(slots, positions, cu, refused)
+
+
+def paged_release(block_table, cache_seqlens, rows, free_pages, free_count, *, page_size):
+    """Rows that have ended give their pages back to the stack, in the order of ``rows`` ((m,)
+    int32): their table entries become -1 and their cache_seqlens 0, in place. A row named twice gives
+    its pages once; numbers outside the batch are passed over."""
+    n, max_pages, stride, dev = _check_tables(block_table, cache_seqlens, free_pages, free_count,
+                                              "paged_release")
+    _ext.same_device(dev, rows=rows)
+    if rows.dtype != torch.int32 or rows.dim() != 1:
+        raise ValueError(f"rows must be (m,) int32; got {tuple(rows.shape)} {rows.dtype}")
+    rows = rows.contiguous()
+    with _ext.on_device(dev):
+        st = _ext.lib().mcamd_paged_release(
+            block_table.data_ptr(), stride, cache_seqlens.data_ptr(), rows.data_ptr(),
+            rows.numel(), n, free_pages.data_ptr(), free_count.data_ptr(), max_pages,
+            free_pages.numel(), check_page_size(page_size), _ext.stream_handle(dev))
+    _ext.check(st, "paged_release")

@@ -25,7 +25,8 @@ import torch
 
 from modelcore_amd import _ext
 
-__all__ = ["rope_norm_scale_append", "rope_norm_scale_append_partials", "default_eps"]
+__all__ = ["rope_norm_scale_append", "rope_norm_scale_append_partials",
+           "rope_norm_scale_append_paged", "default_eps"]
 
 
 def default_eps() -> float:
@@ -173,4 +174,110 @@ def rope_norm_scale_append_partials(qkv, n_head, n_kv_head, cos, sin, cache_seql
         cb, default_eps() if eps is None else float(eps), float(scale), int(with_kv),
         _ext.stream_handle(part.device))
     _ext.check(st, "rope_norm_scale_append_partials")
+    return out
+
+
+def check_pages(k_pages, v_pages, H_kv, D, dtype, device):
+    """The pools of a paged cache, (n_pages, page_size, H_kv, D) with contiguous pages as far apart in
+    both; returns (n_pages, page_size, elements between pages)."""
+    from modelcore_amd.kernels.paged import check_page_size
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] != D \
+            or (H_kv is not None and k_pages.shape[2] != H_kv) or k_pages.shape[0] < 1:
+        raise ValueError(f"k_pages/v_pages must both be (n_pages, page_size, H_kv, D) with H_kv={H_kv}, "
+                         f"D={D}; got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    _ext.same_device(device, k_pages=k_pages, v_pages=v_pages)
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        if t.dtype != dtype:
+            raise TypeError(f"{name} is {t.dtype}, q is {dtype}")
+        if not t[0].is_contiguous():
+            raise ValueError(f"each page of {name} must be contiguous; strides {t.stride()}")
+    n, page = k_pages.shape[0], check_page_size(k_pages.shape[1])
+    if n > 1 and k_pages.stride(0) != v_pages.stride(0):
+        raise ValueError("k_pages and v_pages must have the same page stride")
+    return n, page, k_pages.stride(0) if n > 1 else page * k_pages.shape[2] * D
+
+
+def _packed_rows(t):
+    """t (total, heads, D) with heads and D contiguous and the elements between tokens (a view of a
+    fused projection's output qualifies); else a contiguous copy."""
+    n, heads, D = t.shape
+    if t.stride(2) == 1 and (heads == 1 or t.stride(1) == D) and (n <= 1 or t.stride(0) >= heads * D):
+        return t, t.stride(0) if n > 1 else heads * D
+    return t.contiguous(), heads * D
+
+
+def rope_norm_scale_append_paged(q, cos, sin, positions, k=None, v=None, k_pages=None, v_pages=None,
+                                 slots=None, eps=None, scale=1.2):
+    """rope_norm_scale_append over a paged cache: RoPE + RMS-norm + scale of q (returned) and, when
+    given, of k, which goes with v to each token's slot, in one launch.
+
+    Arithmetic is fp32 throughout and every result is rounded once (rope_norm_scale_append rounds
+    after each operation as the separate torch ops do), so the two agree within those roundings.
+
+    Args:
+        q: (total, H, D) packed queries, bf16 or fp32; q, k and v may be strided views of one fused
+            projection (heads contiguous), read in place.
+        cos, sin: rotary tables that reshape to (n_pos, D/2) in q's dtype.
+        positions: (total,) int32 position of each token within its row (``PagedPlan.positions``).
+        k, v: (total, H_kv, D) new keys/values, or both None (transform q only).
+        k_pages, v_pages: (n_pages, page_size, H_kv, D) pools (a slot view), updated in place.
+        slots: (total,) int64 (``PagedPlan.slots``); required with k and v. Distinct, apart from -1.
+        eps: RMS-norm epsilon; None is ``F.rms_norm``'s default (see ``default_eps``).
+        scale: multiplier after the norm (1.2 in the model).
+
+    A token with a position outside the tables gets NaN in q and writes nothing; one with a slot outside
+    the pool (-1) writes nothing.
+    """
+    _ext.require_rocm(q, cos, sin, k, v, k_pages, v_pages, positions, slots,
+                      what="rope_norm_scale_append_paged")
+    if q.dim() != 3:
+        raise ValueError(f"q must be (total, H, D); got {tuple(q.shape)}")
+    total, H, D = q.shape
+    if D % 2:
+        raise ValueError(f"head_dim must be even for RoPE; got {D}")
+    dt, dev = q.dtype, q.device
+    code = _ext.dtype_code(dt)
+    half = D // 2
+    cos_t, sin_t = _table(cos, half, dt, dev), _table(sin, half, dt, dev)
+    if cos_t.shape != sin_t.shape:
+        raise ValueError(f"cos {tuple(cos_t.shape)} and sin {tuple(sin_t.shape)} differ")
+    if (k is None) != (v is None):
+        raise ValueError("pass both k and v, or neither")
+    _ext.same_device(dev, positions=positions, k=k, v=v, slots=slots)
+    if positions.dtype != torch.int32 or tuple(positions.shape) != (total,):
+        raise ValueError(f"positions must be ({total},) int32; got {tuple(positions.shape)} "
+                         f"{positions.dtype}")
+    positions = positions.contiguous()
+    H_kv, n_pages, page, stride = 1, 0, 0, 0
+    ks = vs = 0
+    if k is not None:
+        if k.dim() != 3 or k.shape != v.shape or k.shape[0] != total or k.shape[2] != D:
+            raise ValueError(f"k/v must be (total, H_kv, D) = ({total}, H_kv, {D}); got "
+                             f"{tuple(k.shape)} and {tuple(v.shape)}")
+        H_kv = k.shape[1]
+        if H_kv == 0 or H % H_kv:
+            raise ValueError(f"n_head {H} is not a multiple of n_kv_head {H_kv}")
+        for name, t in (("k", k), ("v", v)):
+            if t.dtype != dt:
+                raise TypeError(f"{name} is {t.dtype}, q is {dt}")
+        if k_pages is None or v_pages is None or slots is None:
+            raise ValueError("k and v need k_pages, v_pages and slots")
+        n_pages, page, stride = check_pages(k_pages, v_pages, H_kv, D, dt, dev)
+        if slots.dtype != torch.int64 or tuple(slots.shape) != (total,):
+            raise ValueError(f"slots must be ({total},) int64; got {tuple(slots.shape)} {slots.dtype}")
+        slots = slots.contiguous()
+        (k, ks), (v, vs) = _packed_rows(k), _packed_rows(v)
+    q, qs = _packed_rows(q)
+    out = torch.empty((total, H, D), dtype=dt, device=dev)
+    with_kv = k is not None
+    with _ext.on_device(dev):
+        st = _ext.lib().mcamd_qk_rope_norm_append_paged(
+            q.data_ptr(), qs, k.data_ptr() if with_kv else None, ks,
+            v.data_ptr() if with_kv else None, vs, cos_t.data_ptr(), sin_t.data_ptr(),
+            cos_t.shape[0], positions.data_ptr(), slots.data_ptr() if with_kv else None,
+            k_pages.data_ptr() if with_kv else None, v_pages.data_ptr() if with_kv else None,
+            out.data_ptr(), total, H, H_kv, D, n_pages, page, stride,
+            default_eps() if eps is None else float(eps), float(scale), code,
+            _ext.stream_handle(dev))
+    _ext.check(st, "rope_norm_scale_append_paged")
     return out
