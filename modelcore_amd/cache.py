@@ -250,3 +250,180 @@ class PackedPrefill:
         c._pos_uniform = self.lengths[0] if (c._pos_uniform == 0 and every and
                                              len(set(self.lengths)) == 1) else None
         c.shared_prefix = 0
+
+
+class PagedKVCache:
+    """A KV cache whose rows take their memory page by page: K and V in pools of ``n_pages`` pages of
+    ``page_size`` tokens, (n_slots, n_pages, page_size, H_kv, D), and a block table that names each
+    row's pages. A row holds what its tokens need, rounded up to a page, instead of seq_len positions
+    (KVCache, modelcore/cache.py:22-23), so the same memory serves more requests of mixed lengths.
+
+    A forward over it is one call with a ``PagedStep``::
+
+        step = cache.begin([1, 1, 300, 0])          # new tokens of each row: pages, slots, positions
+        logits = model(ids, kv_cache=step)          # ids (1, 302): the rows' tokens one after another
+        cache.release([0])                          # row 0 has ended: its pages are free
+
+    Pages, slots and positions are made on the device (``paged_reserve``) from ``cache_seqlens``; the
+    host keeps its own account of lengths and free pages (``lengths``, ``pages_free``) and raises before
+    a launch where the pool or a row's line of the table is too small, so nothing is read back.
+
+    A step can be captured: ``begin(n)`` in the capture, with the same count for every row, then
+    ``note_device_step(n)`` before each replay, which checks and moves the host's account.
+    """
+
+    def __init__(self, batch_size, n_kv_head, seq_len, head_dim, num_kv_slots, device, dtype, *,
+                 n_pages=None, page_size=16):
+        from modelcore_amd.kernels.paged import check_page_size
+        self.batch_size, self.max_seq_len = batch_size, seq_len
+        self.n_slots, self.n_kv_head, self.head_dim = num_kv_slots, n_kv_head, head_dim
+        self.page_size = check_page_size(page_size)
+        if head_dim > 256:
+            raise ValueError(f"a paged cache takes head dims up to 256; got {head_dim}")
+        self.max_pages = max(1, self._pages(seq_len))
+        self.n_pages = batch_size * self.max_pages if n_pages is None else int(n_pages)
+        if self.n_pages < 1:
+            raise ValueError(f"a paged cache needs at least one page; got {self.n_pages}")
+        shape = (num_kv_slots, self.n_pages, self.page_size, n_kv_head, head_dim)
+        self.k_pages = torch.zeros(shape, device=device, dtype=dtype)
+        self.v_pages = torch.zeros(shape, device=device, dtype=dtype)
+        self.block_table = torch.full((batch_size, self.max_pages), -1, dtype=torch.int32,
+                                      device=device)
+        self.cache_seqlens = torch.zeros(batch_size, dtype=torch.int32, device=device)
+        # The stack of free pages, its first free_count numbers.
+        self.free_pages = torch.arange(self.n_pages - 1, -1, -1, dtype=torch.int32, device=device)
+        self.free_count = torch.full((1,), self.n_pages, dtype=torch.int32, device=device)
+        # The host's account of the same.
+        self.lengths = [0] * batch_size
+        self.pages_free = self.n_pages
+        self._open = False  # a step has begun and not run
+
+    def _pages(self, n):
+        return -(-n // self.page_size)
+
+    def reset(self):
+        """Back to empty; K/V are not zeroed (what no row holds is never read)."""
+        self.block_table.fill_(-1)
+        self.cache_seqlens.zero_()
+        torch.arange(self.n_pages - 1, -1, -1, dtype=torch.int32, out=self.free_pages)
+        self.free_count.fill_(self.n_pages)
+        self.lengths = [0] * self.batch_size
+        self.pages_free = self.n_pages
+        self._open = False
+
+    def get_slot_cache(self, slot):
+        """(k_pages, v_pages) views of one KV slot, each (n_pages, page_size, H_kv, D)."""
+        return self.k_pages[slot], self.v_pages[slot]
+
+    def _lens(self, new_lens):
+        lens = [int(new_lens)] * self.batch_size if isinstance(new_lens, int) \
+            else [int(n) for n in new_lens]
+        assert len(lens) == self.batch_size, \
+            f"{len(lens)} token counts for batch_size {self.batch_size}"
+        assert min(lens, default=0) >= 0, "token counts must not be negative"
+        return lens
+
+    def _room(self, lens):
+        """The pages these new tokens take, checked against the pool and each row's line."""
+        for n, t in zip(self.lengths, lens):
+            assert n + t <= self.max_seq_len, \
+                f"Sequence length {n + t} exceeds cache length {self.max_seq_len}"
+        taken = sum(self._pages(n + t) - self._pages(n) for n, t in zip(self.lengths, lens))
+        assert taken <= self.pages_free, \
+            f"{taken} pages needed, {self.pages_free} of {self.n_pages} free"
+        return taken
+
+    def begin(self, new_lens):
+        """Reserve the pages of each row's next tokens -- a count per row, or one for all -- and return
+        the ``PagedStep`` to run the model with. The step's forward must run before the next begin
+        or release: its pages are the rows' only then (``reset`` is the way out of one that failed)."""
+        from modelcore_amd.kernels.paged import paged_reserve
+        assert not self._open, "the step before has not run"
+        lens = self._lens(new_lens)
+        dev = self.cache_seqlens.device
+        capturing = dev.type == "cuda" and torch.cuda.is_current_stream_capturing()
+        if capturing:
+            if len(set(lens)) > 1:
+                raise RuntimeError("a captured step needs the same count of new tokens for every row")
+        else:
+            self.pages_free -= self._room(lens)
+            self._open = True
+        if len(set(lens)) <= 1:
+            counts = torch.full((self.batch_size,), lens[0] if lens else 0, dtype=torch.int32,
+                                device=dev)
+        else:
+            counts = torch.tensor(lens, dtype=torch.int32, device=dev)
+        plan = paged_reserve(self.block_table, self.cache_seqlens, counts, self.free_pages,
+                             self.free_count, total=sum(lens), page_size=self.page_size)
+        return PagedStep(self, lens, counts, plan, capturing)
+
+    def note_device_step(self, new_lens):
+        """The host's side of a captured begin + forward, before its replay: checked, then moved."""
+        assert not self._open, "the step before has not run"
+        lens = self._lens(new_lens)
+        self.pages_free -= self._room(lens)
+        self.lengths = [n + t for n, t in zip(self.lengths, lens)]
+
+    def release(self, rows):
+        """Rows that have ended give their pages back and are empty."""
+        from modelcore_amd.kernels.paged import paged_release
+        assert not self._open, "the step before has not run"
+        rows = [int(r) for r in rows]
+        assert len(set(rows)) == len(rows), "rows must be distinct"
+        assert all(0 <= r < self.batch_size for r in rows), \
+            f"rows {rows} out of range for batch_size {self.batch_size}"
+        if not rows:
+            return
+        paged_release(self.block_table, self.cache_seqlens,
+                      torch.tensor(rows, dtype=torch.int32, device=self.cache_seqlens.device),
+                      self.free_pages, self.free_count, page_size=self.page_size)
+        for r in rows:
+            self.pages_free += self._pages(self.lengths[r])
+            self.lengths[r] = 0
+
+
+class PagedStep:
+    """One forward over a PagedKVCache (``PagedKVCache.begin``): the rows' new tokens packed one after
+    another, ``model(idx, kv_cache=step)`` with idx (1, total)."""
+
+    shared_prefix = 0
+
+    def __init__(self, cache, lens, counts, plan, captured):
+        self.cache, self.lens, self.plan = cache, lens, plan
+        self.total, self.max_seqlen = sum(lens), max(lens, default=0)
+        # Every row has that many new tokens, or None.
+        self.uniform = self.max_seqlen if lens and len(set(lens)) == 1 else None
+        self.longest = 0 if captured else max((n + t for n, t in zip(cache.lengths, lens)), default=0)
+        self._counts, self._captured, self._done = counts, captured, False
+
+    slots = property(lambda self: self.plan.slots)
+    positions = property(lambda self: self.plan.positions)
+    cu_seqlens = property(lambda self: self.plan.cu_seqlens)
+    cache_seqlens = property(lambda self: self.cache.cache_seqlens)
+    block_table = property(lambda self: self.cache.block_table)
+
+    @property
+    def last(self):
+        """Index of the last token of every row that has any, in the packed sequence."""
+        if self.uniform:
+            return torch.arange(1, self.cache.batch_size + 1,
+                                device=self.cache_seqlens.device) * self.uniform - 1
+        ends, at = [], 0
+        for t in self.lens:
+            at += t
+            if t:
+                ends.append(at - 1)
+        return torch.tensor(ends, dtype=torch.long, device=self.cache_seqlens.device)
+
+    def get_slot_cache(self, slot):
+        return self.cache.get_slot_cache(slot)
+
+    def advance(self, num_tokens):
+        """Each row moves on by its own new tokens (one device add, no host read)."""
+        assert num_tokens == self.total, "a paged forward covers every row's new tokens"
+        assert not self._done, "a step is run once"
+        c = self.cache
+        c.cache_seqlens += self._counts
+        if not self._captured:
+            self._done, c._open = True, False
+            c.lengths = [n + t for n, t in zip(c.lengths, self.lens)]

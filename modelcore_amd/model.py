@@ -27,7 +27,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from modelcore_amd.cache import KVCache, PackedPrefill
+from modelcore_amd.cache import KVCache, PackedPrefill, PagedKVCache, PagedStep
 from modelcore_amd.runtime import Runtime
 
 TYPE_KEY = "#type"
@@ -345,13 +345,16 @@ class Attention(nn.Module):
         each row's position from cache_seqlens on the device (the separate ops slice the tables
         at the host-side position instead)."""
         return kv_cache is not None and self.epilogue is not None and self.fuse_epilogue \
-            and isinstance(self.norm, RMSNorm) and not isinstance(kv_cache, PackedPrefill) \
+            and isinstance(self.norm, RMSNorm) \
+            and not isinstance(kv_cache, (PackedPrefill, PagedStep)) \
             and self.head_dim <= 256  # the fused step's kernel covers head dims up to 256
 
     def forward(self, x, kv_cache, kv_bus):
         B, T, _ = x.size()
         if isinstance(kv_cache, PackedPrefill):
             return self._forward_packed(x, kv_cache, kv_bus)
+        if isinstance(kv_cache, PagedStep):
+            return self._forward_paged(x, kv_cache, kv_bus)
         fused = self.fuses_epilogue(kv_cache)
         if fused:
             part = self._qkv_partials(x)
@@ -401,6 +404,38 @@ class Attention(nn.Module):
             q[0], k_cache, v_cache, k=k[0], v=v[0], cache_seqlens=packed.cache_seqlens,
             cu_seqlens=packed.cu_seqlens, max_seqlen=packed.max_seqlen, rows=packed.rows,
             causal=True, window_size=(self.window, 0)).unsqueeze(0)
+        if "output_gate" in self.features:
+            y = self.features["output_gate"](y, x)
+        return self.c_proj(y.contiguous().view(1, T, -1))
+
+    def _forward_paged(self, x, step, kv_bus):
+        """The layer over a paged cache (x is (1, total, n_embd), the rows' new tokens one after
+        another): a producer rotates, norms and scales q and k and writes k and v to their slots in one
+        launch, a KV-sharing consumer transforms q only, then the operator attends through the block
+        table. With fuse_epilogue off, the reference's separate ops and an operator that appends."""
+        _, T, _ = x.size()
+        q, k, v = self._project(x)
+        k_pages, v_pages = step.get_slot_cache(self.kv_slot)
+        kw = {}
+        if self.epilogue is not None and self.fuse_epilogue and isinstance(self.norm, RMSNorm):
+            from modelcore_amd.kernels.qk_epilogue import rope_norm_scale_append_paged
+            new = (k[0], v[0], k_pages, v_pages, step.slots) if self.produces_kv else ()
+            q = rope_norm_scale_append_paged(q[0], self.rope.cos, self.rope.sin, step.positions, *new,
+                                             eps=self.norm.eps, scale=1.2)
+        else:
+            cos, sin = self.rope.packed_cos_sin(step.positions.clamp(min=0).long())
+            q = (self.norm(rotate(q, cos, sin)) * 1.2)[0]
+            if self.produces_kv:
+                kv_bus[self.kv_slot] = ((self.norm(rotate(k, cos, sin)) * 1.2)[0], v[0])
+            kw["k"], kw["v"] = kv_bus[self.kv_slot]
+        if step.uniform:
+            rows = (-1, step.uniform)
+            q, kw = q.unflatten(0, rows), {n: t.unflatten(0, rows) for n, t in kw.items()}
+        else:
+            kw.update(cu_seqlens=step.cu_seqlens, max_seqlen=step.max_seqlen)
+        y = self.attention.flash_attn_paged_with_kvcache(
+            q, k_pages, v_pages, block_table=step.block_table, cache_seqlens=step.cache_seqlens,
+            causal=True, window_size=(self.window, 0), **kw).view(1, T, self.n_head, self.head_dim)
         if "output_gate" in self.features:
             y = self.features["output_gate"](y, x)
         return self.c_proj(y.contiguous().view(1, T, -1))
@@ -803,6 +838,10 @@ class Model(nn.Module):
             # the packed batch was made, apart from the table's length.
             assert kv_cache.max_seqlen <= kv_cache.cache.max_seq_len
             return
+        if isinstance(kv_cache, PagedStep):  # its pages are reserved: checked by PagedKVCache.begin
+            assert T == kv_cache.total, \
+                "a paged forward takes every row's new tokens as one (1, total) sequence"
+            return
         pos = kv_cache.uniform_pos()
         last = pos + T if pos is not None else int(kv_cache.cache_seqlens.max().item()) + T
         assert last <= kv_cache.max_seq_len, \
@@ -813,19 +852,31 @@ class Model(nn.Module):
             raise NotImplementedError("training loss is not part of the inference path")
         if kv_cache is not None:
             self.check_cache_room(kv_cache, idx.size(1))
+            self._check_paged(idx, kv_cache)
         x = self.embedding(idx)
         x, h = self.body.forward_carry(x, kv_cache)
         if kv_cache is not None:
             kv_cache.advance(idx.size(1))
         return self.unembedding(x, h)
 
+    def _check_paged(self, idx, kv_cache):
+        """A paged forward's tokens come as one sequence, at positions the rotary tables hold."""
+        if isinstance(kv_cache, PagedStep):
+            assert idx.size(0) == 1, \
+                "a paged forward takes every row's new tokens as one (1, total) sequence"
+            n_pos = min(b.mixer.rope.cos.size(1) for b in self.body.blocks)
+            assert kv_cache.longest <= n_pos, \
+                f"Sequence length grew beyond the rotary embeddings cache: {kv_cache.longest} > {n_pos}"
+
     def last_logits(self, idx, kv_cache, last):
         """forward(), but the head runs only at position last[b] of row b: (B, vocab) logits.
         The head is per position, so these equal forward()[b, last[b]]; a prompt prefill needs
         only its last position, and skips the (B, T, vocab) logits of all the others. With a
         PackedPrefill, idx is every prompt's tokens as one (1, total) sequence, `last` is not
-        used, and the logits are those of each prompt's last token, (prompts, vocab)."""
+        used, and the logits are those of each prompt's last token, (prompts, vocab); a PagedStep
+        gives those of the rows that have new tokens, in order, likewise."""
         self.check_cache_room(kv_cache, idx.size(1))
+        self._check_paged(idx, kv_cache)
         if isinstance(kv_cache, PackedPrefill):
             assert idx.size(0) == 1 and idx.size(1) == kv_cache.total, \
                 "a packed prefill takes every prompt's tokens as one (1, total) sequence"
@@ -834,7 +885,7 @@ class Model(nn.Module):
                 f"Sequence length grew beyond the rotary embeddings cache: {kv_cache.max_seqlen} > {n_pos}"
         x, h = self.body.forward_carry(self.embedding(idx), kv_cache)
         kv_cache.advance(idx.size(1))
-        if isinstance(kv_cache, PackedPrefill):  # (prompts, vocab) at each prompt's last token
+        if isinstance(kv_cache, (PackedPrefill, PagedStep)):  # at each prompt's (row's) last token
             last = kv_cache.last
             return self.unembedding(x[0, last].unsqueeze(1),
                                     None if h is None else h[0, last].unsqueeze(1))[:, 0]
@@ -883,6 +934,15 @@ class ModelManager:
         return KVCache(batch_size=batch_size, seq_len=seq_len,
                        device=device or model.get_device(), dtype=self.runtime.compute_dtype,
                        **spec)
+
+    def new_paged_kv_cache(self, model, *, batch_size, seq_len, n_pages=None, page_size=16,
+                           device=None):
+        """A PagedKVCache for the model: rows of at most seq_len tokens that share n_pages pages
+        (default: enough for every row at seq_len)."""
+        spec = kv_cache_spec(model.layer_specs())
+        return PagedKVCache(batch_size=batch_size, seq_len=seq_len, n_pages=n_pages,
+                            page_size=page_size, device=device or model.get_device(),
+                            dtype=self.runtime.compute_dtype, **spec)
 
     def new_decoder(self, model, tokens, *, num_samples=1, max_tokens=None, device=None):
         from modelcore_amd.generate import Decoder
