@@ -53,6 +53,7 @@ SOURCE_FLAGS = {
     "prefill_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "prefill_tiled.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "paged_tiled.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "paged_stream.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "decode_fused.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],  # its shared-prefix jobs
 }
 

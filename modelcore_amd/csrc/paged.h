@@ -51,6 +51,12 @@ __device__ __forceinline__ void row_tokens(const int32_t *cu, int t_new, int tot
   T = cu ? max(min(cu[b + 1], total) - tok0, 0) : t_new;
 }
 
+// Whether a row of T new tokens is one of few pairs, which the streaming kernels take: a single token, or
+// at most `most` (token, head) pairs per KV head; most = 0: none is.
+__device__ __forceinline__ bool few_pairs(int T, int G, int most) {
+  return most > 0 && (T == 1 || int64_t(T) * G <= most);
+}
+
 // A block of queries of a row: its block qt, the row's tokens and its position.
 struct PagedBlock {
   int b, qt, tok0, T, s0;
@@ -60,7 +66,7 @@ struct PagedBlock {
 
 // Block i of a call, blocks with the most keys first: by their number within their row, last first,
 // and rows in order within a number, so that long rows do not fall to one XCD. `pairs` (position,
-// head) pairs make a block; rows of at most `skip` pairs have none. Each wave does this by itself:
+// head) pairs make a block; rows of few_pairs() by `skip` have none. Each wave does this by itself:
 // the rows' counts, four a lane, stay in registers (rows past 256 are read again), and the number is
 // found by bisection over how many blocks there are from it on.
 //
@@ -79,8 +85,8 @@ __device__ __forceinline__ bool find_paged_block(const int32_t *cu, const int32_
     return v.part < v.most && blocks > 0;
   };
   if (!cu) {
-    const int64_t n_pairs = int64_t(t_new) * G;
-    const int each = n_pairs > skip ? int((n_pairs + pairs - 1) / pairs) : 0;
+    const int each =
+        few_pairs(t_new, G, skip) ? 0 : int((int64_t(t_new) * G + pairs - 1) / pairs);
     if (!range_of(each * n_rows)) return false;
     v.qt = each - 1 - i / n_rows;
     v.b = i % n_rows;
@@ -89,8 +95,7 @@ __device__ __forceinline__ bool find_paged_block(const int32_t *cu, const int32_
       if (b >= n_rows) return 0;
       int tok0, T;
       row_tokens(cu, t_new, total, b, tok0, T);
-      const int64_t n = int64_t(T) * G;
-      return n > skip ? int((n + pairs - 1) / pairs) : 0;
+      return few_pairs(T, G, skip) ? 0 : int((int64_t(T) * G + pairs - 1) / pairs);
     };
     int mine[4];
 #pragma unroll
@@ -143,6 +148,10 @@ inline int64_t paged_blocks_bound(const PagedArgs &a, int64_t pairs) {
 }
 
 int launch_paged_append(const PagedArgs &a);
-int launch_paged_tiled(const PagedArgs &a);
+// Rows of few pairs (few_pairs(.., most)) of a bf16 call: append where k_new is given, and attention.
+int launch_paged_stream(const PagedArgs &a, int64_t most);
+size_t paged_stream_bytes(const PagedArgs &a, int64_t most);  // of scratch, to cut long rows' keys
+// Every row but those.
+int launch_paged_tiled(const PagedArgs &a, int64_t skip);
 
 }  // namespace mcamd

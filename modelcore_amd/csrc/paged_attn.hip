@@ -2,6 +2,7 @@
 // their pages, and which kernels a call takes.
 #include "paged.h"
 
+#include <algorithm>
 #include <cmath>
 
 namespace mcamd {
@@ -80,6 +81,8 @@ int check(const PagedArgs &a) {
     return fail(MCAMD_EUNSUPPORTED, "paged attention: more than 64 query heads per KV head");
   if (!a.q || !a.out || !a.k_pages || !a.v_pages || !a.kv.table || !a.seqlens)
     return a.n_rows > 0 && a.total > 0 ? fail(MCAMD_EINVAL, "paged attention: null pointer") : MCAMD_OK;
+  if ((int64_t(a.n_kv_head) << a.kv.shift) * a.head_dim * elem > 0x7fffffff)
+    return fail(MCAMD_EUNSUPPORTED, "paged attention: a page of more than 2 GiB");
   if (!aligned(a.q, 16) || !aligned(a.out, 16) || !aligned(a.k_pages, 16) ||
       !aligned(a.v_pages, 16) || (a.k_new && !aligned(a.k_new, 16)) ||
       (a.v_new && !aligned(a.v_new, 16)) || a.kv.page_stride * elem % 16 != 0 ||
@@ -88,12 +91,31 @@ int check(const PagedArgs &a) {
   return MCAMD_OK;
 }
 
-int launch(const PagedArgs &a) {
-  if (a.k_new) {
-    int st = launch_paged_append(a);
+// Pairs per KV head up to which a row counts as one of few pairs: one block of the streaming kernel.
+constexpr int64_t kFewPairs = 32;
+
+struct Kernels {
+  bool stream, tiles;
+};
+Kernels kernels_of(const PagedArgs &a) {
+  const int64_t G = a.n_head / a.n_kv_head;
+  const bool few = a.t_new == 1 || a.t_new * G <= kFewPairs;  // of every row
+  if (a.dtype != MCAMD_BF16) return {false, true};
+  return {few || a.cu != nullptr, !few};
+}
+
+int launch(PagedArgs a) {
+  const Kernels k = kernels_of(a);
+  if (a.k_new && k.tiles) {  // the streaming kernel appends by itself
+    const int st = launch_paged_append(a);
     if (st != MCAMD_OK) return st;
+    a.k_new = a.v_new = nullptr;
   }
-  return launch_paged_tiled(a);
+  if (k.stream) {
+    const int st = launch_paged_stream(a, kFewPairs);
+    if (st != MCAMD_OK || !k.tiles) return st;
+  }
+  return launch_paged_tiled(a, k.stream ? kFewPairs : 0);
 }
 
 }  // namespace
@@ -126,9 +148,31 @@ extern "C" size_t mcamd_paged_scratch_bytes(int64_t n_rows, int64_t total, int64
                                             int64_t n_head, int64_t n_kv_head, int64_t head_dim,
                                             int64_t max_pages, int64_t page_size, int64_t window,
                                             int dtype) {
-  (void)n_rows, (void)total, (void)max_seqlen, (void)n_head, (void)n_kv_head, (void)head_dim;
-  (void)max_pages, (void)page_size, (void)window, (void)dtype;
-  return 0;
+  if (n_rows <= 0 || total <= 0 || max_seqlen <= 0 || n_kv_head <= 0 || n_head < n_kv_head ||
+      head_dim <= 0 || head_dim > 256 || max_pages <= 0 || page_size < kMinPageSize ||
+      n_head > 65535 || n_rows > 65535 || max_pages > (int64_t(1) << 30) / page_size ||
+      total > (int64_t(1) << 30) / n_head)
+    return 0;
+  PagedArgs a{};
+  while ((int64_t(1) << a.kv.shift) < page_size) ++a.kv.shift;
+  a.kv.max_pages = int(max_pages);
+  a.n_rows = n_rows;
+  a.t_new = max_seqlen;
+  a.total = total;
+  a.n_head = n_head;
+  a.n_kv_head = n_kv_head;
+  a.head_dim = head_dim;
+  a.window = window;
+  a.dtype = dtype;
+  // The sizes do not tell packed rows from uniform ones: room for both.
+  const int32_t packed = 0;
+  size_t most = 0;
+  for (const int32_t *cu : {(const int32_t *)nullptr, &packed}) {
+    a.cu = cu;
+    const Kernels k = kernels_of(a);
+    if (k.stream) most = std::max(most, paged_stream_bytes(a, kFewPairs));
+  }
+  return most;
 }
 
 extern "C" int mcamd_flash_attn_paged_with_kvcache(
