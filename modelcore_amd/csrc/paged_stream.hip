@@ -3,10 +3,12 @@
 // row needs few, go to the matrix cores because they take no time there.
 //
 // Work split. A row's keys are cut into ranges of whole 32-key tiles; a workgroup of four waves owns
-// (row, range, group of up to four KV heads), a wave a KV head of it (with fewer KV heads the waves
-// share a head's tiles). How many ranges a row gets is worked out on the device from the lengths of all
-// rows: ranges of S tiles, S such that the call fills the chip kWorkgroups times, at least kMinTiles.
-// Every wave does this sum by itself, 64 rows at a time.
+// (row, range, group of KV heads). In a large call a wave has a KV head (the four read token rows in runs
+// of four heads, and nothing is shared between them); in one whose tiles are few the four waves take
+// every fourth tile of one head, so that short rows are a tile deep. Which, and how many ranges a row gets,
+// is worked out on the device from the lengths of all rows: ranges of `len` tiles such that all ranges are
+// on the chip at once (kFill workgroups a compute unit), at least kMinTiles. Every wave does this sum by
+// itself, 64 rows at a time.
 //
 // A wave. Its tile of 32 keys is staged in LDS by itself alone, straight from HBM (buffer loads to LDS,
 // 16 bytes a lane, whole rows), so that waves never wait for one another: K of the next tile is under way
@@ -21,10 +23,13 @@
 // LDS rows are swizzled in 16-byte chunks, K so that 16 rows' reads of a chunk fall on all banks, V so
 // that a transpose read's four rows do.
 //
+// The loads are marked non-temporal (the pages are read once per call): 32 rows of up to 8192 keys, 16 / 4
+// heads of 128, 57.7 -> 51.0 us, 60 rows of 32 / 8 heads 196 -> 165 (6.2 TB/s).
+//
 // New tokens come from k_new and v_new where given, and the wave that has a row's last keys puts them in
 // their pages. A row of one range writes its output; otherwise (o, m, l) go to scratch in fp32, a row of
-// floats per pair, and the merge launch adds the ranges up, a wave per pair. Pairs that are not finite
-// are redone (paged_careful.h).
+// floats per pair, and the merge launch adds the ranges up. Pairs that are not finite are redone
+// (paged_careful.h).
 #include "paged_careful.h"
 
 #include <algorithm>
@@ -36,29 +41,29 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int KT = 32;  // keys per tile
-#ifndef MCAMD_STREAM_FILL
-#define MCAMD_STREAM_FILL 2
-#endif
-#ifndef MCAMD_STREAM_MIN_TILES
-#define MCAMD_STREAM_MIN_TILES 4
-#endif
-constexpr int kFill = MCAMD_STREAM_FILL;           // workgroups per compute unit that a call aims at
-constexpr int kMinTiles = MCAMD_STREAM_MIN_TILES;  // of a wave's range, unless the row is shorter
+constexpr int kFill = 2;      // workgroups per compute unit that a call aims at (LDS holds two at DP = 128)
+constexpr int kMinTiles = 2;  // of a wave's range, unless the row is shorter
+// A head per wave from so many tiles a wave on. One row of 16K keys, 8 KV heads (2 a wave): 27.1 us so,
+// 18.8 with four waves a head; 60 rows of 4160 keys on average (15.6): 167.9 and 210.
+constexpr int kDeepTiles = 4;
+constexpr int kNonTemporal = 2;  // cache policy of the pages' loads
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(4))) int32_t *scalar_ints;  // read only, by the scalar unit
 
 struct StreamParams : CarefulParams {
   const void *k_new, *v_new;
   const int32_t *seqlens, *cu;
   float *part_o, *part_ml;  // [slot][pair_slots][DP], [slot][pair_slots][2]
+  int2 *where;              // per row: its first range and the ranges of a block, for the merge
   int n_rows, t_new, total, H, G;
   int most;        // pairs of a row, at most (a single token's rows are always taken)
-  int head_waves;  // KV heads of a workgroup
-  int target;      // ranges a group of KV heads aims at
+  int head_waves;  // KV heads of a workgroup, in a large call
+  int target;      // workgroups a call aims at; 0: no row is cut
   int pair_slots;  // pairs per partial slot
 };
 
@@ -95,18 +100,37 @@ __device__ __forceinline__ int wave_scan(int x, int lane) {
   return x;
 }
 
-// Tiles of a range, at most.
-__device__ __forceinline__ int range_len(const StreamParams &P, int lane, const Row &first) {
-  int64_t work = 0;
+// How a call is cut: KV heads of a workgroup, and tiles of a range, at most.
+struct Cut {
+  int head_waves, len;
+};
+__device__ __forceinline__ Cut cut_of(const StreamParams &P, int lane, const Row &first) {
+  int64_t work = 0, units = 0;
   for (int b = lane; b < P.n_rows; b += 64) {
     const Row r = b == lane ? first : row_of(P, b);
     work += int64_t(r.blocks) * r.tiles;
+    units += r.blocks;
   }
-  work = wave_total64(work);
-  const int64_t len = (work + P.target - 1) / P.target;
-  return int(max(len, int64_t(kMinTiles * kWaves / P.head_waves)));
+  if (__builtin_amdgcn_ballot_w64(work >= (1 << 24)) == 0) {  // the sums fit 32 bits
+    work = wave_total(int(work));
+    units = wave_total(int(units));
+  } else {
+    work = wave_total64(work);
+    units = wave_total64(units);
+  }
+  if (P.target == 0) return Cut{1, 0x7fffffff};
+  Cut c;
+  c.head_waves = work * P.H_kv > int64_t(kDeepTiles * kWaves) * P.target ? P.head_waves : 1;
+  // A row's last range may be shorter than the others: work / len ranges and up to one per block of pairs
+  // more, all of which are to be on the chip at once.
+  const int target = max(1, P.target * c.head_waves / P.H_kv);
+  const int64_t most = max(target - units, int64_t(target + 1) / 2);
+  c.len = int(max((work + most - 1) / most, int64_t(kMinTiles * kWaves / c.head_waves)));
+  return c;
 }
-__device__ __forceinline__ int ranges_of(const Row &r, int len) { return (r.tiles + len - 1) / len; }
+__device__ __forceinline__ int ranges_of(const Row &r, int len) {
+  return int((uint32_t(r.tiles) + uint32_t(len) - 1) / uint32_t(len));
+}
 
 template <int DP>
 struct Shape {
@@ -198,7 +222,8 @@ __device__ __forceinline__ float sum_halves(float x) {
 }
 
 template <int DP>
-__global__ __launch_bounds__(kThreads) void paged_stream_kernel(StreamParams P) {
+__global__ __launch_bounds__(kThreads)
+    __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 2 : 1))) void paged_stream_kernel(StreamParams P) {
   using S_ = Shape<DP>;
   constexpr int CPR = S_::CPR, RPI = S_::RPI, NI = S_::NI, NV = S_::NV, KD = S_::KD, MD = S_::MD;
   // A wave's K tile, then its V tile; at the end its accumulators (32 pairs of DP floats).
@@ -207,13 +232,13 @@ __global__ __launch_bounds__(kThreads) void paged_stream_kernel(StreamParams P) 
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n_groups = P.H_kv / P.head_waves;
+  // This workgroup's heads, row, block of pairs and range.
+  const Row mine = row_of(P, min(lane, P.n_rows - 1));
+  const Cut cut = cut_of(P, lane, mine);
+  const int head_waves = cut.head_waves, len = cut.len;
+  const int n_groups = P.H_kv / head_waves;
   const int group = blockIdx.x % n_groups;
   int id = blockIdx.x / n_groups;  // of the ranges of all rows
-
-  // This workgroup's row, block of pairs and range.
-  const Row mine = row_of(P, min(lane, P.n_rows - 1));
-  const int len = range_len(P, lane, mine);
   int b = -1, ranges = 0;
   Row R;
   for (int b0 = 0; b0 < P.n_rows; b0 += 64) {
@@ -242,9 +267,11 @@ __global__ __launch_bounds__(kThreads) void paged_stream_kernel(StreamParams P) 
   }
   if (b < 0) return;
   const int block = id / ranges, range = id - block * ranges;
+  if (id == 0 && group == 0 && threadIdx.x == 0 && P.where)
+    P.where[b] = make_int2(int(blockIdx.x / n_groups), ranges);
 
-  const int kvh = group * P.head_waves + wave % P.head_waves;
-  const int kw = wave / P.head_waves, n_kw = kWaves / P.head_waves;  // this wave's share of the tiles
+  const int kvh = group * head_waves + wave % head_waves;
+  const int kw = wave / head_waves, n_kw = kWaves / head_waves;  // this wave's share of the tiles
   const int D = P.D;
   const int h = lane >> 5, col = lane & 31;
   const int pairs = R.T * P.G;
@@ -347,7 +374,7 @@ __global__ __launch_bounds__(kThreads) void paged_stream_kernel(StreamParams P) 
         }
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
             rsrc, (__attribute__((address_space(3))) void *)(to + (half * NV + i) * 512), 16, int(o),
-            in_page, 0, 0);
+            in_page, 0, kNonTemporal);
       }
     }
   };
@@ -500,171 +527,191 @@ __global__ __launch_bounds__(kThreads) void paged_stream_kernel(StreamParams P) 
     }
   }
 
-  // The waves of a head: each but the first leaves its sums in its own tiles' place.
+  // The waves of a head leave their sums in their tiles' place; each adds up the dims 32 md .. of every
+  // n_kw-th md, which are its own from here on.
   if (n_kw > 1) {
-    float *so = reinterpret_cast<float *>(s_tiles[wave][0]);
     static_assert(2 * S_::TILE * 2 == 32 * DP * 4, "a wave's sums fit its tiles");
-    if (kw > 0) {
+    float *so = reinterpret_cast<float *>(s_tiles[wave][0]);
 #pragma unroll
-      for (int md = 0; md < MD; ++md)
+    for (int md = 0; md < MD; ++md)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<float4 *>(so + ((md * 4 + j) * 64 + lane) * 4) =
-              make_float4(o[md][4 * j], o[md][4 * j + 1], o[md][4 * j + 2], o[md][4 * j + 3]);
-      if (h == 0) s_ml[wave][0][col] = m, s_ml[wave][1][col] = l;
-    }
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<float4 *>(so + ((md * 4 + j) * 64 + lane) * 4) =
+            make_float4(o[md][4 * j], o[md][4 * j + 1], o[md][4 * j + 2], o[md][4 * j + 3]);
+    if (h == 0) s_ml[wave][0][col] = m, s_ml[wave][1][col] = l;
     __syncthreads();
-    if (kw > 0) return;
-    for (int k = 1; k < n_kw; ++k) {
-      const int w2 = wave + k * P.head_waves;
-      const float m2 = s_ml[w2][0][col], l2 = s_ml[w2][1][col];
-      const float *s2 = reinterpret_cast<const float *>(s_tiles[w2][0]);
-      const float m_new = fmaxf(m, m2);
-      const float a1 = m == -INFINITY ? 0.f : fast_exp2(m - m_new);
-      const float a2 = m2 == -INFINITY ? 0.f : fast_exp2(m2 - m_new);
-      // A wave that saw no key has l = 0; a NaN l must stay.
-      l = l * (m == -INFINITY ? 1.f : a1) + l2 * (m2 == -INFINITY ? 1.f : a2);
-      m = m_new;
+    const int w0 = wave % head_waves;
+    float M = -INFINITY;
+    for (int w = w0; w < kWaves; w += head_waves) M = fmaxf(M, s_ml[w][0][col]);
+    float L = 0.f;
 #pragma unroll
-      for (int md = 0; md < MD; ++md)
+    for (int md = 0; md < MD; ++md)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[md][e] = 0.f;
+    for (int w = w0; w < kWaves; w += head_waves) {
+      const float mw = s_ml[w][0][col];
+      const float a = mw == -INFINITY ? 0.f : fast_exp2(mw - M);
+      L += s_ml[w][1][col] * (mw == -INFINITY ? 1.f : a);  // without a key l = 0; a NaN l must stay
+      const float *s2 = reinterpret_cast<const float *>(s_tiles[w][0]);
+#pragma unroll
+      for (int md = 0; md < MD; ++md) {
+        if (md % n_kw != kw) continue;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float4 x = *reinterpret_cast<const float4 *>(s2 + ((md * 4 + j) * 64 + lane) * 4);
-          o[md][4 * j] = fmaf(x.x, a2, o[md][4 * j] * a1);
-          o[md][4 * j + 1] = fmaf(x.y, a2, o[md][4 * j + 1] * a1);
-          o[md][4 * j + 2] = fmaf(x.z, a2, o[md][4 * j + 2] * a1);
-          o[md][4 * j + 3] = fmaf(x.w, a2, o[md][4 * j + 3] * a1);
+          o[md][4 * j] = fmaf(x.x, a, o[md][4 * j]);
+          o[md][4 * j + 1] = fmaf(x.y, a, o[md][4 * j + 1]);
+          o[md][4 * j + 2] = fmaf(x.z, a, o[md][4 * j + 2]);
+          o[md][4 * j + 3] = fmaf(x.w, a, o[md][4 * j + 3]);
         }
+      }
     }
+    m = M;
+    l = L;
   }
 
   // o[md][4j + i] is dim 32 md + 8 j + 4 h + i of pair `col`.
   if (ranges > 1) {
     if (!live) return;
     const int64_t slot =
-        (int64_t(blockIdx.x) * P.head_waves + wave % P.head_waves) * P.pair_slots + col;
+        (int64_t(blockIdx.x) * head_waves + wave % head_waves) * P.pair_slots + col;
     float *po = P.part_o + slot * DP;
 #pragma unroll
-    for (int md = 0; md < MD; ++md)
+    for (int md = 0; md < MD; ++md) {
+      if (md % n_kw != kw) continue;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (32 * md + 8 * j < D)
           *reinterpret_cast<float4 *>(po + 32 * md + 8 * j + 4 * h) =
               make_float4(o[md][4 * j], o[md][4 * j + 1], o[md][4 * j + 2], o[md][4 * j + 3]);
-    if (h == 0) *reinterpret_cast<float2 *>(P.part_ml + slot * 2) = make_float2(m, l);
+    }
+    if (h == 0 && kw == 0) *reinterpret_cast<float2 *>(P.part_ml + slot * 2) = make_float2(m, l);
     return;
   }
   const float inv = 1.f / l;
-  bool ok = true;
+  uint32_t bad_of = 0;  // lane md: the pairs whose dims 32 md .. are not finite
 #pragma unroll
-  for (int md = 0; md < MD; ++md)
+  for (int md = 0; md < MD; ++md) {
+    if (md % n_kw != kw || 32 * md >= D) continue;
+    bool ok = true;
+    bf16x4 y[4];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      o[md][e] *= inv;
-      ok = ok && (finite(o[md][e]) || 32 * md + 8 * (e >> 2) >= D);
-    }
-  const uint64_t bad64 = __builtin_amdgcn_ballot_w64(live && !ok);
-  const uint32_t bad = uint32_t(bad64) | uint32_t(bad64 >> 32);
-  if (live && !((bad >> col) & 1u)) {
+    for (int j = 0; j < 4; ++j) {
+      f32x4 x;
 #pragma unroll
-    for (int md = 0; md < MD; ++md)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int d = 32 * md + 8 * j + 4 * h;
-        if (d < D) {
-          uint2 u;
-          u.x = f32_to_bf16_bits(o[md][4 * j]) | (uint32_t(f32_to_bf16_bits(o[md][4 * j + 1])) << 16);
-          u.y = f32_to_bf16_bits(o[md][4 * j + 2]) | (uint32_t(f32_to_bf16_bits(o[md][4 * j + 3])) << 16);
-          *reinterpret_cast<uint2 *>(out + d) = u;
-        }
+      for (int i = 0; i < 4; ++i) {
+        x[i] = o[md][4 * j + i] * inv;
+        ok = ok && (finite(x[i]) || 32 * md + 8 * j >= D);
       }
+      y[j] = __builtin_convertvector(x, bf16x4);
+    }
+    const uint64_t bad64 = __builtin_amdgcn_ballot_w64(live && !ok);
+    const uint32_t bad = uint32_t(bad64) | uint32_t(bad64 >> 32);
+    if (live && !((bad >> col) & 1u)) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (32 * md + 8 * j < D)
+          *reinterpret_cast<uint2 *>(out + 32 * md + 8 * j + 4 * h) = __builtin_bit_cast(uint2, y[j]);
+    }
+    bad_of = lane == md ? bad : bad_of;
   }
-  for (uint32_t left = bad; __builtin_expect(left != 0, 0); left &= left - 1) {
-    const int c = __builtin_ctz(left);
-    const int pr = block * 32 + c, t = pr / P.G;
-    const int64_t a = (int64_t(R.tok0 + t) * P.H + kvh * P.G + (pr - t * P.G)) * D;
-    careful_pair<bf16, DP, 8>(P, b, kvh, a, R.s0 + t, lane, 0, D);
-  }
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(bad_of != 0) == 0, 1)) return;
+  for (int md = 0; md < MD; ++md)
+    for (uint32_t left = __builtin_amdgcn_readlane(bad_of, md); left != 0; left &= left - 1) {
+      const int pr = block * 32 + __builtin_ctz(left), t = pr / P.G;
+      careful_pair<bf16, DP, 8>(P, b, kvh,
+                                (int64_t(R.tok0 + t) * P.H + kvh * P.G + (pr - t * P.G)) * D, R.s0 + t,
+                                lane, 32 * md, min(32 * md + 32, D));
+    }
 }
 
-// The ranges of a pair added up, a wave per pair: lane l has dims l, l + 64, ..
-template <int DP>
-__global__ __launch_bounds__(kThreads) void paged_stream_merge_kernel(StreamParams P) {
+// The ranges of a pair added up: a workgroup of MW waves per pair, each of which takes every MW-th range,
+// lane l dims l, l + 64, .. The streaming kernel has left where a row's ranges lie. Bound by the latency of
+// three round trips, and with many pairs by how many workgroups the chip holds: few pairs, whose rows are
+// in many ranges, take eight waves (one row of 16K keys, 64 ranges: 4.2 us, with four 8.5), more than
+// kManyPairs two (60 rows of 32 heads: 6.3 us, with four 7.9, with eight 11.0).
+constexpr int64_t kManyPairs = 1024;
+template <int DP, int MW>
+__global__ __launch_bounds__(64 * MW) void paged_stream_merge_kernel(StreamParams P) {
+  constexpr int N = (DP + 63) / 64, U = 8;
+  __shared__ float s_o[MW][DP], s_ml[MW][2];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kvh = blockIdx.x % P.H_kv;
-  const int pair = (blockIdx.x / P.H_kv) * kWaves + wave;
   const int b = blockIdx.y;
-  const Row mine = row_of(P, b);
-  if (mine.blocks == 0 || pair >= mine.T * P.G || !mine.ok) return;
-  const Row first = row_of(P, min(lane, P.n_rows - 1));
-  const int len = range_len(P, lane, first);
-  const int ranges = ranges_of(mine, len);
+  const int2 where = P.where[b];
+  const Row R = row_of(P, b);
+  if (R.blocks == 0 || !R.ok) return;
+  const int ranges = where.y;
   if (ranges == 1) return;  // written already
-  int64_t before = 0;       // ranges of the rows before this one
-  for (int r0 = lane; r0 < b; r0 += 64) {
-    const Row r = r0 == lane ? first : row_of(P, r0);
-    before += ranges_of(r, len) * r.blocks;
-  }
-  before = wave_total64(before);
-  const int block = pair / 32, n_groups = P.H_kv / P.head_waves;
-  const int64_t unit = before + int64_t(block) * ranges;
-  const int64_t step = int64_t(n_groups) * P.head_waves * P.pair_slots;  // from range to range
-  const int64_t slot = ((unit * n_groups + kvh / P.head_waves) * P.head_waves + kvh % P.head_waves) *
-                           P.pair_slots + (pair & 31);
-  constexpr int N = (DP + 63) / 64, U = 8;
-  float M = -INFINITY, L = 0.f, o[N];
+  const int64_t step = int64_t(P.H_kv) * P.pair_slots;  // from range to range
+  for (int pair = blockIdx.x / P.H_kv; pair < R.T * P.G; pair += gridDim.x / P.H_kv) {
+    const int64_t unit = where.x + int64_t(pair / 32) * ranges;
+    const int64_t slot = (unit * P.H_kv + kvh) * P.pair_slots + pair % 32;
+    float M = -INFINITY, L = 0.f, o[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) o[i] = 0.f;
-  for (int r0 = 0; r0 < ranges; r0 += U) {
-    float2 x[U];
-    float v[U][N];
+    for (int i = 0; i < N; ++i) o[i] = 0.f;
+    auto join = [&](float m2, float l2, const float (&o2)[N]) {
+      const float m_new = fmaxf(M, m2);
+      const float a1 = M == -INFINITY ? 0.f : fast_exp2(M - m_new);
+      const float a2 = m2 == -INFINITY ? 0.f : fast_exp2(m2 - m_new);
+      // A range without a key has l = 0; a NaN l must stay.
+      L = L * (M == -INFINITY ? 1.f : a1) + l2 * (m2 == -INFINITY ? 1.f : a2);
+      M = m_new;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t at = slot + min(r0 + u, ranges - 1) * step;
-      x[u] = *reinterpret_cast<const float2 *>(P.part_ml + at * 2);
+      for (int i = 0; i < N; ++i) o[i] = fmaf(o2[i], a2, o[i] * a1);
+    };
+    for (int r0 = wave; r0 < ranges; r0 += U * MW) {
+      float2 x[U];
+      float v[U][N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[u][i] = P.part_o[at * DP + min(lane + 64 * i, P.D - 1)];
+      for (int u = 0; u < U; ++u) {
+        const int64_t at = slot + min(r0 + u * MW, ranges - 1) * step;
+        x[u] = *reinterpret_cast<const float2 *>(P.part_ml + at * 2);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[u][i] = P.part_o[at * DP + min(lane + 64 * i, P.D - 1)];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r0 + u * MW < ranges) join(x[u].x, x[u].y, v[u]);
     }
-    float m_new = M;
+    __syncthreads();  // the pair before has been added up
 #pragma unroll
-    for (int u = 0; u < U; ++u) m_new = fmaxf(m_new, x[u].x);
-    const float keep = M == -INFINITY ? 0.f : fast_exp2(M - m_new);
-    L *= M == -INFINITY ? 1.f : keep;
+    for (int i = 0; i < N; ++i)
+      if (lane + 64 * i < DP) s_o[wave][lane + 64 * i] = o[i];
+    if (lane == 0) s_ml[wave][0] = M, s_ml[wave][1] = L;
+    __syncthreads();
+    if (wave > 0) continue;
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] *= keep;
-    M = m_new;
+    for (int w = 1; w < MW; ++w) {
+      float o2[N];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (r0 + u >= ranges) break;
-      const float a = x[u].x == -INFINITY ? 0.f : fast_exp2(x[u].x - M);
-      L += x[u].y * (x[u].x == -INFINITY ? 1.f : a);
-#pragma unroll
-      for (int i = 0; i < N; ++i) o[i] = fmaf(v[u][i], a, o[i]);
+      for (int i = 0; i < N; ++i) o2[i] = s_o[w][min(lane + 64 * i, DP - 1)];
+      join(s_ml[w][0], s_ml[w][1], o2);
     }
-  }
-  const float inv = 1.f / L;
-  const int t = pair / P.G;
-  const int64_t at = (int64_t(mine.tok0 + t) * P.H + kvh * P.G + (pair - t * P.G)) * P.D;
-  bool ok = true;
+    const float inv = 1.f / L;
+    const int t = pair / P.G;
+    const int64_t at = (int64_t(R.tok0 + t) * P.H + kvh * P.G + (pair - t * P.G)) * P.D;
+    bool ok = true;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    o[i] *= inv;
-    ok = ok && (finite(o[i]) || lane + 64 * i >= P.D);
-  }
-  if (__builtin_expect(__builtin_amdgcn_ballot_w64(!ok) != 0, 0)) {
-    careful_pair<bf16, DP, 8>(P, b, kvh, at, mine.s0 + t, lane, 0, P.D);
-    return;
-  }
+    for (int i = 0; i < N; ++i) {
+      o[i] *= inv;
+      ok = ok && (finite(o[i]) || lane + 64 * i >= P.D);
+    }
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!ok) != 0, 0)) {
+      careful_pair<bf16, DP, 8>(P, b, kvh, at, R.s0 + t, lane, 0, P.D);
+      continue;
+    }
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (lane + 64 * i < P.D) static_cast<bf16 *>(P.out)[at + lane + 64 * i] = from_f32<bf16>(o[i]);
+    for (int i = 0; i < N; ++i)
+      if (lane + 64 * i < P.D) static_cast<bf16 *>(P.out)[at + lane + 64 * i] = from_f32<bf16>(o[i]);
+  }
 }
 
 struct StreamPlan {
   int head_waves, target, pair_slots;
-  int64_t units;     // blocks of pairs of all rows, at most
-  int64_t max_pairs;  // of a row
+  int64_t units;        // blocks of pairs of all rows, at most
+  int64_t merge_pairs;  // workgroups of the merge per (row, KV head)
   bool cut;
 };
 
@@ -672,34 +719,38 @@ StreamPlan plan_of(const PagedArgs &a, int64_t most) {
   StreamPlan p;
   const int64_t G = a.n_head / a.n_kv_head;
   p.head_waves = a.n_kv_head % 4 == 0 ? 4 : a.n_kv_head % 2 == 0 ? 2 : 1;
-  const int64_t groups = a.n_kv_head / p.head_waves;
-  p.target = int(std::max<int64_t>(1, kFill * device_cus() / groups));
-  p.max_pairs = std::min(a.t_new * G, std::max(most, G));
-  p.units = a.n_rows * ((p.max_pairs + 31) / 32);
-  p.pair_slots = int(std::min<int64_t>(32, p.max_pairs));
+  p.target = kFill * device_cus();
+  const int64_t max_pairs = std::min(a.t_new * G, std::max(most, G));
+  p.merge_pairs = a.cu ? G : max_pairs;  // most rows of a mixture have one token
+  p.units = a.n_rows * ((max_pairs + 31) / 32);
+  p.pair_slots = int(std::min<int64_t>(32, max_pairs));
   const int64_t room = int64_t(a.kv.max_pages) << a.kv.shift;
   const int64_t keys = std::min(room, a.window >= 0 ? a.window + 2 * KT + most : room);
-  p.cut = (keys + KT - 1) / KT > kMinTiles * kWaves / p.head_waves;
+  p.cut = (keys + KT - 1) / KT > kMinTiles * kWaves;
   return p;
 }
 
 int head_pad(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 int64_t slots_of(const PagedArgs &a, const StreamPlan &p) {
-  return (p.units + p.target) * a.n_kv_head * p.pair_slots;
+  // unit ids * H_kv: a call's ranges, at most target * head_waves / H_kv and one per unit.
+  return ((p.units + 1) * a.n_kv_head + int64_t(p.target) * p.head_waves) * p.pair_slots;
 }
 
 template <int DP>
 int run(const StreamParams &P, const PagedArgs &a, const StreamPlan &p) {
-  const int64_t blocks = (p.units + (p.cut ? p.target : 0)) * (a.n_kv_head / p.head_waves);
+  // A KV head at a time, or up to the target.
+  const int64_t blocks = p.units * a.n_kv_head + (p.cut ? std::max<int64_t>(p.target, a.n_kv_head) : 0);
   if (blocks > 0x7fffffff / kThreads || a.n_rows > 65535)
     return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
   hipLaunchKernelGGL(paged_stream_kernel<DP>, dim3(unsigned(blocks)), dim3(kThreads), 0, a.stream, P);
   const int st = launch_status("paged_stream");
   if (st != MCAMD_OK || !p.cut) return st;
-  const unsigned x = unsigned(a.n_kv_head * ((p.max_pairs + kWaves - 1) / kWaves));
-  hipLaunchKernelGGL(paged_stream_merge_kernel<DP>, dim3(x, unsigned(a.n_rows)), dim3(kThreads), 0,
-                     a.stream, P);
+  const dim3 grid{unsigned(a.n_kv_head * p.merge_pairs), unsigned(a.n_rows)};
+  if (int64_t(grid.x) * grid.y > kManyPairs)
+    hipLaunchKernelGGL((paged_stream_merge_kernel<DP, 2>), grid, dim3(128), 0, a.stream, P);
+  else
+    hipLaunchKernelGGL((paged_stream_merge_kernel<DP, 8>), grid, dim3(512), 0, a.stream, P);
   return launch_status("paged_stream_merge");
 }
 
@@ -707,7 +758,7 @@ int run(const StreamParams &P, const PagedArgs &a, const StreamPlan &p) {
 
 size_t paged_stream_bytes(const PagedArgs &a, int64_t most) {
   const StreamPlan p = plan_of(a, most);
-  return p.cut ? size_t(slots_of(a, p)) * (head_pad(a.head_dim) + 2) * 4 : 0;
+  return p.cut ? size_t(slots_of(a, p)) * (head_pad(a.head_dim) + 2) * 4 + size_t(a.n_rows) * 8 : 0;
 }
 
 int launch_paged_stream(const PagedArgs &a, int64_t most) {
@@ -730,6 +781,7 @@ int launch_paged_stream(const PagedArgs &a, int64_t most) {
   P.cu = a.cu;
   P.part_o = static_cast<float *>(a.scratch);
   P.part_ml = P.part_o + slots_of(a, p) * dp;
+  P.where = p.cut ? reinterpret_cast<int2 *>(P.part_ml + slots_of(a, p) * 2) : nullptr;
   P.n_rows = int(a.n_rows);
   P.t_new = int(a.t_new);
   P.total = int(a.total);
@@ -737,7 +789,7 @@ int launch_paged_stream(const PagedArgs &a, int64_t most) {
   P.G = int(a.n_head / a.n_kv_head);
   P.most = int(most);
   P.head_waves = p.head_waves;
-  P.target = p.cut ? p.target : 1;
+  P.target = p.cut ? p.target : 0;
   P.pair_slots = p.pair_slots;
   switch (dp) {
     case 32: return run<32>(P, a, p);
