@@ -140,12 +140,27 @@ __device__ __forceinline__ bool find_paged_block(const int32_t *cu, const int32_
   return true;
 }
 
-// At most so many blocks of `pairs` pairs in a call.
-inline int64_t paged_blocks_bound(const PagedArgs &a, int64_t pairs) {
+// At most so many blocks of `pairs` pairs in a call's rows that are not of few_pairs(.., skip).
+inline int64_t paged_blocks_bound(const PagedArgs &a, int64_t pairs, int64_t skip) {
   const int64_t G = a.n_head / a.n_kv_head;
   if (!a.cu) return a.n_rows * ((a.t_new * G + pairs - 1) / pairs);
-  return a.total * G / pairs + (a.n_rows < a.total ? a.n_rows : a.total);
+  const int64_t shortest = skip > 0 ? (skip / G > 1 ? skip / G : 1) + 1 : 1;  // tokens of such a row
+  const int64_t rows = a.total / shortest < a.n_rows ? a.total / shortest : a.n_rows;
+  return a.total * G / pairs + rows;
 }
+
+// What the tiled kernels of long rows share beyond their own parameters.
+struct PagedTiles {
+  PagedKv kv;
+  int n_rows, total;
+  int skip;         // rows of few_pairs() by it are another launch's
+  int kt, align;    // keys of a tile, and what its first key is a multiple of
+  int groups;       // of 32 pairs, of a block
+  int slots;        // blocks for whose partials there is room, or 0: no block is cut
+  float ratio;      // prefill_split.h's, times the blocks of the call
+  float *part_o;    // [slot][groups of 32 pairs][md][4][64][4], as SplitGeo lays them out
+  float *part_ml;   // [slot][groups][32][2]
+};
 
 int launch_paged_append(const PagedArgs &a);
 // Rows of few pairs (few_pairs(.., most)) of a bf16 call: append where k_new is given, and attention.
@@ -153,5 +168,12 @@ int launch_paged_stream(const PagedArgs &a, int64_t most);
 size_t paged_stream_bytes(const PagedArgs &a, int64_t most);  // of scratch, to cut long rows' keys
 // Every row but those.
 int launch_paged_tiled(const PagedArgs &a, int64_t skip);
+size_t paged_tiled_bytes(const PagedArgs &a, int64_t skip);
+// The same for bf16 and head_dim 128.
+bool paged_mfma_supported(const PagedArgs &a);
+int launch_paged_mfma(const PagedArgs &a, int64_t skip);
+size_t paged_mfma_bytes(const PagedArgs &a, int64_t skip);
+// The ranges of cut blocks (of `pairs` pairs) added up.
+int launch_paged_tiles_merge(const PagedArgs &a, const PagedTiles &t, int pairs);
 
 }  // namespace mcamd

@@ -115,7 +115,8 @@ int launch(PagedArgs a) {
     const int st = launch_paged_stream(a, kFewPairs);
     if (st != MCAMD_OK || !k.tiles) return st;
   }
-  return launch_paged_tiled(a, k.stream ? kFewPairs : 0);
+  const int64_t skip = k.stream ? kFewPairs : 0;
+  return paged_mfma_supported(a) ? launch_paged_mfma(a, skip) : launch_paged_tiled(a, skip);
 }
 
 }  // namespace
@@ -170,7 +171,10 @@ extern "C" size_t mcamd_paged_scratch_bytes(int64_t n_rows, int64_t total, int64
   for (const int32_t *cu : {(const int32_t *)nullptr, &packed}) {
     a.cu = cu;
     const Kernels k = kernels_of(a);
+    const int64_t skip = k.stream ? kFewPairs : 0;
     if (k.stream) most = std::max(most, paged_stream_bytes(a, kFewPairs));
+    if (k.tiles)
+      most = std::max(most, paged_mfma_supported(a) ? paged_mfma_bytes(a, skip) : paged_tiled_bytes(a, skip));
   }
   return most;
 }

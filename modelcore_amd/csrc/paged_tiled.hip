@@ -19,6 +19,7 @@
 #include "prefill_order.h"
 #include "prefill_split.h"
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -38,12 +39,17 @@ typedef __bf16 lds_bf16x4 __attribute__((__vector_size__(4 * sizeof(__bf16))));
 
 struct TiledParams : CarefulParams {
   const int32_t *seqlens, *cu;
-  int n_rows, T_new, total, H, G;
-  int skip;   // rows of few_pairs() by it are another launch's
-  int deal;   // workgroups per round of dealt_block()
-  int slots;  // blocks for whose partials there is room, or 0: no block is cut
-  float ratio;  // the cost rule's, times the blocks of the call
-  SplitGeo split;  // the partials' buffers and pieces
+  int T_new, H, G;
+  int deal;  // workgroups per round of dealt_block()
+  PagedTiles tiles;
+  int md;  // 32-dim pieces of a head
+  // Four dims 32 d + 8 j + 4 (lane / 32) .. of pair lane % 32 of a group's partials.
+  __device__ __forceinline__ float *part_o(int64_t group, int d, int j, int lane) const {
+    return tiles.part_o + ((group * md + d) * 4 + j) * 256 + lane * 4;
+  }
+  __device__ __forceinline__ float *part_ml(int64_t group, int pair) const {
+    return tiles.part_ml + (group * 32 + pair) * 2;
+  }
 };
 
 // Tile geometry of an instantiation (elements of E; DP is head_dim rounded up).
@@ -109,8 +115,8 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
 
   const int id = P.cu ? int(blockIdx.x) : dealt_block(int(blockIdx.x), int(gridDim.x), P.deal);
   PagedBlock blk;
-  if (!find_paged_block(P.cu, P.seqlens, P.n_rows, P.T_new, P.total, P.G, P.H_kv, G_::PAIRS, P.skip,
-                        P.slots, id / P.H_kv, threadIdx.x & 63, blk))
+  if (!find_paged_block(P.cu, P.seqlens, P.tiles.n_rows, P.T_new, P.tiles.total, P.G, P.H_kv,
+                        G_::PAIRS, P.tiles.skip, P.tiles.slots, id / P.H_kv, threadIdx.x & 63, blk))
     return;
   const int kvh = id % P.H_kv, part = blk.part, row = blk.b, T_b = blk.T, s0 = blk.s0;
   const int64_t tok0 = blk.tok0;
@@ -153,7 +159,7 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
   int n_tiles = (hi - lo) / KT + 1;
   bool whole = true;
   if (blk.most > 1) {  // this workgroup's range of the block's tiles
-    const int ranges = best_splits(P.ratio / float(blk.n_blocks), n_tiles, KT, blk.most);
+    const int ranges = best_splits(P.tiles.ratio / float(blk.n_blocks), n_tiles, KT, blk.most);
     if (part >= ranges) return;
     whole = ranges == 1;
     const int t0 = part * n_tiles / ranges, t1 = (part + 1) * n_tiles / ranges;
@@ -361,9 +367,9 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (32 * md < D)
-            store4(P.split.o(g, md, j, lane), f32x4{o[md][4 * j], o[md][4 * j + 1],
+            store4(P.part_o(g, md, j, lane), f32x4{o[md][4 * j], o[md][4 * j + 1],
                                                     o[md][4 * j + 2], o[md][4 * j + 3]});
-      if (h == 0) *reinterpret_cast<float2 *>(P.split.ml(g, col)) = make_float2(m, l);
+      if (h == 0) *reinterpret_cast<float2 *>(P.part_ml(g, col)) = make_float2(m, l);
       return;
     }
     const float inv = 1.f / l;
@@ -446,8 +452,8 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
       const int x = tid & 7;
 #pragma unroll
       for (int i = 0; i < DT / 4; ++i)
-        if (32 * i < D) store4(P.split.o(g, i, x >> 1, 32 * (x & 1) + c), y[i]);
-      if (x == 0) *reinterpret_cast<float2 *>(P.split.ml(g, c)) = make_float2(M, L);
+        if (32 * i < D) store4(P.part_o(g, i, x >> 1, 32 * (x & 1) + c), y[i]);
+      if (x == 0) *reinterpret_cast<float2 *>(P.part_ml(g, c)) = make_float2(M, L);
       return;
     }
     if (c_live && !ok) s_bad[c] = 1;
@@ -467,63 +473,210 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
   }
 }
 
-template <class E, int DP, int KS>
-int run(TiledParams &P, const PagedArgs &a) {
-  using G_ = Geo<E, DP, KS>;
-  const int64_t blocks = paged_blocks_bound(a, G_::PAIRS) * P.H_kv;
-  if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
-  if (blocks == 0) return MCAMD_OK;
-  hipLaunchKernelGGL((paged_tiled_kernel<E, DP, KS>), dim3(unsigned(blocks)), dim3(kThreads), 0,
-                     a.stream, P);
-  return launch_status("paged_tiled");
-}
-
-template <class E, int DP>
-int run_ks(TiledParams &P, const PagedArgs &a, bool over_keys) {
-  if constexpr (DP <= 128) {
-    if (over_keys) return run<E, DP, 4>(P, a);
-  }
-  return run<E, DP, 1>(P, a);
-}
-
+// Merges the partials of key ranges, in the partials' own layout: a workgroup per 32 pairs of a block, a
+// wave per 32 dims of them, eight ranges' loads in flight.
 template <class E>
-int dispatch(TiledParams &P, const PagedArgs &a) {
-  // Fewer workgroups of 128 pairs than compute units: 32 pairs and a quarter of the keys per wave.
-  const bool over_keys = paged_blocks_bound(a, 128) * a.n_kv_head < device_cus();
-  if (P.D <= 32) return run_ks<E, 32>(P, a, over_keys);
-  if (P.D <= 64) return run_ks<E, 64>(P, a, over_keys);
-  if (P.D <= 96) return run_ks<E, 96>(P, a, over_keys);
-  if (P.D <= 128) return run_ks<E, 128>(P, a, over_keys);
-  if (P.D <= 192) return run_ks<E, 192>(P, a, over_keys);
-  return run_ks<E, 256>(P, a, over_keys);
+__global__ __launch_bounds__(kThreads) void paged_merge_kernel(TiledParams P, int pairs) {
+  const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int id = blockIdx.x;
+  const int groups = P.tiles.groups, kt = P.tiles.kt;
+  const int w = id % groups;
+  id /= groups;
+  PagedBlock blk;  // first ranges come first: range 0 of every block
+  if (!find_paged_block(P.cu, P.seqlens, P.tiles.n_rows, P.T_new, P.tiles.total, P.G, P.H_kv, pairs,
+                        P.tiles.skip, P.tiles.slots, id / P.H_kv, lane, blk) ||
+      blk.part > 0 || blk.most == 1)
+    return;
+  const int kvh = id % P.H_kv;
+  if (blk.s0 < 0 || int64_t(blk.s0) + blk.T > int64_t(P.kv.max_pages) << P.kv.shift) return;  // NaN already
+  const int64_t n_pairs = int64_t(blk.T) * P.G, p0 = int64_t(blk.qt) * pairs;
+  const int n = int(min(int64_t(pairs), n_pairs - p0));
+  const int first = blk.s0 + int(p0 / P.G), hi = blk.s0 + int((p0 + n - 1) / P.G);
+  const int lo = (P.window >= 0 ? max(0, first - P.window) : 0) & ~(P.tiles.align - 1);
+  const int ranges =
+      best_splits(P.tiles.ratio / float(blk.n_blocks), (hi - lo) / kt + 1, kt, blk.most);
+  if (ranges == 1) return;  // written by the block itself
+  const int in_block = 32 * w + col;
+  const bool live = in_block < n;
+  const int t = live ? int((p0 + in_block) / P.G) : 0;
+  auto pair_at = [&](int i) {
+    const int tt = int((p0 + i) / P.G);
+    return ((int64_t(blk.tok0) + tt) * P.H + int64_t(kvh) * P.G + int(p0 + i - int64_t(tt) * P.G)) * P.D;
+  };
+  const int64_t at = live ? pair_at(in_block) : 0;
+
+  constexpr int U = 8;
+  const int64_t group = int64_t(id) * groups + w, step = int64_t(blk.n_blocks) * groups;
+  for (int md = wave; md < P.md; md += kWaves) {
+    f32x4 y[4];
+    bool ok = true;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float M = -INFINITY, L = 0.f;
+      y[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int r0 = 0; r0 < ranges; r0 += U) {
+        float2 x[U];
+        f32x4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int64_t g = group + min(r0 + u, ranges - 1) * step;
+          x[u] = *reinterpret_cast<const float2 *>(P.part_ml(g, col));
+          v[u] = *reinterpret_cast<const f32x4 *>(P.part_o(g, md, j, lane));
+        }
+        float m_new = M;
+#pragma unroll
+        for (int u = 0; u < U; ++u) m_new = fmaxf(m_new, x[u].x);
+        const float keep = M == -INFINITY ? 0.f : fast_exp2(M - m_new);
+        L *= M == -INFINITY ? 1.f : keep;  // 0 then, or a NaN that must stay
+        y[j] *= keep;
+        M = m_new;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (r0 + u >= ranges) break;
+          const float a = x[u].x == -INFINITY ? 0.f : fast_exp2(x[u].x - M);
+          L += x[u].y * (x[u].x == -INFINITY ? 1.f : a);
+          y[j] += a * v[u];
+        }
+      }
+      y[j] *= 1.f / L;
+      const int d = 32 * md + 8 * j + 4 * h;
+      ok = ok && ((finite(y[j][0]) && finite(y[j][1]) && finite(y[j][2]) && finite(y[j][3])) || d >= P.D);
+    }
+    const uint64_t bad64 = __builtin_amdgcn_ballot_w64(live && !ok);
+    const uint32_t bad = uint32_t(bad64) | uint32_t(bad64 >> 32);
+    if (live && !((bad >> col) & 1u)) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int d = 32 * md + 8 * j + 4 * h;
+        if (d < P.D) store4(static_cast<E *>(P.out) + at + d, y[j]);
+      }
+    }
+    for (uint32_t left = bad; __builtin_expect(left != 0, 0); left &= left - 1) {
+      const int c = __builtin_ctz(left);
+      careful_pair<E, 256, 4>(P, blk.b, kvh, pair_at(32 * w + c), blk.s0 + __builtin_amdgcn_readlane(t, c),
+                              lane, 32 * md, min(32 * md + 32, P.D));
+    }
+  }
 }
 
-}  // namespace
+// What a call runs: the waves over pairs (KS = 1) or keys (KS = 4), and room for the partials of cut
+// blocks: as many as the chip holds workgroups, where a call can have so few that two ranges of each run
+// side by side.
+struct TiledPlan {
+  int ks, pairs, kt, slots;
+  int64_t bound;  // of blocks
+  float tile_us;
+};
+TiledPlan tiled_plan(const PagedArgs &a, int64_t skip) {
+  const bool bf = a.dtype == MCAMD_BF16;
+  const int64_t cus = device_cus();
+  TiledPlan t;
+  // Fewer workgroups of 128 pairs than compute units: 32 pairs and a quarter of the keys per wave. Head
+  // dims above 128 keep KS = 1 (a tile of four waves' keys outgrows the LDS).
+  t.ks = a.head_dim <= 128 && paged_blocks_bound(a, 128, skip) * a.n_kv_head < cus ? 4 : 1;
+  t.pairs = 128 / t.ks;
+  t.kt = t.ks == 4 ? 128 : bf && a.head_dim <= 128 ? 64 : 32;
+  t.bound = paged_blocks_bound(a, t.pairs, skip);
+  // Measured time of a tile on a compute unit of its own, per head dim (prefill_tiled.hip).
+  t.tile_us = float(a.head_dim) * (t.ks == 4 ? (bf ? 0.027f : 0.085f) : (bf ? 0.012f : 0.035f));
+  t.slots = t.bound * a.n_kv_head < 2 * cus ? int(cus) : 0;
+  return t;
+}
+int64_t slot_floats(const PagedArgs &a, int pairs) {
+  return int64_t(pairs) * ((a.head_dim + 31) / 32 * 32 + 2);
+}
 
-int launch_paged_tiled(const PagedArgs &a, int64_t skip) {
+TiledParams tiled_params(const PagedArgs &a, const PagedTiles &tiles) {
   TiledParams P;
   P.q = a.q;
   P.k_pages = a.k_pages;
   P.v_pages = a.v_pages;
   P.kv = a.kv;
-  P.seqlens = a.seqlens;
-  P.cu = a.cu;
   P.out = a.out;
-  P.n_rows = int(a.n_rows);
-  P.T_new = int(a.t_new);
-  P.total = int(a.total);
-  P.H = int(a.n_head);
   P.H_kv = int(a.n_kv_head);
-  P.G = int(a.n_head / a.n_kv_head);
   P.window = int(a.window < 0 ? -1 : a.window);
   P.D = int(a.head_dim);
-  P.skip = int(skip);
-  P.deal = device_cus();
-  P.slots = 0;
-  P.ratio = 0.f;
   P.scale_log2 = float(kLog2e / std::sqrt(double(a.head_dim)));
-  P.split = SplitGeo{};
-  return a.dtype == MCAMD_BF16 ? dispatch<bf16>(P, a) : dispatch<float>(P, a);
+  P.seqlens = a.seqlens;
+  P.cu = a.cu;
+  P.T_new = int(a.t_new);
+  P.H = int(a.n_head);
+  P.G = int(a.n_head / a.n_kv_head);
+  P.deal = device_cus();
+  P.tiles = tiles;
+  P.md = int((a.head_dim + 31) / 32);
+  return P;
+}
+
+template <class E, int DP, int KS>
+int run(const TiledParams &P, const PagedArgs &a, const TiledPlan &t) {
+  using G_ = Geo<E, DP, KS>;
+  if (t.pairs != G_::PAIRS || t.kt != G_::KT)
+    return fail(MCAMD_EINVAL, "paged attention: plan and kernel disagree");
+  const int64_t blocks = std::max<int64_t>(t.bound * P.H_kv, P.tiles.slots);
+  if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
+  if (blocks == 0) return MCAMD_OK;
+  hipLaunchKernelGGL((paged_tiled_kernel<E, DP, KS>), dim3(unsigned(blocks)), dim3(kThreads), 0,
+                     a.stream, P);
+  const int st = launch_status("paged_tiled");
+  if (st != MCAMD_OK || P.tiles.slots == 0) return st;
+  return launch_paged_tiles_merge(a, P.tiles, t.pairs);
+}
+
+template <class E, int DP>
+int run_ks(const TiledParams &P, const PagedArgs &a, const TiledPlan &t) {
+  if constexpr (DP <= 128) {
+    if (t.ks == 4) return run<E, DP, 4>(P, a, t);
+  }
+  return run<E, DP, 1>(P, a, t);
+}
+
+template <class E>
+int dispatch(const TiledParams &P, const PagedArgs &a, const TiledPlan &t) {
+  if (P.D <= 32) return run_ks<E, 32>(P, a, t);
+  if (P.D <= 64) return run_ks<E, 64>(P, a, t);
+  if (P.D <= 96) return run_ks<E, 96>(P, a, t);
+  if (P.D <= 128) return run_ks<E, 128>(P, a, t);
+  if (P.D <= 192) return run_ks<E, 192>(P, a, t);
+  return run_ks<E, 256>(P, a, t);
+}
+
+}  // namespace
+
+int launch_paged_tiles_merge(const PagedArgs &a, const PagedTiles &tiles, int pairs) {
+  const TiledParams P = tiled_params(a, tiles);
+  const int64_t blocks = paged_blocks_bound(a, pairs, tiles.skip) * P.H_kv * tiles.groups;
+  if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
+  const dim3 grid{unsigned(blocks)}, threads{kThreads};
+  if (a.dtype == MCAMD_BF16)
+    hipLaunchKernelGGL(paged_merge_kernel<bf16>, grid, threads, 0, a.stream, P, pairs);
+  else
+    hipLaunchKernelGGL(paged_merge_kernel<float>, grid, threads, 0, a.stream, P, pairs);
+  return launch_status("paged_merge");
+}
+
+size_t paged_tiled_bytes(const PagedArgs &a, int64_t skip) {
+  const TiledPlan t = tiled_plan(a, skip);
+  return size_t(t.slots) * size_t(slot_floats(a, t.pairs)) * 4;
+}
+
+int launch_paged_tiled(const PagedArgs &a, int64_t skip) {
+  const TiledPlan t = tiled_plan(a, skip);
+  PagedTiles T;
+  T.kv = a.kv;
+  T.n_rows = int(a.n_rows);
+  T.total = int(a.total);
+  T.skip = int(skip);
+  T.kt = t.kt;
+  T.align = 1;
+  T.groups = t.pairs / 32;
+  T.slots = a.scratch && a.scratch_bytes >= paged_tiled_bytes(a, skip) ? t.slots : 0;
+  T.ratio = t.tile_us * MCAMD_SPLIT_BYTES_PER_US / (float(slot_floats(a, t.pairs)) * 8.f);
+  T.part_o = static_cast<float *>(a.scratch);
+  T.part_ml = T.part_o + int64_t(T.slots) * t.pairs * ((a.head_dim + 31) / 32 * 32);
+  const TiledParams P = tiled_params(a, T);
+  return a.dtype == MCAMD_BF16 ? dispatch<bf16>(P, a, t) : dispatch<float>(P, a, t);
 }
 
 }  // namespace mcamd

@@ -54,6 +54,12 @@
 //
 // The shared prompt prefix of a decode step runs inside the fused decode kernel (prefix_mfma.h),
 // built from the same fragments and layouts.
+//
+// A paged cache's long rows (paged.h) run the same schedule: tiles begin at multiples of 64 keys, so the
+// keys of a wave's K loads share at most two pages and those of its V loads one; the pages' numbers are
+// scalars, loaded a tile before their tile's loads. The ranges of cut blocks are merged by
+// paged_tiled.hip, and pairs that are not finite redone (paged_careful.h).
+#include "paged_careful.h"
 #include "prefill_order.h"
 #include "prefill_split.h"
 
@@ -146,12 +152,16 @@ __device__ __forceinline__ float exp2_or_zero(float x) {
   return x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x);
 }
 
+typedef const __attribute__((address_space(4))) int32_t *scalar_ints;  // read only, by the scalar unit
+
 // SPLIT: a workgroup per key range of a block (prefill_split.h), which takes the chunk's own keys from
 // k_new and v_new where they are given (the merge appends them). VARLEN: sequences of their own
-// lengths, packed along the token axis.
-template <bool SPLIT, bool VARLEN>
+// lengths, packed along the token axis. PAGED: keys and values in pages, rows of any lengths, blocks cut
+// where T has room.
+template <bool SPLIT, bool VARLEN, bool PAGED = false>
 __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const SplitGeo *S,
-                                                  const uint16_t *k_new, const uint16_t *v_new) {
+                                                  const uint16_t *k_new, const uint16_t *v_new,
+                                                  const PagedTiles *T = nullptr) {
   __shared__ __attribute__((aligned(1024))) uint16_t sK[4][TILE];
   __shared__ __attribute__((aligned(1024))) uint16_t sV[4][TILE];
 
@@ -175,7 +185,15 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   // rows[b]; a query tile past the sequence's end has nothing to do (a whole workgroup).
   int row = b, T_b = P.T_new, s0;
   int64_t tok0 = int64_t(b) * P.T_new;
-  if constexpr (VARLEN) {
+  PagedBlock blk;
+  if constexpr (PAGED) {
+    if (!find_paged_block(P.cu, P.seqlens, T->n_rows, P.T_new, T->total, P.G, P.H_kv, P.QT * P.G, T->skip,
+                          T->slots, int(blockIdx.x) / P.H_kv, lane, blk))
+      return;
+    kvh = int(blockIdx.x) % P.H_kv;
+    part = blk.part;
+    b = row = blk.b, qt = blk.qt, tok0 = blk.tok0, T_b = blk.T, s0 = blk.s0;
+  } else if constexpr (VARLEN) {
     const int n_seqs = P.n_bh / P.H_kv;
     if (n_seqs <= kOrderedSeqs) {
       VarlenBlock v;
@@ -232,8 +250,21 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   const int p_last = s0 + q_end - 1;
   int lo = P.window >= 0 ? max(0, p_first - P.window) : 0;
   int hi = p_last;
+  const int seen_from = lo;  // PAGED: tiles begin before it, at a multiple of their keys
+  if constexpr (PAGED) lo &= ~(KT - 1);
   const int lo_block = lo;
   bool whole = true;
+  if constexpr (PAGED) {
+    if (blk.most > 1) {
+      const int tiles = (hi - lo) / KT + 1;
+      const int ranges = best_splits(T->ratio / float(blk.n_blocks), tiles, KT, blk.most);
+      if (part >= ranges) return;
+      whole = ranges == 1;
+      const int t0 = part * tiles / ranges, t1 = (part + 1) * tiles / ranges;
+      hi = min(hi, lo + t1 * KT - 1);
+      lo += t0 * KT;
+    }
+  }
   if constexpr (SPLIT) {  // this workgroup's range of the block's tiles
     const int tiles = (hi - lo) / KT + 1;
     const int ranges = block_splits(*S, s0, T_b, tiles);
@@ -245,8 +276,9 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   }
 
   const int64_t tok = int64_t(P.H_kv) * D;
-  const uint16_t *kbase = P.k_cache + int64_t(row) * P.cache_b + int64_t(kvh) * D;
-  const uint16_t *vbase = P.v_cache + int64_t(row) * P.cache_b + int64_t(kvh) * D;
+  const int64_t row_at = PAGED ? 0 : int64_t(row) * P.cache_b;
+  const uint16_t *kbase = P.k_cache + row_at + int64_t(kvh) * D;
+  const uint16_t *vbase = P.v_cache + row_at + int64_t(kvh) * D;
 
   // A tile takes 32 DMA instructions of 1 KiB (16 K fragments, 16 blocks of 4 V rows); wave w
   // issues K fragments 2w, 2w + 1 and V blocks 2w, 2w + 1. Keys past `hi` re-read key `hi` (they
@@ -271,8 +303,35 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
     const char *base = reinterpret_cast<const char *>(is_new ? fresh + new_at : cached);
     return base + __umul24(uint32_t(is_new ? key - s0 : key), tok_bytes);
   };
+  // PAGED: the pages of the keys this wave loads of the next tile to load: of its K fragments' first and
+  // last 16 keys, and of its V rows.
+  int page_k[2] = {0, 0}, page_v = 0;
+  bool lost = false;  // a page outside the pool
+  auto load_pages = [&](int k0) {
+    if constexpr (PAGED) {
+      const scalar_ints pages = (scalar_ints)(T->kv.table + row * T->kv.table_stride);
+      auto page_of = [&](int k) { return pages[max(seen_from, min(k, hi)) >> T->kv.shift]; };
+      page_k[0] = page_of(k0 + 32 * (wave_s >> 2));
+      page_k[1] = page_of(k0 + 32 * (wave_s >> 2) + 16);
+      page_v = page_of(k0 + 8 * wave_s);
+    }
+  };
   auto issue_part = [&](int k0, int buf, int i) {
     const int f = 2 * wave_s + (i >> 1);
+    if constexpr (PAGED) {
+      const bool is_k = (i & 1) == 0;
+      const int key = min(k0 + (is_k ? 32 * (f >> 3) + col : 4 * f + (lane >> 4)), hi);
+      const int64_t tokens = int64_t(P.H_kv) * D;
+      const uint32_t at = __umul24(uint32_t(T->kv.in_page(key)), tok_bytes) +
+                          (is_k ? uint32_t(32 * (f & 7)) + k_lane_off : (v_chunk ^ uint32_t(f & 3)) << 4);
+      const uint16_t *base = is_k ? kbase + T->kv.offset(col < 16 ? page_k[0] : page_k[1], 0, tokens)
+                                  : vbase + T->kv.offset(page_v, 0, tokens);
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void *)(reinterpret_cast<const char *>(base) + at),
+          (__attribute__((address_space(3))) void *)(is_k ? &sK[buf][f * 512] : &sV[buf][f * 512]),
+          16, 0, 0);
+      return;
+    }
     if constexpr (SPLIT) {
       const bool is_k = (i & 1) == 0;
       const int key = min(k0 + (is_k ? 32 * (f >> 3) + col : 4 * f + (lane >> 4)), hi);
@@ -301,6 +360,13 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   auto issue_tile = [&](int k0, int buf) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) issue_part(k0, buf, i);
+  };
+  // PAGED: after a tile's loads have been issued, the pages of the tile after it.
+  auto next_pages = [&](int k0) {
+    if constexpr (PAGED) {
+      lost = lost || !T->kv.is_page(page_k[0]) || !T->kv.is_page(page_k[1]) || !T->kv.is_page(page_v);
+      load_pages(k0);
+    }
   };
 
   f32x16 o[4];
@@ -419,13 +485,19 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   const int lag = wave >= 4 ? 1 : 0;
   f32x16 sc[2];
   bf16x8 pk[4];
-  const bool later = SPLIT && part > 0;
+  const bool later = (SPLIT || PAGED) && part > 0;
   if (later) {  // the block's first keys, into the buffer that is taken last
+    load_pages(lo_block);
     issue_part(lo_block, 3, 0);
     issue_part(lo_block, 3, 2);
   }
+  load_pages(lo);
   issue_tile(lo, 0);
-  if (n_tiles > 1) issue_tile(lo + KT, 1);
+  next_pages(lo + KT);
+  if (n_tiles > 1) {
+    issue_tile(lo + KT, 1);
+    next_pages(lo + 2 * KT);
+  }
   if (later) {
     // A later range starts from the maximum over the block's first tile, as the whole block's walk
     // does: its weights are then rounded to bf16 as they are there, and the ranges differ from the walk
@@ -460,7 +532,10 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
     // last read in slot - 1; the four parts are spread over the slot's work.
     const int dma_tile = ((slot & 1) == 0 && slot / 2 + 2 < n_tiles) ? slot / 2 + 2 : -1;
     auto dma_part = [&](int i) {
-      if (dma_tile >= 0) issue_part(lo + dma_tile * KT, dma_tile % 4, i);
+      if (dma_tile >= 0) {
+        issue_part(lo + dma_tile * KT, dma_tile % 4, i);
+        if (i == 3) next_pages(lo + (dma_tile + 1) * KT);
+      }
     };
     const int ph = slot - lag;  // this wave's phase index
     if (ph < 0 || ph > 2 * n_tiles) {
@@ -506,7 +581,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
     } else {
       const int t = ph / 2 - 1;  // M(t)
       // SPLIT: all parts before the fragments are live (their 64-bit addresses take registers).
-      if constexpr (SPLIT)
+      if constexpr (SPLIT || PAGED)
         for (int i = 0; i < 4; ++i) dma_part(i);
       // The matrix phase at raised wave priority: when the matrix core frees, the SIMD issues
       // this wave's next product before its partner's VALU work (measured: +1.4-2.3% on the 16K
@@ -556,7 +631,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
           pair(ks_c, std::integral_constant<int, 1>{});
           pair(ks_c, std::integral_constant<int, 2>{});
           pair(ks_c, std::integral_constant<int, 3>{});
-          if constexpr (!SPLIT) dma_part(ks);
+          if constexpr (!SPLIT && !PAGED) dma_part(ks);
         };
         auto issue = [&](auto ks_c, int buf) {
           issue_i(ks_c, std::integral_constant<int, 0>{}, buf);
@@ -573,7 +648,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
           pv_step(pk[ks], ks, sV[t % 4]);
-          if constexpr (!SPLIT) dma_part(ks);
+          if constexpr (!SPLIT && !PAGED) dma_part(ks);
         }
       }
       __builtin_amdgcn_s_setprio(0);
@@ -581,8 +656,40 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   }
 
   // Normalise and write: o[md][4j + i] is dim 32 md + 8 j + 4 h + i of pair `col`.
-  const float lt = sum_halves(l);
+  float lt = sum_halves(l);
+  if constexpr (PAGED)
+    if (__syncthreads_or(lost)) lt = NAN;
   const float inv = 1.f / lt;
+  if constexpr (PAGED) {
+    if (!whole) {
+      if (!live) return;
+      const int64_t g = int64_t(blockIdx.x) * kWaves + wave;
+#pragma unroll
+      for (int md = 0; md < 4; ++md)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<float4 *>(T->part_o + ((g * 4 + md) * 4 + j) * 256 + lane * 4) =
+              make_float4(o[md][4 * j], o[md][4 * j + 1], o[md][4 * j + 2], o[md][4 * j + 3]);
+      if (h == 0) *reinterpret_cast<float2 *>(T->part_ml + (g * 32 + col) * 2) = make_float2(m, lt);
+      return;
+    }
+    bool ok = true;
+#pragma unroll
+    for (int md = 0; md < 4; ++md)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) ok = ok && finite(o[md][e] * inv);
+    const uint64_t bad64 = __builtin_amdgcn_ballot_w64(live && !ok);
+    if (__builtin_expect(bad64 != 0, 0)) {
+      const CarefulParams C{P.q, P.k_cache, P.v_cache, T->kv, P.out, P.H_kv, P.window, D, P.scale_log2};
+      for (uint32_t left = uint32_t(bad64) | uint32_t(bad64 >> 32); left != 0; left &= left - 1) {
+        const int pr2 = wave * 32 + __builtin_ctz(left), t = q0 + pr2 / P.G;
+        careful_pair<bf16, D, 8>(C, row, kvh,
+                                 ((tok0 + t) * P.H + int64_t(kvh) * P.G + (pr2 - pr2 / P.G * P.G)) * D,
+                                 s0 + t, lane, 0, D);
+      }
+      if ((uint32_t(bad64 >> col) | uint32_t(bad64 >> (32 + col))) & 1u) return;
+    }
+  }
   if (!live) return;
   if constexpr (SPLIT) {
     if (!whole) {
@@ -618,6 +725,9 @@ __global__ __launch_bounds__(kThreads, 1) void prefill_mfma_kernel(MfmaParams P)
 }
 __global__ __launch_bounds__(kThreads, 1) void prefill_mfma_varlen_kernel(MfmaParams P) {
   prefill_mfma_body<false, true>(P, nullptr, nullptr, nullptr);
+}
+__global__ __launch_bounds__(kThreads, 1) void paged_mfma_kernel(MfmaParams P, PagedTiles T) {
+  prefill_mfma_body<false, false, true>(P, nullptr, nullptr, nullptr, &T);
 }
 __global__ __launch_bounds__(kThreads, 1) void prefill_mfma_split_kernel(
     MfmaParams P, SplitGeo S, const uint16_t *k_new, const uint16_t *v_new) {
@@ -695,6 +805,70 @@ int launch_prefill_mfma(const AttnArgs &a) {
   const int st = launch_status("prefill_mfma");
   if (st != MCAMD_OK) return st;
   return launch_prefill_combine(a, geo, false);
+}
+
+// A long row's blocks over a paged cache.
+bool paged_mfma_supported(const PagedArgs &a) {
+  // In-page offsets are products of 24 bits.
+  return a.dtype == MCAMD_BF16 && a.head_dim == D && a.n_kv_head * D * 2 < (1 << 24) && a.kv.shift <= 24;
+}
+
+namespace {
+
+// Room for the partials of a workgroup per compute unit, where a call can have so few blocks that two
+// ranges of each run side by side.
+int64_t paged_slots(const PagedArgs &a, int64_t blocks) {
+  const int64_t cus = device_cus();
+  return blocks * a.n_kv_head < 2 * cus ? cus : 0;
+}
+constexpr int64_t kSlotFloats = int64_t(kPairs) * (D + 2);
+
+}  // namespace
+
+size_t paged_mfma_bytes(const PagedArgs &a, int64_t skip) {
+  const int64_t G = a.n_head / a.n_kv_head;
+  return size_t(paged_slots(a, paged_blocks_bound(a, kPairs / G * G, skip)) * kSlotFloats * 4);
+}
+
+int launch_paged_mfma(const PagedArgs &a, int64_t skip) {
+  MfmaParams P{};
+  P.q = static_cast<const uint16_t *>(a.q);
+  P.k_cache = static_cast<const uint16_t *>(a.k_pages);
+  P.v_cache = static_cast<const uint16_t *>(a.v_pages);
+  P.seqlens = a.seqlens;
+  P.cu = a.cu;
+  P.out = static_cast<uint16_t *>(a.out);
+  P.T_new = int(a.t_new);
+  P.H = int(a.n_head);
+  P.H_kv = int(a.n_kv_head);
+  P.G = int(a.n_head / a.n_kv_head);
+  P.QT = kPairs / P.G;
+  P.T_max = a.kv.max_pages << a.kv.shift;
+  P.window = int(a.window < 0 ? -1 : a.window);
+  P.n_bh = P.H_kv;
+  P.n_qt = 1;
+  P.scale_log2 = float(kLog2e / std::sqrt(double(D)));
+  PagedTiles T{};
+  T.kv = a.kv;
+  T.n_rows = int(a.n_rows);
+  T.total = int(a.total);
+  T.skip = int(skip);
+  T.kt = T.align = KT;
+  T.groups = kWaves;
+  const int64_t bound = paged_blocks_bound(a, P.QT * P.G, skip);
+  T.slots = int(paged_slots(a, bound));
+  if (!a.scratch || a.scratch_bytes < size_t(T.slots * kSlotFloats * 4)) T.slots = 0;
+  // A tile of 64 keys takes 256 pairs 1.4 us; a range's partials are written and read.
+  T.ratio = 1.4f * MCAMD_SPLIT_BYTES_PER_US / (float(kSlotFloats) * 8.f);
+  T.part_o = static_cast<float *>(a.scratch);
+  T.part_ml = T.part_o + int64_t(T.slots) * kPairs * D;
+  const int64_t blocks = std::max<int64_t>(bound * P.H_kv, T.slots);
+  if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
+  if (blocks == 0) return MCAMD_OK;
+  hipLaunchKernelGGL(paged_mfma_kernel, dim3(unsigned(blocks)), dim3(kThreads), 0, a.stream, P, T);
+  const int st = launch_status("paged_mfma");
+  if (st != MCAMD_OK || T.slots == 0) return st;
+  return launch_paged_tiles_merge(a, T, P.QT * P.G);
 }
 
 }  // namespace mcamd
