@@ -473,16 +473,20 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
   }
 }
 
-// Merges the partials of key ranges, in the partials' own layout: a workgroup per 32 pairs of a block, a
-// wave per 32 dims of them, eight ranges' loads in flight.
+// Merges the partials of key ranges, in the partials' own layout: a workgroup per 32 pairs and 32 dims of
+// a block, a wave per step j of them, eight ranges' loads in flight.
 template <class E>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(TiledParams P, int pairs) {
   const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int id = blockIdx.x;
+  const int j = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int groups = P.tiles.groups, kt = P.tiles.kt;
+  int id = blockIdx.x;
+  const int md = id % P.md;
+  id /= P.md;
   const int w = id % groups;
   id /= groups;
+  const int d = 32 * md + 8 * j;  // this wave's dims d .. d + 7, lane half h d + 4h ..
+  if (d >= P.D) return;
   PagedBlock blk;  // first ranges come first: range 0 of every block
   if (!find_paged_block(P.cu, P.seqlens, P.tiles.n_rows, P.T_new, P.tiles.total, P.G, P.H_kv, pairs,
                         P.tiles.skip, P.tiles.slots, id / P.H_kv, lane, blk) ||
@@ -504,59 +508,45 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(TiledParams P, in
     const int tt = int((p0 + i) / P.G);
     return ((int64_t(blk.tok0) + tt) * P.H + int64_t(kvh) * P.G + int(p0 + i - int64_t(tt) * P.G)) * P.D;
   };
-  const int64_t at = live ? pair_at(in_block) : 0;
 
   constexpr int U = 8;
   const int64_t group = int64_t(id) * groups + w, step = int64_t(blk.n_blocks) * groups;
-  for (int md = wave; md < P.md; md += kWaves) {
-    f32x4 y[4];
-    bool ok = true;
+  float M = -INFINITY, L = 0.f;
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+  for (int r0 = 0; r0 < ranges; r0 += U) {
+    float2 x[U];
+    f32x4 v[U];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float M = -INFINITY, L = 0.f;
-      y[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      for (int r0 = 0; r0 < ranges; r0 += U) {
-        float2 x[U];
-        f32x4 v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int64_t g = group + min(r0 + u, ranges - 1) * step;
-          x[u] = *reinterpret_cast<const float2 *>(P.part_ml(g, col));
-          v[u] = *reinterpret_cast<const f32x4 *>(P.part_o(g, md, j, lane));
-        }
-        float m_new = M;
-#pragma unroll
-        for (int u = 0; u < U; ++u) m_new = fmaxf(m_new, x[u].x);
-        const float keep = M == -INFINITY ? 0.f : fast_exp2(M - m_new);
-        L *= M == -INFINITY ? 1.f : keep;  // 0 then, or a NaN that must stay
-        y[j] *= keep;
-        M = m_new;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (r0 + u >= ranges) break;
-          const float a = x[u].x == -INFINITY ? 0.f : fast_exp2(x[u].x - M);
-          L += x[u].y * (x[u].x == -INFINITY ? 1.f : a);
-          y[j] += a * v[u];
-        }
-      }
-      y[j] *= 1.f / L;
-      const int d = 32 * md + 8 * j + 4 * h;
-      ok = ok && ((finite(y[j][0]) && finite(y[j][1]) && finite(y[j][2]) && finite(y[j][3])) || d >= P.D);
+    for (int u = 0; u < U; ++u) {
+      const int64_t g = group + min(r0 + u, ranges - 1) * step;
+      x[u] = *reinterpret_cast<const float2 *>(P.part_ml(g, col));
+      v[u] = *reinterpret_cast<const f32x4 *>(P.part_o(g, md, j, lane));
     }
-    const uint64_t bad64 = __builtin_amdgcn_ballot_w64(live && !ok);
-    const uint32_t bad = uint32_t(bad64) | uint32_t(bad64 >> 32);
-    if (live && !((bad >> col) & 1u)) {
+    float m_new = M;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int d = 32 * md + 8 * j + 4 * h;
-        if (d < P.D) store4(static_cast<E *>(P.out) + at + d, y[j]);
-      }
+    for (int u = 0; u < U; ++u) m_new = fmaxf(m_new, x[u].x);
+    const float keep = M == -INFINITY ? 0.f : fast_exp2(M - m_new);
+    L *= M == -INFINITY ? 1.f : keep;  // 0 then, or a NaN that must stay
+    y *= keep;
+    M = m_new;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (r0 + u >= ranges) break;
+      const float a = x[u].x == -INFINITY ? 0.f : fast_exp2(x[u].x - M);
+      L += x[u].y * (x[u].x == -INFINITY ? 1.f : a);
+      y += a * v[u];
     }
-    for (uint32_t left = bad; __builtin_expect(left != 0, 0); left &= left - 1) {
-      const int c = __builtin_ctz(left);
-      careful_pair<E, 256, 4>(P, blk.b, kvh, pair_at(32 * w + c), blk.s0 + __builtin_amdgcn_readlane(t, c),
-                              lane, 32 * md, min(32 * md + 32, P.D));
-    }
+  }
+  y *= 1.f / L;
+  const bool ok = (finite(y[0]) && finite(y[1]) && finite(y[2]) && finite(y[3])) || d + 4 * h >= P.D;
+  const uint64_t bad64 = __builtin_amdgcn_ballot_w64(live && !ok);
+  const uint32_t bad = uint32_t(bad64) | uint32_t(bad64 >> 32);
+  if (live && !((bad >> col) & 1u) && d + 4 * h < P.D)
+    store4(static_cast<E *>(P.out) + pair_at(in_block) + d + 4 * h, y);
+  for (uint32_t left = bad; __builtin_expect(left != 0, 0); left &= left - 1) {
+    const int c = __builtin_ctz(left);
+    careful_pair<E, 256, 4>(P, blk.b, kvh, pair_at(32 * w + c), blk.s0 + __builtin_amdgcn_readlane(t, c),
+                            lane, d, min(d + 8, P.D));
   }
 }
 
@@ -646,7 +636,7 @@ int dispatch(const TiledParams &P, const PagedArgs &a, const TiledPlan &t) {
 
 int launch_paged_tiles_merge(const PagedArgs &a, const PagedTiles &tiles, int pairs) {
   const TiledParams P = tiled_params(a, tiles);
-  const int64_t blocks = paged_blocks_bound(a, pairs, tiles.skip) * P.H_kv * tiles.groups;
+  const int64_t blocks = paged_blocks_bound(a, pairs, tiles.skip) * P.H_kv * tiles.groups * P.md;
   if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
   const dim3 grid{unsigned(blocks)}, threads{kThreads};
   if (a.dtype == MCAMD_BF16)

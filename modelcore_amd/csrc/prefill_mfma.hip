@@ -55,9 +55,12 @@
 // The shared prompt prefix of a decode step runs inside the fused decode kernel (prefix_mfma.h),
 // built from the same fragments and layouts.
 //
-// A paged cache's long rows (paged.h) run the same schedule: tiles begin at multiples of 64 keys, so the
-// keys of a wave's K loads share at most two pages and those of its V loads one; the pages' numbers are
-// scalars, loaded a tile before their tile's loads. The ranges of cut blocks are merged by
+// A paged cache's long rows (paged.h) run the same schedule: tiles begin at multiples of 64 keys, and a
+// wave's K loads take 16 keys by 32 dims each (K blocks of 1 KiB are [4 chunks][16 keys] there, whose
+// fragments are read in runs of 256 bytes), its V loads 8 keys, so that a load's keys share a page: its
+// number is a scalar, loaded a tile ahead, and the page a buffer resource, whose offsets are as cheap as
+// those of a contiguous cache. (With K fragments of 32 keys, two pages and 64-bit addresses per lane, a
+// chunk of 8 x 512 tokens after 8192 keys took 660 us.) The ranges of cut blocks are merged by
 // paged_tiled.hip, and pairs that are not finite redone (paged_careful.h).
 #include "paged_careful.h"
 #include "prefill_order.h"
@@ -222,7 +225,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   const bool row_ok = s0 >= 0 && int64_t(s0) + T_b <= P.T_max;
 
   const int pr = wave * 32 + col;
-  const bool live = pr < P.QT * P.G && q0 + pr / P.G < q_end;
+  bool live = pr < P.QT * P.G && q0 + pr / P.G < q_end;
   const int pos = live ? q0 + pr / P.G : q0;  // dead pairs compute on a live position
   const int head = live ? pr - (pr / P.G) * P.G : 0;
   uint16_t *out = P.out + ((tok0 + pos) * P.H + int64_t(kvh) * P.G + head) * D;
@@ -303,35 +306,58 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
     const char *base = reinterpret_cast<const char *>(is_new ? fresh + new_at : cached);
     return base + __umul24(uint32_t(is_new ? key - s0 : key), tok_bytes);
   };
-  // PAGED: the pages of the keys this wave loads of the next tile to load: of its K fragments' first and
-  // last 16 keys, and of its V rows.
-  int page_k[2] = {0, 0}, page_v = 0;
+  // PAGED: the page of the 16 keys of which this wave loads K, and of half of which V, in the next tile to
+  // load; and where a tile's loads begin and end, made from it once a tile.
+  int page_id = 0;
   bool lost = false;  // a page outside the pool
-  auto load_pages = [&](int k0) {
+  const int first16 = 16 * (wave_s >> 1);
+  auto load_page = [&](int k0) {
     if constexpr (PAGED) {
       const scalar_ints pages = (scalar_ints)(T->kv.table + row * T->kv.table_stride);
-      auto page_of = [&](int k) { return pages[max(seen_from, min(k, hi)) >> T->kv.shift]; };
-      page_k[0] = page_of(k0 + 32 * (wave_s >> 2));
-      page_k[1] = page_of(k0 + 32 * (wave_s >> 2) + 16);
-      page_v = page_of(k0 + 8 * wave_s);
+      page_id = pages[uint32_t(max(seen_from, min(k0 + first16, hi))) >> T->kv.shift];
+    }
+  };
+  struct PageAt {
+    const char *k, *v;
+    int from, end;  // the first key's place in the page; past `end` (past key hi) loads give zeros
+  };
+  auto page_at = [&](int k0) {
+    PageAt p{};
+    if constexpr (PAGED) {
+      const bool ok = T->kv.is_page(page_id);
+      lost = lost || !ok;
+      const uint64_t off = uint64_t(ok ? uint32_t(page_id) : 0u) * uint32_t(T->kv.page_stride * 2);
+      p.k = reinterpret_cast<const char *>(kbase) + off;
+      p.v = reinterpret_cast<const char *>(vbase) + off;
+      const int page = 1 << T->kv.shift, first = k0 + first16;
+      p.from = (first & (page - 1)) * int(tok_bytes);
+      p.end = min(page, max(0, hi + 1 - (first & -page))) * int(tok_bytes) - kvh * D * 2;
+    }
+    return p;
+  };
+  // This lane's part of the loads' offsets: K key lane % 16 and chunk lane / 16, V key lane / 16 (of the
+  // wave's half of the 16) and its chunk.
+  uint32_t k_in = 0, v_in = 0;
+  if constexpr (PAGED) {
+    k_in = __umul24(uint32_t(lane & 15), tok_bytes) + 16u * uint32_t(lane >> 4);
+    v_in = __umul24(uint32_t(8 * (wave_s & 1) + (lane >> 4)), tok_bytes) +
+           ((v_chunk ^ uint32_t(2 * (wave_s & 1))) << 4);
+  }
+  auto issue_paged = [&](const PageAt &p, int buf, int i) {
+    if constexpr (PAGED) {
+      const int f = 2 * wave_s + (i >> 1);
+      const bool is_k = (i & 1) == 0;
+      const __amdgpu_buffer_rsrc_t rsrc =
+          __builtin_amdgcn_make_buffer_rsrc((void *)(is_k ? p.k : p.v), 0, p.end, 0x00020000);
+      // V's second four keys: the lowest bit of their chunks is the other one (a token is whole 32 bytes).
+      const uint32_t at = is_k ? k_in : i < 2 ? v_in : v_in ^ 16u;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rsrc, (__attribute__((address_space(3))) void *)(is_k ? &sK[buf][f * 512] : &sV[buf][f * 512]),
+          16, int(at), p.from + (is_k ? 64 * (f & 3) : i < 2 ? 0 : 4 * int(tok_bytes)), 0, 0);
     }
   };
   auto issue_part = [&](int k0, int buf, int i) {
     const int f = 2 * wave_s + (i >> 1);
-    if constexpr (PAGED) {
-      const bool is_k = (i & 1) == 0;
-      const int key = min(k0 + (is_k ? 32 * (f >> 3) + col : 4 * f + (lane >> 4)), hi);
-      const int64_t tokens = int64_t(P.H_kv) * D;
-      const uint32_t at = __umul24(uint32_t(T->kv.in_page(key)), tok_bytes) +
-                          (is_k ? uint32_t(32 * (f & 7)) + k_lane_off : (v_chunk ^ uint32_t(f & 3)) << 4);
-      const uint16_t *base = is_k ? kbase + T->kv.offset(col < 16 ? page_k[0] : page_k[1], 0, tokens)
-                                  : vbase + T->kv.offset(page_v, 0, tokens);
-      __builtin_amdgcn_global_load_lds(
-          (const __attribute__((address_space(1))) void *)(reinterpret_cast<const char *>(base) + at),
-          (__attribute__((address_space(3))) void *)(is_k ? &sK[buf][f * 512] : &sV[buf][f * 512]),
-          16, 0, 0);
-      return;
-    }
     if constexpr (SPLIT) {
       const bool is_k = (i & 1) == 0;
       const int key = min(k0 + (is_k ? 32 * (f >> 3) + col : 4 * f + (lane >> 4)), hi);
@@ -361,12 +387,11 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
 #pragma unroll
     for (int i = 0; i < 4; ++i) issue_part(k0, buf, i);
   };
-  // PAGED: after a tile's loads have been issued, the pages of the tile after it.
-  auto next_pages = [&](int k0) {
-    if constexpr (PAGED) {
-      lost = lost || !T->kv.is_page(page_k[0]) || !T->kv.is_page(page_k[1]) || !T->kv.is_page(page_v);
-      load_pages(k0);
-    }
+  auto issue_pages = [&](int k0, int buf, bool only_k) {
+    const PageAt p = page_at(k0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (!only_k || (i & 1) == 0) issue_paged(p, buf, i);
   };
 
   f32x16 o[4];
@@ -398,6 +423,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
     vofs[4 + md] = 2 * (r1 * D + (((cc >> 3) ^ swz(r1)) << 3) + (cc & 7));
   }
 
+  const int k_lane = (col >> 4) * 2048 + h * 128 + (col & 15) * 8;  // PAGED: of this lane's fragments
   // Scores of one tile in log2 units less the running maximum: s[mk][4j + i] is key
   // k0 + 32 mk + 8 j + 4 h + i of pair `col`.
   auto scores = [&](f32x16 (&s)[2], const uint16_t *tK) {
@@ -405,8 +431,9 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
     for (int kd = 0; kd < 8; ++kd)
 #pragma unroll
       for (int mk = 0; mk < 2; ++mk) {
-        const bf16x8 a = __builtin_bit_cast(
-            bf16x8, *reinterpret_cast<const uint4 *>(&tK[(mk * 8 + kd) * 512 + lane * 8]));
+        const int at = PAGED ? mk * 4096 + (kd >> 1) * 512 + (kd & 1) * 256 + k_lane
+                             : (mk * 8 + kd) * 512 + lane * 8;
+        const bf16x8 a = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4 *>(&tK[at]));
         s[mk] = mfma(a, qf[kd], kd == 0 ? negm : s[mk]);
       }
   };
@@ -487,16 +514,23 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   bf16x8 pk[4];
   const bool later = (SPLIT || PAGED) && part > 0;
   if (later) {  // the block's first keys, into the buffer that is taken last
-    load_pages(lo_block);
-    issue_part(lo_block, 3, 0);
-    issue_part(lo_block, 3, 2);
+    if constexpr (PAGED) {
+      load_page(lo_block);
+      issue_pages(lo_block, 3, true);
+    } else {
+      issue_part(lo_block, 3, 0);
+      issue_part(lo_block, 3, 2);
+    }
   }
-  load_pages(lo);
-  issue_tile(lo, 0);
-  next_pages(lo + KT);
-  if (n_tiles > 1) {
-    issue_tile(lo + KT, 1);
-    next_pages(lo + 2 * KT);
+  if constexpr (PAGED) {
+    load_page(lo);
+    issue_pages(lo, 0, false);
+    load_page(lo + KT);
+    if (n_tiles > 1) issue_pages(lo + KT, 1, false);
+    load_page(lo + 2 * KT);
+  } else {
+    issue_tile(lo, 0);
+    if (n_tiles > 1) issue_tile(lo + KT, 1);
   }
   if (later) {
     // A later range starts from the maximum over the block's first tile, as the whole block's walk
@@ -532,18 +566,32 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
     // last read in slot - 1; the four parts are spread over the slot's work.
     const int dma_tile = ((slot & 1) == 0 && slot / 2 + 2 < n_tiles) ? slot / 2 + 2 : -1;
     auto dma_part = [&](int i) {
-      if (dma_tile >= 0) {
-        issue_part(lo + dma_tile * KT, dma_tile % 4, i);
-        if (i == 3) next_pages(lo + (dma_tile + 1) * KT);
-      }
+      if (dma_tile >= 0) issue_part(lo + dma_tile * KT, dma_tile % 4, i);
     };
+    // PAGED: the four parts in one piece, in which a page's place stays scalar.
+    auto dma_paged = [&]() {
+      if (dma_tile >= 0) issue_pages(lo + dma_tile * KT, dma_tile % 4, false);
+    };
+    if constexpr (PAGED) {
+      // With a vector phase, whichever of the two slots that is, and outside its branch, where the page
+      // would not be a scalar: a load under way would hold up the matrix phase's counted waits for LDS
+      // reads. Waves 0-3 load the next even slot's tile, waves 4-7 this one's.
+      const int ahead = wave_s < 4 ? 1 : 0;
+      if ((slot & 1) == ahead) load_page(lo + min(slot / 2 + 2 + ahead, n_tiles) * KT);
+    }
     const int ph = slot - lag;  // this wave's phase index
     if (ph < 0 || ph > 2 * n_tiles) {
-      for (int i = 0; i < 4; ++i) dma_part(i);
+      if constexpr (PAGED)
+        dma_paged();
+      else
+        for (int i = 0; i < 4; ++i) dma_part(i);
       continue;
     }
     if (ph == 0) {
-      for (int i = 0; i < 4; ++i) dma_part(i);
+      if constexpr (PAGED)
+        dma_paged();
+      else
+        for (int i = 0; i < 4; ++i) dma_part(i);
       scores(sc, sK[0]);
     } else if (ph & 1) {
       const int t = (ph - 1) / 2;  // V(t)
@@ -558,8 +606,12 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
       for (int ks = 0; ks < 4; ++ks) pk[ks] = weights(sc, ks, ts[ks]);
       float tl = (ts[0] + ts[1]) + (ts[2] + ts[3]);
       // The DMA parts after the weights (measured: ~1% faster than interleaved with them).
+      if constexpr (PAGED) {
+        dma_paged();
+      } else {
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) dma_part(ks);
+        for (int ks = 0; ks < 4; ++ks) dma_part(ks);
+      }
       if (__builtin_amdgcn_ballot_w64(!(tl <= kTileSumLimit) || m == -INFINITY) != 0) {
         const float mx = tile_max(sc) + m_try;
         const float m_new = fmaxf(m, mx);
@@ -581,8 +633,9 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
     } else {
       const int t = ph / 2 - 1;  // M(t)
       // SPLIT: all parts before the fragments are live (their 64-bit addresses take registers).
-      if constexpr (SPLIT || PAGED)
+      if constexpr (SPLIT)
         for (int i = 0; i < 4; ++i) dma_part(i);
+      if constexpr (PAGED) dma_paged();
       // The matrix phase at raised wave priority: when the matrix core frees, the SIMD issues
       // this wave's next product before its partner's VALU work (measured: +1.4-2.3% on the 16K
       // chunked prefill; the opposite preference costs 7%).
@@ -591,7 +644,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
         // The two products interleaved; the twelve LDS reads of step ks + 1 (four K fragments,
         // four V^T fragments of two transpose reads) are issued before the eight products of
         // step ks, so the reads stream while the matrix core works.
-        const uint32_t ka = lds_addr(&sK[(t + 1) % 4][lane * 8]);
+        const uint32_t ka = lds_addr(&sK[(t + 1) % 4][PAGED ? k_lane : lane * 8]);
         const uint32_t vb = lds_addr(sV[t % 4]);
         uint32_t va[8];
 #pragma unroll
@@ -604,7 +657,9 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
         // over the step instead of in one burst of twelve.
         auto issue_i = [&](auto ks_c, auto i_c, int buf) {
           constexpr int ks = decltype(ks_c)::value, i = decltype(i_c)::value;
-          ds_read_b128<((i & 1) * 8 + 2 * ks + (i >> 1)) * 1024>(kf[buf][i], ka);
+          constexpr int kOff = PAGED ? (i & 1) * 8192 + ks * 1024 + (i >> 1) * 512
+                                     : ((i & 1) * 8 + 2 * ks + (i >> 1)) * 1024;
+          ds_read_b128<kOff>(kf[buf][i], ka);
           ds_read_tr<4096 * ks>(vf[buf][i][0], va[i]);
           ds_read_tr<4096 * ks>(vf[buf][i][1], va[4 + i]);
         };
@@ -657,6 +712,13 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
 
   // Normalise and write: o[md][4j + i] is dim 32 md + 8 j + 4 h + i of pair `col`.
   float lt = sum_halves(l);
+  if constexpr (PAGED) {  // made again: no registers are kept for it through the loop
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    const int pr2 = wave_s * 32 + (ln & 31), at_q = pr2 / P.G;
+    live = pr2 < P.QT * P.G && q0 + at_q < q_end;
+    out = P.out + ((tok0 + q0 + at_q) * P.H + int64_t(kvh) * P.G + (pr2 - at_q * P.G)) * D;
+  }
   if constexpr (PAGED)
     if (__syncthreads_or(lost)) lt = NAN;
   const float inv = 1.f / lt;
