@@ -331,7 +331,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
       p.v = reinterpret_cast<const char *>(vbase) + off;
       const int page = 1 << T->kv.shift, first = k0 + first16;
       p.from = (first & (page - 1)) * int(tok_bytes);
-      p.end = min(page, max(0, hi + 1 - (first & -page))) * int(tok_bytes) - kvh * D * 2;
+      p.end = max(0, min(page, hi + 1 - (first & -page)) * int(tok_bytes) - kvh * D * 2);
     }
     return p;
   };
@@ -871,8 +871,9 @@ int launch_prefill_mfma(const AttnArgs &a) {
 
 // A long row's blocks over a paged cache.
 bool paged_mfma_supported(const PagedArgs &a) {
-  // In-page offsets are products of 24 bits.
-  return a.dtype == MCAMD_BF16 && a.head_dim == D && a.n_kv_head * D * 2 < (1 << 24) && a.kv.shift <= 24;
+  // In-page offsets are products of 24 bits, and 31 bits hold a page's bytes and the way to the next one.
+  return a.dtype == MCAMD_BF16 && a.head_dim == D && a.n_kv_head * D * 2 < (1 << 24) &&
+         a.kv.shift <= 24 && a.kv.page_stride < (int64_t(1) << 30);
 }
 
 namespace {
