@@ -150,8 +150,10 @@ def dtype_code(dtype) -> int:
 
 
 def stream_handle(device) -> int:
-    """hipStream_t of torch's current stream on `device`, as an integer for ctypes."""
-    return torch.cuda.current_stream(device).cuda_stream
+    """hipStream_t of torch's current stream on `device`, as an integer for ctypes: the handle alone, without
+    a Stream object around it (0.2 us against 1.8)."""
+    return torch._C._cuda_getCurrentRawStream(
+        torch.cuda.current_device() if device.index is None else device.index)
 
 
 _WORKSPACES: dict[int, torch.Tensor] = {}
@@ -201,7 +203,7 @@ def on_device(device):
 def require_rocm(*tensors, what: str):
     """Every tensor must live on a ROCm device: the HIP kernels are the only implementation."""
     for t in tensors:
-        if t is not None and t.device.type != "cuda":
+        if t is not None and not t.is_cuda:
             raise RuntimeError(
                 f"{what}: modelcore_amd runs its KV path only as HIP kernels on a ROCm device; "
                 f"got a tensor on {t.device}")

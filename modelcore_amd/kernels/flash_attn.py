@@ -29,6 +29,7 @@ from types import SimpleNamespace
 import torch
 
 from modelcore_amd import _ext
+from modelcore_amd.kernels.qk_epilogue import check_pages
 
 # -----------------------------------------------------------------------------------------------
 # Backend switch, kept for signature parity with modelcore/kernels/flash_attn.py:64-93.
@@ -410,7 +411,6 @@ def flash_attn_paged_with_kvcache(q, k_pages, v_pages, k=None, v=None, *, block_
             if t.dtype != dt:
                 raise TypeError(f"{name} is {t.dtype}, q is {dt}")
         H_kv = k.shape[-2]
-    from modelcore_amd.kernels.qk_epilogue import check_pages
     n_pages, page, stride = check_pages(k_pages, v_pages, H_kv, D, dt, dev)
     H_kv = k_pages.shape[2]
     if H_kv == 0 or H % H_kv:

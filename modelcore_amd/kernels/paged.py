@@ -93,7 +93,7 @@ def paged_reserve(block_table, cache_seqlens, new_lens, free_pages, free_count, 
     if total < 0:
         raise ValueError(f"total must not be negative; got {total}")
     ints = torch.empty(2 * n + 2 + total, dtype=torch.int32, device=dev)
-    cu, refused, scratch, positions = ints.split([n + 1, 1, n, total])
+    cu, refused, positions, scratch = torch.split_with_sizes(ints, [n + 1, 1, total, n])
     slots = torch.empty(total, dtype=torch.int64, device=dev)
     with _ext.on_device(dev):
         st = _ext.lib().mcamd_paged_reserve(

@@ -24,15 +24,19 @@ from __future__ import annotations
 import torch
 
 from modelcore_amd import _ext
+from modelcore_amd.kernels.paged import check_page_size
 
 __all__ = ["rope_norm_scale_append", "rope_norm_scale_append_partials",
            "rope_norm_scale_append_paged", "default_eps"]
 
 
+_F32_EPS = float(torch.finfo(torch.float32).eps)
+
+
 def default_eps() -> float:
     """The epsilon ``F.rms_norm(x, eps=None)`` adds: float32's, for fp32 and reduced-precision
     inputs alike (the computation is upcast to fp32 before the epsilon is chosen)."""
-    return float(torch.finfo(torch.float32).eps)
+    return _F32_EPS
 
 
 def _table(t: torch.Tensor, half: int, dt: torch.dtype, device) -> torch.Tensor:
@@ -42,7 +46,7 @@ def _table(t: torch.Tensor, half: int, dt: torch.dtype, device) -> torch.Tensor:
         raise ValueError(f"rotary table is on {t.device}, q on {device}")
     if t.shape[-1] != half or t.numel() % half != 0:
         raise ValueError(f"rotary table must end in head_dim/2 = {half}; got {tuple(t.shape)}")
-    return t.reshape(-1, half).contiguous()
+    return (t if t.dim() == 2 else t.view(-1, half)) if t.is_contiguous() else t.reshape(-1, half).contiguous()
 
 
 def _token_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
@@ -180,16 +184,16 @@ def rope_norm_scale_append_partials(qkv, n_head, n_kv_head, cos, sin, cache_seql
 def check_pages(k_pages, v_pages, H_kv, D, dtype, device):
     """The pools of a paged cache, (n_pages, page_size, H_kv, D) with contiguous pages as far apart in
     both; returns (n_pages, page_size, elements between pages)."""
-    from modelcore_amd.kernels.paged import check_page_size
     if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] != D \
             or (H_kv is not None and k_pages.shape[2] != H_kv) or k_pages.shape[0] < 1:
         raise ValueError(f"k_pages/v_pages must both be (n_pages, page_size, H_kv, D) with H_kv={H_kv}, "
                          f"D={D}; got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
     _ext.same_device(device, k_pages=k_pages, v_pages=v_pages)
+    in_page = (k_pages.shape[2] * D, D, 1)
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
         if t.dtype != dtype:
             raise TypeError(f"{name} is {t.dtype}, q is {dtype}")
-        if not t[0].is_contiguous():
+        if t.stride()[1:] != in_page and not t[0].is_contiguous():
             raise ValueError(f"each page of {name} must be contiguous; strides {t.stride()}")
     n, page = k_pages.shape[0], check_page_size(k_pages.shape[1])
     if n > 1 and k_pages.stride(0) != v_pages.stride(0):
