@@ -70,7 +70,7 @@ struct PagedBlock {
 // rows' lengths and positions are loaded at once and stay in registers, R a lane (rows past 64 R are read
 // again), and the number is found by bisection over how many blocks there are from it on. (With the
 // found row's numbers read again from memory, and R = 4 for eight rows too, eight prompts of 37 to 4001
-// tokens took 5% longer.)
+// tokens took 2% longer.)
 //
 // Where the partials of `slots` blocks have room, fewer blocks than half of that may be cut into key
 // ranges: the first ranges of all blocks come first, then the second ones, and so on.
@@ -207,6 +207,9 @@ int launch_paged_append(const PagedArgs &a);
 // Rows of few pairs (few_pairs(.., most)) of a bf16 call: append where k_new is given, and attention.
 int launch_paged_stream(const PagedArgs &a, int64_t most);
 size_t paged_stream_bytes(const PagedArgs &a, int64_t most);  // of scratch, to cut long rows' keys
+// Single tokens of an fp32 call, the same.
+int launch_paged_stream_f32(const PagedArgs &a);
+size_t paged_stream_f32_bytes(const PagedArgs &a);
 // Every row but those.
 int launch_paged_tiled(const PagedArgs &a, int64_t skip);
 size_t paged_tiled_bytes(const PagedArgs &a, int64_t skip);

@@ -91,16 +91,16 @@ int check(const PagedArgs &a) {
   return MCAMD_OK;
 }
 
-// Pairs per KV head up to which a row counts as one of few pairs: one block of the streaming kernel.
-constexpr int64_t kFewPairs = 32;
+// Pairs per KV head up to which a row counts as one of few pairs (few_pairs()): one block of the bf16
+// streaming kernel, and single tokens for the fp32 one.
+int64_t few_of(const PagedArgs &a) { return a.dtype == MCAMD_BF16 ? 32 : 1; }
 
 struct Kernels {
   bool stream, tiles;
 };
 Kernels kernels_of(const PagedArgs &a) {
   const int64_t G = a.n_head / a.n_kv_head;
-  const bool few = a.t_new == 1 || a.t_new * G <= kFewPairs;  // of every row
-  if (a.dtype != MCAMD_BF16) return {false, true};
+  const bool few = a.t_new == 1 || a.t_new * G <= few_of(a);  // of every row
   return {few || a.cu != nullptr, !few};
 }
 
@@ -112,10 +112,10 @@ int launch(PagedArgs a) {
     a.k_new = a.v_new = nullptr;
   }
   if (k.stream) {
-    const int st = launch_paged_stream(a, kFewPairs);
+    const int st = a.dtype == MCAMD_BF16 ? launch_paged_stream(a, few_of(a)) : launch_paged_stream_f32(a);
     if (st != MCAMD_OK || !k.tiles) return st;
   }
-  const int64_t skip = k.stream ? kFewPairs : 0;
+  const int64_t skip = k.stream ? few_of(a) : 0;
   return paged_mfma_supported(a) ? launch_paged_mfma(a, skip) : launch_paged_tiled(a, skip);
 }
 
@@ -171,8 +171,9 @@ extern "C" size_t mcamd_paged_scratch_bytes(int64_t n_rows, int64_t total, int64
   for (const int32_t *cu : {(const int32_t *)nullptr, &packed}) {
     a.cu = cu;
     const Kernels k = kernels_of(a);
-    const int64_t skip = k.stream ? kFewPairs : 0;
-    if (k.stream) most = std::max(most, paged_stream_bytes(a, kFewPairs));
+    const int64_t skip = k.stream ? few_of(a) : 0;
+    if (k.stream)
+      most = std::max(most, a.dtype == MCAMD_BF16 ? paged_stream_bytes(a, few_of(a)) : paged_stream_f32_bytes(a));
     if (k.tiles)
       most = std::max(most, paged_mfma_supported(a) ? paged_mfma_bytes(a, skip) : paged_tiled_bytes(a, skip));
   }

@@ -330,6 +330,70 @@ def test_offsets_past_32_bits(T, dtype, D):
     assert same_bits(kg[n - 17], k_all[4 * page:])
 
 
+@pytest.mark.parametrize("dtype,T", [(BF, 1), (BF, 40), (F32, 1), (F32, 40)])
+@pytest.mark.parametrize("past", [-16, 16])
+def test_pages_far_apart(dtype, T, past):
+    """Pages 2 GiB apart, a little less and a little more, as in the views of one layer of a stacked pool."""
+    page, H_kv, D = 16, 2, 128
+    step = ((1 << 31) + past) // dtype.itemsize  # elements between pages
+    flat = torch.empty(2 * step + page * H_kv * D * 2, dtype=dtype, device=DEV)
+    shape, strides = (3, page, H_kv, D), (step, H_kv * D, D, 1)
+    kg = torch.as_strided(flat, shape, strides)
+    vg = torch.as_strided(flat, shape, strides, page * H_kv * D)
+    g = torch.Generator().manual_seed(16)
+    pos = 3 * page - T
+    k_all, v_all = randn(g, 3 * page, H_kv, D, dtype=dtype), randn(g, 3 * page, H_kv, D, dtype=dtype)
+    for i, p in enumerate((2, 0, 1)):
+        kg[p], vg[p] = k_all[i * page:(i + 1) * page].to(DEV), v_all[i * page:(i + 1) * page].to(DEV)
+    q = randn(g, 1, T, 8, D, dtype=dtype)
+    y = _op()(q.to(DEV), kg, vg, block_table=i32([[2, 0, 1]]), cache_seqlens=i32([pos]), causal=True)
+    want, tol = attend(q[0], k_all, v_all, pos, -1)
+    close(y[0], want, tol)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("H", [5, 8, 33, 40, 64])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_a_new_value_that_is_not_finite(dtype, H, value):
+    """Heads in several blocks all see the token's own value, which its page does not hold before."""
+    pool = Pool([20, 4], 16, 1, 128, dtype, stale=3.0)
+    g = torch.Generator().manual_seed(18)
+    q = randn(g, 2, 1, H, 128, dtype=dtype)
+    k, v = randn(g, 2, 1, 1, 128, dtype=dtype), randn(g, 2, 1, 1, 128, dtype=dtype)
+    v[0, 0, 0, 7] = value
+    y = _call(pool, q, [19, 3], k, v)
+    for b, p in enumerate((19, 3)):
+        pool.k[pool.place(b, p)], pool.v[pool.place(b, p)] = k[b, 0], v[b, 0]
+    other = [d for d in range(128) if d != 7]
+    for b, p in enumerate((19, 3)):
+        kk, vv = pool.rows(b, p + 1)
+        want, tol = attend(q[b], kk, vv.nan_to_num(0.0, 0.0), p, -1)
+        close(y[b][..., other], want[..., other], tol[..., other])
+        if b == 1:
+            close(y[b], want, tol)
+    assert (y[0, ..., 7].isnan() if value != value else y[0, ..., 7] == value).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("H,H_kv", [(16, 1), (32, 1), (33, 1), (64, 1), (6, 6), (20, 5), (48, 12)])
+def test_rows_at_the_edge_of_few_pairs(H, H_kv, dtype):
+    """Rows of 31 to 66 pairs, uniform and packed, of one block of queries and of two."""
+    G = H // H_kv
+    near = sorted({max(1, 32 // G + i) for i in (-1, 0, 1)} | {1, 2})
+    for T in near:
+        run_attention([21, 300], [T, T], H, H_kv, 64, 16, dtype, seed=T)
+    run_attention([21 * i for i in range(len(near))], near, H, H_kv, 128, 32, dtype, window=50, packed=True)
+
+
+@pytest.mark.parametrize("H,H_kv,D", [(12, 12, 64), (8, 4, 32), (4, 1, 128), (6, 2, 256), (9, 1, 40)])
+def test_single_tokens_of_many_keys_fp32(H, H_kv, D):
+    """Cut into ranges, with a head to a wave and a head to a workgroup, with and without a window."""
+    run_attention([4000, 0, 777, 16, 2047], [1] * 5, H, H_kv, D, 16, F32)
+    run_attention([4000, 0, 777, 16, 2047], [1] * 5, H, H_kv, D, 64, F32, window=900)
+    run_attention([300 + 13 * b for b in range(70)], [1] * 70, H, H_kv, D, 16, F32)
+    run_attention([1500, 3, 900, 0], [1, 20, 1, 1], H, H_kv, D, 16, F32, pad=3)
+
+
 def test_same_bits_again_and_on_two_streams():
     """A call gives the same bits each time, also with another at work on another stream."""
     g = torch.Generator().manual_seed(8)
