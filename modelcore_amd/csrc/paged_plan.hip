@@ -22,7 +22,7 @@ namespace {
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
 constexpr int kOneLaunchTokens = 4096;
-constexpr int kTokens = 4;  // consecutive tokens of a thread
+constexpr int kTokens = 4;  // tokens of a thread
 
 struct PlanParams {
   int32_t *table;
@@ -64,46 +64,59 @@ __device__ __forceinline__ int64_t group_scan(int64_t x, int64_t &carry, int64_t
   return y;
 }
 
-__device__ __forceinline__ void write_tokens(const PlanParams &P, int t0) {
-  if (t0 >= P.total) return;
-  // The row of token t0: the last one that begins at or before it, past any empty ones.
-  int lo = 0, hi = P.n_rows;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (P.cu[mid] <= t0)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  int b = lo, end = P.cu[b + 1];
-  const int page_mask = (1 << P.shift) - 1;
+// What the tokens need to know of the rows: in LDS where kThreads rows are the most, else where it lies.
+struct SharedRows {
+  int cu[kThreads + 1], first[kThreads], len[kThreads];
+};
+struct GlobalRows {
+  const int32_t *cu, *first, *len;
+};
+
+// kTokens tokens, `step` apart from t0 on.
+template <class Rows>
+__device__ __forceinline__ void write_tokens(const PlanParams &P, const Rows &rows, int t0, int step) {
+  int row[kTokens];
 #pragma unroll
   for (int u = 0; u < kTokens; ++u) {
-    const int t = t0 + u;
-    if (t >= P.total) return;
-    while (t >= end && b + 1 < P.n_rows) end = P.cu[++b + 1];
-    int64_t slot = -1;
-    int pos = -1;
-    const int first = P.first[b];
-    if (t < end && first >= 0) {
-      const int len = P.seqlens[b];
-      pos = len + t - P.cu[b];
-      const int have = int((int64_t(len) + page_mask) >> P.shift), page = pos >> P.shift;
-      int id;
-      if (page < have) {
-        id = P.table[b * P.table_stride + page];
-      } else {
-        id = P.free_pages[first - (page - have)];
-        if ((pos & page_mask) == 0) P.table[b * P.table_stride + page] = id;
-      }
-      slot = id < 0 ? -1 : (int64_t(id) << P.shift) + (pos & page_mask);
+    // The row of the token: the last one that begins at or before it (those before it may be empty).
+    int lo = 0, hi = P.n_rows;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (rows.cu[mid] <= t0 + u * step)
+        lo = mid;
+      else
+        hi = mid;
     }
-    P.slots[t] = slot;
-    P.positions[t] = pos;
+    row[u] = lo;
+  }
+  // The numbers of all of its pages are asked for before any is used; a token without one asks for the
+  // stack's first.
+  const int page_mask = (1 << P.shift) - 1;
+  int pos[kTokens], id[kTokens];
+  int32_t *named[kTokens];  // where a page that is taken goes
+#pragma unroll
+  for (int u = 0; u < kTokens; ++u) {
+    const int t = t0 + u * step, b = row[u];
+    const int first = rows.first[b], len = rows.len[b], begin = rows.cu[b];
+    const bool planned = t < rows.cu[b + 1] && first >= 0;
+    pos[u] = planned ? len + t - begin : -1;
+    const int have = int((int64_t(len) + page_mask) >> P.shift), page = pos[u] >> P.shift;
+    int32_t *const line = P.table + b * P.table_stride + page;
+    id[u] = *(!planned ? P.free_pages : page < have ? line : P.free_pages + (first - (page - have)));
+    named[u] = planned && page >= have && (pos[u] & page_mask) == 0 ? line : nullptr;
+  }
+#pragma unroll
+  for (int u = 0; u < kTokens; ++u) {
+    const int t = t0 + u * step;
+    if (t >= P.total) return;
+    if (named[u]) *named[u] = id[u];
+    P.slots[t] = pos[u] < 0 || id[u] < 0 ? -1 : (int64_t(id[u]) << P.shift) + (pos[u] & page_mask);
+    P.positions[t] = pos[u];
   }
 }
 
 __global__ __launch_bounds__(kThreads) void reserve_kernel(PlanParams P, int with_tokens) {
+  __shared__ SharedRows s_rows;
   __shared__ int64_t s_sum[kWaves];
   __shared__ int s_refused;
   const int tid = threadIdx.x;
@@ -129,48 +142,82 @@ __global__ __launch_bounds__(kThreads) void reserve_kernel(PlanParams P, int wit
     const bool ok = fits && (take == 0 || upto <= stack);
     if (here) {
       // A row that takes none has no first page; any index but -1 will do.
-      P.first[b] = !ok ? -1 : take == 0 ? 0 : int(stack - 1 - (upto - take));
+      const int first = !ok ? -1 : take == 0 ? 0 : int(stack - 1 - (upto - take));
+      P.first[b] = first;
       P.cu[b + 1] = int(end);
+      if (b < kThreads) {
+        s_rows.first[b] = first;
+        s_rows.cu[b + 1] = int(end);
+        s_rows.len[b] = int(len);
+      }
       if (!ok) atomicAdd(&s_refused, 1);
       given += ok ? take : 0;
     }
   }
   group_scan(given, kept, s_sum);
   if (tid == 0) {
-    P.cu[0] = 0;
+    P.cu[0] = s_rows.cu[0] = 0;
     P.free_count[0] = int(stack - kept);
     P.refused[0] = s_refused;
   }
   if (!with_tokens) return;
   __syncthreads();  // the rows' numbers are written
-  for (int t = tid * kTokens; t < P.total; t += kThreads * kTokens) write_tokens(P, t);
+  for (int t = tid; t < P.total; t += kThreads * kTokens) {
+    if (P.n_rows <= kThreads)
+      write_tokens(P, s_rows, t, kThreads);
+    else
+      write_tokens(P, GlobalRows{P.cu, P.first, P.seqlens}, t, kThreads);
+  }
 }
 
 __global__ __launch_bounds__(256) void tokens_kernel(PlanParams P) {
-  write_tokens(P, (int(blockIdx.x) * 256 + int(threadIdx.x)) * kTokens);
+  __shared__ SharedRows s_rows;
+  const int t = int(blockIdx.x) * 256 * kTokens + int(threadIdx.x);
+  if (P.n_rows > kThreads) {
+    write_tokens(P, GlobalRows{P.cu, P.first, P.seqlens}, t, 256);
+    return;
+  }
+  for (int b = threadIdx.x; b < P.n_rows; b += 256) {
+    s_rows.cu[b + 1] = P.cu[b + 1];
+    s_rows.first[b] = P.first[b];
+    s_rows.len[b] = P.seqlens[b];
+  }
+  if (threadIdx.x == 0) s_rows.cu[0] = 0;
+  __syncthreads();
+  write_tokens(P, s_rows, t, 256);
 }
 
 // Rows rows[0 .. n) give their pages back, in order, and are empty then. A row that is named twice
-// gives them once; a row outside the batch, or a page outside the pool, is passed over.
+// gives them where it is named first; a row outside the batch is passed over.
 __global__ __launch_bounds__(kThreads) void release_kernel(int32_t *table, int64_t table_stride,
                                                            int32_t *seqlens, const int32_t *rows,
                                                            int n, int n_rows, int32_t *free_pages,
                                                            int32_t *free_count, int max_pages,
                                                            int n_pages, int shift) {
   __shared__ int64_t s_sum[kWaves];
-  __shared__ int s_row[kThreads], s_end[kThreads];
+  __shared__ __attribute__((aligned(16))) int s_row[kThreads], s_end[kThreads];
   const int tid = threadIdx.x;
   int64_t top = min(max(free_count[0], 0), n_pages);
   for (int i0 = 0; i0 < n; i0 += kThreads) {
     const int i = i0 + tid;
     int row = i < n ? rows[i] : -1;
-    if (row >= n_rows) row = -1;
-    const int len = row >= 0 ? atomicExch(&seqlens[row], 0) : 0;
+    if (row < 0 || row >= n_rows) row = -1;
+    s_row[tid] = row;
+    __syncthreads();
+    int again = 0;  // names of the same row before this one
+#pragma unroll 8
+    for (int j = 0; j < (row < 0 ? 0 : tid >> 2); ++j) {
+      const int4 x = reinterpret_cast<const int4 *>(s_row)[j];
+      again |= int(x.x == row) | int(x.y == row) | int(x.z == row) | int(x.w == row);
+    }
+    for (int j = tid & ~3; j < tid; ++j) again |= int(s_row[j] == row);
+    if (again) row = -1;
+    const int len = row >= 0 ? seqlens[row] : 0;
+    if (row >= 0) seqlens[row] = 0;
     const int64_t held =
         min((max(int64_t(len), int64_t(0)) + (1 << shift) - 1) >> shift, int64_t(max_pages));
     const int64_t base = top;
     const int64_t end = group_scan(held, top, s_sum) - base;
-    s_row[tid] = row;
     s_end[tid] = int(end);
     __syncthreads();
     const int64_t all = top - base;

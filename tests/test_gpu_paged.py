@@ -498,6 +498,30 @@ def test_release_rows_twice_and_outside():
     assert dc.tolist() == [count[0] + 2]
 
 
+def test_rows_named_twice_give_their_pages_where_named_first():
+    """Whichever wave comes first: the stack is the same every time, for names a few and a thousand apart."""
+    from modelcore_amd.kernels.paged import paged_release
+    n = 900
+    lens = [16 + b % 40 for b in range(n)]
+    g = torch.Generator().manual_seed(12)
+    once = torch.randperm(n, generator=g).tolist()
+    for names in (once[:70] + once[:70] + once[60:130], once + once[::-1] + once,
+                  [x for b in once[:300] for x in (b, b, b)]):
+        table, free, count = _plan_state(lens, 4, 16, 3)
+        dt, dl, df, dc = i32(table), i32(lens), i32(free), i32(count)
+        paged_release(dt, dl, i32(names), df, dc, page_size=16)
+        held = list(lens)
+        release(table, held, names, free, count, 16)
+        assert dt.tolist() == table and dl.tolist() == held and dc.tolist() == count
+        assert df.tolist()[:count[0]] == free[:count[0]]
+
+
+@pytest.mark.parametrize("rows", [1024, 1025])
+def test_reserve_more_tokens_than_one_launch_takes(rows):
+    _check_plan([(7 * b) % 100 for b in range(rows)], [(0, 3, 11, 0, 1)[b % 5] * 2 for b in range(rows)], 10, 16,
+                2 * rows)
+
+
 def test_pages_change_hands_without_loss():
     """Forty rounds of rows that end and start anew: every page is free or held once."""
     from modelcore_amd.kernels.paged import paged_release, paged_reserve
