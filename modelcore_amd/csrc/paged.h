@@ -10,6 +10,7 @@
 #pragma once
 
 #include "kernels.h"
+#include "prefill_split.h"
 
 namespace mcamd {
 
@@ -202,6 +203,16 @@ struct PagedTiles {
   float *part_o;    // [slot][groups of 32 pairs][md][4][64][4], as SplitGeo lays them out
   float *part_ml;   // [slot][groups][32][2]
 };
+
+// Room for the partials of a workgroup per compute unit, where a call of at most `blocks` blocks can have so
+// few that two ranges of each run side by side, and a block (of at most 256 positions) keys for two. Uniform
+// rows have that many blocks; packed ones mostly fewer than their bound, by up to about four times.
+inline int paged_slots(const PagedArgs &a, int64_t blocks) {
+  const int64_t cus = device_cus(), room = int64_t(a.kv.max_pages) << a.kv.shift;
+  const int64_t keys = a.window < 0 ? room : std::min<int64_t>(room, a.window + 256 + 64);
+  const int64_t most = a.cu ? 2 * cus : cus / 2;  // workgroups of uncut blocks
+  return blocks * a.n_kv_head <= most && keys >= 2 * kMinRangeKeys ? int(cus) : 0;
+}
 
 int launch_paged_append(const PagedArgs &a);
 // Rows of few pairs (few_pairs(.., most)) of a bf16 call: append where k_new is given, and attention.

@@ -163,7 +163,7 @@ extern "C" size_t mcamd_paged_scratch_bytes(int64_t n_rows, int64_t total, int64
   a.n_head = n_head;
   a.n_kv_head = n_kv_head;
   a.head_dim = head_dim;
-  a.window = window;
+  a.window = std::min(window, int64_t(1) << 30);  // no position is past it
   a.dtype = dtype;
   // The sizes do not tell packed rows from uniform ones: room for both.
   const int32_t packed = 0;
@@ -224,7 +224,7 @@ extern "C" int mcamd_flash_attn_paged_with_kvcache(
   a.n_head = n_head;
   a.n_kv_head = n_kv_head;
   a.head_dim = head_dim;
-  a.window = window;
+  a.window = std::min(window, int64_t(1) << 30);  // no position is past it
   a.dtype = dtype;
   a.scratch = scratch;
   a.scratch_bytes = scratch_bytes;

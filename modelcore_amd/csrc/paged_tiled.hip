@@ -551,8 +551,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(TiledParams P, in
 }
 
 // What a call runs: the waves over pairs (KS = 1) or keys (KS = 4), and room for the partials of cut
-// blocks: as many as the chip holds workgroups, where a call can have so few that two ranges of each run
-// side by side.
+// blocks.
 struct TiledPlan {
   int ks, pairs, kt, slots;
   int64_t bound;  // of blocks
@@ -570,7 +569,7 @@ TiledPlan tiled_plan(const PagedArgs &a, int64_t skip) {
   t.bound = paged_blocks_bound(a, t.pairs, skip);
   // Measured time of a tile on a compute unit of its own, per head dim (prefill_tiled.hip).
   t.tile_us = float(a.head_dim) * (t.ks == 4 ? (bf ? 0.027f : 0.085f) : (bf ? 0.012f : 0.035f));
-  t.slots = t.bound * a.n_kv_head < 2 * cus ? int(cus) : 0;
+  t.slots = paged_slots(a, t.bound);
   return t;
 }
 int64_t slot_floats(const PagedArgs &a, int pairs) {

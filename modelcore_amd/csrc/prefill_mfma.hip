@@ -878,12 +878,6 @@ bool paged_mfma_supported(const PagedArgs &a) {
 
 namespace {
 
-// Room for the partials of a workgroup per compute unit, where a call can have so few blocks that two
-// ranges of each run side by side.
-int64_t paged_slots(const PagedArgs &a, int64_t blocks) {
-  const int64_t cus = device_cus();
-  return blocks * a.n_kv_head < 2 * cus ? cus : 0;
-}
 constexpr int64_t kSlotFloats = int64_t(kPairs) * (D + 2);
 
 }  // namespace

@@ -112,6 +112,12 @@ def test_chunk_lengths(T, window):
     run_attention([17], [T], 2, 2, 64, 16, F32, window, seed=T)
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 40])
+def test_windows_wider_than_any_row(window):
+    run_attention([40, 0, 300], [1, 70, 9], 4, 2, 128, 16, BF, window)
+    run_attention([40, 0, 300], [1, 70, 9], 4, 2, 64, 16, F32, window)
+
+
 @pytest.mark.parametrize("dtype,H,H_kv,D", [(BF, 8, 2, 128), (BF, 6, 6, 64), (F32, 4, 2, 128), (BF, 4, 1, 256)])
 @pytest.mark.parametrize("window", [-1, 33])
 def test_mixed_rows(dtype, H, H_kv, D, window):
