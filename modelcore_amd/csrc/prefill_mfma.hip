@@ -60,8 +60,12 @@
 // fragments are read in runs of 256 bytes), its V loads 8 keys, so that a load's keys share a page: its
 // number is a scalar, loaded a tile ahead, and the page a buffer resource, whose offsets are as cheap as
 // those of a contiguous cache. (With K fragments of 32 keys, two pages and 64-bit addresses per lane, a
-// chunk of 8 x 512 tokens after 8192 keys took 660 us.) The ranges of cut blocks are merged by
-// paged_tiled.hip, and pairs that are not finite redone (paged_careful.h).
+// chunk of 8 x 512 tokens after 8192 keys took 660 us.) Their q enters as it is and the scores are
+// multiplied by the scale where exp2 takes them: the one rounding but the output's is then that of the
+// weights to bf16, and the outputs' error against 64 bits 2.3e-3 of their norm, of which the output's
+// rounding alone makes 1.7e-3; with q scaled and rounded 3.4e-3, for 579 instead of 606 us (8 x 512 tokens
+// after 8192 keys, 32 / 8 heads: 936 TFLOP/s). The ranges of cut blocks are merged by paged_tiled.hip, and
+// pairs that are not finite redone (paged_careful.h).
 #include "paged_careful.h"
 #include "prefill_order.h"
 #include "prefill_split.h"
@@ -237,7 +241,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
 
   // Q^T fragments: B[k = dim][n = pair], lane holds pair `col`, dims 16 kd + 8 h .. + 7, each
   // element multiplied by scale_log2 and rounded to bf16 once, so the products give scores in
-  // log2 units with no per-score scaling.
+  // log2 units with no per-score scaling. PAGED: as it is, which halves the outputs' error.
   bf16x8 qf[8];
   {
     const uint16_t *qp = P.q + ((tok0 + pos) * P.H + int64_t(kvh) * P.G + head) * D + 8 * h;
@@ -245,7 +249,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
     for (int kd = 0; kd < 8; ++kd) {
       const bf16x8 raw =
           __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4 *>(qp + 16 * kd));
-      qf[kd] = __builtin_convertvector(__builtin_convertvector(raw, f32x8) * P.scale_log2, bf16x8);
+      qf[kd] = PAGED ? raw : __builtin_convertvector(__builtin_convertvector(raw, f32x8) * P.scale_log2, bf16x8);
     }
   }
   const int p_abs = s0 + pos;
@@ -401,9 +405,9 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
     for (int e = 0; e < 16; ++e) o[md][e] = 0.f;
   float m = -INFINITY;
   float l = 0.f;
-  // The score products start from -m (the running maximum, 0 while the pair has none) in every
-  // accumulator instead of zero, so a tile's scores arrive already shifted: the weights are
-  // exp2 of them as they are. All sixteen accumulators of a lane belong to its one pair.
+  // The score products start from -m (the running maximum in the scores' units, 0 while the pair has
+  // none) in every accumulator instead of zero, so a tile's scores arrive already shifted: the weights
+  // are exp2 of them as they are. All sixteen accumulators of a lane belong to its one pair.
   f32x16 negm;
 #pragma unroll
   for (int e = 0; e < 16; ++e) negm[e] = 0.f;
@@ -480,10 +484,12 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   auto sum8 = [](const f32x8 &pv) {
     return ((pv[0] + pv[1]) + (pv[2] + pv[3])) + ((pv[4] + pv[5]) + (pv[6] + pv[7]));
   };
+  // PAGED: scores are of q as it is, and get their scale here.
+  auto in_log2 = [&](float s) { return PAGED ? s * P.scale_log2 : s; };
   auto weights = [&](const f32x16 (&s)[2], int ks, float &ts) {
     f32x8 pv;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) pv[e] = __builtin_amdgcn_exp2f(s[ks >> 1][8 * (ks & 1) + e]);
+    for (int e = 0; e < 8; ++e) pv[e] = __builtin_amdgcn_exp2f(in_log2(s[ks >> 1][8 * (ks & 1) + e]));
     ts = sum8(pv);
     return __builtin_convertvector(pv, bf16x8);
   };
@@ -491,7 +497,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
     f32x8 pv;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      pv[e] = __builtin_amdgcn_exp2f(s[ks >> 1][8 * (ks & 1) + e] - shift);
+      pv[e] = __builtin_amdgcn_exp2f(in_log2(s[ks >> 1][8 * (ks & 1) + e] - shift));
     ts = sum8(pv);
     return __builtin_convertvector(pv, bf16x8);
   };
@@ -615,7 +621,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
       if (__builtin_amdgcn_ballot_w64(!(tl <= kTileSumLimit) || m == -INFINITY) != 0) {
         const float mx = tile_max(sc) + m_try;
         const float m_new = fmaxf(m, mx);
-        const float alpha = m_new == -INFINITY ? 1.f : exp2_or_zero(m - m_new);
+        const float alpha = m_new == -INFINITY ? 1.f : exp2_or_zero(in_log2(m - m_new));
         l *= alpha;
 #pragma unroll
         for (int md = 0; md < 4; ++md)
@@ -732,7 +738,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
         for (int j = 0; j < 4; ++j)
           *reinterpret_cast<float4 *>(T->part_o + ((g * 4 + md) * 4 + j) * 256 + lane * 4) =
               make_float4(o[md][4 * j], o[md][4 * j + 1], o[md][4 * j + 2], o[md][4 * j + 3]);
-      if (h == 0) *reinterpret_cast<float2 *>(T->part_ml + (g * 32 + col) * 2) = make_float2(m, lt);
+      if (h == 0) *reinterpret_cast<float2 *>(T->part_ml + (g * 32 + col) * 2) = make_float2(in_log2(m), lt);
       return;
     }
     bool ok = true;

@@ -41,11 +41,10 @@ def attend(q, k, v, pos, window):
     """q (T, H, D) at positions pos .. against keys k, v (pos + T, H_kv, D): the outputs in 64 bits and,
     per output element, how far the kernels may be off.
 
-    A score's terms are products of D pairs. With bf16 operands their sum is exact to 2^-24 a step, but
-    the bf16 / 128 kernels round q, multiplied by the softmax scale, once to bf16, so a score is off by at
-    most d = (2^-8 + D 2^-24) sum |q k| scale; in fp32 d = (D + 4) 2^-24 sum |q k| scale. exp2 of it adds
-    a few units of its argument's last place. A weight is so off by a factor within exp(+-d'), its sum
-    alike; bf16 weights are rounded once more (2^-8) before they meet V, and the sums over n keys, the
+    A score's terms are products of D pairs, which no kernel rounds to fewer than 32 bits: its sum is off by
+    at most d = (D + 4) 2^-24 sum |q k| scale. exp2 of it adds a few units of its argument's last place. A
+    weight is so off by a factor within exp(+-d'), its sum alike; the weights of the bf16 / 128 kernel for
+    long rows are rounded once more (2^-8) before they meet V, and the sums over n keys, the
     ranges' merge and the final division take fewer than (n + 64) steps of 2^-24. Outputs are weighted
     means, so all of this is at most (2 d' + ..) sum w |v|, and the last rounding half a step of the
     result."""
@@ -67,7 +66,7 @@ def attend(q, k, v, pos, window):
         mean = torch.einsum("hn,nhd->hd", w, vv.abs())
         n = p + 1 - lo
         step = 2.0 ** -24
-        d = ((u if q.dtype == torch.bfloat16 else 0) + (D + 4) * step) * size + 8 * step * (1 + size)
+        d = (D + 4) * step * size + 8 * step * (1 + size)
         rel = 2 * d + (u if q.dtype == torch.bfloat16 else 0) + (n + 64) * step
         tol[t] = torch.expm1(rel)[:, None] * mean + u * out[t].abs() * (1 + torch.expm1(rel)[:, None])
     return out, tol
