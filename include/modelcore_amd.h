@@ -386,7 +386,7 @@ int mcamd_paged_reserve(int32_t *block_table, int64_t table_stride, const int32_
 /*
  * Rows rows[0 .. n_release) end: their pages go onto the stack of free pages, in the order of `rows`
  * and of their tables, their table entries become -1 and their cache_seqlens 0. A row named twice
- * gives its pages once; numbers outside [0, n_rows) are passed over.
+ * gives its pages where it is named first; numbers outside [0, n_rows) are passed over.
  */
 int mcamd_paged_release(int32_t *block_table, int64_t table_stride, int32_t *cache_seqlens,
                         const int32_t *rows, int64_t n_release, int64_t n_rows,
@@ -428,7 +428,7 @@ size_t mcamd_paged_scratch_bytes(int64_t n_rows, int64_t total, int64_t max_seql
  * 256, at most 64 query heads share a KV head. cache_seqlens is only read.
  * A row whose positions fall outside [0, max_pages * page_size) gets NaN output and appends nothing; a
  * query that sees a key in a page outside the pool is NaN, and nothing is appended there. Tokens past the
- * last row's are not read, and their outputs not written. The scratch (16-byte aligned) belongs to the
+ * last row's, and a row's past max_seqlen, are not read, and their outputs not written. The scratch (16-byte aligned) belongs to the
  * call until it ends on the stream. No two rows may append to one page.
  */
 int mcamd_flash_attn_paged_with_kvcache(

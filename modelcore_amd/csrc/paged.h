@@ -45,11 +45,12 @@ struct PagedArgs {
   hipStream_t stream;
 };
 
-// The new tokens of row b: [tok0, tok0 + T) of q, whatever cu holds.
+// The new tokens of row b: [tok0, tok0 + T) of q, and no more than t_new, by which grids and scratch are
+// sized, whatever cu holds.
 __device__ __forceinline__ void row_tokens(const int32_t *cu, int t_new, int total, int b, int &tok0,
                                            int &T) {
   tok0 = cu ? max(cu[b], 0) : b * t_new;
-  T = cu ? max(min(cu[b + 1], total) - tok0, 0) : t_new;
+  T = cu ? min(max(min(cu[b + 1], total) - tok0, 0), t_new) : t_new;
 }
 
 // Whether a row of T new tokens is one of few pairs, which the streaming kernels take: a single token, or

@@ -359,7 +359,8 @@ def flash_attn_paged_with_kvcache(q, k_pages, v_pages, k=None, v=None, *, block_
         cu_seqlens: (B + 1,) int32 on the device, ascending from 0 (``PagedPlan.cu_seqlens``); a row
             may have no tokens, and tokens past the last row's are left out (their outputs are not
             written)
-        max_seqlen: with cu_seqlens, at least the longest row's new tokens (host int)
+        max_seqlen: with cu_seqlens, at least the longest row's new tokens (host int); a row's tokens past
+            it are left out
         causal: accepted for signature parity; attention is always causal
         window_size: (left, right); left = -1 means unlimited
 

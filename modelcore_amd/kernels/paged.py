@@ -108,7 +108,7 @@ def paged_reserve(block_table, cache_seqlens, new_lens, free_pages, free_count, 
 def paged_release(block_table, cache_seqlens, rows, free_pages, free_count, *, page_size):
     """Rows that have ended give their pages back to the stack, in the order of ``rows`` ((m,)
     int32): their table entries become -1 and their cache_seqlens 0, in place. A row named twice gives
-    its pages once; numbers outside the batch are passed over."""
+    its pages where it is named first; numbers outside the batch are passed over."""
     n, max_pages, stride, dev = _check_tables(block_table, cache_seqlens, free_pages, free_count,
                                               "paged_release")
     _ext.same_device(dev, rows=rows)

@@ -400,6 +400,35 @@ def test_single_tokens_of_many_keys_fp32(H, H_kv, D):
     run_attention([1500, 3, 900, 0], [1, 20, 1, 1], H, H_kv, D, 16, F32, pad=3)
 
 
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (BF, 64), (F32, 64)])
+@pytest.mark.parametrize("longest", [1, 3, 40])
+def test_tokens_past_max_seqlen_are_left_out(dtype, D, longest):
+    """Rows longer than the call was told: their first tokens as in a call that was told right, the others
+    neither read nor written, and the rows beside them whole."""
+    new, pos = [20, 1, 70, 2], [30, 700, 10, 5]
+    g = torch.Generator().manual_seed(20)
+    pool = Pool([p + t for p, t in zip(pos, new)], 16, 2, D, dtype, stale=9.0)
+    kp, vp = pool.k.clone(), pool.v.clone()
+    q, k, v = (randn(g, sum(new), h, D, dtype=dtype) for h in (8, 2, 2))
+    cu = [0, 20, 21, 91, 93]
+    for b, (p, t) in enumerate(zip(pos, new)):
+        for i in range(t):
+            where = pool.place(b, p + i)
+            kp[where], vp[where] = 9.0, 9.0
+            here = i < longest
+            pool.k[where] = k[cu[b] + i] if here else 9.0
+            pool.v[where] = v[cu[b] + i] if here else 9.0
+    kg, vg = kp.to(DEV), vp.to(DEV)
+    y = _op()(q.to(DEV), kg, vg, k=k.to(DEV), v=v.to(DEV), block_table=pool.table.to(DEV),
+              cache_seqlens=i32(pos), cu_seqlens=i32(cu), max_seqlen=longest, causal=True)
+    torch.cuda.synchronize()
+    assert same_bits(kg, pool.k) and same_bits(vg, pool.v)
+    for b, (p, t) in enumerate(zip(pos, new)):
+        n = min(t, longest)
+        want, tol = attend(q[cu[b]:cu[b] + n], *pool.rows(b, p + n), p, -1)
+        close(y[cu[b]:cu[b] + n], want, tol, f"row {b}")
+
+
 def test_same_bits_again_and_on_two_streams():
     """A call gives the same bits each time, also with another at work on another stream."""
     g = torch.Generator().manual_seed(8)
