@@ -429,6 +429,91 @@ def test_tokens_past_max_seqlen_are_left_out(dtype, D, longest):
         close(y[cu[b]:cu[b] + n], want, tol, f"row {b}")
 
 
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (BF, 64), (F32, 64)])
+def test_captured_calls_follow_their_inputs(dtype, D):
+    """Two graphs out of one memory pool, of a mixed call and of single tokens: each replay, with eager calls
+    and synchronizations in between, gives the bits of an eager call on what the buffers hold then."""
+    g = torch.Generator().manual_seed(22)
+    pool = Pool([1400, 60, 900], 16, 2, D, dtype, stale=0.0)
+    kg, vg, table = pool.k.to(DEV), pool.v.to(DEV), pool.table.to(DEV)
+    calls = []
+    for new in ([1, 40, 5], [1, 1, 1]):
+        n = sum(new)
+        bufs = {"q": randn(g, n, 8, D, dtype=dtype).to(DEV), "k": randn(g, n, 2, D, dtype=dtype).to(DEV),
+                "v": randn(g, n, 2, D, dtype=dtype).to(DEV), "pos": i32([0, 0, 0])}
+        cu = i32([0, new[0], new[0] + new[1], n])
+        calls.append((bufs, lambda kk, vv, b=bufs, cu=cu, m=max(new): _op()(
+            b["q"], kk, vv, k=b["k"], v=b["v"], block_table=table, cache_seqlens=b["pos"], cu_seqlens=cu,
+            max_seqlen=m, causal=True)))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _, call in calls:
+            call(kg, vg)
+    torch.cuda.current_stream().wait_stream(side)
+    share, graphs, outs = torch.cuda.graph_pool_handle(), [], []
+    for _, call in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side, pool=share):
+            outs.append(call(kg, vg))
+    for i in range(6):
+        got, want = [], []
+        ke, ve = kg.clone(), vg.clone()
+        for bufs, call in calls:
+            for name in ("q", "k", "v"):
+                bufs[name].copy_(randn(g, *bufs[name].shape, dtype=dtype))
+            bufs["pos"].copy_(torch.tensor([(i * 271 + 3) % 1390, i, (i * 97) % 850], dtype=torch.int32))
+        for (bufs, call), graph, out in zip(calls, graphs, outs):
+            graph.replay()
+            got.append(out.clone())
+            want.append(call(ke, ve))
+            if i % 2:
+                torch.cuda.synchronize()
+        for a, b in zip(got + [kg, vg], want + [ke, ve]):
+            assert same_bits(a, b), i
+
+
+def _attention_args(**kw):
+    z = lambda *shape, dtype=BF: torch.zeros(*shape, dtype=dtype, device=DEV)  # noqa: E731
+    args = {"q": z(2, 1, 4, 64), "k_pages": z(4, 16, 2, 64), "v_pages": z(4, 16, 2, 64),
+            "block_table": z(2, 2, dtype=torch.int32), "cache_seqlens": z(2, dtype=torch.int32)}
+    args.update({n: x(z) if callable(x) else x for n, x in kw.items()})
+    return args
+
+
+@pytest.mark.parametrize("error,words,kw", [
+    (ValueError, "q must be", {"q": lambda z: z(2, 4, 64)}),
+    (ValueError, "block_table", {"block_table": lambda z: z(2, 2, dtype=torch.int64)}),
+    (ValueError, "block_table", {"block_table": lambda z: z(2, 4, dtype=torch.int32)[:, ::2]}),
+    (ValueError, "block_table", {"block_table": None}),
+    (ValueError, "rows", {"block_table": lambda z: z(3, 2, dtype=torch.int32)}),
+    (ValueError, "cache_seqlens", {"cache_seqlens": None}),
+    (ValueError, "cache_seqlens", {"cache_seqlens": lambda z: z(3, dtype=torch.int32)}),
+    (ValueError, "both k and v", {"k": lambda z: z(2, 1, 2, 64)}),
+    (ValueError, "k/v must be", {"k": lambda z: z(2, 2, 2, 64), "v": lambda z: z(2, 2, 2, 64)}),
+    (TypeError, "k is", {"k": lambda z: z(2, 1, 2, 64, dtype=F32), "v": lambda z: z(2, 1, 2, 64, dtype=F32)}),
+    (TypeError, "k_pages is", {"k_pages": lambda z: z(4, 16, 2, 64, dtype=F32)}),
+    (ValueError, "contiguous", {"k_pages": lambda z: z(4, 2, 16, 64).transpose(1, 2)}),
+    (ValueError, "page stride", {"v_pages": lambda z: z(4, 2, 16, 2, 64)[:, 0]}),
+    (ValueError, "power of two", {"k_pages": lambda z: z(4, 24, 2, 64), "v_pages": lambda z: z(4, 24, 2, 64)}),
+    (ValueError, "power of two", {"k_pages": lambda z: z(4, 8, 2, 64), "v_pages": lambda z: z(4, 8, 2, 64)}),
+    (ValueError, "multiple", {"q": lambda z: z(2, 1, 5, 64)}),
+    (ValueError, "cu_seqlens", {"q": lambda z: z(2, 4, 64), "cu_seqlens": lambda z: z(2, dtype=torch.int32),
+                                "max_seqlen": 1}),
+    (ValueError, "max_seqlen", {"q": lambda z: z(2, 4, 64), "cu_seqlens": lambda z: z(3, dtype=torch.int32)}),
+    (ValueError, "less than", {"q": lambda z: z(2, 3, 4, 64), "max_seqlen": 2}),
+    (TypeError, "bfloat16 or float32", {"q": lambda z: z(2, 1, 4, 64, dtype=torch.float16)}),
+    (RuntimeError, "64 query heads", {"q": lambda z: z(2, 1, 130, 64)}),
+    (RuntimeError, "at most 256", {"q": lambda z: z(2, 1, 4, 264), "k_pages": lambda z: z(4, 16, 2, 264),
+                                   "v_pages": lambda z: z(4, 16, 2, 264)}),
+    (NotImplementedError, "forward-only", {"q": lambda z: z(2, 1, 4, 64).requires_grad_()}),
+])
+def test_attention_refuses_before_launching(error, words, kw):
+    args = _attention_args(**kw)
+    with pytest.raises(error, match=words):
+        _op()(args.pop("q"), args.pop("k_pages"), args.pop("v_pages"), **args)
+
+
 def test_same_bits_again_and_on_two_streams():
     """A call gives the same bits each time, also with another at work on another stream."""
     g = torch.Generator().manual_seed(8)
