@@ -13,7 +13,10 @@
 // reserve: one workgroup sums over the rows (integer sums: the same pages whatever the timing), then
 // tokens are dealt to threads. A page that is taken begins at its first new token, which writes its
 // number into the table. Up to kOneLaunchTokens tokens the same workgroup does both; more take a
-// second launch, bound by the slots and positions it writes.
+// second launch, bound by the slots and positions it writes. Rows' offsets, lengths and first pages are
+// searched in LDS (up to kThreads rows), the page numbers of all of a thread's tokens asked for before any
+// is used. 64 rows of a token: 6.3 us (8.8 with the search in memory), three scans and two round trips;
+// 512 rows of a million tokens, 12.6 MB written: 4.5 + 8.6.
 #include "paged.h"
 
 namespace mcamd {

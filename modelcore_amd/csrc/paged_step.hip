@@ -10,7 +10,9 @@
 //
 // LPI lanes per head: lane L holds dims VEC L .. of the first half and their partners in the second,
 // so a rotation needs no exchange and the sum of squares log2(LPI) steps. VEC is 16 bytes where rows
-// and tables are made of such pieces, else one element with 64 lanes a head.
+// and tables are made of such pieces, else one element with 64 lanes a head. 4096 tokens of 32 / 8 heads
+// of 128 in bf16, 102 MB: 20.9 us, 4.86 TB/s, what a copy reaches; 64 tokens 4.1, one round trip for the
+// position, one for its table rows.
 //
 // A token whose position is outside the tables gets NaN in q and writes nothing; one whose slot is
 // outside the pool writes nothing.

@@ -15,6 +15,8 @@
 //  * Not finite: a pair whose result is not finite is redone over the keys it sees alone
 //    (careful_pair()), and so is every pair of a block that met a page outside the pool, which leaves
 //    NaN to those that see such a page.
+// Two prompts of 512, 12 heads of 64 in fp32: 31 us (0.81 GFLOP; the contiguous kernel's 30), a tile's loads
+// and its products in series.
 #include "paged_careful.h"
 #include "prefill_order.h"
 #include "prefill_split.h"
