@@ -354,7 +354,8 @@ def flash_attn_paged_with_kvcache(q, k_pages, v_pages, k=None, v=None, *, block_
         k, v: new keys/values, of q's layout with H_kv heads, written to their pages, or both None
             (they are there: ``rope_norm_scale_append_paged`` wrote them)
         block_table: (B, max_pages) int32; position t of row b is token t % page_size of page
-            block_table[b, t // page_size]. Rows may read the same pages; no two rows may write one.
+            block_table[b, t // page_size]. Rows may read the same pages, but a page that takes
+            new tokens in this call is its own row's alone.
         cache_seqlens: (B,) int32 position of each row before the new tokens (read only)
         cu_seqlens: (B + 1,) int32 on the device, ascending from 0 (``PagedPlan.cu_seqlens``); a row
             may have no tokens, and tokens past the last row's are left out (their outputs are not
