@@ -193,10 +193,13 @@ def same_device(device, **tensors):
             raise ValueError(f"{name} is on {t.device}, not on {device}")
 
 
+_HERE = contextlib.nullcontext()
+
+
 def on_device(device):
     """A context in which `device` is the current one, as a launch on its streams needs."""
     if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+        return _HERE
     return torch.cuda.device(device)
 
 

@@ -371,33 +371,37 @@ def flash_attn_paged_with_kvcache(q, k_pages, v_pages, k=None, v=None, *, block_
         checked mode (``set_checked``) such a call raises IndexError instead.
     """
     what = "flash_attn_paged_with_kvcache"
-    _ext.require_rocm(q, k_pages, v_pages, k, v, block_table, cache_seqlens, cu_seqlens, what=what)
+    _ext.require_rocm(q, what=what)  # the others are on its device, checked below
     packed = cu_seqlens is not None
-    if q.dim() != (3 if packed else 4):
+    shape = q.shape
+    if len(shape) != (3 if packed else 4):
         raise ValueError(f"q must be {'(total, H, D)' if packed else '(B, T_new, H, D)'}; got "
-                         f"{tuple(q.shape)}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v)):
+                         f"{tuple(shape)}")
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)
+                                    or (v is not None and v.requires_grad)):
         raise NotImplementedError(f"{what} is forward-only (no autograd)")
-    H, D = q.shape[-2:]
+    H, D = shape[-2], shape[-1]
     dt, dev = q.dtype, q.device
     code = _ext.dtype_code(dt)
-    if block_table is None or block_table.dtype != torch.int32 or block_table.dim() != 2 \
-            or block_table.shape[1] < 1 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+    lines, at = ((), ()) if block_table is None else (block_table.shape, block_table.stride())
+    if len(lines) != 2 or block_table.dtype != torch.int32 or lines[1] < 1 \
+            or (lines[1] > 1 and at[1] != 1):
         raise ValueError("block_table is required: (B, max_pages) int32 with contiguous lines")
-    B, max_pages = block_table.shape
+    B, max_pages = lines
+    line = at[0] if B > 1 else max(at[0], max_pages)  # one line has no stride of its own
     if packed:
-        if cu_seqlens.dtype != torch.int32 or tuple(cu_seqlens.shape) != (B + 1,):
+        if cu_seqlens.dtype != torch.int32 or cu_seqlens.shape != (B + 1,):
             raise ValueError(f"cu_seqlens must be ({B + 1},) int32; got {tuple(cu_seqlens.shape)} "
                              f"{cu_seqlens.dtype}")
         if max_seqlen is None or int(max_seqlen) < 0:
             raise ValueError("max_seqlen (at least the longest row's new tokens) is required with "
                              "cu_seqlens")
-        total, longest = q.shape[0], min(int(max_seqlen), q.shape[0])
+        total, longest = shape[0], min(int(max_seqlen), shape[0])
         cu_seqlens = cu_seqlens.contiguous()
     else:
-        if q.shape[0] != B:
-            raise ValueError(f"q has {q.shape[0]} rows, block_table {B}")
-        longest = q.shape[1]
+        if shape[0] != B:
+            raise ValueError(f"q has {shape[0]} rows, block_table {B}")
+        longest = shape[1]
         if max_seqlen is not None and int(max_seqlen) < longest:
             raise ValueError(f"max_seqlen {max_seqlen} is less than q's {longest} tokens")
         total = B * longest
@@ -405,14 +409,14 @@ def flash_attn_paged_with_kvcache(q, k_pages, v_pages, k=None, v=None, *, block_
         raise ValueError("pass both k and v, or neither")
     H_kv = None
     if k is not None:
-        if k.shape != v.shape or k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] \
-                or k.shape[-1] != D:
-            raise ValueError(f"k/v must be of q's layout {tuple(q.shape)} with H_kv heads; got "
-                             f"{tuple(k.shape)} and {tuple(v.shape)}")
+        new = k.shape
+        if new != v.shape or len(new) != len(shape) or new[:-2] != shape[:-2] or new[-1] != D:
+            raise ValueError(f"k/v must be of q's layout {tuple(shape)} with H_kv heads; got "
+                             f"{tuple(new)} and {tuple(v.shape)}")
         for name, t in (("k", k), ("v", v)):
             if t.dtype != dt:
                 raise TypeError(f"{name} is {t.dtype}, q is {dt}")
-        H_kv = k.shape[-2]
+        H_kv = new[-2]
     n_pages, page, stride = check_pages(k_pages, v_pages, H_kv, D, dt, dev)
     H_kv = k_pages.shape[2]
     if H_kv == 0 or H % H_kv:
@@ -423,27 +427,26 @@ def flash_attn_paged_with_kvcache(q, k_pages, v_pages, k=None, v=None, *, block_
     if CHECK_POSITIONS and B > 0:
         lens = [longest] * B
         if packed:
-            at = cu_seqlens.tolist()
-            if at[0] != 0 or at[-1] > total or any(y - x < 0 or y - x > longest
-                                                   for x, y in zip(at, at[1:])):
+            ends = cu_seqlens.tolist()
+            if ends[0] != 0 or ends[-1] > total or any(y - x < 0 or y - x > longest
+                                                       for x, y in zip(ends, ends[1:])):
                 raise IndexError(f"{what}: cu_seqlens must ascend from 0 to at most {total} in "
                                  f"steps of at most max_seqlen {longest}")
-            lens = [y - x for x, y in zip(at, at[1:])]
+            lens = [y - x for x, y in zip(ends, ends[1:])]
         _check_paged_positions(block_table, seqlens, lens, n_pages, page, w)
     q = q.contiguous()
     if k is not None:
         k, v = k.contiguous(), v.contiguous()
-    out = torch.empty(q.shape, dtype=dt, device=dev)
+    out = torch.empty_like(q)
     with _ext.on_device(dev):
         nbytes = _paged_scratch_bytes(dev.index, B, total, longest, H, H_kv, D, max_pages, page, w,
                                       code)
         # Scratch of the call's own: calls on several streams, and captured graphs, share nothing.
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         st = _ext.lib().mcamd_flash_attn_paged_with_kvcache(
             q.data_ptr(), k.data_ptr() if k is not None else None,
             v.data_ptr() if v is not None else None, k_pages.data_ptr(), v_pages.data_ptr(),
-            block_table.data_ptr(), max(block_table.stride(0), max_pages) if B <= 1
-            else block_table.stride(0), seqlens.data_ptr(),
+            block_table.data_ptr(), line, seqlens.data_ptr(),
             cu_seqlens.data_ptr() if packed else None, out.data_ptr(), B, total, longest, H, H_kv, D,
             n_pages, page, stride, max_pages, w, int(bool(causal)), code,
             ws.data_ptr() if ws is not None else None, nbytes, _ext.stream_handle(dev))

@@ -39,29 +39,26 @@ def check_page_size(page_size) -> int:
 
 
 def _check_tables(block_table, cache_seqlens, free_pages, free_count, what):
-    _ext.require_rocm(block_table, cache_seqlens, free_pages, free_count, what=what)
+    _ext.require_rocm(block_table, what=what)
     dev = block_table.device
     _ext.same_device(dev, cache_seqlens=cache_seqlens, free_pages=free_pages, free_count=free_count)
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[1] < 1 \
-            or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
+    lines, at = block_table.shape, block_table.stride()
+    if block_table.dtype != torch.int32 or len(lines) != 2 or lines[1] < 1 \
+            or (at[1] != 1 and lines[1] > 1):
         raise ValueError("block_table must be (rows, max_pages) int32 with contiguous lines; got "
-                         f"{tuple(block_table.shape)} {block_table.dtype}")
-    n = block_table.shape[0]
+                         f"{tuple(lines)} {block_table.dtype}")
+    n, max_pages = lines
     for name, t, shape in (("cache_seqlens", cache_seqlens, (n,)),
-                           ("free_pages", free_pages, tuple(free_pages.shape[:1])),
+                           ("free_pages", free_pages, free_pages.shape[:1]),
                            ("free_count", free_count, (1,))):
-        if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
-            raise ValueError(f"{name} must be {shape} int32, contiguous; got {tuple(t.shape)} "
+        if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{name} must be {tuple(shape)} int32, contiguous; got {tuple(t.shape)} "
                              f"{t.dtype}")
-    if free_pages.numel() < 1:
+    n_pages = free_pages.numel()
+    if n_pages < 1:
         raise ValueError("free_pages must have room for every page of the pool")
-    return n, block_table.shape[1], _line_stride(block_table), dev
-
-
-def _line_stride(block_table):
-    """Numbers between lines of a block table (a single line has none of its own)."""
-    return max(block_table.stride(0), block_table.shape[1]) if block_table.shape[0] <= 1 \
-        else block_table.stride(0)
+    # A single line has no stride of its own.
+    return n, max_pages, at[0] if n > 1 else max(at[0], max_pages), n_pages, dev
 
 
 def paged_reserve(block_table, cache_seqlens, new_lens, free_pages, free_count, *, total,
@@ -82,25 +79,25 @@ def paged_reserve(block_table, cache_seqlens, new_lens, free_pages, free_count, 
         PagedPlan. A row whose pages the stack does not hold, or that would outgrow its line of the
         table, takes none; its tokens get slot and position -1 and ``refused`` counts it.
     """
-    n, max_pages, stride, dev = _check_tables(block_table, cache_seqlens, free_pages, free_count,
-                                              "paged_reserve")
+    n, max_pages, stride, n_pages, dev = _check_tables(block_table, cache_seqlens, free_pages,
+                                                       free_count, "paged_reserve")
     _ext.same_device(dev, new_lens=new_lens)
-    if new_lens.dtype != torch.int32 or tuple(new_lens.shape) != (n,):
+    if new_lens.dtype != torch.int32 or new_lens.shape != (n,):
         raise ValueError(f"new_lens must be ({n},) int32; got {tuple(new_lens.shape)} "
                          f"{new_lens.dtype}")
     new_lens = new_lens.contiguous()
     total, page_size = int(total), check_page_size(page_size)
     if total < 0:
         raise ValueError(f"total must not be negative; got {total}")
-    ints = torch.empty(2 * n + 2 + total, dtype=torch.int32, device=dev)
+    ints = new_lens.new_empty(2 * n + 2 + total)
     cu, refused, positions, scratch = torch.split_with_sizes(ints, [n + 1, 1, total, n])
-    slots = torch.empty(total, dtype=torch.int64, device=dev)
+    slots = new_lens.new_empty(total, dtype=torch.int64)
     with _ext.on_device(dev):
         st = _ext.lib().mcamd_paged_reserve(
             block_table.data_ptr(), stride, cache_seqlens.data_ptr(), new_lens.data_ptr(),
             free_pages.data_ptr(), free_count.data_ptr(), scratch.data_ptr(), cu.data_ptr(),
             slots.data_ptr(), positions.data_ptr(), refused.data_ptr(), n, max_pages,
-            free_pages.numel(), page_size, total, _ext.stream_handle(dev))
+            n_pages, page_size, total, _ext.stream_handle(dev))
     _ext.check(st, "paged_reserve")
     return PagedPlan(slots, positions, cu, refused)
 
@@ -109,8 +106,8 @@ def paged_release(block_table, cache_seqlens, rows, free_pages, free_count, *, p
     """Rows that have ended give their pages back to the stack, in the order of ``rows`` ((m,)
     int32): their table entries become -1 and their cache_seqlens 0, in place. A row named twice gives
     its pages where it is named first; numbers outside the batch are passed over."""
-    n, max_pages, stride, dev = _check_tables(block_table, cache_seqlens, free_pages, free_count,
-                                              "paged_release")
+    n, max_pages, stride, n_pages, dev = _check_tables(block_table, cache_seqlens, free_pages,
+                                                       free_count, "paged_release")
     _ext.same_device(dev, rows=rows)
     if rows.dtype != torch.int32 or rows.dim() != 1:
         raise ValueError(f"rows must be (m,) int32; got {tuple(rows.shape)} {rows.dtype}")
@@ -119,5 +116,5 @@ def paged_release(block_table, cache_seqlens, rows, free_pages, free_count, *, p
         st = _ext.lib().mcamd_paged_release(
             block_table.data_ptr(), stride, cache_seqlens.data_ptr(), rows.data_ptr(),
             rows.numel(), n, free_pages.data_ptr(), free_count.data_ptr(), max_pages,
-            free_pages.numel(), check_page_size(page_size), _ext.stream_handle(dev))
+            n_pages, check_page_size(page_size), _ext.stream_handle(dev))
     _ext.check(st, "paged_release")

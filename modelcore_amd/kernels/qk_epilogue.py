@@ -39,14 +39,18 @@ def default_eps() -> float:
     return _F32_EPS
 
 
-def _table(t: torch.Tensor, half: int, dt: torch.dtype, device) -> torch.Tensor:
+def _check_table(t: torch.Tensor, half: int, dt: torch.dtype, device) -> None:
     if t.dtype != dt:
         raise TypeError(f"rotary table is {t.dtype}, q is {dt}")
     if t.device != device:
         raise ValueError(f"rotary table is on {t.device}, q on {device}")
     if t.shape[-1] != half or t.numel() % half != 0:
         raise ValueError(f"rotary table must end in head_dim/2 = {half}; got {tuple(t.shape)}")
-    return (t if t.dim() == 2 else t.view(-1, half)) if t.is_contiguous() else t.reshape(-1, half).contiguous()
+
+
+def _table(t: torch.Tensor, half: int, dt: torch.dtype, device) -> torch.Tensor:
+    _check_table(t, half, dt, device)
+    return t.reshape(-1, half).contiguous()
 
 
 def _token_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
@@ -184,16 +188,21 @@ def rope_norm_scale_append_partials(qkv, n_head, n_kv_head, cos, sin, cache_seql
 def check_pages(k_pages, v_pages, H_kv, D, dtype, device):
     """The pools of a paged cache, (n_pages, page_size, H_kv, D) with contiguous pages as far apart in
     both; returns (n_pages, page_size, elements between pages)."""
+    shape, at = k_pages.shape, k_pages.stride()
+    if len(shape) == 4 and shape[0] > 1 and shape == v_pages.shape and at == v_pages.stride() \
+            and at[1:] == (shape[2] * D, D, 1) and shape[3] == D and H_kv in (None, shape[2]) \
+            and k_pages.dtype == dtype == v_pages.dtype and k_pages.device == device == v_pages.device:
+        return shape[0], check_page_size(shape[1]), at[0]
+    # What is not as usual, check by check.
     if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] != D \
             or (H_kv is not None and k_pages.shape[2] != H_kv) or k_pages.shape[0] < 1:
         raise ValueError(f"k_pages/v_pages must both be (n_pages, page_size, H_kv, D) with H_kv={H_kv}, "
                          f"D={D}; got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
     _ext.same_device(device, k_pages=k_pages, v_pages=v_pages)
-    in_page = (k_pages.shape[2] * D, D, 1)
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
         if t.dtype != dtype:
             raise TypeError(f"{name} is {t.dtype}, q is {dtype}")
-        if t.stride()[1:] != in_page and not t[0].is_contiguous():
+        if not t[0].is_contiguous():
             raise ValueError(f"each page of {name} must be contiguous; strides {t.stride()}")
     n, page = k_pages.shape[0], check_page_size(k_pages.shape[1])
     if n > 1 and k_pages.stride(0) != v_pages.stride(0):
@@ -201,12 +210,12 @@ def check_pages(k_pages, v_pages, H_kv, D, dtype, device):
     return n, page, k_pages.stride(0) if n > 1 else page * k_pages.shape[2] * D
 
 
-def _packed_rows(t):
-    """t (total, heads, D) with heads and D contiguous and the elements between tokens (a view of a
+def _packed_rows(t, n, heads, D):
+    """t (n tokens, heads, D) with heads and D contiguous and the elements between tokens (a view of a
     fused projection's output qualifies); else a contiguous copy."""
-    n, heads, D = t.shape
-    if t.stride(2) == 1 and (heads == 1 or t.stride(1) == D) and (n <= 1 or t.stride(0) >= heads * D):
-        return t, t.stride(0) if n > 1 else heads * D
+    token, head, one = t.stride()
+    if one == 1 and (heads == 1 or head == D) and (n <= 1 or token >= heads * D):
+        return t, token if n > 1 else heads * D
     return t.contiguous(), heads * D
 
 
@@ -232,8 +241,7 @@ def rope_norm_scale_append_paged(q, cos, sin, positions, k=None, v=None, k_pages
     A token with a position outside the tables gets NaN in q and writes nothing; one with a slot outside
     the pool (-1) writes nothing.
     """
-    _ext.require_rocm(q, cos, sin, k, v, k_pages, v_pages, positions, slots,
-                      what="rope_norm_scale_append_paged")
+    _ext.require_rocm(q, what="rope_norm_scale_append_paged")  # the others are on its device, checked below
     if q.dim() != 3:
         raise ValueError(f"q must be (total, H, D); got {tuple(q.shape)}")
     total, H, D = q.shape
@@ -242,13 +250,16 @@ def rope_norm_scale_append_paged(q, cos, sin, positions, k=None, v=None, k_pages
     dt, dev = q.dtype, q.device
     code = _ext.dtype_code(dt)
     half = D // 2
-    cos_t, sin_t = _table(cos, half, dt, dev), _table(sin, half, dt, dev)
-    if cos_t.shape != sin_t.shape:
-        raise ValueError(f"cos {tuple(cos_t.shape)} and sin {tuple(sin_t.shape)} differ")
+    _check_table(cos, half, dt, dev)
+    _check_table(sin, half, dt, dev)
+    n_pos = cos.numel() // half
+    if sin.numel() != cos.numel():
+        raise ValueError(f"cos {tuple(cos.shape)} and sin {tuple(sin.shape)} differ")
+    cos, sin = cos.contiguous(), sin.contiguous()
     if (k is None) != (v is None):
         raise ValueError("pass both k and v, or neither")
     _ext.same_device(dev, positions=positions, k=k, v=v, slots=slots)
-    if positions.dtype != torch.int32 or tuple(positions.shape) != (total,):
+    if positions.dtype != torch.int32 or positions.shape != (total,):
         raise ValueError(f"positions must be ({total},) int32; got {tuple(positions.shape)} "
                          f"{positions.dtype}")
     positions = positions.contiguous()
@@ -267,18 +278,18 @@ def rope_norm_scale_append_paged(q, cos, sin, positions, k=None, v=None, k_pages
         if k_pages is None or v_pages is None or slots is None:
             raise ValueError("k and v need k_pages, v_pages and slots")
         n_pages, page, stride = check_pages(k_pages, v_pages, H_kv, D, dt, dev)
-        if slots.dtype != torch.int64 or tuple(slots.shape) != (total,):
+        if slots.dtype != torch.int64 or slots.shape != (total,):
             raise ValueError(f"slots must be ({total},) int64; got {tuple(slots.shape)} {slots.dtype}")
         slots = slots.contiguous()
-        (k, ks), (v, vs) = _packed_rows(k), _packed_rows(v)
-    q, qs = _packed_rows(q)
-    out = torch.empty((total, H, D), dtype=dt, device=dev)
+        (k, ks), (v, vs) = _packed_rows(k, total, H_kv, D), _packed_rows(v, total, H_kv, D)
+    q, qs = _packed_rows(q, total, H, D)
+    out = q.new_empty((total, H, D))
     with_kv = k is not None
     with _ext.on_device(dev):
         st = _ext.lib().mcamd_qk_rope_norm_append_paged(
             q.data_ptr(), qs, k.data_ptr() if with_kv else None, ks,
-            v.data_ptr() if with_kv else None, vs, cos_t.data_ptr(), sin_t.data_ptr(),
-            cos_t.shape[0], positions.data_ptr(), slots.data_ptr() if with_kv else None,
+            v.data_ptr() if with_kv else None, vs, cos.data_ptr(), sin.data_ptr(),
+            n_pos, positions.data_ptr(), slots.data_ptr() if with_kv else None,
             k_pages.data_ptr() if with_kv else None, v_pages.data_ptr() if with_kv else None,
             out.data_ptr(), total, H, H_kv, D, n_pages, page, stride,
             default_eps() if eps is None else float(eps), float(scale), code,
