@@ -203,6 +203,19 @@ struct PagedTiles {
   float ratio;      // prefill_split.h's, times the blocks of the call
   float *part_o;    // [slot][groups of 32 pairs][md][4][64][4], as SplitGeo lays them out
   float *part_ml;   // [slot][groups][32][2]
+  struct Cut {      // a block, for the merge
+    int b, qt, tok0, T, s0, ranges, unused[2];
+  };
+  Cut *cuts;        // [slots / 2]: the blocks of a call that may be cut, by their number
+  int *n_cuts;      // and how many
+
+  // Left for the merge by a call's first workgroup, and by the first range of each block.
+  __device__ __forceinline__ void note_call(bool found, const PagedBlock &v) const {
+    if (slots > 0) *n_cuts = found && v.most > 1 ? v.n_blocks : 0;
+  }
+  __device__ __forceinline__ void note_block(int id, const PagedBlock &v, int ranges) const {
+    cuts[id] = Cut{v.b, v.qt, v.tok0, v.T, v.s0, ranges, {0, 0}};
+  }
 };
 
 // Room for the partials of a workgroup per compute unit, where a call of at most `blocks` blocks can have so
@@ -213,6 +226,19 @@ inline int paged_slots(const PagedArgs &a, int64_t blocks) {
   const int64_t keys = a.window < 0 ? room : std::min<int64_t>(room, a.window + 256 + 64);
   const int64_t most = a.cu ? 2 * cus : cus / 2;  // workgroups of uncut blocks
   return blocks * a.n_kv_head <= most && keys >= 2 * kMinRangeKeys ? int(cus) : 0;
+}
+
+inline size_t paged_tiles_bytes(int64_t slots, int64_t slot_floats) {
+  return slots == 0 ? 0 : size_t(slots) * size_t(slot_floats) * 4 + size_t(slots / 2) * sizeof(PagedTiles::Cut) + 16;
+}
+// Lays out the scratch of a call with so many slots, if it is large enough; else no block is cut.
+inline void paged_tiles_buffers(const PagedArgs &a, PagedTiles &t, int64_t slots, int64_t slot_floats,
+                                int64_t ml_floats) {
+  t.slots = a.scratch && a.scratch_bytes >= paged_tiles_bytes(slots, slot_floats) ? int(slots) : 0;
+  t.part_o = static_cast<float *>(a.scratch);
+  t.part_ml = t.part_o + t.slots * (slot_floats - ml_floats);
+  t.cuts = reinterpret_cast<PagedTiles::Cut *>(t.part_o + t.slots * slot_floats);
+  t.n_cuts = reinterpret_cast<int *>(t.cuts + t.slots / 2);
 }
 
 int launch_paged_append(const PagedArgs &a);
@@ -230,6 +256,6 @@ bool paged_mfma_supported(const PagedArgs &a);
 int launch_paged_mfma(const PagedArgs &a, int64_t skip);
 size_t paged_mfma_bytes(const PagedArgs &a, int64_t skip);
 // The ranges of cut blocks (of `pairs` pairs) added up.
-int launch_paged_tiles_merge(const PagedArgs &a, const PagedTiles &t, int pairs);
+int launch_paged_tiles_merge(const PagedArgs &a, const PagedTiles &t, int pairs, int64_t bound);
 
 }  // namespace mcamd

@@ -163,6 +163,9 @@ __device__ __forceinline__ Range find_range(const StreamParams &P, int lane, Row
 // in many ranges, take eight waves (one row of 16K keys, 64 ranges: 4.2 us, with four 8.5), more than
 // kManyPairs two (60 rows of 32 heads: 6.3 us, with four 7.9, with eight 11.0).
 constexpr int64_t kManyPairs = 1024;
+// Workgroups of a packed call's merge, at most, beyond one per head of each row: three rows of 8 to 57
+// tokens of one head per KV head took 37 us with a workgroup a row and KV head.
+constexpr int64_t kMergeGroups = 1024;
 template <class E, int DP, int MW, int PB>
 __global__ __launch_bounds__(64 * MW) void paged_stream_merge_kernel(StreamParams P) {
   constexpr int N = (DP + 63) / 64, U = 8;
@@ -254,7 +257,8 @@ StreamPlan stream_plan(const PagedArgs &a, int64_t most, int64_t block, int fill
   p.head_waves = a.n_kv_head % 4 == 0 ? 4 : a.n_kv_head % 2 == 0 ? 2 : 1;
   p.target = fill * device_cus();
   const int64_t max_pairs = std::min(a.t_new * G, std::max(most, G));
-  p.merge_pairs = a.cu ? G : max_pairs;  // most rows of a mixture have one token
+  // Of a mixture most rows have one token; a workgroup of more goes round.
+  p.merge_pairs = a.cu ? std::max(G, std::min(max_pairs, kMergeGroups / (a.n_rows * a.n_kv_head))) : max_pairs;
   p.units = a.n_rows * ((max_pairs + block - 1) / block);
   p.pair_slots = int(std::min<int64_t>(block, max_pairs));
   const int64_t room = int64_t(a.kv.max_pages) << a.kv.shift;
@@ -315,7 +319,7 @@ int launch_stream(K kernel, const StreamParams &P, const PagedArgs &a, const Str
   const int st = launch_status("paged_stream");
   if (st != MCAMD_OK || !p.cut) return st;
   const dim3 grid{unsigned(a.n_kv_head * p.merge_pairs), unsigned(a.n_rows)};
-  if (int64_t(grid.x) * grid.y > kManyPairs)
+  if ((a.cu ? a.n_rows * a.n_head : int64_t(grid.x) * grid.y) > kManyPairs)  // of a mixture, the single tokens
     hipLaunchKernelGGL((paged_stream_merge_kernel<E, DP, 2, PB>), grid, dim3(128), 0, a.stream, P);
   else
     hipLaunchKernelGGL((paged_stream_merge_kernel<E, DP, 8, PB>), grid, dim3(512), 0, a.stream, P);

@@ -20,7 +20,7 @@
 // The loads are marked non-temporal (the pages are read once per call): 32 rows of up to 8192 keys, 16 / 4
 // heads of 128, 57.7 -> 51.0 us, 60 rows of 32 / 8 heads 196 -> 165 (6.2 TB/s).
 //
-// New tokens come from k_new and v_new where given, and the wave that has a row's last keys puts them in
+// New tokens come from k_new and v_new where given, and a wave of the row's last range puts them in
 // their pages. A row of one range writes its output; otherwise (o, m, l) go to scratch in fp32, a row of
 // floats per pair, and the merge launch adds the ranges up. Pairs that are not finite are redone
 // (paged_careful.h).
@@ -386,9 +386,9 @@ __global__ __launch_bounds__(kThreads)
   l = sum_halves(l);
   if (lost) l = NAN;
 
-  // The new tokens into their pages: the wave that has the row's last keys. In every block, so that a redo
-  // below finds them whichever other block has come how far; they write the same.
-  if (fresh && range == ranges - 1 && kw == 0) {
+  // The new tokens into their pages: in the row's last range, by the wave that has the fewest tiles. In every
+  // block, so that a redo below finds them whichever other block has come how far; they write the same.
+  if (fresh && range == ranges - 1 && kw == n_kw - 1) {
     const int units = D / 8;  // of 16 bytes, of K and of V
     for (int i = lane; i < R.T * units; i += 64) {
       const int t = i / units, u = i - t * units, key = R.s0 + t;

@@ -202,9 +202,9 @@ __global__ __launch_bounds__(kThreads)
     if (lost) l[g] = NAN;
   }
 
-  // The new token into its page: the wave that has the row's last keys. In every block, so that a redo below
-  // finds it whichever other block has come how far; they write the same.
-  if (fresh && mine.range == ranges - 1 && kw == 0 && lane < LPK && d < D) {
+  // The new token into its page: in the row's last range, by the wave that has the fewest tiles. In every
+  // block, so that a redo below finds it whichever other block has come how far; they write the same.
+  if (fresh && mine.range == ranges - 1 && kw == n_kw - 1 && lane < LPK && d < D) {
     const int id = P.kv.table[b * P.kv.table_stride + (s0 >> P.kv.shift)];
     if (P.kv.is_page(id)) {
       const int64_t to = 4 * (P.kv.offset(id, P.kv.in_page(s0), int64_t(P.H_kv) * D) + d) + head_at;

@@ -117,9 +117,11 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
 
   const int id = P.cu ? int(blockIdx.x) : dealt_block(int(blockIdx.x), int(gridDim.x), P.deal);
   PagedBlock blk;
-  if (!find_paged_block(P.cu, P.seqlens, P.tiles.n_rows, P.T_new, P.tiles.total, P.G, P.H_kv,
-                        G_::PAIRS, P.tiles.skip, P.tiles.slots, id / P.H_kv, threadIdx.x & 63, blk))
-    return;
+  const bool found =
+      find_paged_block(P.cu, P.seqlens, P.tiles.n_rows, P.T_new, P.tiles.total, P.G, P.H_kv, G_::PAIRS,
+                       P.tiles.skip, P.tiles.slots, id / P.H_kv, threadIdx.x & 63, blk);
+  if (id == 0 && threadIdx.x == 0) P.tiles.note_call(found, blk);
+  if (!found) return;
   const int kvh = id % P.H_kv, part = blk.part, row = blk.b, T_b = blk.T, s0 = blk.s0;
   const int64_t tok0 = blk.tok0;
   // This workgroup's pairs: n of them from pair p0 on, which is head r0 of position q0.
@@ -149,6 +151,7 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
   const int64_t at = pair_at(pr);
   E *out = static_cast<E *>(P.out) + at;
   if (!row_ok) {
+    if (blk.most > 1 && part == 0 && tid == 0) P.tiles.note_block(id, blk, 1);
     if (live && part == 0 && (KS == 1 || wave == 0))
       for (int d = h; d < D; d += 2) out[d] = from_f32<E>(NAN);
     return;
@@ -163,6 +166,7 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
   if (blk.most > 1) {  // this workgroup's range of the block's tiles
     const int ranges = best_splits(P.tiles.ratio / float(blk.n_blocks), n_tiles, KT, blk.most);
     if (part >= ranges) return;
+    if (part == 0 && tid == 0) P.tiles.note_block(id, blk, ranges);
     whole = ranges == 1;
     const int t0 = part * n_tiles / ranges, t1 = (part + 1) * n_tiles / ranges;
     hi = min(hi, lo + t1 * KT - 1);
@@ -476,33 +480,27 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
 }
 
 // Merges the partials of key ranges, in the partials' own layout: a workgroup per 32 pairs and 32 dims of
-// a block, a wave per step j of them, eight ranges' loads in flight.
+// a block, a wave per step j of them, eight ranges' loads in flight. What the blocks are, and whether any is
+// cut, the kernel before has left (each workgroup finding its block again took 10.4 us where none was cut:
+// 17 rows of up to 10 tokens, 32 / 8 heads).
 template <class E>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(TiledParams P, int pairs) {
   const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
   const int j = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int groups = P.tiles.groups, kt = P.tiles.kt;
+  const int groups = P.tiles.groups;
   int id = blockIdx.x;
   const int md = id % P.md;
   id /= P.md;
   const int w = id % groups;
-  id /= groups;
+  id /= groups;  // the block
   const int d = 32 * md + 8 * j;  // this wave's dims d .. d + 7, lane half h d + 4h ..
-  if (d >= P.D) return;
-  PagedBlock blk;  // first ranges come first: range 0 of every block
-  if (!find_paged_block(P.cu, P.seqlens, P.tiles.n_rows, P.T_new, P.tiles.total, P.G, P.H_kv, pairs,
-                        P.tiles.skip, P.tiles.slots, id / P.H_kv, lane, blk) ||
-      blk.part > 0 || blk.most == 1)
-    return;
+  const int n_blocks = *P.tiles.n_cuts;
+  const PagedTiles::Cut blk = P.tiles.cuts[id];
+  const int ranges = blk.ranges;
+  if (d >= P.D || id >= n_blocks || ranges == 1) return;  // of one range: written by the block itself
   const int kvh = id % P.H_kv;
-  if (blk.s0 < 0 || int64_t(blk.s0) + blk.T > int64_t(P.kv.max_pages) << P.kv.shift) return;  // NaN already
   const int64_t n_pairs = int64_t(blk.T) * P.G, p0 = int64_t(blk.qt) * pairs;
   const int n = int(min(int64_t(pairs), n_pairs - p0));
-  const int first = blk.s0 + int(p0 / P.G), hi = blk.s0 + int((p0 + n - 1) / P.G);
-  const int lo = (P.window >= 0 ? max(0, first - P.window) : 0) & ~(P.tiles.align - 1);
-  const int ranges =
-      best_splits(P.tiles.ratio / float(blk.n_blocks), (hi - lo) / kt + 1, kt, blk.most);
-  if (ranges == 1) return;  // written by the block itself
   const int in_block = 32 * w + col;
   const bool live = in_block < n;
   const int t = live ? int((p0 + in_block) / P.G) : 0;
@@ -512,7 +510,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(TiledParams P, in
   };
 
   constexpr int U = 8;
-  const int64_t group = int64_t(id) * groups + w, step = int64_t(blk.n_blocks) * groups;
+  const int64_t group = int64_t(id) * groups + w, step = int64_t(n_blocks) * groups;
   float M = -INFINITY, L = 0.f;
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
   for (int r0 = 0; r0 < ranges; r0 += U) {
@@ -612,7 +610,7 @@ int run(const TiledParams &P, const PagedArgs &a, const TiledPlan &t) {
                      a.stream, P);
   const int st = launch_status("paged_tiled");
   if (st != MCAMD_OK || P.tiles.slots == 0) return st;
-  return launch_paged_tiles_merge(a, P.tiles, t.pairs);
+  return launch_paged_tiles_merge(a, P.tiles, t.pairs, t.bound);
 }
 
 template <class E, int DP>
@@ -635,9 +633,10 @@ int dispatch(const TiledParams &P, const PagedArgs &a, const TiledPlan &t) {
 
 }  // namespace
 
-int launch_paged_tiles_merge(const PagedArgs &a, const PagedTiles &tiles, int pairs) {
+int launch_paged_tiles_merge(const PagedArgs &a, const PagedTiles &tiles, int pairs, int64_t bound) {
   const TiledParams P = tiled_params(a, tiles);
-  const int64_t blocks = paged_blocks_bound(a, pairs, tiles.skip) * P.H_kv * tiles.groups * P.md;
+  // Blocks of which two ranges do not fit the slots are not cut.
+  const int64_t blocks = std::min<int64_t>(bound * P.H_kv, tiles.slots / 2) * tiles.groups * P.md;
   if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
   const dim3 grid{unsigned(blocks)}, threads{kThreads};
   if (a.dtype == MCAMD_BF16)
@@ -649,7 +648,7 @@ int launch_paged_tiles_merge(const PagedArgs &a, const PagedTiles &tiles, int pa
 
 size_t paged_tiled_bytes(const PagedArgs &a, int64_t skip) {
   const TiledPlan t = tiled_plan(a, skip);
-  return size_t(t.slots) * size_t(slot_floats(a, t.pairs)) * 4;
+  return paged_tiles_bytes(t.slots, slot_floats(a, t.pairs));
 }
 
 int launch_paged_tiled(const PagedArgs &a, int64_t skip) {
@@ -662,10 +661,8 @@ int launch_paged_tiled(const PagedArgs &a, int64_t skip) {
   T.kt = t.kt;
   T.align = 1;
   T.groups = t.pairs / 32;
-  T.slots = a.scratch && a.scratch_bytes >= paged_tiled_bytes(a, skip) ? t.slots : 0;
+  paged_tiles_buffers(a, T, t.slots, slot_floats(a, t.pairs), t.pairs * 2);
   T.ratio = t.tile_us * MCAMD_SPLIT_BYTES_PER_US / (float(slot_floats(a, t.pairs)) * 8.f);
-  T.part_o = static_cast<float *>(a.scratch);
-  T.part_ml = T.part_o + int64_t(T.slots) * t.pairs * ((a.head_dim + 31) / 32 * 32);
   const TiledParams P = tiled_params(a, T);
   return a.dtype == MCAMD_BF16 ? dispatch<bf16>(P, a, t) : dispatch<float>(P, a, t);
 }

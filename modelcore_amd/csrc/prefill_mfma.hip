@@ -194,9 +194,10 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   int64_t tok0 = int64_t(b) * P.T_new;
   PagedBlock blk;
   if constexpr (PAGED) {
-    if (!find_paged_block(P.cu, P.seqlens, T->n_rows, P.T_new, T->total, P.G, P.H_kv, P.QT * P.G, T->skip,
-                          T->slots, int(blockIdx.x) / P.H_kv, lane, blk))
-      return;
+    const bool found = find_paged_block(P.cu, P.seqlens, T->n_rows, P.T_new, T->total, P.G, P.H_kv,
+                                        P.QT * P.G, T->skip, T->slots, int(blockIdx.x) / P.H_kv, lane, blk);
+    if (blockIdx.x == 0 && tid == 0) T->note_call(found, blk);
+    if (!found) return;
     kvh = int(blockIdx.x) % P.H_kv;
     part = blk.part;
     b = row = blk.b, qt = blk.qt, tok0 = blk.tok0, T_b = blk.T, s0 = blk.s0;
@@ -234,6 +235,8 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   const int head = live ? pr - (pr / P.G) * P.G : 0;
   uint16_t *out = P.out + ((tok0 + pos) * P.H + int64_t(kvh) * P.G + head) * D;
   if (!row_ok) {
+    if constexpr (PAGED)
+      if (blk.most > 1 && part == 0 && tid == 0) T->note_block(int(blockIdx.x), blk, 1);
     if (live && part == 0)
       for (int d = h * 64; d < h * 64 + 64; ++d) out[d] = 0x7fc0;
     return;
@@ -266,6 +269,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
       const int tiles = (hi - lo) / KT + 1;
       const int ranges = best_splits(T->ratio / float(blk.n_blocks), tiles, KT, blk.most);
       if (part >= ranges) return;
+      if (part == 0 && tid == 0) T->note_block(int(blockIdx.x), blk, ranges);
       whole = ranges == 1;
       const int t0 = part * tiles / ranges, t1 = (part + 1) * tiles / ranges;
       hi = min(hi, lo + t1 * KT - 1);
@@ -890,7 +894,7 @@ constexpr int64_t kSlotFloats = int64_t(kPairs) * (D + 2);
 
 size_t paged_mfma_bytes(const PagedArgs &a, int64_t skip) {
   const int64_t G = a.n_head / a.n_kv_head;
-  return size_t(paged_slots(a, paged_blocks_bound(a, kPairs / G * G, skip)) * kSlotFloats * 4);
+  return paged_tiles_bytes(paged_slots(a, paged_blocks_bound(a, kPairs / G * G, skip)), kSlotFloats);
 }
 
 int launch_paged_mfma(const PagedArgs &a, int64_t skip) {
@@ -919,19 +923,16 @@ int launch_paged_mfma(const PagedArgs &a, int64_t skip) {
   T.kt = T.align = KT;
   T.groups = kWaves;
   const int64_t bound = paged_blocks_bound(a, P.QT * P.G, skip);
-  T.slots = int(paged_slots(a, bound));
-  if (!a.scratch || a.scratch_bytes < size_t(T.slots * kSlotFloats * 4)) T.slots = 0;
+  paged_tiles_buffers(a, T, paged_slots(a, bound), kSlotFloats, kPairs * 2);
   // A tile of 64 keys takes 256 pairs 1.4 us; a range's partials are written and read.
   T.ratio = 1.4f * MCAMD_SPLIT_BYTES_PER_US / (float(kSlotFloats) * 8.f);
-  T.part_o = static_cast<float *>(a.scratch);
-  T.part_ml = T.part_o + int64_t(T.slots) * kPairs * D;
   const int64_t blocks = std::max<int64_t>(bound * P.H_kv, T.slots);
   if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
   if (blocks == 0) return MCAMD_OK;
   hipLaunchKernelGGL(paged_mfma_kernel, dim3(unsigned(blocks)), dim3(kThreads), 0, a.stream, P, T);
   const int st = launch_status("paged_mfma");
   if (st != MCAMD_OK || T.slots == 0) return st;
-  return launch_paged_tiles_merge(a, T, P.QT * P.G);
+  return launch_paged_tiles_merge(a, T, P.QT * P.G, bound);
 }
 
 }  // namespace mcamd
