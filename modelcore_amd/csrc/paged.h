@@ -201,6 +201,7 @@ struct PagedTiles {
   int groups;       // of 32 pairs, of a block
   int slots;        // blocks for whose partials there is room, or 0: no block is cut
   float ratio;      // prefill_split.h's, times the blocks of the call
+  int min_tiles;    // of a range, about
   float *part_o;    // [slot][groups of 32 pairs][md][4][64][4], as SplitGeo lays them out
   float *part_ml;   // [slot][groups][32][2]
   struct Cut {      // a block, for the merge
@@ -209,6 +210,12 @@ struct PagedTiles {
   Cut *cuts;        // [slots / 2]: the blocks of a call that may be cut, by their number
   int *n_cuts;      // and how many
 
+  // Ranges of a block of n tiles: what pays for their partials, by the cost rule of prefill_split.h, none
+  // much shorter than what starting it takes.
+  __device__ __forceinline__ int ranges_of(const PagedBlock &v, int n) const {
+    const int most = min(v.most, n / min_tiles), s = int(sqrtf(float(n) * ratio / float(v.n_blocks)));
+    return max(1, min(s, most));
+  }
   // Left for the merge by a call's first workgroup, and by the first range of each block.
   __device__ __forceinline__ void note_call(bool found, const PagedBlock &v) const {
     if (slots > 0) *n_cuts = found && v.most > 1 ? v.n_blocks : 0;
@@ -218,14 +225,18 @@ struct PagedTiles {
   }
 };
 
-// Room for the partials of a workgroup per compute unit, where a call of at most `blocks` blocks can have so
-// few that two ranges of each run side by side, and a block (of at most 256 positions) keys for two. Uniform
-// rows have that many blocks; packed ones mostly fewer than their bound, by up to about four times.
-inline int paged_slots(const PagedArgs &a, int64_t blocks) {
-  const int64_t cus = device_cus(), room = int64_t(a.kv.max_pages) << a.kv.shift;
-  const int64_t keys = a.window < 0 ? room : std::min<int64_t>(room, a.window + 256 + 64);
-  const int64_t most = a.cu ? 2 * cus : cus / 2;  // workgroups of uncut blocks
-  return blocks * a.n_kv_head <= most && keys >= 2 * kMinRangeKeys ? int(cus) : 0;
+// Keys of a block, at most.
+inline int64_t paged_keys(const PagedArgs &a) {
+  const int64_t room = int64_t(a.kv.max_pages) << a.kv.shift;
+  return a.window < 0 ? room : std::min<int64_t>(room, a.window + 256 + 64);
+}
+
+// Room for the partials of `per_cu` workgroups per compute unit, where a call of at most `blocks` blocks can
+// have so few that two ranges of each run side by side, and a block keys for two of min_keys. Uniform rows have that many blocks; packed ones mostly fewer than their bound, by up to about
+// four times.
+inline int paged_slots(const PagedArgs &a, int64_t blocks, int per_cu, int64_t min_keys) {
+  const int64_t slots = int64_t(per_cu) * device_cus();
+  return blocks * a.n_kv_head <= (a.cu ? 2 * slots : slots / 2) && paged_keys(a) >= 2 * min_keys ? int(slots) : 0;
 }
 
 inline size_t paged_tiles_bytes(int64_t slots, int64_t slot_floats) {

@@ -164,7 +164,7 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
   int n_tiles = (hi - lo) / KT + 1;
   bool whole = true;
   if (blk.most > 1) {  // this workgroup's range of the block's tiles
-    const int ranges = best_splits(P.tiles.ratio / float(blk.n_blocks), n_tiles, KT, blk.most);
+    const int ranges = P.tiles.ranges_of(blk, n_tiles);
     if (part >= ranges) return;
     if (part == 0 && tid == 0) P.tiles.note_block(id, blk, ranges);
     whole = ranges == 1;
@@ -553,24 +553,36 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(TiledParams P, in
 // What a call runs: the waves over pairs (KS = 1) or keys (KS = 4), and room for the partials of cut
 // blocks.
 struct TiledPlan {
-  int ks, pairs, kt, slots;
+  int ks, pairs, kt, slots, min_tiles;
   int64_t bound;  // of blocks
   float tile_us;
 };
+constexpr float kShortUs = 30.f;
+constexpr float kRangeUs = 3.f;  // of a range, at least: starting one takes about as long
 TiledPlan tiled_plan(const PagedArgs &a, int64_t skip) {
   const bool bf = a.dtype == MCAMD_BF16;
-  const int64_t cus = device_cus();
-  TiledPlan t;
-  // Fewer workgroups of 128 pairs than compute units: 32 pairs and a quarter of the keys per wave. Head
-  // dims above 128 keep KS = 1 (a tile of four waves' keys outgrows the LDS).
-  t.ks = a.head_dim <= 128 && paged_blocks_bound(a, 128, skip) * a.n_kv_head < cus ? 4 : 1;
-  t.pairs = 128 / t.ks;
-  t.kt = t.ks == 4 ? 128 : bf && a.head_dim <= 128 ? 64 : 32;
-  t.bound = paged_blocks_bound(a, t.pairs, skip);
-  // Measured time of a tile on a compute unit of its own, per head dim (prefill_tiled.hip).
-  t.tile_us = float(a.head_dim) * (t.ks == 4 ? (bf ? 0.027f : 0.085f) : (bf ? 0.012f : 0.035f));
-  t.slots = paged_slots(a, t.bound);
-  return t;
+  auto plan = [&](int ks) {
+    TiledPlan t;
+    t.ks = ks;
+    t.pairs = 128 / ks;
+    t.kt = ks == 4 ? 128 : bf && a.head_dim <= 128 ? 64 : 32;
+    t.bound = paged_blocks_bound(a, t.pairs, skip);
+    // Measured time of a tile on a compute unit of its own, per head dim (prefill_tiled.hip).
+    t.tile_us = float(a.head_dim) * (ks == 4 ? (bf ? 0.027f : 0.085f) : (bf ? 0.012f : 0.035f));
+    t.min_tiles = std::max(1, int(kRangeUs / t.tile_us));
+    t.slots = paged_slots(a, t.bound, a.head_dim <= 128 ? 2 : 1, int64_t(t.min_tiles) * t.kt);
+    return t;
+  };
+  const TiledPlan whole = plan(1);
+  if (a.head_dim > 128) return whole;  // a tile of four waves' keys outgrows the LDS
+  // KS = 4 takes twice to four times as long for the same pairs and keys, and is for calls that cannot fill
+  // the chip otherwise: fewer blocks of 128 pairs than compute units, and rows of so few pairs that half of
+  // such a block would be empty, or too few keys for ranges that are worth their merge (kShortUs).
+  const TiledPlan four = plan(4);
+  const bool fills = whole.bound * a.n_kv_head >= device_cus();
+  const bool few = a.t_new * (a.n_head / a.n_kv_head) <= 64;
+  const bool brief = float(paged_keys(a)) / float(four.kt) * four.tile_us <= kShortUs;
+  return !fills && (few || brief || whole.slots == 0) ? four : whole;
 }
 int64_t slot_floats(const PagedArgs &a, int pairs) {
   return int64_t(pairs) * ((a.head_dim + 31) / 32 * 32 + 2);
@@ -662,6 +674,7 @@ int launch_paged_tiled(const PagedArgs &a, int64_t skip) {
   T.align = 1;
   T.groups = t.pairs / 32;
   paged_tiles_buffers(a, T, t.slots, slot_floats(a, t.pairs), t.pairs * 2);
+  T.min_tiles = t.min_tiles;
   T.ratio = t.tile_us * MCAMD_SPLIT_BYTES_PER_US / (float(slot_floats(a, t.pairs)) * 8.f);
   const TiledParams P = tiled_params(a, T);
   return a.dtype == MCAMD_BF16 ? dispatch<bf16>(P, a, t) : dispatch<float>(P, a, t);

@@ -267,7 +267,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   if constexpr (PAGED) {
     if (blk.most > 1) {
       const int tiles = (hi - lo) / KT + 1;
-      const int ranges = best_splits(T->ratio / float(blk.n_blocks), tiles, KT, blk.most);
+      const int ranges = T->ranges_of(blk, tiles);
       if (part >= ranges) return;
       if (part == 0 && tid == 0) T->note_block(int(blockIdx.x), blk, ranges);
       whole = ranges == 1;
@@ -894,7 +894,8 @@ constexpr int64_t kSlotFloats = int64_t(kPairs) * (D + 2);
 
 size_t paged_mfma_bytes(const PagedArgs &a, int64_t skip) {
   const int64_t G = a.n_head / a.n_kv_head;
-  return paged_tiles_bytes(paged_slots(a, paged_blocks_bound(a, kPairs / G * G, skip)), kSlotFloats);
+  return paged_tiles_bytes(paged_slots(a, paged_blocks_bound(a, kPairs / G * G, skip), 1, kMinRangeKeys),
+                           kSlotFloats);
 }
 
 int launch_paged_mfma(const PagedArgs &a, int64_t skip) {
@@ -923,7 +924,8 @@ int launch_paged_mfma(const PagedArgs &a, int64_t skip) {
   T.kt = T.align = KT;
   T.groups = kWaves;
   const int64_t bound = paged_blocks_bound(a, P.QT * P.G, skip);
-  paged_tiles_buffers(a, T, paged_slots(a, bound), kSlotFloats, kPairs * 2);
+  paged_tiles_buffers(a, T, paged_slots(a, bound, 1, kMinRangeKeys), kSlotFloats, kPairs * 2);
+  T.min_tiles = kMinRangeKeys / KT;
   // A tile of 64 keys takes 256 pairs 1.4 us; a range's partials are written and read.
   T.ratio = 1.4f * MCAMD_SPLIT_BYTES_PER_US / (float(kSlotFloats) * 8.f);
   const int64_t blocks = std::max<int64_t>(bound * P.H_kv, T.slots);
