@@ -15,8 +15,8 @@
 //  * Not finite: a pair whose result is not finite is redone over the keys it sees alone
 //    (careful_pair()), and so is every pair of a block that met a page outside the pool, which leaves
 //    NaN to those that see such a page.
-// Two prompts of 512, 12 heads of 64 in fp32: 31 us (0.81 GFLOP; the contiguous kernel's 30), a tile's loads
-// and its products in series.
+// Two prompts of 512, 12 heads of 64 in fp32: 22.6 us (0.81 GFLOP), with the staged tile in registers (31 with
+// half of it in scratch memory); 344 tokens after 3639, 16 / 4 heads of 256 in bf16: 56 (95).
 #include "paged_careful.h"
 #include "prefill_order.h"
 #include "prefill_split.h"
@@ -37,6 +37,7 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 lds_bf16x4 __attribute__((__vector_size__(4 * sizeof(__bf16))));
 
 struct TiledParams : CarefulParams {
@@ -206,7 +207,7 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
   // The next tile, on its way to LDS (see above where it waits): piece c = tid + 256 i is 16 bytes of key c / (DP / VEC).
   // Keys past `hi` re-read key `hi` (they are masked); K's dims past the head_dim are zero, V's
   // re-read the last ones (they reach no output).
-  uint4 kr[CH], vr[CH];
+  u32x4 kr[CH], vr[CH];  // as uint4, a struct, the compiler keeps V's in scratch memory
   auto load_tile = [&](int k0) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
@@ -215,8 +216,8 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
       const int d = (c % (DP / VEC)) * VEC;
       const int64_t off = P.kv.offset(page[i], P.kv.in_page(key), tok) + min(d, D - VEC);
       lost = lost || !P.kv.is_page(page[i]);
-      kr[i] = *reinterpret_cast<const uint4 *>(kbase + off);
-      vr[i] = *reinterpret_cast<const uint4 *>(vbase + off);
+      kr[i] = *reinterpret_cast<const u32x4 *>(kbase + off);
+      vr[i] = *reinterpret_cast<const u32x4 *>(vbase + off);
     }
   };
   auto store_tile = [&]() {
@@ -225,8 +226,8 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
       const int c = tid + kThreads * i;
       const int key = c / (DP / VEC), d = (c % (DP / VEC)) * VEC;
       // The zeroes go in here and not at the load, all of which would then be waited for at once.
-      *reinterpret_cast<uint4 *>(&sK[key * KSTR + d]) = d < D ? kr[i] : make_uint4(0, 0, 0, 0);
-      *reinterpret_cast<uint4 *>(&sV[key * VSTR + d]) = vr[i];
+      *reinterpret_cast<u32x4 *>(&sK[key * KSTR + d]) = d < D ? kr[i] : u32x4{0, 0, 0, 0};
+      *reinterpret_cast<u32x4 *>(&sV[key * VSTR + d]) = vr[i];
     }
   };
 
