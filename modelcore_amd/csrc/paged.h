@@ -252,14 +252,14 @@ inline void paged_tiles_buffers(const PagedArgs &a, PagedTiles &t, int64_t slots
   t.n_cuts = reinterpret_cast<int *>(t.cuts + t.slots / 2);
 }
 
-int launch_paged_append(const PagedArgs &a);
-// Rows of few pairs (few_pairs(.., most)) of a bf16 call: append where k_new is given, and attention.
-int launch_paged_stream(const PagedArgs &a, int64_t most);
+// Rows of few pairs (few_pairs(.., most)) of a bf16 call: append where k_new is given, with `others` of the
+// other rows too, and attention.
+int launch_paged_stream(const PagedArgs &a, int64_t most, bool others);
 size_t paged_stream_bytes(const PagedArgs &a, int64_t most);  // of scratch, to cut long rows' keys
 // Single tokens of an fp32 call, the same.
-int launch_paged_stream_f32(const PagedArgs &a);
+int launch_paged_stream_f32(const PagedArgs &a, bool others);
 size_t paged_stream_f32_bytes(const PagedArgs &a);
-// Every row but those.
+// Every row but those, whose new tokens are in their pages.
 int launch_paged_tiled(const PagedArgs &a, int64_t skip);
 size_t paged_tiled_bytes(const PagedArgs &a, int64_t skip);
 // The same for bf16 and head_dim 128.

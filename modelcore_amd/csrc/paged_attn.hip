@@ -1,6 +1,6 @@
 // The attention operator over a paged cache: its argument checks, the append of new tokens into
 // their pages, and which kernels a call takes.
-#include "paged.h"
+#include "paged_append.h"
 
 #include <algorithm>
 #include <cmath>
@@ -8,61 +8,8 @@
 namespace mcamd {
 namespace {
 
-constexpr int kThreads = 256;
-
-// New tokens' K and V into their pages, bit for bit: kTokens tokens a workgroup, whose places its
-// first threads find, then 16-byte pieces by all of them. A row that does not fit its line of the
-// table, and a token whose page is outside the pool, are passed over.
-constexpr int kTokens = 8;
-
-struct PagedAppend {
-  const uint4 *k, *v;
-  uint4 *k_pages, *v_pages;
-  PagedKv kv;  // page_stride in pieces
-  const int32_t *seqlens, *cu;
-  int n_rows, t_new, total, units;
-};
-
-__global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedAppend A) {
-  __shared__ int64_t s_at[kTokens];
-  const int t0 = blockIdx.x * kTokens;
-  if (threadIdx.x < kTokens) {
-    const int t = t0 + threadIdx.x;
-    int64_t at = -1;
-    if (t < A.total) {
-      int b, tok0, T;
-      if (A.cu) {
-        int lo = 0, hi = A.n_rows;  // the last row that begins at or before t
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (A.cu[mid] <= t)
-            lo = mid;
-          else
-            hi = mid;
-        }
-        b = lo;
-      } else {
-        b = t / A.t_new;
-      }
-      row_tokens(A.cu, A.t_new, A.total, b, tok0, T);
-      const int64_t s0 = A.seqlens[b], pos = s0 + (t - tok0);
-      if (t >= tok0 && t < tok0 + T && s0 >= 0 && s0 + T <= int64_t(A.kv.max_pages) << A.kv.shift) {
-        const int id = A.kv.table[b * A.kv.table_stride + (pos >> A.kv.shift)];
-        if (A.kv.is_page(id)) at = A.kv.offset(id, A.kv.in_page(int(pos)), A.units);
-      }
-    }
-    s_at[threadIdx.x] = at;
-  }
-  __syncthreads();
-  const int n = min(kTokens, A.total - t0) * A.units;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const int t = i / A.units, u = i - t * A.units;
-    const int64_t at = s_at[t], from = (int64_t(t0) + t) * A.units + u;
-    if (at < 0) continue;
-    const uint4 x = A.k[from], y = A.v[from];
-    A.k_pages[at + u] = x;
-    A.v_pages[at + u] = y;
-  }
+__global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(PagedAppend A) {
+  append_tokens(A, blockIdx.x);
 }
 
 int check(const PagedArgs &a) {
@@ -104,15 +51,25 @@ Kernels kernels_of(const PagedArgs &a) {
   return {few || a.cu != nullptr, !few};
 }
 
+// New tokens of a mixed call up to which the streaming kernel's launch appends those of the long rows too.
+// Three rows of 97 tokens 12.6 us in two launches, 10.4 in one; 60 single tokens beside four chunks, 2100
+// tokens, 171 and 179, eight prompts of 16384 18 and 23: more workgroups stand in the way of ranges that
+// are all to be on the chip at once.
+constexpr int64_t kAppendWithin = 512;
+
 int launch(PagedArgs a) {
   const Kernels k = kernels_of(a);
-  if (a.k_new && k.tiles) {  // the streaming kernel appends by itself
-    const int st = launch_paged_append(a);
+  const bool within = k.stream && (!k.tiles || a.total <= kAppendWithin);
+  if (a.k_new && !within) {
+    hipLaunchKernelGGL(paged_append_kernel, dim3(unsigned(paged_append_blocks(a))), dim3(kAppendThreads), 0,
+                       a.stream, paged_append(a, 0));
+    const int st = launch_status("paged_append");
     if (st != MCAMD_OK) return st;
     a.k_new = a.v_new = nullptr;
   }
   if (k.stream) {
-    const int st = a.dtype == MCAMD_BF16 ? launch_paged_stream(a, few_of(a)) : launch_paged_stream_f32(a);
+    const int st = a.dtype == MCAMD_BF16 ? launch_paged_stream(a, few_of(a), k.tiles)
+                                         : launch_paged_stream_f32(a, k.tiles);
     if (st != MCAMD_OK || !k.tiles) return st;
   }
   const int64_t skip = k.stream ? few_of(a) : 0;
@@ -120,27 +77,6 @@ int launch(PagedArgs a) {
 }
 
 }  // namespace
-
-int launch_paged_append(const PagedArgs &a) {
-  const int64_t elem = a.dtype == MCAMD_F32 ? 4 : 2;
-  PagedAppend A;
-  A.k = static_cast<const uint4 *>(a.k_new);
-  A.v = static_cast<const uint4 *>(a.v_new);
-  A.k_pages = static_cast<uint4 *>(a.k_pages);
-  A.v_pages = static_cast<uint4 *>(a.v_pages);
-  A.kv = a.kv;
-  A.kv.page_stride = a.kv.page_stride * elem / 16;
-  A.seqlens = a.seqlens;
-  A.cu = a.cu;
-  A.n_rows = int(a.n_rows);
-  A.t_new = int(a.t_new);
-  A.total = int(a.total);
-  A.units = int(a.n_kv_head * a.head_dim * elem / 16);
-  const int64_t blocks = (a.total + kTokens - 1) / kTokens;
-  hipLaunchKernelGGL(paged_append_kernel, dim3(unsigned(blocks)), dim3(kThreads), 0, a.stream, A);
-  return launch_status("paged_append");
-}
-
 }  // namespace mcamd
 
 using namespace mcamd;

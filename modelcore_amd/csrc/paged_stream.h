@@ -9,6 +9,7 @@
 // itself, 64 rows at a time.
 #pragma once
 
+#include "paged_append.h"
 #include "paged_careful.h"
 
 #include <algorithm>
@@ -38,6 +39,8 @@ struct StreamParams : CarefulParams {
   int head_waves;  // KV heads of a workgroup, in a large call
   int target;      // workgroups a call aims at; 0: no row is cut
   int pair_slots;  // pairs per partial slot
+  PagedAppend append;
+  int blocks;      // workgroups from that one on append
 };
 
 // The rows' shares of a call. A row has `blocks` blocks of PB pairs and `tiles` tiles; a range is at most
@@ -305,14 +308,17 @@ StreamParams stream_params(const PagedArgs &a, const StreamPlan &p, int64_t most
   P.head_waves = p.head_waves;
   P.target = p.cut ? p.target : 0;
   P.pair_slots = p.pair_slots;
+  P.append = paged_append(a, most);
+  // A KV head at a time, or up to the target.
+  P.blocks = int(std::min<int64_t>(
+      p.units * a.n_kv_head + (p.cut ? std::max<int64_t>(p.target, a.n_kv_head) : 0), 0x7fffffff));
   return P;
 }
 
 // kernel: the launch of a call's ranges, by E, DP (head dims, rounded up) and blocks of PB pairs.
 template <class E, int DP, int PB, class K>
-int launch_stream(K kernel, const StreamParams &P, const PagedArgs &a, const StreamPlan &p) {
-  // A KV head at a time, or up to the target.
-  const int64_t blocks = p.units * a.n_kv_head + (p.cut ? std::max<int64_t>(p.target, a.n_kv_head) : 0);
+int launch_stream(K kernel, const StreamParams &P, const PagedArgs &a, const StreamPlan &p, bool others) {
+  const int64_t blocks = P.blocks + (a.k_new && others ? paged_append_blocks(a) : 0);
   if (blocks > 0x7fffffff / kThreads || a.n_rows > 65535)
     return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
   hipLaunchKernelGGL(kernel, dim3(unsigned(blocks)), dim3(kThreads), 0, a.stream, P);

@@ -139,6 +139,7 @@ __global__ __launch_bounds__(kThreads)
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // This workgroup's heads, row, block of pairs and range.
+  if (int(blockIdx.x) >= P.blocks) return append_tokens(P.append, int(blockIdx.x) - P.blocks);
   Row R;
   const Range mine = find_range<kPairs>(P, lane, R);
   if (mine.b < 0) return;
@@ -507,15 +508,15 @@ size_t paged_stream_bytes(const PagedArgs &a, int64_t most) {
   return stream_bytes(a, stream_plan(a, most, kPairs, kFill));
 }
 
-int launch_paged_stream(const PagedArgs &a, int64_t most) {
+int launch_paged_stream(const PagedArgs &a, int64_t most, bool others) {
   StreamPlan p = stream_plan(a, most, kPairs, kFill);
   if (p.cut && (!a.scratch || a.scratch_bytes < stream_bytes(a, p))) p.cut = false;
   const StreamParams P = stream_params(a, p, most);
   switch (head_pad(a.head_dim)) {
-    case 32: return launch_stream<bf16, 32, kPairs>(paged_stream_kernel<32>, P, a, p);
-    case 64: return launch_stream<bf16, 64, kPairs>(paged_stream_kernel<64>, P, a, p);
-    case 128: return launch_stream<bf16, 128, kPairs>(paged_stream_kernel<128>, P, a, p);
-    default: return launch_stream<bf16, 256, kPairs>(paged_stream_kernel<256>, P, a, p);
+    case 32: return launch_stream<bf16, 32, kPairs>(paged_stream_kernel<32>, P, a, p, others);
+    case 64: return launch_stream<bf16, 64, kPairs>(paged_stream_kernel<64>, P, a, p, others);
+    case 128: return launch_stream<bf16, 128, kPairs>(paged_stream_kernel<128>, P, a, p, others);
+    default: return launch_stream<bf16, 256, kPairs>(paged_stream_kernel<256>, P, a, p, others);
   }
 }
 

@@ -65,6 +65,7 @@ __global__ __launch_bounds__(kThreads)
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (int(blockIdx.x) >= P.blocks) return append_tokens(P.append, int(blockIdx.x) - P.blocks);
   Row R;
   const Range mine = find_range<GP>(P, lane, R);
   if (mine.b < 0) return;
@@ -263,12 +264,12 @@ __global__ __launch_bounds__(kThreads)
 }
 
 template <int GP>
-int run(const StreamParams &P, const PagedArgs &a, const StreamPlan &p) {
+int run(const StreamParams &P, const PagedArgs &a, const StreamPlan &p, bool others) {
   switch (head_pad(a.head_dim)) {
-    case 32: return launch_stream<float, 32, GP>(paged_stream_f32_kernel<32, GP>, P, a, p);
-    case 64: return launch_stream<float, 64, GP>(paged_stream_f32_kernel<64, GP>, P, a, p);
-    case 128: return launch_stream<float, 128, GP>(paged_stream_f32_kernel<128, GP>, P, a, p);
-    default: return launch_stream<float, 256, GP>(paged_stream_f32_kernel<256, GP>, P, a, p);
+    case 32: return launch_stream<float, 32, GP>(paged_stream_f32_kernel<32, GP>, P, a, p, others);
+    case 64: return launch_stream<float, 64, GP>(paged_stream_f32_kernel<64, GP>, P, a, p, others);
+    case 128: return launch_stream<float, 128, GP>(paged_stream_f32_kernel<128, GP>, P, a, p, others);
+    default: return launch_stream<float, 256, GP>(paged_stream_f32_kernel<256, GP>, P, a, p, others);
   }
 }
 
@@ -286,14 +287,14 @@ StreamPlan plan_of(const PagedArgs &a) {
 
 size_t paged_stream_f32_bytes(const PagedArgs &a) { return stream_bytes(a, plan_of(a)); }
 
-int launch_paged_stream_f32(const PagedArgs &a) {
+int launch_paged_stream_f32(const PagedArgs &a, bool others) {
   StreamPlan p = plan_of(a);
   if (p.cut && (!a.scratch || a.scratch_bytes < stream_bytes(a, p))) p.cut = false;
   const StreamParams P = stream_params(a, p, 1);
   switch (heads_of(a)) {
-    case 1: return run<1>(P, a, p);
-    case 2: return run<2>(P, a, p);
-    default: return run<4>(P, a, p);
+    case 1: return run<1>(P, a, p, others);
+    case 2: return run<2>(P, a, p, others);
+    default: return run<4>(P, a, p, others);
   }
 }
 

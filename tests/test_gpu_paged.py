@@ -146,6 +146,22 @@ def test_long_rows_are_cut(dtype, H, H_kv, D):
     run_attention([2100], [1], H, H_kv, D, 16, dtype, window=1500)
 
 
+@pytest.mark.parametrize("dtype,H,H_kv,D", [(BF, 8, 2, 128), (BF, 8, 2, 64), (F32, 8, 2, 64), (BF, 6, 2, 96)])
+def test_long_chunks_of_few_rows(dtype, H, H_kv, D):
+    """Blocks of many pairs that are cut, rows that end inside one, more new tokens than one launch appends."""
+    run_attention([1900], [150], H, H_kv, D, 16, dtype)
+    run_attention([1500, 0, 300], [200, 33, 90], H, H_kv, D, 32, dtype, pad=3)
+    run_attention([1800], [70], H, H_kv, D, 16, dtype, window=1200)
+    run_attention([30, 200, 900, 0, 5], [1, 400, 2, 0, 130], H, H_kv, D, 16, dtype)
+
+
+@pytest.mark.parametrize("dtype,T", [(BF, 7), (F32, 1)])
+def test_many_rows_of_a_few_tokens_are_cut(dtype, T):
+    """More pairs than the merge has workgroups for."""
+    run_attention([500 + 3 * b for b in range(90)], [T - b % 2 if T > 1 else 1 for b in range(90)], 16, 4, 64, 16,
+                  dtype, packed=True)
+
+
 @pytest.mark.parametrize("dtype,D", [(BF, 128), (BF, 64), (F32, 64)])
 def test_without_append(dtype, D):
     run_attention([30, 100, 0], [1, 20, 5], 4, 2, D, 16, dtype, append=False)
