@@ -56,7 +56,7 @@ __device__ __forceinline__ void row_tokens(const int32_t *cu, int t_new, int tot
 // Whether a row of T new tokens is one of few pairs, which the streaming kernels take: a single token, or
 // at most `most` (token, head) pairs per KV head; most = 0: none is.
 __device__ __forceinline__ bool few_pairs(int T, int G, int most) {
-  return most > 0 && (T == 1 || int64_t(T) * G <= most);
+  return most > 0 && (T == 1 || T * G <= most);  // a call's pairs per KV head fit 30 bits
 }
 
 // A block of queries of a row: its block qt, the row's tokens and its position.
@@ -82,16 +82,18 @@ struct PagedCall {
   const int32_t *cu, *seqlens;
   int n_rows, t_new, total, G, H_kv, pairs, skip, slots;
   __device__ __forceinline__ int blocks_of(int T) const {
-    return few_pairs(T, G, skip) ? 0 : int((int64_t(T) * G + pairs - 1) / pairs);
+    return few_pairs(T, G, skip) ? 0 : int((uint32_t(T * G) + uint32_t(pairs) - 1) / uint32_t(pairs));
   }
   // The key range that i is of, and i's block; false past the last.
   __device__ __forceinline__ bool range_of(int blocks, int &i, PagedBlock &v) const {
-    if (blocks == 0) return false;
     v.n_blocks = blocks * H_kv;
-    v.most = max(1, min(slots / v.n_blocks, kMaxPagedSplits));
-    v.part = i / blocks;
-    i -= v.part * blocks;
-    return v.part < v.most;
+    v.part = 0, v.most = 1;
+    if (blocks > 0 && slots >= 2 * v.n_blocks) {
+      v.most = min(slots / v.n_blocks, kMaxPagedSplits);
+      v.part = i / blocks;
+      i -= v.part * blocks;
+    }
+    return i < blocks && v.part < v.most;
   }
 };
 
