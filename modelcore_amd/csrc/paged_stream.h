@@ -58,7 +58,7 @@ __device__ __forceinline__ Row row_of(const StreamParams &P, int b) {
   r.ok = r.s0 >= 0 && int64_t(r.s0) + r.T <= int64_t(P.kv.max_pages) << P.kv.shift;
   r.lo = r.ok && P.window >= 0 ? max(0, r.s0 - P.window) : 0;
   r.hi = r.ok ? r.s0 + r.T - 1 : 0;
-  r.blocks = few_pairs(r.T, P.G, P.most) ? int((int64_t(r.T) * P.G + PB - 1) / PB) : 0;
+  r.blocks = few_pairs(r.T, P.G, P.most) ? int(uint32_t(r.T * P.G + PB - 1) / PB) : 0;
   r.tiles = r.ok ? (r.hi / KT) - (r.lo / KT) + 1 : 1;
   return r;
 }
@@ -89,21 +89,21 @@ __device__ __forceinline__ Cut cut_of(const StreamParams &P, int lane, const Row
     work += int64_t(r.blocks) * r.tiles;
     units += r.blocks;
   }
-  if (__builtin_amdgcn_ballot_w64(work >= (1 << 24)) == 0) {  // the sums fit 32 bits
-    work = wave_total(int(work));
-    units = wave_total(int(units));
-  } else {
-    work = wave_total64(work);
-    units = wave_total64(units);
-  }
   if (P.target == 0) return Cut{1, 0x7fffffff};
   Cut c;
-  c.head_waves = work * P.H_kv > int64_t(kDeepTiles * kWaves) * P.target ? P.head_waves : 1;
-  // A row's last range may be shorter than the others: work / len ranges and up to one per block of pairs
-  // more, all of which are to be on the chip at once.
-  const int target = max(1, P.target * c.head_waves / P.H_kv);
-  const int64_t most = max(target - units, int64_t(target + 1) / 2);
-  c.len = int(max((work + most - 1) / most, int64_t(kMinTiles * kWaves / c.head_waves)));
+  auto cut = [&](auto work, auto units) {
+    using T = decltype(work);
+    c.head_waves = int64_t(work) * P.H_kv > int64_t(kDeepTiles * kWaves) * P.target ? P.head_waves : 1;
+    // A row's last range may be shorter than the others: work / len ranges and up to one per block of pairs
+    // more, all of which are to be on the chip at once.
+    const int target = max(1, int(uint32_t(P.target * c.head_waves) / uint32_t(P.H_kv)));
+    const T most = units < T(target / 2) ? T(target) - units : T((target + 1) / 2);
+    c.len = int(max((work + most - 1) / most, T(kMinTiles * kWaves) / T(c.head_waves)));
+  };
+  if (__builtin_amdgcn_ballot_w64(work >= (1 << 24)) == 0)  // the sums fit 32 bits
+    cut(uint32_t(wave_total(int(work))), uint32_t(wave_total(int(units))));
+  else
+    cut(uint64_t(wave_total64(work)), uint64_t(wave_total64(units)));
   c.head_waves = __builtin_amdgcn_readfirstlane(c.head_waves);  // so the compiler knows as well
   c.len = __builtin_amdgcn_readfirstlane(c.len);
   return c;
@@ -116,6 +116,7 @@ __device__ __forceinline__ int ranges_of(const Row &r, int len) {
 // which of the row's ranges.
 struct Range {
   int head_waves, n_groups, group, b, block, range, ranges;
+  int t0, t1;  // its tiles, from the row's first one on
 };
 template <int PB>
 __device__ __forceinline__ Range find_range(const StreamParams &P, int lane, Row &R) {
@@ -153,8 +154,12 @@ __device__ __forceinline__ Range find_range(const StreamParams &P, int lane, Row
     break;
   }
   if (v.b < 0) return v;
-  v.block = id / v.ranges;
+  v.block = int(uint32_t(id) / uint32_t(v.ranges));
   v.range = id - v.block * v.ranges;
+  // Tiles from range * tiles / ranges on, of the row's.
+  const uint32_t each = uint32_t(R.tiles) / uint32_t(v.ranges), rest = R.tiles - each * v.ranges;
+  v.t0 = int(each * v.range + rest * v.range / v.ranges);
+  v.t1 = int(each * (v.range + 1) + rest * (v.range + 1) / v.ranges);
   if (id == 0 && v.group == 0 && threadIdx.x == 0 && P.where)
     P.where[v.b] = make_int2(int(blockIdx.x / v.n_groups), v.ranges);
   return v;

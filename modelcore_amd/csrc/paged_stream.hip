@@ -168,8 +168,7 @@ __global__ __launch_bounds__(kThreads)
   const int t_first = block * 32 / P.G, t_last = min(block * 32 + 31, pairs - 1) / P.G;
   const int p_abs = R.s0 + t_q;
   const int first_tile = R.lo / KT;
-  const int t0 = first_tile + int(int64_t(range) * R.tiles / ranges);
-  const int t1 = first_tile + int(int64_t(range + 1) * R.tiles / ranges);  // past the last tile
+  const int t0 = first_tile + mine.t0, t1 = first_tile + mine.t1;
 
   const uint16_t *q = static_cast<const uint16_t *>(P.q) + at;
   bf16x8 qf[KD];

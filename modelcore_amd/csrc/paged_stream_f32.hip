@@ -92,8 +92,7 @@ __global__ __launch_bounds__(kThreads)
   }
 
   const int first_tile = R.lo / KT;
-  const int t0 = first_tile + int(int64_t(mine.range) * R.tiles / ranges);
-  const int t1 = first_tile + int(int64_t(mine.range + 1) * R.tiles / ranges);  // past the last tile
+  const int t0 = first_tile + mine.t0, t1 = first_tile + mine.t1;
   const int seen_from = R.lo, s0 = R.s0;  // the keys the token sees, itself the last
   const bool fresh = P.k_new != nullptr;
   const int tok_bytes = P.H_kv * D * 4;
