@@ -1,5 +1,7 @@
 """The paged KV cache's operators on the GPU against plain 64-bit forms: pages and slots, the
 pre-attention step by slot, and attention over pages for single tokens, chunks and mixtures of them."""
+import random
+
 import pytest
 import torch
 
@@ -160,6 +162,33 @@ def test_many_rows_of_a_few_tokens_are_cut(dtype, T):
     """More pairs than the merge has workgroups for."""
     run_attention([500 + 3 * b for b in range(90)], [T - b % 2 if T > 1 else 1 for b in range(90)], 16, 4, 64, 16,
                   dtype, packed=True)
+
+
+@pytest.mark.parametrize("seed", range(48))
+def test_random_calls(seed):
+    """Rows, heads, pages, windows and lengths at random, every third seed of bf16 / 128."""
+    rng = random.Random(seed)
+    dtype = rng.choice([BF, BF, F32])
+    D = rng.choice([8, 16, 24, 40, 64, 64, 72, 96, 128, 136, 192, 256])
+    if seed % 3 == 0:
+        dtype, D = BF, 128
+    G = rng.choice([1, 1, 2, 3, 4, 5, 7, 8, 16, 64])
+    H_kv = rng.choice([1, 2, 3, 4, 8]) if G < 16 else 1
+    rows = rng.choice([1, 2, 5, 9, 30, 70])
+    deep = rng.choice([30, 200, 900, 2500 if rows < 9 else 300])
+    pos = [rng.randint(0, deep) for _ in range(rows)]
+    kind = rng.choice(["ones", "same", "mixed", "mixed", "mixed"])
+    if kind == "ones":
+        new = [1] * rows
+    elif kind == "same":
+        new = [rng.randint(1, 300 // rows + 1)] * rows
+    else:
+        new = [rng.choice([0, 1, 1, 1, rng.randint(2, 9), rng.randint(1, 240 // rows + 2)]) for _ in range(rows)]
+    if sum(new) == 0:
+        new[0] = 1
+    run_attention(pos, new, G * H_kv, H_kv, D, rng.choice([16, 16, 32, 64, 256 if rows > 5 else 1024]), dtype,
+                  window=rng.choice([-1, -1, 0, 5, 33, 300]), append=rng.random() < 0.8, seed=seed,
+                  pad=rng.choice([0, 0, 3]), packed=True if rng.random() < 0.3 else None)
 
 
 @pytest.mark.parametrize("dtype,D", [(BF, 128), (BF, 64), (F32, 64)])
