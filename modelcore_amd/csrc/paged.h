@@ -64,7 +64,19 @@ struct PagedBlock {
   int b, qt, tok0, T, s0;
   int n_blocks;    // of the whole call, its KV heads counted
   int part, most;  // which key range of the block, of how many at most
+  bool noted;      // blocks of the call may be cut: the merge is told what each has become
+  int half;        // the block is cut in two, whose second range is number `half` of the call; else -1
 };
+
+// Inclusive sum over the wave.
+__device__ __forceinline__ int wave_upto(int x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
 
 // Block i of a call, blocks with the most keys first: by their number within their row, last first,
 // and rows in order within a number, so that long rows do not fall to one XCD. `pairs` (position,
@@ -74,24 +86,41 @@ struct PagedBlock {
 // found row's numbers read again from memory, and R = 4 for eight rows too, eight prompts of 37 to 4001
 // tokens took 2% longer.)
 //
-// Where the partials of `slots` blocks have room, fewer blocks than half of that may be cut into key
-// ranges: the first ranges of all blocks come first, then the second ones, and so on.
+// Where the partials of `slots` blocks have room, at most half as many blocks may be cut into key
+// ranges: the first ranges of all blocks come first, then the second ones, and so on. With more blocks, of
+// packed rows without a window, the deepest ones are cut in two, as many as there are slots left, none of
+// half the deepest's keys or less: their second ranges come after all first ones, without gaps, since
+// workgroups are dealt to the chip's parts in turn and one that finds no room in its part holds up all
+// behind it.
 constexpr int kMaxPagedSplits = 32;
 
 struct PagedCall {
   const int32_t *cu, *seqlens;
-  int n_rows, t_new, total, G, H_kv, pairs, skip, slots;
+  int n_rows, t_new, total, G, H_kv, pairs, skip, slots, room, halve;
+  // The keys of a row's last block, and of its block qt; 0 for a row that does not fit its line.
+  __device__ __forceinline__ int depth_of(int T, int s0) const { return s0 >= 0 && s0 <= room - T ? s0 + T : 0; }
+  __device__ __forceinline__ int depth_of(int T, int s0, int qt) const {
+    return depth_of(T, s0) == 0 ? 0 : s0 + min(int(uint32_t(qt + 1) * uint32_t(pairs) / uint32_t(G)), T);
+  }
+  // Blocks of a row, its last ones, that have more than `keys` keys.
+  __device__ __forceinline__ int deeper(int T, int s0, int blocks, int keys) const {
+    if (blocks == 0 || depth_of(T, s0) <= keys) return 0;
+    const int from = max(keys - s0 + 1, 0);  // at most T
+    const int shallow = int((uint32_t(from) * uint32_t(G) + uint32_t(pairs) - 1) / uint32_t(pairs)) - 1;
+    return blocks - max(shallow, 0);
+  }
   __device__ __forceinline__ int blocks_of(int T) const {
     return few_pairs(T, G, skip) ? 0 : int((uint32_t(T * G) + uint32_t(pairs) - 1) / uint32_t(pairs));
   }
   // The key range that i is of, and i's block; false past the last.
   __device__ __forceinline__ bool range_of(int blocks, int &i, PagedBlock &v) const {
     v.n_blocks = blocks * H_kv;
-    v.part = 0, v.most = 1;
+    v.part = 0, v.most = 1, v.half = -1, v.noted = false;
     if (blocks > 0 && slots >= 2 * v.n_blocks) {
       v.most = min(slots / v.n_blocks, kMaxPagedSplits);
       v.part = i / blocks;
       i -= v.part * blocks;
+      v.noted = true;
     }
     return i < blocks && v.part < v.most;
   }
@@ -125,7 +154,59 @@ __device__ __forceinline__ bool find_packed_block(const PagedCall &c, int i, int
     for (int b = 64 * R + lane; b < c.n_rows; b += 64) n += max(far(b) - k, 0);
     return wave_total(n);
   };
-  if (!c.range_of(from(0), i, v)) return false;
+  const int blocks = from(0);
+  const int spare = c.halve > 0 && c.n_rows <= 64 * R && c.slots < 2 * blocks * c.H_kv
+                        ? (c.slots - blocks * c.H_kv) / c.H_kv : 0;
+  const bool fits = c.range_of(blocks, i, v);
+  int keys = 0, cut[R];  // blocks of more keys are cut in two: so many of each row
+  if (spare > 0) {
+    v.noted = true;
+    int deep = 0;
+#pragma unroll
+    for (int u = 0; u < R; ++u) deep = max(deep, mine[u] > 0 ? c.depth_of(T[u], s0[u]) : 0);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) deep = max(deep, __shfl_xor(deep, o, 64));
+    deep = __builtin_amdgcn_readfirstlane(deep);
+    auto all = [&](int k) {
+      int n = 0;
+#pragma unroll
+      for (int u = 0; u < R; ++u) n += cut[u] = c.deeper(T[u], s0[u], mine[u], k);
+      return wave_total(n);
+    };
+    int under = max(deep >> 1, c.halve - 1);
+    keys = max(deep, under);
+    for (int step = 0; step < 5 && keys - under > 1; ++step) {
+      const int mid = (under + keys) >> 1;
+      if (all(mid) <= spare)
+        keys = mid;
+      else
+        under = mid;
+    }
+    const int halves = all(keys);
+    if (!fits) {  // the second range of one of them
+      int nth = i - blocks;
+      if (nth >= halves) return false;
+      v.part = 1, v.most = 2, v.half = i;
+#pragma unroll
+      for (int u = 0; u < R; ++u) {
+        const int upto = wave_upto(cut[u], lane);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(upto > nth);
+        if (past == 0) {
+          nth -= __builtin_amdgcn_readlane(upto, 63);
+          continue;
+        }
+        const int l = __builtin_ctzll(past);
+        v.b = 64 * u + l;
+        v.tok0 = __builtin_amdgcn_readlane(tok0[u], l);
+        v.T = __builtin_amdgcn_readlane(T[u], l);
+        v.s0 = __builtin_amdgcn_readlane(s0[u], l);
+        v.qt = __builtin_amdgcn_readlane(mine[u], l) - 1 - (nth - __builtin_amdgcn_readlane(upto - cut[u], l));
+        return true;
+      }
+      return false;
+    }
+  }
+  if (!fits) return false;
   for (int b = 64 * R + lane; b < c.n_rows; b += 64) deepest = max(deepest, far(b));
   int lo = 0, hi = 1;  // more than i blocks from lo on; at most i from hi on
   while (__builtin_amdgcn_ballot_w64(deepest > hi) != 0 && from(hi) > i) lo = hi, hi *= 2;
@@ -159,7 +240,16 @@ __device__ __forceinline__ bool find_packed_block(const PagedCall &c, int i, int
     v.T = __builtin_amdgcn_readlane(T[u], l);
     v.s0 = __builtin_amdgcn_readlane(s0[u], l);
   }
-  if (v.b >= 0) return true;
+  if (v.b >= 0) {
+    if (spare > 0 && c.depth_of(v.T, v.s0, v.qt) > keys) {
+      int before = 0;  // halves of rows before it
+#pragma unroll
+      for (int u = 0; u < R; ++u) before += 64 * u + lane < v.b ? cut[u] : 0;
+      v.most = 2;
+      v.half = blocks + wave_total(before) + c.blocks_of(v.T) - 1 - v.qt;
+    }
+    return true;
+  }
   for (int b0 = 64 * R; b0 < c.n_rows; b0 += 64) {
     const int l = look(far(b0 + lane));
     if (l < 0) continue;
@@ -173,9 +263,17 @@ __device__ __forceinline__ bool find_packed_block(const PagedCall &c, int i, int
 
 __device__ __forceinline__ bool find_paged_block(const int32_t *cu, const int32_t *seqlens, int n_rows,
                                                  int t_new, int total, int G, int H_kv, int pairs,
-                                                 int skip, int slots, int i, int lane, PagedBlock &v) {
-  const PagedCall c{cu, seqlens, n_rows, t_new, total, G, H_kv, pairs, skip, slots};
-  if (cu) return n_rows <= 64 ? find_packed_block<1>(c, i, lane, v) : find_packed_block<4>(c, i, lane, v);
+                                                 int skip, int slots, int room, int halve, int i,
+                                                 int lane, PagedBlock &v) {
+  const PagedCall c{cu, seqlens, n_rows, t_new, total, G, H_kv, pairs, skip, slots, room, halve};
+  if (cu) {
+    const bool found =
+        n_rows <= 64 ? find_packed_block<1>(c, i, lane, v) : find_packed_block<4>(c, i, lane, v);
+    for (int *x : {&v.b, &v.qt, &v.tok0, &v.T, &v.s0, &v.n_blocks, &v.part, &v.most, &v.half})
+      *x = __builtin_amdgcn_readfirstlane(*x);  // so the compiler knows as well
+    v.noted = __builtin_amdgcn_readfirstlane(v.noted);
+    return __builtin_amdgcn_readfirstlane(found);
+  }
   const int each = c.blocks_of(t_new);
   if (!c.range_of(each * n_rows, i, v)) return false;
   v.qt = each - 1 - i / n_rows;
@@ -204,26 +302,29 @@ struct PagedTiles {
   int slots;        // blocks for whose partials there is room, or 0: no block is cut
   float ratio;      // prefill_split.h's, times the blocks of the call
   int min_tiles;    // of a range, about
+  int halve;        // keys from which on a block may be cut in two, or 0: none is
   float *part_o;    // [slot][groups of 32 pairs][md][4][64][4], as SplitGeo lays them out
   float *part_ml;   // [slot][groups][32][2]
   struct Cut {      // a block, for the merge
-    int b, qt, tok0, T, s0, ranges, unused[2];
+    int b, qt, tok0, T, s0, ranges, second, unused;  // second: the slot of its second range
   };
-  Cut *cuts;        // [slots / 2]: the blocks of a call that may be cut, by their number
+  Cut *cuts;        // [slots]: the blocks of a call that may be cut, by their number
   int *n_cuts;      // and how many
 
   // Ranges of a block of n tiles: what pays for their partials, by the cost rule of prefill_split.h, none
   // much shorter than what starting it takes.
   __device__ __forceinline__ int ranges_of(const PagedBlock &v, int n) const {
+    if (v.half >= 0) return 2;
     const int most = min(v.most, n / min_tiles), s = int(sqrtf(float(n) * ratio / float(v.n_blocks)));
     return max(1, min(s, most));
   }
   // Left for the merge by a call's first workgroup, and by the first range of each block.
   __device__ __forceinline__ void note_call(bool found, const PagedBlock &v) const {
-    if (slots > 0) *n_cuts = found && v.most > 1 ? v.n_blocks : 0;
+    if (slots > 0) *n_cuts = found && v.noted ? v.n_blocks : 0;
   }
-  __device__ __forceinline__ void note_block(int id, const PagedBlock &v, int ranges) const {
-    cuts[id] = Cut{v.b, v.qt, v.tok0, v.T, v.s0, ranges, {0, 0}};
+  __device__ __forceinline__ void note_block(int id, const PagedBlock &v, int ranges, int H_kv) const {
+    cuts[id] = Cut{v.b, v.qt, v.tok0, v.T, v.s0, ranges,
+                   v.half >= 0 ? v.half * H_kv + id % H_kv : id + v.n_blocks, 0};
   }
 };
 
@@ -234,15 +335,16 @@ inline int64_t paged_keys(const PagedArgs &a) {
 }
 
 // Room for the partials of `per_cu` workgroups per compute unit, where a call of at most `blocks` blocks can
-// have so few that two ranges of each run side by side, and a block keys for two of min_keys. Uniform rows have that many blocks; packed ones mostly fewer than their bound, by up to about
-// four times.
-inline int paged_slots(const PagedArgs &a, int64_t blocks, int per_cu, int64_t min_keys) {
+// have so few that ranges of some run side by side, and a block keys for two of min_keys. Uniform rows have
+// that many blocks, packed ones about as many as their tokens fill, or more.
+inline int paged_slots(const PagedArgs &a, int64_t blocks, int64_t pairs, int per_cu, int64_t min_keys) {
   const int64_t slots = int64_t(per_cu) * device_cus();
-  return blocks * a.n_kv_head <= (a.cu ? 2 * slots : slots / 2) && paged_keys(a) >= 2 * min_keys ? int(slots) : 0;
+  const int64_t least = (a.cu ? a.total * (a.n_head / a.n_kv_head) / pairs : 2 * blocks) * a.n_kv_head;
+  return least <= slots && paged_keys(a) >= 2 * min_keys ? int(slots) : 0;
 }
 
 inline size_t paged_tiles_bytes(int64_t slots, int64_t slot_floats) {
-  return slots == 0 ? 0 : size_t(slots) * size_t(slot_floats) * 4 + size_t(slots / 2) * sizeof(PagedTiles::Cut) + 16;
+  return slots == 0 ? 0 : size_t(slots) * size_t(slot_floats) * 4 + size_t(slots) * sizeof(PagedTiles::Cut) + 16;
 }
 // Lays out the scratch of a call with so many slots, if it is large enough; else no block is cut.
 inline void paged_tiles_buffers(const PagedArgs &a, PagedTiles &t, int64_t slots, int64_t slot_floats,
@@ -251,7 +353,8 @@ inline void paged_tiles_buffers(const PagedArgs &a, PagedTiles &t, int64_t slots
   t.part_o = static_cast<float *>(a.scratch);
   t.part_ml = t.part_o + t.slots * (slot_floats - ml_floats);
   t.cuts = reinterpret_cast<PagedTiles::Cut *>(t.part_o + t.slots * slot_floats);
-  t.n_cuts = reinterpret_cast<int *>(t.cuts + t.slots / 2);
+  t.n_cuts = reinterpret_cast<int *>(t.cuts + t.slots);
+  t.halve = a.window < 0 ? 2 * t.min_tiles * t.kt : 0;
 }
 
 // Rows of few pairs (few_pairs(.., most)) of a bf16 call: append where k_new is given, with `others` of the

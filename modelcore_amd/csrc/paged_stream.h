@@ -68,14 +68,6 @@ __device__ __forceinline__ int64_t wave_total64(int64_t x) {
   for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
   return x;
 }
-__device__ __forceinline__ int wave_scan(int x, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
-  }
-  return x;
-}
 
 // How a call is cut: KV heads of a workgroup, and tiles of a range, at most.
 struct Cut {
@@ -134,7 +126,7 @@ __device__ __forceinline__ Range find_range(const StreamParams &P, int lane, Row
     if (b0 > 0) r = row_of<PB>(P, min(b0 + lane, P.n_rows - 1));
     const int rr = ranges_of(r, cut.len);
     const int n = b0 + lane < P.n_rows ? rr * r.blocks : 0;
-    const int upto = wave_scan(n, lane);
+    const int upto = wave_upto(n, lane);
     const uint64_t past = __builtin_amdgcn_ballot_w64(upto > id);
     if (past == 0) {
       id -= __builtin_amdgcn_readlane(upto, 63);

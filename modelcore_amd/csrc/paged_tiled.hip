@@ -120,7 +120,8 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
   PagedBlock blk;
   const bool found =
       find_paged_block(P.cu, P.seqlens, P.tiles.n_rows, P.T_new, P.tiles.total, P.G, P.H_kv, G_::PAIRS,
-                       P.tiles.skip, P.tiles.slots, id / P.H_kv, threadIdx.x & 63, blk);
+                       P.tiles.skip, P.tiles.slots, P.kv.max_pages << P.kv.shift, P.tiles.halve,
+                       id / P.H_kv, threadIdx.x & 63, blk);
   if (id == 0 && threadIdx.x == 0) P.tiles.note_call(found, blk);
   if (!found) return;
   const int kvh = id % P.H_kv, part = blk.part, row = blk.b, T_b = blk.T, s0 = blk.s0;
@@ -152,7 +153,7 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
   const int64_t at = pair_at(pr);
   E *out = static_cast<E *>(P.out) + at;
   if (!row_ok) {
-    if (blk.most > 1 && part == 0 && tid == 0) P.tiles.note_block(id, blk, 1);
+    if (blk.noted && part == 0 && tid == 0) P.tiles.note_block(id, blk, 1, P.H_kv);
     if (live && part == 0 && (KS == 1 || wave == 0))
       for (int d = h; d < D; d += 2) out[d] = from_f32<E>(NAN);
     return;
@@ -164,10 +165,10 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
   int lo = P.window >= 0 ? max(0, p_first - P.window) : 0, hi = last;
   int n_tiles = (hi - lo) / KT + 1;
   bool whole = true;
-  if (blk.most > 1) {  // this workgroup's range of the block's tiles
+  if (blk.noted) {  // this workgroup's range of the block's tiles
     const int ranges = P.tiles.ranges_of(blk, n_tiles);
     if (part >= ranges) return;
-    if (part == 0 && tid == 0) P.tiles.note_block(id, blk, ranges);
+    if (part == 0 && tid == 0) P.tiles.note_block(id, blk, ranges, P.H_kv);
     whole = ranges == 1;
     const int t0 = part * n_tiles / ranges, t1 = (part + 1) * n_tiles / ranges;
     hi = min(hi, lo + t1 * KT - 1);
@@ -512,6 +513,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(TiledParams P, in
 
   constexpr int U = 8;
   const int64_t group = int64_t(id) * groups + w, step = int64_t(n_blocks) * groups;
+  const int64_t second = int64_t(blk.second) * groups + w;
   float M = -INFINITY, L = 0.f;
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
   for (int r0 = 0; r0 < ranges; r0 += U) {
@@ -519,7 +521,8 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(TiledParams P, in
     f32x4 v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t g = group + min(r0 + u, ranges - 1) * step;
+      const int r = min(r0 + u, ranges - 1);
+      const int64_t g = r == 0 ? group : second + (r - 1) * step;
       x[u] = *reinterpret_cast<const float2 *>(P.part_ml(g, col));
       v[u] = *reinterpret_cast<const f32x4 *>(P.part_o(g, md, j, lane));
     }
@@ -573,7 +576,7 @@ TiledPlan tiled_plan(const PagedArgs &a, int64_t skip) {
     // Measured time of a tile on a compute unit of its own, per head dim (prefill_tiled.hip).
     t.tile_us = float(a.head_dim) * (ks == 4 ? (bf ? 0.027f : 0.085f) : (bf ? 0.012f : 0.035f));
     t.min_tiles = std::max(1, int(kRangeUs / t.tile_us));
-    t.slots = paged_slots(a, t.bound, a.head_dim <= 128 ? 2 : 1, int64_t(t.min_tiles) * t.kt);
+    t.slots = paged_slots(a, t.bound, t.pairs, a.head_dim <= 128 ? 2 : 1, int64_t(t.min_tiles) * t.kt);
     return t;
   };
   const TiledPlan whole = plan(1);
@@ -653,8 +656,8 @@ int dispatch(const TiledParams &P, const PagedArgs &a, const TiledPlan &t) {
 
 int launch_paged_tiles_merge(const PagedArgs &a, const PagedTiles &tiles, int pairs, int64_t bound) {
   const TiledParams P = tiled_params(a, tiles);
-  // Blocks of which two ranges do not fit the slots are not cut.
-  const int64_t blocks = std::min<int64_t>(bound * P.H_kv, tiles.slots / 2) * tiles.groups * P.md;
+  // Of more blocks than slots none is cut.
+  const int64_t blocks = std::min<int64_t>(bound * P.H_kv, tiles.slots) * tiles.groups * P.md;
   if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
   const dim3 grid{unsigned(blocks)}, threads{kThreads};
   if (a.dtype == MCAMD_BF16)
@@ -679,8 +682,8 @@ int launch_paged_tiled(const PagedArgs &a, int64_t skip) {
   T.kt = t.kt;
   T.align = 1;
   T.groups = t.pairs / 32;
-  paged_tiles_buffers(a, T, t.slots, slot_floats(a, t.pairs), t.pairs * 2);
   T.min_tiles = t.min_tiles;
+  paged_tiles_buffers(a, T, t.slots, slot_floats(a, t.pairs), t.pairs * 2);
   T.ratio = t.tile_us * MCAMD_SPLIT_BYTES_PER_US / (float(slot_floats(a, t.pairs)) * 8.f);
   const TiledParams P = tiled_params(a, T);
   return a.dtype == MCAMD_BF16 ? dispatch<bf16>(P, a, t) : dispatch<float>(P, a, t);

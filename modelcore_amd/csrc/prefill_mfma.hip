@@ -195,7 +195,8 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   PagedBlock blk;
   if constexpr (PAGED) {
     const bool found = find_paged_block(P.cu, P.seqlens, T->n_rows, P.T_new, T->total, P.G, P.H_kv,
-                                        P.QT * P.G, T->skip, T->slots, int(blockIdx.x) / P.H_kv, lane, blk);
+                                        P.QT * P.G, T->skip, T->slots, int(P.T_max), T->halve,
+                                        int(blockIdx.x) / P.H_kv, lane, blk);
     if (blockIdx.x == 0 && tid == 0) T->note_call(found, blk);
     if (!found) return;
     kvh = int(blockIdx.x) % P.H_kv;
@@ -236,7 +237,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   uint16_t *out = P.out + ((tok0 + pos) * P.H + int64_t(kvh) * P.G + head) * D;
   if (!row_ok) {
     if constexpr (PAGED)
-      if (blk.most > 1 && part == 0 && tid == 0) T->note_block(int(blockIdx.x), blk, 1);
+      if (blk.noted && part == 0 && tid == 0) T->note_block(int(blockIdx.x), blk, 1, P.H_kv);
     if (live && part == 0)
       for (int d = h * 64; d < h * 64 + 64; ++d) out[d] = 0x7fc0;
     return;
@@ -265,11 +266,11 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   const int lo_block = lo;
   bool whole = true;
   if constexpr (PAGED) {
-    if (blk.most > 1) {
+    if (blk.noted) {
       const int tiles = (hi - lo) / KT + 1;
       const int ranges = T->ranges_of(blk, tiles);
       if (part >= ranges) return;
-      if (part == 0 && tid == 0) T->note_block(int(blockIdx.x), blk, ranges);
+      if (part == 0 && tid == 0) T->note_block(int(blockIdx.x), blk, ranges, P.H_kv);
       whole = ranges == 1;
       const int t0 = part * tiles / ranges, t1 = (part + 1) * tiles / ranges;
       hi = min(hi, lo + t1 * KT - 1);
@@ -894,7 +895,8 @@ constexpr int64_t kSlotFloats = int64_t(kPairs) * (D + 2);
 
 size_t paged_mfma_bytes(const PagedArgs &a, int64_t skip) {
   const int64_t G = a.n_head / a.n_kv_head;
-  return paged_tiles_bytes(paged_slots(a, paged_blocks_bound(a, kPairs / G * G, skip), 1, kMinRangeKeys),
+  const int64_t pairs = kPairs / G * G;
+  return paged_tiles_bytes(paged_slots(a, paged_blocks_bound(a, pairs, skip), pairs, 1, kMinRangeKeys),
                            kSlotFloats);
 }
 
@@ -924,8 +926,8 @@ int launch_paged_mfma(const PagedArgs &a, int64_t skip) {
   T.kt = T.align = KT;
   T.groups = kWaves;
   const int64_t bound = paged_blocks_bound(a, P.QT * P.G, skip);
-  paged_tiles_buffers(a, T, paged_slots(a, bound, 1, kMinRangeKeys), kSlotFloats, kPairs * 2);
   T.min_tiles = kMinRangeKeys / KT;
+  paged_tiles_buffers(a, T, paged_slots(a, bound, P.QT * P.G, 1, kMinRangeKeys), kSlotFloats, kPairs * 2);
   // A tile of 64 keys takes 256 pairs 1.4 us; a range's partials are written and read.
   T.ratio = 1.4f * MCAMD_SPLIT_BYTES_PER_US / (float(kSlotFloats) * 8.f);
   const int64_t blocks = std::max<int64_t>(bound * P.H_kv, T.slots);

@@ -157,6 +157,36 @@ def test_long_chunks_of_few_rows(dtype, H, H_kv, D):
     run_attention([30, 200, 900, 0, 5], [1, 400, 2, 0, 130], H, H_kv, D, 16, dtype)
 
 
+@pytest.mark.parametrize("dtype,H,H_kv,D", [(BF, 32, 32, 128), (BF, 64, 32, 64), (F32, 32, 32, 64), (BF, 48, 24, 128)])
+def test_the_deepest_blocks_are_halved(dtype, H, H_kv, D):
+    """More blocks than may be cut at will, fewer than the chip takes at once: the deepest in two."""
+    run_attention([900, 20, 700, 0, 350], [40, 33, 64, 50, 35], H, H_kv, D, 16, dtype)
+    run_attention([30, 1200, 0, 640, 5, 1100], [1, 40, 45, 36, 1, 34], H, H_kv, D, 64, dtype, seed=1)
+    run_attention([600, 500, 9], [290, 40, 1], H, H_kv, D, 16, dtype, seed=2, append=False)
+    run_attention([900, 20, 800, 0, 350], [40, 33, 64, 50, 35], H, H_kv, D, 16, dtype, window=600)
+
+
+def test_halved_blocks_beside_a_row_that_does_not_fit():
+    """Its outputs are NaN, the others' those of a call without it, and the same again."""
+    g = torch.Generator().manual_seed(24)
+    new, pos = [40, 33, 64, 50], [900, 700, 1100, 5]
+    pool = Pool([p + t for p, t in zip(pos, new)], 16, 32, 128, BF, stale=1.0)
+    q = randn(g, sum(new), 32, 128, dtype=BF)
+    kg, vg, table = pool.k.to(DEV), pool.v.to(DEV), pool.table.to(DEV)
+    cu = i32([0, 40, 73, 137, 187])
+
+    def call(pos):
+        return _op()(q.to(DEV), kg, vg, block_table=table, cache_seqlens=i32(pos), cu_seqlens=cu, max_seqlen=64,
+                     causal=True).cpu()
+    for lost in (2 ** 31 - 1, -1, 16 * pool.table.shape[1] - 49):
+        y = call([900, 700, 1100, lost])
+        assert y[137:].isnan().all() and torch.equal(y[:137], call([900, 700, 1100, lost])[:137])
+        for b in range(3):
+            a, e = [0, 40, 73][b], [40, 73, 137][b]
+            want, tol = attend(q[a:e], *pool.rows(b, pos[b] + new[b]), pos[b], -1)
+            close(y[a:e], want, tol)
+
+
 @pytest.mark.parametrize("dtype,T", [(BF, 7), (F32, 1)])
 def test_many_rows_of_a_few_tokens_are_cut(dtype, T):
     """More pairs than the merge has workgroups for."""
