@@ -428,9 +428,9 @@ size_t mcamd_paged_scratch_bytes(int64_t n_rows, int64_t total, int64_t max_seql
  * 256, at most 64 query heads share a KV head. cache_seqlens is only read.
  * A row whose positions fall outside [0, max_pages * page_size) gets NaN output and appends nothing; a
  * query that sees a key in a page outside the pool is NaN, and nothing is appended there. Tokens past the
- * last row's, and a row's past max_seqlen, are not read, and their outputs not written. The scratch (16-byte aligned) belongs to the
- * call until it ends on the stream. A page that a call appends to is its own row's alone (others may share
- * theirs).
+ * last row's, and a row's past max_seqlen, are not read, and their outputs not written. The scratch
+ * (16-byte aligned) belongs to the call until it ends on the stream. A page that a call appends to is its
+ * own row's alone (others may share theirs).
  */
 int mcamd_flash_attn_paged_with_kvcache(
     const void *q, const void *k, const void *v, void *k_pages, void *v_pages,

@@ -205,7 +205,7 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
       page[i] = pages[min(k0 + (tid + kThreads * i) / (DP / VEC), hi) >> P.kv.shift];
   };
 
-  // The next tile, on its way to LDS (see above where it waits): piece c = tid + 256 i is 16 bytes of key c / (DP / VEC).
+  // The next tile, on its way to LDS: piece c = tid + 256 i is 16 bytes of key c / (DP / VEC).
   // Keys past `hi` re-read key `hi` (they are masked); K's dims past the head_dim are zero, V's
   // re-read the last ones (they reach no output).
   u32x4 kr[CH], vr[CH];  // as uint4, a struct, the compiler keeps V's in scratch memory
