@@ -373,7 +373,8 @@ int mcamd_residual_rmsnorm(const void *x, const float *part, int64_t splits, con
  * position cache_seqlens[b] + i - cu_seqlens[b] and its slot, page * page_size + position % page_size.
  * A row whose pages the stack does not hold, or that would outgrow the table, or with a negative
  * length, takes none and its tokens get position and slot -1, as do tokens past the last row's;
- * *refused becomes the number of such rows. Tokens past `total` are not planned and get no pages.
+ * *refused becomes the number of such rows. Tokens past `total` are not planned and get no pages. The
+ * lengths of refused rows must not move on.
  * row_scratch: n_rows int32, the call's own until it ends on the stream. cache_seqlens is only read:
  * the caller advances it after the forward, as with the contiguous cache.
  */
@@ -386,7 +387,9 @@ int mcamd_paged_reserve(int32_t *block_table, int64_t table_stride, const int32_
 /*
  * Rows rows[0 .. n_release) end: their pages go onto the stack of free pages, in the order of `rows`
  * and of their tables, their table entries become -1 and their cache_seqlens 0. A row named twice
- * gives its pages where it is named first; numbers outside [0, n_rows) are passed over.
+ * gives its pages where it is named first; numbers outside [0, n_rows) are passed over, and so are
+ * table entries that are no page of the pool (a row that was refused holds fewer pages than its length
+ * says if it moves on all the same).
  */
 int mcamd_paged_release(int32_t *block_table, int64_t table_stride, int32_t *cache_seqlens,
                         const int32_t *rows, int64_t n_release, int64_t n_rows,

@@ -191,14 +191,15 @@ __global__ __launch_bounds__(256) void tokens_kernel(PlanParams P) {
 }
 
 // Rows rows[0 .. n) give their pages back, in order, and are empty then. A row that is named twice
-// gives them where it is named first; a row outside the batch is passed over.
+// gives them where it is named first; a row outside the batch is passed over, and so is a number in the
+// table that is no page.
 __global__ __launch_bounds__(kThreads) void release_kernel(int32_t *table, int64_t table_stride,
                                                            int32_t *seqlens, const int32_t *rows,
                                                            int n, int n_rows, int32_t *free_pages,
                                                            int32_t *free_count, int max_pages,
                                                            int n_pages, int shift) {
-  __shared__ int64_t s_sum[kWaves];
-  __shared__ __attribute__((aligned(16))) int s_row[kThreads], s_end[kThreads];
+  __shared__ int64_t s_sum[kWaves], s_end[kThreads];
+  __shared__ __attribute__((aligned(16))) int s_row[kThreads];
   const int tid = threadIdx.x;
   int64_t top = min(max(free_count[0], 0), n_pages);
   for (int i0 = 0; i0 < n; i0 += kThreads) {
@@ -219,24 +220,30 @@ __global__ __launch_bounds__(kThreads) void release_kernel(int32_t *table, int64
     if (row >= 0) seqlens[row] = 0;
     const int64_t held =
         min((max(int64_t(len), int64_t(0)) + (1 << shift) - 1) >> shift, int64_t(max_pages));
-    const int64_t base = top;
-    const int64_t end = group_scan(held, top, s_sum) - base;
-    s_end[tid] = int(end);
+    int64_t all = 0;
+    s_end[tid] = group_scan(held, all, s_sum);
     __syncthreads();
-    const int64_t all = top - base;
-    for (int64_t p = tid; p < all; p += kThreads) {
-      int lo = 0, hi = kThreads - 1;  // the first row whose pages end past p
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (s_end[mid] > p)
-          hi = mid;
-        else
-          lo = mid + 1;
+    for (int64_t p0 = 0; p0 < all; p0 += kThreads) {
+      const int64_t p = p0 + tid;
+      int id = -1;
+      if (p < all) {
+        int lo = 0, hi = kThreads - 1;  // the first row whose pages end past p
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (s_end[mid] > p)
+            hi = mid;
+          else
+            lo = mid + 1;
+        }
+        const int64_t at = s_row[lo] * table_stride + p - (lo ? s_end[lo - 1] : 0);
+        id = table[at];
+        table[at] = -1;
       }
-      const int64_t at = s_row[lo] * table_stride + p - (lo ? s_end[lo - 1] : 0);
-      const int id = table[at];
-      table[at] = -1;
-      if (base + p < n_pages) free_pages[base + p] = id;
+      // What is no page of the pool, as in a row that was refused and moved on all the same, is not one to
+      // give: the pages move up.
+      const bool page = uint32_t(id) < uint32_t(n_pages);
+      const int64_t to = group_scan(int64_t(page), top, s_sum) - 1;
+      if (page && to < n_pages) free_pages[to] = id;
     }
     __syncthreads();  // s_row and s_end have been read
   }

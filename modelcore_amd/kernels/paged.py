@@ -77,7 +77,8 @@ def paged_reserve(block_table, cache_seqlens, new_lens, free_pages, free_count, 
 
     Returns:
         PagedPlan. A row whose pages the stack does not hold, or that would outgrow its line of the
-        table, takes none; its tokens get slot and position -1 and ``refused`` counts it.
+        table, takes none; its tokens get slot and position -1 and ``refused`` counts it. The length of
+        such a row must not move on.
     """
     n, max_pages, stride, n_pages, dev = _check_tables(block_table, cache_seqlens, free_pages,
                                                        free_count, "paged_reserve")
@@ -105,7 +106,8 @@ def paged_reserve(block_table, cache_seqlens, new_lens, free_pages, free_count, 
 def paged_release(block_table, cache_seqlens, rows, free_pages, free_count, *, page_size):
     """Rows that have ended give their pages back to the stack, in the order of ``rows`` ((m,)
     int32): their table entries become -1 and their cache_seqlens 0, in place. A row named twice gives
-    its pages where it is named first; numbers outside the batch are passed over."""
+    its pages where it is named first; numbers outside the batch are passed over, and so are table entries
+    that are no page of the pool."""
     n, max_pages, stride, n_pages, dev = _check_tables(block_table, cache_seqlens, free_pages,
                                                        free_count, "paged_release")
     _ext.same_device(dev, rows=rows)
