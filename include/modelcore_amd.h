@@ -373,8 +373,9 @@ int mcamd_residual_rmsnorm(const void *x, const float *part, int64_t splits, con
  * position cache_seqlens[b] + i - cu_seqlens[b] and its slot, page * page_size + position % page_size.
  * A row whose pages the stack does not hold, or that would outgrow the table, or with a negative
  * length, takes none and its tokens get position and slot -1, as do tokens past the last row's;
- * *refused becomes the number of such rows. Tokens past `total` are not planned and get no pages. The
- * lengths of refused rows must not move on.
+ * *refused becomes the number of such rows, and of numbers taken off the stack that are no page of the
+ * pool (the table gets -1 for them, and their tokens slot -1). Tokens past `total` are not planned and
+ * get no pages. The lengths of refused rows must not move on.
  * row_scratch: n_rows int32, the call's own until it ends on the stream. cache_seqlens is only read:
  * the caller advances it after the forward, as with the contiguous cache.
  */

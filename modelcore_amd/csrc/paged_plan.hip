@@ -8,7 +8,8 @@
 // A row whose pages the stack no longer holds, or that would outgrow the table, or whose lengths are
 // negative, takes none and its tokens get slot and position -1 (`refused` counts such rows). Token i
 // of row b is at position len + i, slot table[b][position / P] * P + position % P; tokens past the
-// last row's get -1.
+// last row's get -1, and so do tokens whose page, taken now or before, is none of the pool (`refused`
+// counts those taken now).
 //
 // reserve: one workgroup sums over the rows (integer sums: the same pages whatever the timing), then
 // tokens are dealt to threads. A page that is taken begins at its first new token, which writes its
@@ -75,9 +76,10 @@ struct GlobalRows {
   const int32_t *cu, *first, *len;
 };
 
-// kTokens tokens, `step` apart from t0 on.
+// kTokens tokens, `step` apart from t0 on; returns how many of the pages taken for them are no pages, whose
+// tokens get no slot.
 template <class Rows>
-__device__ __forceinline__ void write_tokens(const PlanParams &P, const Rows &rows, int t0, int step) {
+__device__ __forceinline__ int write_tokens(const PlanParams &P, const Rows &rows, int t0, int step) {
   int row[kTokens];
 #pragma unroll
   for (int u = 0; u < kTokens; ++u) {
@@ -108,14 +110,20 @@ __device__ __forceinline__ void write_tokens(const PlanParams &P, const Rows &ro
     id[u] = *(!planned ? P.free_pages : page < have ? line : P.free_pages + (first - (page - have)));
     named[u] = planned && page >= have && (pos[u] & page_mask) == 0 ? line : nullptr;
   }
+  int lost = 0;
 #pragma unroll
   for (int u = 0; u < kTokens; ++u) {
     const int t = t0 + u * step;
-    if (t >= P.total) return;
-    if (named[u]) *named[u] = id[u];
-    P.slots[t] = pos[u] < 0 || id[u] < 0 ? -1 : (int64_t(id[u]) << P.shift) + (pos[u] & page_mask);
+    if (t >= P.total) break;
+    const bool page = uint32_t(id[u]) < uint32_t(P.n_pages);
+    if (named[u]) {
+      *named[u] = page ? id[u] : -1;
+      lost += !page;
+    }
+    P.slots[t] = pos[u] < 0 || !page ? -1 : (int64_t(id[u]) << P.shift) + (pos[u] & page_mask);
     P.positions[t] = pos[u];
   }
+  return lost;
 }
 
 __global__ __launch_bounds__(kThreads) void reserve_kernel(PlanParams P, int with_tokens) {
@@ -161,33 +169,39 @@ __global__ __launch_bounds__(kThreads) void reserve_kernel(PlanParams P, int wit
   if (tid == 0) {
     P.cu[0] = s_rows.cu[0] = 0;
     P.free_count[0] = int(stack - kept);
-    P.refused[0] = s_refused;
   }
-  if (!with_tokens) return;
   __syncthreads();  // the rows' numbers are written
-  for (int t = tid; t < P.total; t += kThreads * kTokens) {
-    if (P.n_rows <= kThreads)
-      write_tokens(P, s_rows, t, kThreads);
-    else
-      write_tokens(P, GlobalRows{P.cu, P.first, P.seqlens}, t, kThreads);
+  if (with_tokens) {
+    int lost = 0;
+    for (int t = tid; t < P.total; t += kThreads * kTokens) {
+      if (P.n_rows <= kThreads)
+        lost += write_tokens(P, s_rows, t, kThreads);
+      else
+        lost += write_tokens(P, GlobalRows{P.cu, P.first, P.seqlens}, t, kThreads);
+    }
+    if (lost > 0) atomicAdd(&s_refused, lost);
+    __syncthreads();
   }
+  if (tid == 0) P.refused[0] = s_refused;
 }
 
 __global__ __launch_bounds__(256) void tokens_kernel(PlanParams P) {
   __shared__ SharedRows s_rows;
   const int t = int(blockIdx.x) * 256 * kTokens + int(threadIdx.x);
+  int lost;
   if (P.n_rows > kThreads) {
-    write_tokens(P, GlobalRows{P.cu, P.first, P.seqlens}, t, 256);
-    return;
+    lost = write_tokens(P, GlobalRows{P.cu, P.first, P.seqlens}, t, 256);
+  } else {
+    for (int b = threadIdx.x; b < P.n_rows; b += 256) {
+      s_rows.cu[b + 1] = P.cu[b + 1];
+      s_rows.first[b] = P.first[b];
+      s_rows.len[b] = P.seqlens[b];
+    }
+    if (threadIdx.x == 0) s_rows.cu[0] = 0;
+    __syncthreads();
+    lost = write_tokens(P, s_rows, t, 256);
   }
-  for (int b = threadIdx.x; b < P.n_rows; b += 256) {
-    s_rows.cu[b + 1] = P.cu[b + 1];
-    s_rows.first[b] = P.first[b];
-    s_rows.len[b] = P.seqlens[b];
-  }
-  if (threadIdx.x == 0) s_rows.cu[0] = 0;
-  __syncthreads();
-  write_tokens(P, s_rows, t, 256);
+  if (lost > 0) atomicAdd(P.refused, lost);  // whole numbers: the same in any order
 }
 
 // Rows rows[0 .. n) give their pages back, in order, and are empty then. A row that is named twice

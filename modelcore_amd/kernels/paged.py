@@ -28,7 +28,7 @@ class PagedPlan(NamedTuple):
     slots: torch.Tensor       # (total,) int64: page * page_size + token of the page, or -1
     positions: torch.Tensor   # (total,) int32: position within the row, or -1
     cu_seqlens: torch.Tensor  # (rows + 1,) int32: the rows' offsets
-    refused: torch.Tensor     # (1,) int32: rows that got no pages
+    refused: torch.Tensor     # (1,) int32: rows that got no pages, and pages outside the pool
 
 
 def check_page_size(page_size) -> int:
@@ -78,7 +78,8 @@ def paged_reserve(block_table, cache_seqlens, new_lens, free_pages, free_count, 
     Returns:
         PagedPlan. A row whose pages the stack does not hold, or that would outgrow its line of the
         table, takes none; its tokens get slot and position -1 and ``refused`` counts it. The length of
-        such a row must not move on.
+        such a row must not move on. A number on the stack that is no page of the pool is counted too, and
+        the tokens it was taken for get slot -1.
     """
     n, max_pages, stride, n_pages, dev = _check_tables(block_table, cache_seqlens, free_pages,
                                                        free_count, "paged_reserve")

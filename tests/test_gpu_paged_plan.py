@@ -40,3 +40,26 @@ def test_a_row_longer_than_its_pages_gives_back_those_it_has(rows):
     given = [s for s in slots if s >= 0]
     assert len(set(given)) == len(given) and all(s < 16 * n_pages for s in given)
     assert (plan.refused.item() == 0) == (len(given) == len(slots))
+
+
+@pytest.mark.parametrize("tokens", [20, 3000])  # in one launch, and in two
+@pytest.mark.parametrize("bad", [-1, 7000, 2 ** 31 - 1])
+def test_numbers_on_the_stack_that_are_no_pages(tokens, bad):
+    """Their tokens get no slot, the table -1, and `refused` says that something was not given."""
+    from modelcore_amd.kernels.paged import paged_reserve
+    rows, pages = 3, 600
+    free = list(range(pages))
+    need = -(-tokens // 16)
+    free[pages - 1 - need] = bad  # the first page of the second row
+    table = torch.full((rows, need + 2), -1, dtype=torch.int32, device=DEV)
+    count = i32([pages])
+    plan = paged_reserve(table, i32([0] * rows), i32([tokens] * rows), i32(free), count,
+                         total=rows * tokens, page_size=16)
+    want = []
+    for b in range(rows):
+        for t in range(tokens):
+            page = free[pages - 1 - b * need - t // 16]
+            want.append(page * 16 + t % 16 if 0 <= page < pages else -1)
+    assert plan.slots.tolist() == want
+    assert plan.refused.tolist() == [1] and count.tolist() == [pages - rows * need]
+    assert table[1].tolist()[:2] == [-1, free[pages - 2 - need] if need > 1 else -1]
