@@ -391,6 +391,8 @@ int mcamd_paged_reserve(int32_t *block_table, int64_t table_stride, const int32_
  * gives its pages where it is named first; numbers outside [0, n_rows) are passed over, and so are
  * table entries that are no page of the pool (a row that was refused holds fewer pages than its length
  * says if it moves on all the same).
+ * A page goes onto the stack once for each row that gives it: one that several rows share must be given
+ * by one of them alone, the last that reads it.
  */
 int mcamd_paged_release(int32_t *block_table, int64_t table_stride, int32_t *cache_seqlens,
                         const int32_t *rows, int64_t n_release, int64_t n_rows,

@@ -104,20 +104,51 @@ def paged_reserve(block_table, cache_seqlens, new_lens, free_pages, free_count, 
     return PagedPlan(slots, positions, cu, refused)
 
 
+def _check_release(block_table, cache_seqlens, rows, free_pages, free_count, page_size):
+    """Checked mode: every page of the rows that end is one of the pool, held by no other row and not free."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("paged_release: checked mode reads the block table on the host and cannot run "
+                           "under graph capture; call set_checked(False) first")
+    table, lens, width = block_table.tolist(), cache_seqlens.tolist(), block_table.shape[1]
+    n_pages = free_pages.numel()
+    held = {}
+    for b, n in enumerate(lens):
+        for page in table[b][:min(-(-max(n, 0) // page_size), width)]:
+            held.setdefault(page, []).append(b)
+    free = set(free_pages.tolist()[:min(max(free_count.item(), 0), n_pages)])
+    for b in rows.tolist():
+        if not 0 <= b < len(lens):
+            continue
+        for page in table[b][:min(-(-max(lens[b], 0) // page_size), width)]:
+            if not 0 <= page < n_pages:
+                raise IndexError(f"paged_release: page {page} of row {b} is not one of the pool's {n_pages}")
+            if page in free or len(held[page]) > 1:
+                raise ValueError(f"paged_release: page {page} of row {b} is also "
+                                 f"{'free' if page in free else f'held by rows {held[page]}'}")
+
+
 def paged_release(block_table, cache_seqlens, rows, free_pages, free_count, *, page_size):
     """Rows that have ended give their pages back to the stack, in the order of ``rows`` ((m,)
     int32): their table entries become -1 and their cache_seqlens 0, in place. A row named twice gives
     its pages where it is named first; numbers outside the batch are passed over, and so are table entries
-    that are no page of the pool."""
+    that are no page of the pool.
+
+    Every page goes onto the stack once for each row that gives it: rows whose lines share pages (which the
+    attention only reads) must not be released through more than one of them. Checked mode
+    (``flash_attn.set_checked``) reads the tables back and raises where a page is shared, free already or
+    outside the pool."""
     n, max_pages, stride, n_pages, dev = _check_tables(block_table, cache_seqlens, free_pages,
                                                        free_count, "paged_release")
     _ext.same_device(dev, rows=rows)
     if rows.dtype != torch.int32 or rows.dim() != 1:
         raise ValueError(f"rows must be (m,) int32; got {tuple(rows.shape)} {rows.dtype}")
-    rows = rows.contiguous()
+    rows, page_size = rows.contiguous(), check_page_size(page_size)
+    from modelcore_amd.kernels import flash_attn
+    if flash_attn.CHECK_POSITIONS:
+        _check_release(block_table, cache_seqlens, rows, free_pages, free_count, page_size)
     with _ext.on_device(dev):
         st = _ext.lib().mcamd_paged_release(
             block_table.data_ptr(), stride, cache_seqlens.data_ptr(), rows.data_ptr(),
             rows.numel(), n, free_pages.data_ptr(), free_count.data_ptr(), max_pages,
-            n_pages, check_page_size(page_size), _ext.stream_handle(dev))
+            n_pages, page_size, _ext.stream_handle(dev))
     _ext.check(st, "paged_release")

@@ -63,3 +63,33 @@ def test_numbers_on_the_stack_that_are_no_pages(tokens, bad):
     assert plan.slots.tolist() == want
     assert plan.refused.tolist() == [1] and count.tolist() == [pages - rows * need]
     assert table[1].tolist()[:2] == [-1, free[pages - 2 - need] if need > 1 else -1]
+
+
+def test_checked_mode_finds_pages_that_would_be_given_twice():
+    """Rows whose lines share pages, pages that are free already, numbers that are no pages: refused before
+    anything is launched, where checked mode is on."""
+    from modelcore_amd.kernels import flash_attn as fa
+    from modelcore_amd.kernels.paged import paged_release
+    free, count = i32([9, 8, 7, 6, 5] + [-1] * 5), i32([5])
+    lens = [20, 16, 40, 0]
+    lines = [[0, 1, -1], [0, -1, -1], [2, 3, 4], [2, -1, -1]]
+
+    def release(rows, lines):
+        table, n = i32(lines), i32(lens)
+        paged_release(table, n, i32(rows), free, count, page_size=16)
+        return table, n
+    fa.set_checked(True)
+    try:
+        for rows in ([0], [2, 1], [0, 1]):
+            with pytest.raises(ValueError, match="page 0 of row . is also held by rows"):
+                release(rows, lines)
+        with pytest.raises(ValueError, match="page 6 of row 1 is also free"):
+            release([1], [lines[0], [6, -1, -1]] + lines[2:])
+        with pytest.raises(IndexError, match="page 10 of row 1 is not one of the pool"):
+            release([1], [lines[0], [10, -1, -1]] + lines[2:])
+        assert count.tolist() == [5]
+        table, n = release([2, 3, 2, 77], lines)  # what row 3 names, it does not hold
+        assert count.tolist() == [8] and free.tolist()[5:8] == [2, 3, 4]
+        assert n.tolist() == [20, 16, 0, 0] and table.tolist()[2] == [-1] * 3
+    finally:
+        fa.set_checked(False)
