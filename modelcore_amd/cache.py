@@ -269,7 +269,8 @@ class PagedKVCache:
     a launch where the pool or a row's line of the table is too small, so nothing is read back.
 
     A step can be captured: ``begin(n)`` in the capture, with the same count for every row, then
-    ``note_device_step(n)`` before each replay, which checks and moves the host's account.
+    ``note_device_step(n)`` before each replay, which checks and moves the host's account. The model that
+    runs the captured step bounds the replays' positions by its rotary tables (``PagedStep.bound_positions``).
     """
 
     def __init__(self, batch_size, n_kv_head, seq_len, head_dim, num_kv_slots, device, dtype, *,
@@ -297,6 +298,7 @@ class PagedKVCache:
         self.lengths = [0] * batch_size
         self.pages_free = self.n_pages
         self._open = False  # a step has begun and not run
+        self._replay_positions = None  # that the models of captured steps have in their rotary tables
 
     def _pages(self, n):
         return -(-n // self.page_size)
@@ -361,8 +363,12 @@ class PagedKVCache:
         """The host's side of a captured begin + forward, before its replay: checked, then moved."""
         assert not self._open, "the step before has not run"
         lens = self._lens(new_lens)
-        self.pages_free -= self._room(lens)
-        self.lengths = [n + t for n, t in zip(self.lengths, lens)]
+        taken = self._room(lens)
+        lengths = [n + t for n, t in zip(self.lengths, lens)]
+        if self._replay_positions is not None:
+            _check_rotary(max(lengths, default=0), self._replay_positions)
+        self.pages_free -= taken
+        self.lengths = lengths
 
     def release(self, rows):
         """Rows that have ended give their pages back and are empty."""
@@ -382,6 +388,11 @@ class PagedKVCache:
             self.lengths[r] = 0
 
 
+def _check_rotary(longest, n_pos):
+    assert longest <= n_pos, \
+        f"Sequence length grew beyond the rotary embeddings cache: {longest} > {n_pos}"
+
+
 class PagedStep:
     """One forward over a PagedKVCache (``PagedKVCache.begin``): the rows' new tokens packed one after
     another, ``model(idx, kv_cache=step)`` with idx (1, total)."""
@@ -395,6 +406,15 @@ class PagedStep:
         self.uniform = self.max_seqlen if lens and len(set(lens)) == 1 else None
         self.longest = 0 if captured else max((n + t for n, t in zip(cache.lengths, lens)), default=0)
         self._counts, self._captured, self._done = counts, captured, False
+
+    def bound_positions(self, n_pos):
+        """The model that runs the step has n_pos positions in its rotary tables: checked here, or, of a step
+        that is captured, before each replay (``PagedKVCache.note_device_step``)."""
+        if self._captured:
+            c = self.cache
+            c._replay_positions = min(n_pos, n_pos if c._replay_positions is None else c._replay_positions)
+        else:
+            _check_rotary(self.longest, n_pos)
 
     slots = property(lambda self: self.plan.slots)
     positions = property(lambda self: self.plan.positions)

@@ -864,9 +864,7 @@ class Model(nn.Module):
         if isinstance(kv_cache, PagedStep):
             assert idx.size(0) == 1, \
                 "a paged forward takes every row's new tokens as one (1, total) sequence"
-            n_pos = min(b.mixer.rope.cos.size(1) for b in self.body.blocks)
-            assert kv_cache.longest <= n_pos, \
-                f"Sequence length grew beyond the rotary embeddings cache: {kv_cache.longest} > {n_pos}"
+            kv_cache.bound_positions(min(b.mixer.rope.cos.size(1) for b in self.body.blocks))
 
     def last_logits(self, idx, kv_cache, last):
         """forward(), but the head runs only at position last[b] of row b: (B, vocab) logits.
