@@ -297,7 +297,7 @@ class PagedKVCache:
         # The host's account of the same.
         self.lengths = [0] * batch_size
         self.pages_free = self.n_pages
-        self._open = False  # a step has begun and not run
+        self._open = None  # the step that has begun and not run
         self._replay_positions = None  # that the models of captured steps have in their rotary tables
 
     def _pages(self, n):
@@ -311,7 +311,7 @@ class PagedKVCache:
         self.free_count.fill_(self.n_pages)
         self.lengths = [0] * self.batch_size
         self.pages_free = self.n_pages
-        self._open = False
+        self._open = None
 
     def get_slot_cache(self, slot):
         """(k_pages, v_pages) views of one KV slot, each (n_pages, page_size, H_kv, D)."""
@@ -349,7 +349,6 @@ class PagedKVCache:
                 raise RuntimeError("a captured step needs the same count of new tokens for every row")
         else:
             self.pages_free -= self._room(lens)
-            self._open = True
         if len(set(lens)) <= 1:
             counts = torch.full((self.batch_size,), lens[0] if lens else 0, dtype=torch.int32,
                                 device=dev)
@@ -357,7 +356,10 @@ class PagedKVCache:
             counts = torch.tensor(lens, dtype=torch.int32, device=dev)
         plan = paged_reserve(self.block_table, self.cache_seqlens, counts, self.free_pages,
                              self.free_count, total=sum(lens), page_size=self.page_size)
-        return PagedStep(self, lens, counts, plan, capturing)
+        step = PagedStep(self, lens, counts, plan, capturing)
+        if not capturing:
+            self._open = step
+        return step
 
     def note_device_step(self, new_lens):
         """The host's side of a captured begin + forward, before its replay: checked, then moved."""
@@ -407,6 +409,12 @@ class PagedStep:
         self.longest = 0 if captured else max((n + t for n, t in zip(cache.lengths, lens)), default=0)
         self._counts, self._captured, self._done = counts, captured, False
 
+    def check_open(self):
+        """The step is the one its cache has begun: its slots are its rows' only until it has run, or until
+        the cache is reset."""
+        assert not self._done, "a step is run once"
+        assert self._captured or self.cache._open is self, "the cache was reset after the step began"
+
     def bound_positions(self, n_pos):
         """The model that runs the step has n_pos positions in its rotary tables: checked here, or, of a step
         that is captured, before each replay (``PagedKVCache.note_device_step``)."""
@@ -441,9 +449,9 @@ class PagedStep:
     def advance(self, num_tokens):
         """Each row moves on by its own new tokens (one device add, no host read)."""
         assert num_tokens == self.total, "a paged forward covers every row's new tokens"
-        assert not self._done, "a step is run once"
+        self.check_open()
         c = self.cache
         c.cache_seqlens += self._counts
         if not self._captured:
-            self._done, c._open = True, False
+            self._done, c._open = True, None
             c.lengths = [n + t for n, t in zip(c.lengths, self.lens)]

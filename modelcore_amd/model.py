@@ -839,6 +839,7 @@ class Model(nn.Module):
             assert kv_cache.max_seqlen <= kv_cache.cache.max_seq_len
             return
         if isinstance(kv_cache, PagedStep):  # its pages are reserved: checked by PagedKVCache.begin
+            kv_cache.check_open()
             assert T == kv_cache.total, \
                 "a paged forward takes every row's new tokens as one (1, total) sequence"
             return
