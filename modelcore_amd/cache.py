@@ -344,11 +344,9 @@ class PagedKVCache:
         lens = self._lens(new_lens)
         dev = self.cache_seqlens.device
         capturing = dev.type == "cuda" and torch.cuda.is_current_stream_capturing()
-        if capturing:
-            if len(set(lens)) > 1:
-                raise RuntimeError("a captured step needs the same count of new tokens for every row")
-        else:
-            self.pages_free -= self._room(lens)
+        if capturing and len(set(lens)) > 1:
+            raise RuntimeError("a captured step needs the same count of new tokens for every row")
+        taken = 0 if capturing else self._room(lens)
         if len(set(lens)) <= 1:
             counts = torch.full((self.batch_size,), lens[0] if lens else 0, dtype=torch.int32,
                                 device=dev)
@@ -357,8 +355,9 @@ class PagedKVCache:
         plan = paged_reserve(self.block_table, self.cache_seqlens, counts, self.free_pages,
                              self.free_count, total=sum(lens), page_size=self.page_size)
         step = PagedStep(self, lens, counts, plan, capturing)
-        if not capturing:
+        if not capturing:  # the host's account moves once the plan is under way
             self._open = step
+            self.pages_free -= taken
         return step
 
     def note_device_step(self, new_lens):

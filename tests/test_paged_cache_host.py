@@ -99,3 +99,14 @@ def test_a_step_that_is_not_its_caches_open_one_runs_no_layer(plans):
     assert layers.runs == 1 and cache.lengths == [0, 0]
     model(ids[:, :2], kv_cache=anew)
     assert layers.runs == 2 and cache.lengths == [1, 1] == cache.cache_seqlens.tolist()
+
+
+def test_a_plan_that_fails_leaves_the_account(plans):
+    cache = make()
+    plans.fail = True
+    with pytest.raises(RuntimeError, match="no launch"):
+        cache.begin([20, 3])
+    assert cache.pages_free == cache.n_pages and cache.lengths == [0, 0]
+    plans.fail = False
+    step = cache.begin([20, 3])
+    assert cache.pages_free == cache.n_pages - 3 and plans == [[20, 3]] and step.total == 23
