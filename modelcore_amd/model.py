@@ -438,7 +438,7 @@ class Attention(nn.Module):
             causal=True, window_size=(self.window, 0), **kw).view(1, T, self.n_head, self.head_dim)
         if "output_gate" in self.features:
             y = self.features["output_gate"](y, x)
-        return self.c_proj(y.contiguous().view(1, T, -1))
+        return self.c_proj(y.contiguous().view(1, T, self.n_head * self.head_dim))  # T may be 0
 
     def _extensions(self, kv_cache):
         """Operator keywords beyond the reference's, for an operator that takes them: the

@@ -1,4 +1,4 @@
-"""Captured steps of a paged cache where the eager step would raise."""
+"""Steps of a paged cache at their edges: replays where the eager step would raise, steps of no tokens."""
 import pytest
 import torch
 
@@ -51,3 +51,20 @@ def test_replays_stop_at_the_rotary_table(fused):
         cache.note_device_step(1)
         graph.replay()
         assert out.isfinite().all() and cache.cache_seqlens.tolist() == [1, 1]
+
+
+@pytest.mark.parametrize("fused", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_step_of_no_tokens(dtype, fused):
+    mgr = ModelManager(Runtime(dtype))
+    model = awake(mgr.create_model(config(layers=2), device=DEV, seed=0))
+    model.set_fused_epilogue(fused)
+    none = torch.zeros(1, 0, dtype=torch.long, device=DEV)
+    with torch.inference_mode():
+        cache = mgr.new_paged_kv_cache(model, batch_size=2, seq_len=64)
+        model(torch.arange(6, device=DEV)[None], kv_cache=cache.begin(3))
+        assert model(none, kv_cache=cache.begin(0)).shape == (1, 0, 500)
+        assert model.last_logits(none, cache.begin([0, 0]), None).shape == (0, 500)
+        assert cache.lengths == [3, 3] == cache.cache_seqlens.tolist()
+        model(torch.arange(2, device=DEV)[None], kv_cache=cache.begin(1))
+        assert cache.lengths == [4, 4]
