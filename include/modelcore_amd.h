@@ -358,7 +358,7 @@ int mcamd_residual_rmsnorm(const void *x, const float *part, int64_t splits, con
  * The paged KV cache: K and V in pools of n_pages pages, (n_pages, page_size, H_kv, D) per slot, each
  * page contiguous and pages `page_stride` elements apart, and per row a line of a block table,
  * (n_rows, max_pages) int32 with lines `table_stride` numbers apart: position t of row b is token
- * t % page_size of page block_table[b][t / page_size]. page_size is a power of two, at least 16
+ * t % page_size of page block_table[b][t / page_size]. page_size is a power of two from 16 to 2^30
  * (MCAMD_EINVAL otherwise). Entries of pages a row does not hold are not read; a page number outside
  * [0, n_pages) that is needed is never followed. It has no counterpart in the reference, whose cache
  * reserves T_max positions per row (modelcore/cache.py:22-23).

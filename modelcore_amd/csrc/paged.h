@@ -14,7 +14,14 @@
 
 namespace mcamd {
 
-constexpr int64_t kMinPageSize = 16;
+constexpr int64_t kMinPageSize = 16, kMaxPageSize = int64_t(1) << 30;
+
+// The power of two that a page size is; false where it is none that the kernels take.
+inline bool page_shift(int64_t page_size, int &shift) {
+  if (page_size < kMinPageSize || page_size > kMaxPageSize || (page_size & (page_size - 1)) != 0) return false;
+  for (shift = 0; (int64_t(1) << shift) < page_size;) ++shift;
+  return true;
+}
 
 struct PagedKv {
   const int32_t *table;

@@ -86,12 +86,11 @@ extern "C" size_t mcamd_paged_scratch_bytes(int64_t n_rows, int64_t total, int64
                                             int64_t max_pages, int64_t page_size, int64_t window,
                                             int dtype) {
   if (n_rows <= 0 || total <= 0 || max_seqlen <= 0 || n_kv_head <= 0 || n_head < n_kv_head ||
-      head_dim <= 0 || head_dim > 256 || max_pages <= 0 || page_size < kMinPageSize ||
-      n_head > 65535 || n_rows > 65535 || max_pages > (int64_t(1) << 30) / page_size ||
+      head_dim <= 0 || head_dim > 256 || max_pages <= 0 || n_head > 65535 || n_rows > 65535 ||
       total > (int64_t(1) << 30) / n_head)
     return 0;
   PagedArgs a{};
-  while ((int64_t(1) << a.kv.shift) < page_size) ++a.kv.shift;
+  if (!page_shift(page_size, a.kv.shift) || max_pages > (int64_t(1) << 30) / page_size) return 0;
   a.kv.max_pages = int(max_pages);
   a.n_rows = n_rows;
   a.t_new = max_seqlen;
@@ -127,18 +126,19 @@ extern "C" int mcamd_flash_attn_paged_with_kvcache(
   if ((k == nullptr) != (v == nullptr))
     return fail(MCAMD_EINVAL, "flash_attn_paged_with_kvcache: pass both k and v, or neither");
   PagedArgs a{};
-  while ((int64_t(1) << a.kv.shift) < page_size) ++a.kv.shift;
-  if (page_size < kMinPageSize || (int64_t(1) << a.kv.shift) != page_size)
-    return fail(MCAMD_EINVAL, "paged attention: page_size must be a power of two, at least 16");
+  if (!page_shift(page_size, a.kv.shift))
+    return fail(MCAMD_EINVAL, "paged attention: page_size must be a power of two from 16 to 2^30");
   if (n_pages <= 0 || max_pages <= 0 || max_seqlen < 0)
     return fail(MCAMD_EINVAL, "paged attention: empty pool or block table, or negative max_seqlen");
+  if (n_pages > 0x7fffffff / page_size || max_pages > (int64_t(1) << 30) / page_size ||
+      n_rows > 65535 || n_head > 65535 || n_kv_head > 65535 || head_dim > 65535 ||
+      total > (int64_t(1) << 30) / (n_head > 0 ? n_head : 1) ||
+      (!cu_seqlens && max_seqlen > int64_t(1) << 30))
+    return fail(MCAMD_EUNSUPPORTED, "paged attention: sizes beyond the 32-bit index range of the kernels");
   if (page_stride < page_size * n_kv_head * head_dim)
     return fail(MCAMD_EINVAL, "paged attention: page_stride smaller than page_size*H_kv*D");
   if (table_stride < max_pages)
     return fail(MCAMD_EINVAL, "paged attention: table_stride smaller than max_pages");
-  if (n_pages * page_size > 0x7fffffff || max_pages > (int64_t(1) << 30) / page_size ||
-      n_rows > 65535 || n_head > 65535 || total > (int64_t(1) << 30) / (n_head > 0 ? n_head : 1))
-    return fail(MCAMD_EUNSUPPORTED, "paged attention: sizes beyond the 32-bit index range of the kernels");
   if (!cu_seqlens && total != n_rows * max_seqlen)
     return fail(MCAMD_EINVAL, "paged attention: without cu_seqlens every row has max_seqlen tokens");
   a.q = q;

@@ -264,12 +264,6 @@ __global__ __launch_bounds__(kThreads) void release_kernel(int32_t *table, int64
   if (tid == 0) free_count[0] = int(min(top, int64_t(n_pages)));
 }
 
-bool page_size_ok(int64_t page_size, int &shift) {
-  shift = 0;
-  while ((int64_t(1) << shift) < page_size) ++shift;
-  return page_size >= kMinPageSize && (int64_t(1) << shift) == page_size;
-}
-
 constexpr int64_t kMax31 = 0x7fffffff;
 
 }  // namespace
@@ -287,12 +281,12 @@ extern "C" int mcamd_paged_reserve(int32_t *block_table, int64_t table_stride,
   PlanParams P{};
   if (n_rows < 0 || total < 0 || max_pages <= 0 || n_pages <= 0)
     return fail(MCAMD_EINVAL, "paged_reserve: sizes must be positive (n_rows, total may be 0)");
-  if (!page_size_ok(page_size, P.shift))
-    return fail(MCAMD_EINVAL, "paged_reserve: page_size must be a power of two, at least 16");
+  if (!page_shift(page_size, P.shift))
+    return fail(MCAMD_EINVAL, "paged_reserve: page_size must be a power of two from 16 to 2^30");
   if (table_stride < max_pages)
     return fail(MCAMD_EINVAL, "paged_reserve: table_stride smaller than max_pages");
   if (n_rows >= kMax31 - kThreads || total > kMax31 - kThreads * kTokens ||
-      n_pages * page_size > kMax31 || max_pages * page_size > kMax31)
+      n_pages > kMax31 / page_size || max_pages > kMax31 / page_size)
     return fail(MCAMD_EUNSUPPORTED, "paged_reserve: sizes beyond 31 bits");
   if (!free_count || !cu_seqlens || !refused ||
       (n_rows > 0 && (!block_table || !cache_seqlens || !new_lens || !free_pages || !row_scratch)) ||
@@ -333,12 +327,12 @@ extern "C" int mcamd_paged_release(int32_t *block_table, int64_t table_stride,
   int shift = 0;
   if (n_rows < 0 || n_release < 0 || max_pages <= 0 || n_pages <= 0)
     return fail(MCAMD_EINVAL, "paged_release: sizes must be positive (n_rows, n_release may be 0)");
-  if (!page_size_ok(page_size, shift))
-    return fail(MCAMD_EINVAL, "paged_release: page_size must be a power of two, at least 16");
+  if (!page_shift(page_size, shift))
+    return fail(MCAMD_EINVAL, "paged_release: page_size must be a power of two from 16 to 2^30");
   if (table_stride < max_pages)
     return fail(MCAMD_EINVAL, "paged_release: table_stride smaller than max_pages");
   if (n_rows >= kMax31 - kThreads || n_release >= kMax31 - kThreads ||
-      n_pages * page_size > kMax31 || max_pages * page_size > kMax31)
+      n_pages > kMax31 / page_size || max_pages > kMax31 / page_size)
     return fail(MCAMD_EUNSUPPORTED, "paged_release: sizes beyond 31 bits");
   if (n_release == 0 || n_rows == 0) {
     clear_error();

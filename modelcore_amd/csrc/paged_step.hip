@@ -141,8 +141,8 @@ int run(const StepParams &P, hipStream_t stream) {
   int lpi = 64;
   if (whole)
     for (lpi = 1; lpi * N < half;) lpi *= 2;
+  if (P.n_items_all > 0x7fffffff / lpi) return fail(MCAMD_EUNSUPPORTED, "rope_norm_append_paged: grid too large");
   const int64_t blocks = (P.n_items_all * lpi + kThreads - 1) / kThreads;
-  if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "rope_norm_append_paged: grid too large");
   const dim3 grid{unsigned(blocks)}, threads{kThreads};
 #define MCAMD_STEP(VEC, LPI, R) \
   hipLaunchKernelGGL((paged_step_kernel<T, VEC, LPI, R>), grid, threads, 0, stream, P)
@@ -181,6 +181,8 @@ extern "C" int mcamd_qk_rope_norm_append_paged(
     return fail(MCAMD_EINVAL, "rope_norm_append_paged: dtype must be MCAMD_F32 or MCAMD_BF16");
   if (total < 0 || n_head <= 0 || n_kv_head <= 0 || n_pos <= 0)
     return fail(MCAMD_EINVAL, "rope_norm_append_paged: sizes must be positive (total may be 0)");
+  if (total > 0x7fffffff || n_head > 0x7fffffff / 2 || n_kv_head > 0x7fffffff / 4)
+    return fail(MCAMD_EUNSUPPORTED, "rope_norm_append_paged: sizes too large");
   if (head_dim <= 0 || head_dim % 2 != 0 || head_dim > 256)
     return fail(MCAMD_EUNSUPPORTED, "rope_norm_append_paged: head_dim must be even and <= 256");
   if ((k == nullptr) != (v == nullptr))
@@ -190,19 +192,18 @@ extern "C" int mcamd_qk_rope_norm_append_paged(
   const bool with_kv = k != nullptr;
   StepParams P{};
   if (with_kv) {
-    while ((int64_t(1) << P.shift) < page_size) ++P.shift;
-    if (page_size < kMinPageSize || (int64_t(1) << P.shift) != page_size)
+    if (!page_shift(page_size, P.shift))
       return fail(MCAMD_EINVAL,
-                  "rope_norm_append_paged: page_size must be a power of two, at least 16");
-    if (n_pages <= 0 || page_stride < page_size * n_kv_head * head_dim)
+                  "rope_norm_append_paged: page_size must be a power of two from 16 to 2^30");
+    if (n_pages <= 0 || page_stride / page_size < n_kv_head * head_dim)
       return fail(MCAMD_EINVAL, "rope_norm_append_paged: empty pool, or page_stride smaller than "
                                 "page_size*H_kv*D");
+    if (n_pages > (int64_t(1) << 62) / page_size)
+      return fail(MCAMD_EUNSUPPORTED, "rope_norm_append_paged: sizes too large");
   }
   if (q_token_stride < n_head * head_dim ||
       (with_kv && (k_token_stride < n_kv_head * head_dim || v_token_stride < n_kv_head * head_dim)))
     return fail(MCAMD_EINVAL, "rope_norm_append_paged: a token stride is smaller than heads * head_dim");
-  if (total > 0x7fffffff || n_head + 2 * n_kv_head > 0x7fffffff)
-    return fail(MCAMD_EUNSUPPORTED, "rope_norm_append_paged: sizes too large");
   if (total == 0) {
     clear_error();
     return MCAMD_OK;
