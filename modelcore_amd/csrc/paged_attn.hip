@@ -93,7 +93,7 @@ extern "C" size_t mcamd_paged_scratch_bytes(int64_t n_rows, int64_t total, int64
   if (!page_shift(page_size, a.kv.shift) || max_pages > (int64_t(1) << 30) / page_size) return 0;
   a.kv.max_pages = int(max_pages);
   a.n_rows = n_rows;
-  a.t_new = max_seqlen;
+  a.t_new = std::min(max_seqlen, total);  // no row has more, and 31 bits hold it
   a.total = total;
   a.n_head = n_head;
   a.n_kv_head = n_kv_head;
@@ -155,7 +155,7 @@ extern "C" int mcamd_flash_attn_paged_with_kvcache(
   a.cu = cu_seqlens;
   a.out = out;
   a.n_rows = n_rows;
-  a.t_new = max_seqlen;
+  a.t_new = std::min(max_seqlen, total);  // no row has more, and 31 bits hold it
   a.total = total;
   a.n_head = n_head;
   a.n_kv_head = n_kv_head;

@@ -47,3 +47,16 @@ def test_steps_of_more_heads_than_a_grid_are_refused(total, H, H_kv, q_tok):
     assert _ext.lib().mcamd_qk_rope_norm_append_paged(
         FAKE, q_tok, FAKE, TOP, FAKE, TOP, FAKE, FAKE, 64, FAKE, FAKE, FAKE, FAKE, FAKE, total, H, H_kv, 128, 4, 16,
         TOP, 1e-6, 1.2, _ext.BF16, None) == _ext.EUNSUPPORTED
+
+
+@pytest.mark.parametrize("dtype", [_ext.BF16, _ext.F32])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_bound_on_rows_past_their_tokens_is_one_by_them(dtype, D):
+    """max_seqlen says "at most": past a call's tokens it changes nothing, past 31 bits too."""
+    def scratch(longest, total=20):
+        return _ext.lib().mcamd_paged_scratch_bytes(3, total, longest, 8, 8, D, 4000, 16, -1, dtype)
+    want = scratch(20)
+    assert want > 0
+    for longest in (21, 1000, (1 << 31) - 1, 1 << 31, (1 << 32) + 1, TOP):
+        assert scratch(longest) == want, longest
+    assert attention(longest=TOP, total=0) == _ext.OK
