@@ -237,27 +237,46 @@ __global__ __launch_bounds__(kThreads) void release_kernel(int32_t *table, int64
     int64_t all = 0;
     s_end[tid] = group_scan(held, all, s_sum);
     __syncthreads();
-    for (int64_t p0 = 0; p0 < all; p0 += kThreads) {
-      const int64_t p = p0 + tid;
-      int id = -1;
-      if (p < all) {
-        int lo = 0, hi = kThreads - 1;  // the first row whose pages end past p
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          if (s_end[mid] > p)
-            hi = mid;
-          else
-            lo = mid + 1;
-        }
-        const int64_t at = s_row[lo] * table_stride + p - (lo ? s_end[lo - 1] : 0);
-        id = table[at];
-        table[at] = -1;
+    auto entry = [&](int64_t p) {  // of page p of this round's rows in the table
+      int lo = 0, hi = kThreads - 1;  // the first row whose pages end past p
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (s_end[mid] > p)
+          hi = mid;
+        else
+          lo = mid + 1;
       }
+      return s_row[lo] * table_stride + p - (lo ? s_end[lo - 1] : 0);
+    };
+    auto taken_from = [&](int64_t p) {
+      const int64_t at = entry(p);
+      const int id = table[at];
+      table[at] = -1;
+      return id;
+    };
+    auto is_page = [&](int id) { return uint32_t(id) < uint32_t(n_pages); };
+    const int64_t base = top;
+    bool odd = false;  // an entry is no page, or there are more than the stack has room for
+    for (int64_t p = tid; p < all; p += kThreads) {
+      if (base + p < n_pages) {
+        const int id = taken_from(p);
+        free_pages[base + p] = id;
+        odd = odd || !is_page(id);
+      } else {
+        odd = true;
+      }
+    }
+    top += all;
+    if (__syncthreads_or(odd)) {
       // What is no page of the pool, as in a row that was refused and moved on all the same, is not one to
-      // give: the pages move up.
-      const bool page = uint32_t(id) < uint32_t(n_pages);
-      const int64_t to = group_scan(int64_t(page), top, s_sum) - 1;
-      if (page && to < n_pages) free_pages[to] = id;
+      // give: the pages behind it move up, none past where its own thread has read it.
+      top = base;
+      for (int64_t p0 = 0; p0 < all; p0 += kThreads) {
+        const int64_t p = p0 + tid;
+        const int id = p >= all ? -1 : base + p < n_pages ? free_pages[base + p] : taken_from(p);
+        const int64_t to = group_scan(int64_t(is_page(id)), top, s_sum) - 1;
+        if (is_page(id) && to < n_pages) free_pages[to] = id;
+      }
     }
     __syncthreads();  // s_row and s_end have been read
   }

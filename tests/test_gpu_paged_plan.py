@@ -93,3 +93,18 @@ def test_checked_mode_finds_pages_that_would_be_given_twice():
         assert n.tolist() == [20, 16, 0, 0] and table.tolist()[2] == [-1] * 3
     finally:
         fa.set_checked(False)
+
+
+@pytest.mark.parametrize("rows", [5, 1100])
+def test_entries_without_a_page_beside_a_full_stack(rows):
+    """The lines say more pages than the stack has room for: those there are fill it, in order."""
+    from modelcore_amd.kernels.paged import paged_release
+    n_pages = 2 * rows
+    g = torch.Generator().manual_seed(rows)
+    ids = torch.randperm(n_pages, generator=g).tolist()
+    table = [[-1, ids[2 * b], -1, n_pages, ids[2 * b + 1]] for b in range(rows - 1)] + [ids[-2:] + [-1] * 3]
+    dt, dl = i32(table), i32([80] * (rows - 1) + [32])
+    df, dc = i32([-7] * n_pages), i32([0])
+    paged_release(dt, dl, i32(list(range(rows))), df, dc, page_size=16)
+    assert df.tolist() == ids and dc.tolist() == [n_pages]
+    assert (dt == -1).all() and (dl == 0).all()
