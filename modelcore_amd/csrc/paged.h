@@ -304,7 +304,7 @@ struct PagedTiles {
   PagedKv kv;
   int n_rows, total;
   int skip;         // rows of few_pairs() by it are another launch's
-  int kt, align;    // keys of a tile, and what its first key is a multiple of
+  int kt;           // keys of a tile
   int groups;       // of 32 pairs, of a block
   int slots;        // blocks for whose partials there is room, or 0: no block is cut
   float ratio;      // prefill_split.h's, times the blocks of the call

@@ -680,7 +680,6 @@ int launch_paged_tiled(const PagedArgs &a, int64_t skip) {
   T.total = int(a.total);
   T.skip = int(skip);
   T.kt = t.kt;
-  T.align = 1;
   T.groups = t.pairs / 32;
   T.min_tiles = t.min_tiles;
   paged_tiles_buffers(a, T, t.slots, slot_floats(a, t.pairs), t.pairs * 2);

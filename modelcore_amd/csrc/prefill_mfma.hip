@@ -923,7 +923,7 @@ int launch_paged_mfma(const PagedArgs &a, int64_t skip) {
   T.n_rows = int(a.n_rows);
   T.total = int(a.total);
   T.skip = int(skip);
-  T.kt = T.align = KT;
+  T.kt = KT;
   T.groups = kWaves;
   const int64_t bound = paged_blocks_bound(a, P.QT * P.G, skip);
   T.min_tiles = kMinRangeKeys / KT;
