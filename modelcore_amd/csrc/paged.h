@@ -335,7 +335,7 @@ struct PagedTiles {
   }
 };
 
-// Keys of a block, at most.
+// Keys of a block, at most: by the width of the table's lines, since the rows' lengths are the device's.
 inline int64_t paged_keys(const PagedArgs &a) {
   const int64_t room = int64_t(a.kv.max_pages) << a.kv.shift;
   return a.window < 0 ? room : std::min<int64_t>(room, a.window + 256 + 64);

@@ -14,10 +14,13 @@
 // reserve: one workgroup sums over the rows (integer sums: the same pages whatever the timing), then
 // tokens are dealt to threads. A page that is taken begins at its first new token, which writes its
 // number into the table. Up to kOneLaunchTokens tokens the same workgroup does both; more take a
-// second launch, bound by the slots and positions it writes. Rows' offsets, lengths and first pages are
-// searched in LDS (up to kThreads rows), the page numbers of all of a thread's tokens asked for before any
-// is used. 64 rows of a token: 6.3 us (8.8 with the search in memory), three scans and two round trips;
-// 512 rows of a million tokens, 12.6 MB written: 4.5 + 8.6.
+// second launch. Rows' offsets, lengths and first pages are searched in LDS (up to kThreads rows), the page
+// numbers of all of a thread's tokens asked for before any is used. 64 rows of a token: 6.4 us (8.8 with the
+// search in memory), three scans and two round trips; 512 rows of a million tokens, 12.6 MB written: 4.5 + 9.0,
+// 1.4 TB/s: 2.2 are every workgroup's copy of the rows' numbers and a thread's four searches among them (8 rows
+// of as many tokens take 6.8), the rest the launch, a round trip for the page numbers, and stores of 4 and 8 bytes.
+//
+// release: one workgroup; 128 rows of up to 32 pages 7.8 us, 512 rows of 8000 pages 20.
 #include "paged.h"
 
 namespace mcamd {

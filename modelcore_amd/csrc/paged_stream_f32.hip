@@ -11,7 +11,8 @@
 //
 // Bound by the stream from HBM: 32 rows of 512 to 8191 keys, 16 / 4 heads of 128, 571 MB in 98 us with the
 // append (5.8 TB/s; the tiled kernel 547), 64 rows of 512 to 1023 keys, 12 heads of 64, 302 MB in 55. Two rows of 80
-// keys take 6.6, start-up. Registers set how many workgroups a compute unit holds: four instead of three at
+// keys take 6.6, start-up, and where the table has room for more than 256 keys a merge of nothing (1.9 traced, 3.5 us
+// of the call). Registers set how many workgroups a compute unit holds: four instead of three at
 // head dim 64 spill with four heads (50.9 -> 77.0 us) and gain 3% with one.
 //
 #include "paged_stream.h"

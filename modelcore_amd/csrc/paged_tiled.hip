@@ -583,9 +583,10 @@ TiledPlan tiled_plan(const PagedArgs &a, int64_t skip) {
   if (a.head_dim > 128) return whole;  // a tile of four waves' keys outgrows the LDS
   // KS = 4 takes twice to four times as long for the same pairs and keys, and is for calls that cannot fill
   // the chip otherwise: fewer blocks of 128 pairs than compute units, and rows of so few pairs that half of
-  // such a block would be empty, or too few keys for ranges that are worth their merge (kShortUs). Four waves
-  // on the keys against ranges with their merge: two prompts of 512, 12 heads of 64 in fp32 (24 us by that
-  // count) 22.8 and 33.3; two prompts of 830, 12 / 4 heads of 128 in fp32 (71) 93 and 86; two chunks of 512
+  // such a block would be empty, or too few keys for ranges that are worth their merge (kShortUs). The keys
+  // are those that the table has room for: the lengths are not known here, and the same prompts under a
+  // table of 2048 positions are cut. Four waves on the keys against ranges with their merge: two prompts of
+  // 512, 12 heads of 64 in fp32 (24 us by that count, in a table of 576) 22.6 and 33.1; two prompts of 830, 12 / 4 heads of 128 in fp32 (71) 93 and 86; two chunks of 512
   // after 2000, 12 heads of 64 in bf16 (55) 37 and 33.
   const TiledPlan four = plan(4);
   const bool fills = whole.bound * a.n_kv_head >= device_cus();
