@@ -33,8 +33,8 @@ class PagedPlan(NamedTuple):
 
 def check_page_size(page_size) -> int:
     page_size = int(page_size)
-    if page_size < 16 or page_size & (page_size - 1):
-        raise ValueError(f"page_size must be a power of two, at least 16; got {page_size}")
+    if not 16 <= page_size <= 1 << 30 or page_size & (page_size - 1):
+        raise ValueError(f"page_size must be a power of two from 16 to 2^30; got {page_size}")
     return page_size
 
 
@@ -73,7 +73,7 @@ def paged_reserve(block_table, cache_seqlens, new_lens, free_pages, free_count, 
         free_count: (1,) int32, updated in place
         total: the sum of new_lens, known to the host (the forward's token count). Tokens past it
             are not planned; where it is larger, the tokens past the last row's get -1.
-        page_size: tokens per page, a power of two, at least 16
+        page_size: tokens per page, a power of two from 16 to 2^30
 
     Returns:
         PagedPlan. A row whose pages the stack does not hold, or that would outgrow its line of the

@@ -60,3 +60,11 @@ def test_a_bound_on_rows_past_their_tokens_is_one_by_them(dtype, D):
     for longest in (21, 1000, (1 << 31) - 1, 1 << 31, (1 << 32) + 1, TOP):
         assert scratch(longest) == want, longest
     assert attention(longest=TOP, total=0) == _ext.OK
+
+
+def test_page_sizes_end_in_python_too():
+    from modelcore_amd.kernels.paged import check_page_size
+    assert check_page_size(1 << 30) == 1 << 30
+    for n in (1 << 31, 1 << 62):
+        with pytest.raises(ValueError, match="power of two"):
+            check_page_size(n)
