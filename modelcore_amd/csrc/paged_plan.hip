@@ -240,7 +240,7 @@ __global__ __launch_bounds__(kThreads) void release_kernel(int32_t *table, int64
     int64_t all = 0;
     s_end[tid] = group_scan(held, all, s_sum);
     __syncthreads();
-    auto entry = [&](int64_t p) {  // of page p of this round's rows in the table
+    auto entry = [&](int64_t p) {  // of page p of these rows, in the table
       int lo = 0, hi = kThreads - 1;  // the first row whose pages end past p
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
