@@ -446,6 +446,91 @@ int mcamd_flash_attn_paged_with_kvcache(
     int64_t page_stride, int64_t max_pages, int64_t window, int causal, int dtype, void *scratch,
     size_t scratch_bytes, void *stream);
 
+/*
+ * Drafted trees over the paged cache. A row's new tokens are nodes: node i, its index among them, is a guess at
+ * what follows node parents[i], one before it (-1: what follows the row itself), and lies behind the row's
+ * tokens like any new token, at slot position cache_seqlens[b] + i. Its mask is `mask_words` words (1 to 16) of
+ * 64 bits: bit j, j <= i, says that j is i itself or one of its ancestors. It stands at position
+ * cache_seqlens[b] + depth, depth being the number of its bits less one. A forward over them is
+ * mcamd_paged_reserve, mcamd_paged_tree, the layers with the two positions' rules below, then
+ * mcamd_verify_drafts and mcamd_paged_keep. No counterpart in the reference, whose decode loop takes a token a
+ * step (modelcore/generate.py:82-94).
+ */
+
+/*
+ * Masks, (total, mask_words), and positions, (total), of the nodes of all rows, packed by cu_seqlens
+ * (n_rows + 1). A node whose chain of parents does not go down (a parent that is not before its child, or
+ * below -1), one of a row of negative length, one at a position past 31 bits, one past 64 * mask_words of its
+ * row and tokens past the last row's get position -1 and no bits.
+ */
+int mcamd_paged_tree(const int32_t *parents, const int32_t *cu_seqlens, const int32_t *cache_seqlens,
+                     int32_t *positions, uint64_t *masks, int64_t n_rows, int64_t total,
+                     int64_t mask_words, void *stream);
+
+/*
+ * mcamd_flash_attn_paged_with_kvcache() for such nodes: node i of row b is written at position
+ * cache_seqlens[b] + i, and attends the row's tokens and the nodes of its mask, tree_masks (total,
+ * mask_words). With a window >= 0 it attends those at most `window` positions before its own: the row's tokens
+ * from cache_seqlens[b] + depth - window on, and the window + 1 last of its bits. Bits past a node's own do not
+ * count; a node that attends nothing at all (no bit, and no token of the row) gets zeros. max_seqlen is at most
+ * 64 * mask_words. All else is as there, with mcamd_paged_tree_scratch_bytes() of scratch.
+ */
+size_t mcamd_paged_tree_scratch_bytes(int64_t n_rows, int64_t total, int64_t max_seqlen, int64_t n_head,
+                                      int64_t n_kv_head, int64_t head_dim, int64_t max_pages,
+                                      int64_t page_size, int64_t window, int dtype);
+int mcamd_flash_attn_paged_tree_with_kvcache(
+    const void *q, const void *k, const void *v, void *k_pages, void *v_pages,
+    const int32_t *block_table, int64_t table_stride, const int32_t *cache_seqlens,
+    const int32_t *cu_seqlens, const uint64_t *tree_masks, int64_t mask_words, void *out, int64_t n_rows,
+    int64_t total, int64_t max_seqlen, int64_t n_head, int64_t n_kv_head, int64_t head_dim,
+    int64_t n_pages, int64_t page_size, int64_t page_stride, int64_t max_pages, int64_t window, int dtype,
+    void *scratch, size_t scratch_bytes, void *stream);
+
+/*
+ * How far the drafts of each row go, from the target's logits at every node, (total, vocab) fp32 with rows
+ * logits_stride apart, and a random number from [0, 1) for every node. tokens (total) are the nodes' tokens, node
+ * 0 the one the row ended with; the walk begins there. At a node with p = softmax(logits / temperature) its
+ * children are tried in the order of their indices:
+ *  - draft_probs (total, vocab) given, row i of which is the distribution q that the children of node i were
+ *    drawn from, independently: x is accepted if numbers[i] * Z * q(x) < max(p(x) - a q(x), 0); a = 0 and Z = 1
+ *    before the first, a + Z and sum(max(p - a q, 0)) after each that is refused;
+ *  - NULL, the drafts are guesses: x is accepted if numbers[i] * Z < p(x), Z = 1 - the p of those refused before
+ *    (a token that was refused there before has none left);
+ *  - temperature 0: x is accepted if it is the first of the largest logits (draft_probs is not read).
+ * Where none is, the row's last token is the first whose running sum of what is left, max(p - a q, 0) or p
+ * without the refused, passes numbers[node 0] times the whole (of p, where nothing is left). Probabilities and
+ * sums are in 64 bits. A NaN logit and -inf are probability 0, +inf logits share it all; of a node with no other
+ * logits nothing is accepted and the last token is 0. A child with a token outside [0, vocab) is passed over.
+ * kept (n_rows, max_seqlen) gets the accepted nodes, the root first, counts (n_rows) how many, out_tokens
+ * (n_rows, max_seqlen) the tokens after the root: those of the accepted nodes, then the last one, so as many;
+ * -1 past them. A row without nodes has counts 0. max_seqlen (at most 1024): nodes past it are left out.
+ * scratch: mcamd_verify_drafts_scratch_bytes(), 16-byte aligned, the call's own until it ends on the stream.
+ */
+size_t mcamd_verify_drafts_scratch_bytes(int64_t total, int64_t vocab);
+int mcamd_verify_drafts(const float *logits, int64_t logits_stride, const float *draft_probs,
+                        int64_t draft_stride, const int64_t *tokens, const int32_t *parents,
+                        const int32_t *cu_seqlens, const float *numbers, int32_t *kept, int32_t *counts,
+                        int64_t *out_tokens, int64_t n_rows, int64_t total, int64_t max_seqlen,
+                        int64_t vocab, float temperature, void *scratch, size_t scratch_bytes,
+                        void *stream);
+
+/*
+ * The rows keep the nodes that were accepted. Row b's nodes kept[b][0 .. counts[b]) (ascending indices, kept
+ * (n_rows, max_kept)) become its next tokens: in each of n_slots KV slots, slot_stride elements apart, the key
+ * and value of node kept[b][j] move to where node j's are (a node outside [j, new_lens[b]) stays where it is).
+ * Then cache_seqlens[b] goes up by counts[b], and the pages past it that the row's new_lens[b] nodes were given
+ * go back onto the stack, the rows in order, their table entries becoming -1. counts above new_lens[b] or
+ * max_kept count as that, negative ones as 0. A row that was refused its pages (the page of its last node is
+ * none of the pool) keeps nothing, and one whose nodes do not fit its line is left as it is. row_elems: H_kv * D.
+ * Pages that a row's nodes lie in are its own alone.
+ */
+int mcamd_paged_keep(void *k_pages, void *v_pages, int64_t n_slots, int64_t slot_stride,
+                     int32_t *block_table, int64_t table_stride, int32_t *cache_seqlens,
+                     const int32_t *new_lens, const int32_t *kept, int64_t max_kept,
+                     const int32_t *counts, int32_t *free_pages, int32_t *free_count, int64_t n_rows,
+                     int64_t max_pages, int64_t n_pages, int64_t page_size, int64_t page_stride,
+                     int64_t row_elems, int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -23,7 +23,7 @@ LIB_PATH = Path(os.environ.get("MODELCORE_AMD_LIB",
 F32, BF16 = 0, 1
 ACT_SILU = 0  # mcamd_linear_bf16_gated activations
 OK, EINVAL, EUNSUPPORTED, EWORKSPACE, ELAUNCH = 0, -1, -2, -3, -4
-ABI_VERSION = 8
+ABI_VERSION = 9
 NOALLOC_SCRATCH_BYTES = 32 << 20  # MCAMD_NOALLOC_SCRATCH_BYTES
 
 _i64 = ctypes.c_int64
@@ -92,6 +92,18 @@ SIGNATURES = {
                                                    _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64,
                                                    _i64, _i64, _i64, _i64, _i64, _int, _int, _ptr,
                                                    _size, _ptr]),
+    "mcamd_paged_tree": (_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _ptr]),
+    "mcamd_paged_tree_scratch_bytes": (_size, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                               _int]),
+    "mcamd_flash_attn_paged_tree_with_kvcache": (_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr,
+                                                        _ptr, _ptr, _i64, _ptr, _i64, _i64, _i64, _i64,
+                                                        _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int,
+                                                        _ptr, _size, _ptr]),
+    "mcamd_verify_drafts_scratch_bytes": (_size, [_i64, _i64]),
+    "mcamd_verify_drafts": (_int, [_ptr, _i64, _ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
+                                   _i64, _i64, _i64, _i64, ctypes.c_float, _ptr, _size, _ptr]),
+    "mcamd_paged_keep": (_int, [_ptr, _ptr, _i64, _i64, _ptr, _i64, _ptr, _ptr, _ptr, _i64, _ptr, _ptr,
+                                _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _int, _ptr]),
 }
 
 _LIB = None

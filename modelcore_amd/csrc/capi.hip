@@ -49,7 +49,7 @@ int check_attn_shapes(const AttnArgs &a, bool need_workspace) {
 
 using namespace mcamd;
 
-extern "C" int mcamd_abi_version(void) { return 8; }
+extern "C" int mcamd_abi_version(void) { return 9; }
 
 extern "C" const char *mcamd_last_error(void) { return g_last_error.c_str(); }
 

@@ -11,6 +11,7 @@
 
 #include "kernels.h"
 #include "prefill_split.h"
+#include "tree_bits.h"
 
 namespace mcamd {
 
@@ -44,6 +45,7 @@ struct PagedArgs {
   void *k_pages, *v_pages;
   PagedKv kv;
   const int32_t *seqlens, *cu;  // cu: packed rows of their own lengths; NULL = t_new tokens each
+  TreeMasks tree;               // masks: the new tokens are nodes of drafted trees; NULL = they follow one another
   void *out;
   int64_t n_rows, t_new, total, n_head, n_kv_head, head_dim, window;
   int dtype;
@@ -317,6 +319,7 @@ struct PagedTiles {
   };
   Cut *cuts;        // [slots]: the blocks of a call that may be cut, by their number
   int *n_cuts;      // and how many
+  TreeMasks tree;
 
   // Ranges of a block of n tiles: what pays for their partials, by the cost rule of prefill_split.h, none
   // much shorter than what starting it takes.

@@ -39,15 +39,17 @@ int check(const PagedArgs &a) {
 }
 
 // Pairs per KV head up to which a row counts as one of few pairs (few_pairs()): one block of the bf16
-// streaming kernel, and single tokens for the fp32 one.
-int64_t few_of(const PagedArgs &a) { return a.dtype == MCAMD_BF16 ? 32 : 1; }
+// streaming kernel, and single tokens for the fp32 one, which knows no trees.
+int64_t few_of(const PagedArgs &a) { return a.dtype == MCAMD_BF16 ? 32 : a.tree.masks ? 0 : 1; }
 
 struct Kernels {
   bool stream, tiles;
 };
 Kernels kernels_of(const PagedArgs &a) {
   const int64_t G = a.n_head / a.n_kv_head;
-  const bool few = a.t_new == 1 || a.t_new * G <= few_of(a);  // of every row
+  const int64_t most = few_of(a);
+  if (most == 0) return {false, true};
+  const bool few = a.t_new == 1 || a.t_new * G <= most;  // of every row
   return {few || a.cu != nullptr, !few};
 }
 
@@ -76,15 +78,8 @@ int launch(PagedArgs a) {
   return paged_mfma_supported(a) ? launch_paged_mfma(a, skip) : launch_paged_tiled(a, skip);
 }
 
-}  // namespace
-}  // namespace mcamd
-
-using namespace mcamd;
-
-extern "C" size_t mcamd_paged_scratch_bytes(int64_t n_rows, int64_t total, int64_t max_seqlen,
-                                            int64_t n_head, int64_t n_kv_head, int64_t head_dim,
-                                            int64_t max_pages, int64_t page_size, int64_t window,
-                                            int dtype) {
+size_t scratch_bytes(int64_t n_rows, int64_t total, int64_t max_seqlen, int64_t n_head, int64_t n_kv_head,
+                     int64_t head_dim, int64_t max_pages, int64_t page_size, int64_t window, int dtype, bool tree) {
   if (n_rows <= 0 || total <= 0 || max_seqlen <= 0 || n_kv_head <= 0 || n_head < n_kv_head ||
       head_dim <= 0 || head_dim > 256 || max_pages <= 0 || n_head > 65535 || n_rows > 65535 ||
       total > (int64_t(1) << 30) / n_head)
@@ -100,6 +95,8 @@ extern "C" size_t mcamd_paged_scratch_bytes(int64_t n_rows, int64_t total, int64
   a.head_dim = head_dim;
   a.window = std::min(window, int64_t(1) << 30);  // no position is past it
   a.dtype = dtype;
+  const uint64_t none = 0;
+  if (tree) a.tree.masks = &none;
   // The sizes do not tell packed rows from uniform ones: room for both.
   const int32_t packed = 0;
   size_t most = 0;
@@ -115,14 +112,35 @@ extern "C" size_t mcamd_paged_scratch_bytes(int64_t n_rows, int64_t total, int64
   return most;
 }
 
-extern "C" int mcamd_flash_attn_paged_with_kvcache(
-    const void *q, const void *k, const void *v, void *k_pages, void *v_pages,
-    const int32_t *block_table, int64_t table_stride, const int32_t *cache_seqlens,
-    const int32_t *cu_seqlens, void *out, int64_t n_rows, int64_t total, int64_t max_seqlen,
-    int64_t n_head, int64_t n_kv_head, int64_t head_dim, int64_t n_pages, int64_t page_size,
-    int64_t page_stride, int64_t max_pages, int64_t window, int causal, int dtype, void *scratch,
-    size_t scratch_bytes, void *stream) {
-  (void)causal;
+}  // namespace
+}  // namespace mcamd
+
+using namespace mcamd;
+
+extern "C" size_t mcamd_paged_scratch_bytes(int64_t n_rows, int64_t total, int64_t max_seqlen,
+                                            int64_t n_head, int64_t n_kv_head, int64_t head_dim,
+                                            int64_t max_pages, int64_t page_size, int64_t window,
+                                            int dtype) {
+  return scratch_bytes(n_rows, total, max_seqlen, n_head, n_kv_head, head_dim, max_pages, page_size, window, dtype,
+                       false);
+}
+
+extern "C" size_t mcamd_paged_tree_scratch_bytes(int64_t n_rows, int64_t total, int64_t max_seqlen,
+                                                 int64_t n_head, int64_t n_kv_head, int64_t head_dim,
+                                                 int64_t max_pages, int64_t page_size, int64_t window,
+                                                 int dtype) {
+  return scratch_bytes(n_rows, total, max_seqlen, n_head, n_kv_head, head_dim, max_pages, page_size, window, dtype,
+                       true);
+}
+
+namespace {
+
+int paged_attention(const void *q, const void *k, const void *v, void *k_pages, void *v_pages,
+                    const int32_t *block_table, int64_t table_stride, const int32_t *cache_seqlens,
+                    const int32_t *cu_seqlens, TreeMasks tree, void *out, int64_t n_rows, int64_t total,
+                    int64_t max_seqlen, int64_t n_head, int64_t n_kv_head, int64_t head_dim, int64_t n_pages,
+                    int64_t page_size, int64_t page_stride, int64_t max_pages, int64_t window, int dtype,
+                    void *scratch, size_t scratch_bytes, void *stream) {
   if ((k == nullptr) != (v == nullptr))
     return fail(MCAMD_EINVAL, "flash_attn_paged_with_kvcache: pass both k and v, or neither");
   PagedArgs a{};
@@ -153,6 +171,7 @@ extern "C" int mcamd_flash_attn_paged_with_kvcache(
   a.kv.max_pages = int(max_pages);
   a.seqlens = cache_seqlens;
   a.cu = cu_seqlens;
+  a.tree = tree;
   a.out = out;
   a.n_rows = n_rows;
   a.t_new = std::min(max_seqlen, total);  // no row has more, and 31 bits hold it
@@ -172,4 +191,40 @@ extern "C" int mcamd_flash_attn_paged_with_kvcache(
     return MCAMD_OK;
   }
   return launch(a);
+}
+
+}  // namespace
+
+extern "C" int mcamd_flash_attn_paged_with_kvcache(
+    const void *q, const void *k, const void *v, void *k_pages, void *v_pages,
+    const int32_t *block_table, int64_t table_stride, const int32_t *cache_seqlens,
+    const int32_t *cu_seqlens, void *out, int64_t n_rows, int64_t total, int64_t max_seqlen,
+    int64_t n_head, int64_t n_kv_head, int64_t head_dim, int64_t n_pages, int64_t page_size,
+    int64_t page_stride, int64_t max_pages, int64_t window, int causal, int dtype, void *scratch,
+    size_t scratch_bytes, void *stream) {
+  (void)causal;
+  return paged_attention(q, k, v, k_pages, v_pages, block_table, table_stride, cache_seqlens, cu_seqlens,
+                         TreeMasks{nullptr, 0}, out, n_rows, total, max_seqlen, n_head, n_kv_head, head_dim,
+                         n_pages, page_size, page_stride, max_pages, window, dtype, scratch, scratch_bytes,
+                         stream);
+}
+
+extern "C" int mcamd_flash_attn_paged_tree_with_kvcache(
+    const void *q, const void *k, const void *v, void *k_pages, void *v_pages,
+    const int32_t *block_table, int64_t table_stride, const int32_t *cache_seqlens,
+    const int32_t *cu_seqlens, const uint64_t *tree_masks, int64_t mask_words, void *out, int64_t n_rows,
+    int64_t total, int64_t max_seqlen, int64_t n_head, int64_t n_kv_head, int64_t head_dim, int64_t n_pages,
+    int64_t page_size, int64_t page_stride, int64_t max_pages, int64_t window, int dtype, void *scratch,
+    size_t scratch_bytes, void *stream) {
+  if (mask_words < 1 || mask_words > kMaxTreeWords || max_seqlen > 64 * mask_words)
+    return fail(MCAMD_EINVAL, "flash_attn_paged_tree_with_kvcache: a node has a mask of 1 to 16 words, 64 of a "
+                              "row's nodes a word");
+  if (!aligned(tree_masks, 8))
+    return fail(MCAMD_EINVAL, "flash_attn_paged_tree_with_kvcache: the masks must be 8-byte aligned");
+  if (!tree_masks && n_rows > 0 && total > 0 && max_seqlen > 0)
+    return fail(MCAMD_EINVAL, "flash_attn_paged_tree_with_kvcache: null pointer");
+  return paged_attention(q, k, v, k_pages, v_pages, block_table, table_stride, cache_seqlens, cu_seqlens,
+                         TreeMasks{tree_masks, int(mask_words)}, out, n_rows, total, max_seqlen, n_head,
+                         n_kv_head, head_dim, n_pages, page_size, page_stride, max_pages, window, dtype,
+                         scratch, scratch_bytes, stream);
 }

@@ -17,15 +17,16 @@ struct CarefulParams {
   void *out;
   int H_kv, window, D;
   float scale_log2;
+  TreeMasks tree;  // of calls over trees
 };
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
 // Dims [d0, d1) of one pair redone by a wave over the keys it sees alone, for pairs whose result is not
 // finite: 64 keys a step, a key per lane for its score, then a dim per lane (l, l + 64, ..) for the sums.
-template <class E, int DP, int LOADS = 32>  // LOADS: values (and 16-byte pieces of keys) in flight
+template <class E, int DP, int LOADS = 32, bool TREE = false>  // LOADS: values (and 16-byte pieces of keys) in flight
 __device__ void careful_pair(const CarefulParams &P, int row, int kvh, int64_t at, int p, int lane,
-                             int d0, int d1) {
+                             int d0, int d1, int64_t token = 0, int node = 0) {
   constexpr int N = (DP + 63) / 64, VEC = Vec<E>::N, U = N == 3 ? LOADS / 4 : LOADS / N;
   static_assert(64 % U == 0, "whole batches per step");
   const int D = P.D;
@@ -40,7 +41,13 @@ __device__ void careful_pair(const CarefulParams &P, int row, int kvh, int64_t a
 #pragma unroll
   for (int i = 0; i < N; ++i) o[i] = 0.f;
   float m = -INFINITY, l = 0.f;  // l: of this lane's keys
-  for (int t0 = key_lo(p, P.window); t0 <= p; t0 += 64) {
+  int from = key_lo(p, P.window);
+  TreeNode N_;  // TREE: node `node` of its row, token `token` of the call
+  if constexpr (TREE) {
+    N_ = TreeNode(P.tree, token, node, p - node, P.window);
+    from = N_.first();
+  }
+  for (int t0 = from; t0 <= p; t0 += 64) {
     const int t = min(t0 + lane, p);
     const int64_t t_at = key_at(t);
     float s = 0.f;
@@ -60,8 +67,10 @@ __device__ void careful_pair(const CarefulParams &P, int row, int kvh, int64_t a
         s = c0 + c * VEC < D ? dot : s;
       }
     }
-    if (t0 + lane > p) s = -INFINITY;
-    if (!P.kv.is_page(pages[t >> P.kv.shift])) s = NAN;
+    bool hidden = t0 + lane > p;
+    if constexpr (TREE) hidden = hidden || !((N_.seen(t0) >> lane) & 1);
+    if (hidden) s = -INFINITY;
+    if ((!TREE || !hidden) && !P.kv.is_page(pages[t >> P.kv.shift])) s = NAN;
     if (__builtin_amdgcn_ballot_w64(s != s) != 0) {  // a NaN key makes the output NaN, as in the softmax
       l = NAN;
       break;
@@ -90,7 +99,8 @@ __device__ void careful_pair(const CarefulParams &P, int row, int kvh, int64_t a
       }
     }
   }
-  const float inv = 1.f / wave_sum<64>(l);
+  const float all = wave_sum<64>(l);
+  const float inv = TREE && all == 0.f ? 0.f : 1.f / all;  // a node that sees no key at all gets zeros
 #pragma unroll
   for (int i = 0; i < N; ++i)
     if (lane + 64 * i >= d0 && lane + 64 * i < d1) out[lane + 64 * i] = from_f32<E>(o[i] * inv);

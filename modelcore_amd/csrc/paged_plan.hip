@@ -21,13 +21,11 @@
 // of as many tokens take 6.8), the rest the launch, a round trip for the page numbers, and stores of 4 and 8 bytes.
 //
 // release: one workgroup; 128 rows of up to 32 pages 7.8 us, 512 rows of 8000 pages 20.
-#include "paged.h"
+#include "paged_stack.h"
 
 namespace mcamd {
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / 64;
 constexpr int kOneLaunchTokens = 4096;
 constexpr int kTokens = 4;  // tokens of a thread
 
@@ -42,34 +40,6 @@ struct PlanParams {
   int64_t table_stride;
   int n_rows, max_pages, n_pages, shift, total;
 };
-
-// Inclusive sum over the wave.
-__device__ __forceinline__ int64_t wave_scan(int64_t x, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int64_t y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
-  }
-  return x;
-}
-
-// Inclusive sum of x over the workgroup, after `carry`; carry becomes the whole sum.
-__device__ __forceinline__ int64_t group_scan(int64_t x, int64_t &carry, int64_t *s_sum) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t y = wave_scan(x, lane);
-  __syncthreads();  // the sums of the scan before have been read
-  if (lane == 63) s_sum[wave] = y;
-  __syncthreads();
-  int64_t all = 0, before = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) before += s_sum[w];
-    all += s_sum[w];
-  }
-  y += carry + before;
-  carry += all;
-  return y;
-}
 
 // What the tokens need to know of the rows: in LDS where kThreads rows are the most, else where it lies.
 struct SharedRows {
@@ -240,47 +210,8 @@ __global__ __launch_bounds__(kThreads) void release_kernel(int32_t *table, int64
     int64_t all = 0;
     s_end[tid] = group_scan(held, all, s_sum);
     __syncthreads();
-    auto entry = [&](int64_t p) {  // of page p of these rows, in the table
-      int lo = 0, hi = kThreads - 1;  // the first row whose pages end past p
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (s_end[mid] > p)
-          hi = mid;
-        else
-          lo = mid + 1;
-      }
-      return s_row[lo] * table_stride + p - (lo ? s_end[lo - 1] : 0);
-    };
-    auto taken_from = [&](int64_t p) {
-      const int64_t at = entry(p);
-      const int id = table[at];
-      table[at] = -1;
-      return id;
-    };
-    auto is_page = [&](int id) { return uint32_t(id) < uint32_t(n_pages); };
-    const int64_t base = top;
-    bool odd = false;  // an entry is no page, or there are more than the stack has room for
-    for (int64_t p = tid; p < all; p += kThreads) {
-      if (base + p < n_pages) {
-        const int id = taken_from(p);
-        free_pages[base + p] = id;
-        odd = odd || !is_page(id);
-      } else {
-        odd = true;
-      }
-    }
-    top += all;
-    if (__syncthreads_or(odd)) {
-      // What is no page of the pool, as in a row that was refused and moved on all the same, is not one to
-      // give: the pages behind it move up, none past where its own thread has read it.
-      top = base;
-      for (int64_t p0 = 0; p0 < all; p0 += kThreads) {
-        const int64_t p = p0 + tid;
-        const int id = p >= all ? -1 : base + p < n_pages ? free_pages[base + p] : taken_from(p);
-        const int64_t to = group_scan(int64_t(is_page(id)), top, s_sum) - 1;
-        if (is_page(id) && to < n_pages) free_pages[to] = id;
-      }
-    }
+    top = push_pages(table, s_end, all, top, free_pages, n_pages, s_sum,
+                     [&](int i) { return s_row[i] * table_stride; });
     __syncthreads();  // s_row and s_end have been read
   }
   if (tid == 0) free_count[0] = int(min(top, int64_t(n_pages)));

@@ -39,6 +39,7 @@ struct StreamParams : CarefulParams {
   int head_waves;  // KV heads of a workgroup, in a large call
   int target;      // workgroups a call aims at; 0: no row is cut
   int pair_slots;  // pairs per partial slot
+  int early;       // of trees 1: a node without a bit stands a position before the row's next
   PagedAppend append;
   int blocks;      // workgroups from that one on append
 };
@@ -56,7 +57,7 @@ __device__ __forceinline__ Row row_of(const StreamParams &P, int b) {
   row_tokens(P.cu, P.t_new, P.total, b, r.tok0, r.T);
   r.s0 = P.seqlens[b];
   r.ok = r.s0 >= 0 && int64_t(r.s0) + r.T <= int64_t(P.kv.max_pages) << P.kv.shift;
-  r.lo = r.ok && P.window >= 0 ? max(0, r.s0 - P.window) : 0;
+  r.lo = r.ok && P.window >= 0 ? max(0, r.s0 - P.window - P.early) : 0;
   r.hi = r.ok ? r.s0 + r.T - 1 : 0;
   r.blocks = few_pairs(r.T, P.G, P.most) ? int(uint32_t(r.T * P.G + PB - 1) / PB) : 0;
   r.tiles = r.ok ? (r.hi / KT) - (r.lo / KT) + 1 : 1;
@@ -166,7 +167,7 @@ constexpr int64_t kManyPairs = 1024;
 // Workgroups of a packed call's merge, at most, beyond one per head of each row: three rows of 8 to 57
 // tokens of one head per KV head took 37 us with a workgroup a row and KV head.
 constexpr int64_t kMergeGroups = 1024;
-template <class E, int DP, int MW, int PB>
+template <class E, int DP, int MW, int PB, bool TREE>
 __global__ __launch_bounds__(64 * MW) void paged_stream_merge_kernel(StreamParams P) {
   constexpr int N = (DP + 63) / 64, U = 8;
   __shared__ float s_o[MW][DP], s_ml[MW][2];
@@ -234,7 +235,7 @@ __global__ __launch_bounds__(64 * MW) void paged_stream_merge_kernel(StreamParam
       ok = ok && (finite(o[i]) || lane + 64 * i >= P.D);
     }
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(!ok) != 0, 0)) {
-      careful_pair<E, DP, 8>(P, b, kvh, at, R.s0 + t, lane, 0, P.D);
+      careful_pair<E, DP, 8, TREE>(P, b, kvh, at, R.s0 + t, lane, 0, P.D, R.tok0 + t, t);
       continue;
     }
 #pragma unroll
@@ -305,6 +306,8 @@ StreamParams stream_params(const PagedArgs &a, const StreamPlan &p, int64_t most
   P.head_waves = p.head_waves;
   P.target = p.cut ? p.target : 0;
   P.pair_slots = p.pair_slots;
+  P.tree = a.tree;
+  P.early = a.tree.masks ? 1 : 0;
   P.append = paged_append(a, most);
   // A KV head at a time, or up to the target.
   P.blocks = int(std::min<int64_t>(
@@ -313,7 +316,7 @@ StreamParams stream_params(const PagedArgs &a, const StreamPlan &p, int64_t most
 }
 
 // kernel: the launch of a call's ranges, by E, DP (head dims, rounded up) and blocks of PB pairs.
-template <class E, int DP, int PB, class K>
+template <class E, int DP, int PB, bool TREE = false, class K>
 int launch_stream(K kernel, const StreamParams &P, const PagedArgs &a, const StreamPlan &p, bool others) {
   const int64_t blocks = P.blocks + (a.k_new && others ? paged_append_blocks(a) : 0);
   if (blocks > 0x7fffffff / kThreads || a.n_rows > 65535)
@@ -323,9 +326,9 @@ int launch_stream(K kernel, const StreamParams &P, const PagedArgs &a, const Str
   if (st != MCAMD_OK || !p.cut) return st;
   const dim3 grid{unsigned(a.n_kv_head * p.merge_pairs), unsigned(a.n_rows)};
   if ((a.cu ? a.n_rows * a.n_head : int64_t(grid.x) * grid.y) > kManyPairs)  // of a mixture, the single tokens
-    hipLaunchKernelGGL((paged_stream_merge_kernel<E, DP, 2, PB>), grid, dim3(128), 0, a.stream, P);
+    hipLaunchKernelGGL((paged_stream_merge_kernel<E, DP, 2, PB, TREE>), grid, dim3(128), 0, a.stream, P);
   else
-    hipLaunchKernelGGL((paged_stream_merge_kernel<E, DP, 8, PB>), grid, dim3(512), 0, a.stream, P);
+    hipLaunchKernelGGL((paged_stream_merge_kernel<E, DP, 8, PB, TREE>), grid, dim3(512), 0, a.stream, P);
   return launch_status("paged_stream_merge");
 }
 

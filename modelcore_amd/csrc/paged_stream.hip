@@ -127,7 +127,7 @@ __device__ __forceinline__ float sum_halves(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-template <int DP>
+template <int DP, bool TREE>
 __global__ __launch_bounds__(kThreads)
     __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 2 : 1))) void paged_stream_kernel(StreamParams P) {
   using S_ = Shape<DP>;
@@ -321,8 +321,15 @@ __global__ __launch_bounds__(kThreads)
     if (more) load_k(tile + n_kw, next);
 
     // Keys the pair may not see.
-    if (k0 + KT - 1 > R.s0 + t_first || k0 < seen_from ||
-        (P.window >= 0 && k0 < R.s0 + t_last - P.window)) {
+    if constexpr (TREE) {
+      if (k0 + KT - 1 >= R.s0 || (P.window >= 0 && k0 < R.s0 + t_last - P.window)) {
+        const uint64_t seen = TreeNode(P.tree, R.tok0 + t_q, t_q, R.s0, P.window).seen(k0) >> (4 * h);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (!((seen >> (8 * (e >> 2) + (e & 3))) & 1)) s[e] = -INFINITY;
+      }
+    } else if (k0 + KT - 1 > R.s0 + t_first || k0 < seen_from ||
+               (P.window >= 0 && k0 < R.s0 + t_last - P.window)) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int gap = p_abs - (k0 + 8 * (e >> 2) + 4 * h + (e & 3));
@@ -495,10 +502,20 @@ __global__ __launch_bounds__(kThreads)
   for (int md = 0; md < MD; ++md)
     for (uint32_t left = __builtin_amdgcn_readlane(bad_of, md); left != 0; left &= left - 1) {
       const int pr = block * 32 + __builtin_ctz(left), t = pr / P.G;
-      careful_pair<bf16, DP, 8>(P, b, kvh,
-                                (int64_t(R.tok0 + t) * P.H + kvh * P.G + (pr - t * P.G)) * D, R.s0 + t,
-                                lane, 32 * md, min(32 * md + 32, D));
+      careful_pair<bf16, DP, 8, TREE>(P, b, kvh,
+                                      (int64_t(R.tok0 + t) * P.H + kvh * P.G + (pr - t * P.G)) * D,
+                                      R.s0 + t, lane, 32 * md, min(32 * md + 32, D), R.tok0 + t, t);
     }
+}
+
+template <bool TREE>
+int run(const StreamParams &P, const PagedArgs &a, const StreamPlan &p, bool others) {
+  switch (head_pad(a.head_dim)) {
+    case 32: return launch_stream<bf16, 32, kPairs, TREE>(paged_stream_kernel<32, TREE>, P, a, p, others);
+    case 64: return launch_stream<bf16, 64, kPairs, TREE>(paged_stream_kernel<64, TREE>, P, a, p, others);
+    case 128: return launch_stream<bf16, 128, kPairs, TREE>(paged_stream_kernel<128, TREE>, P, a, p, others);
+    default: return launch_stream<bf16, 256, kPairs, TREE>(paged_stream_kernel<256, TREE>, P, a, p, others);
+  }
 }
 
 }  // namespace
@@ -511,12 +528,7 @@ int launch_paged_stream(const PagedArgs &a, int64_t most, bool others) {
   StreamPlan p = stream_plan(a, most, kPairs, kFill);
   if (p.cut && (!a.scratch || a.scratch_bytes < stream_bytes(a, p))) p.cut = false;
   const StreamParams P = stream_params(a, p, most);
-  switch (head_pad(a.head_dim)) {
-    case 32: return launch_stream<bf16, 32, kPairs>(paged_stream_kernel<32>, P, a, p, others);
-    case 64: return launch_stream<bf16, 64, kPairs>(paged_stream_kernel<64>, P, a, p, others);
-    case 128: return launch_stream<bf16, 128, kPairs>(paged_stream_kernel<128>, P, a, p, others);
-    default: return launch_stream<bf16, 256, kPairs>(paged_stream_kernel<256>, P, a, p, others);
-  }
+  return a.tree.masks ? run<true>(P, a, p, others) : run<false>(P, a, p, others);
 }
 
 }  // namespace mcamd

@@ -106,7 +106,7 @@ __device__ __forceinline__ void store4(bf16 *p, const f32x4 &x) {
       __builtin_bit_cast(uint2, __builtin_convertvector(x, bf16x4));
 }
 
-template <class E, int DP, int KS>
+template <class E, int DP, int KS, bool TREE>
 __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
   using G_ = Geo<E, DP, KS>;
   constexpr bool kBf16 = G_::kBf16;
@@ -162,7 +162,7 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
   const int p_abs = s0 + tq;
   const int p_first = s0 + q0;
   const int last = s0 + pair_pos(n - 1);  // the last key any pair of the workgroup sees
-  int lo = P.window >= 0 ? max(0, p_first - P.window) : 0, hi = last;
+  int lo = P.window >= 0 ? max(0, (TREE ? s0 - 1 : p_first) - P.window) : 0, hi = last;
   int n_tiles = (hi - lo) / KT + 1;
   bool whole = true;
   if (blk.noted) {  // this workgroup's range of the block's tiles
@@ -284,7 +284,16 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
       if constexpr (!kBf16) s[mk] = (sc[0] + sc[1]) + (sc[2] + sc[3]);
     }
     // Keys the pair may not see, in tiles that straddle the diagonal or the window's edge.
-    if (k0 + KW - 1 > p_first || (P.window >= 0 && k0 < last - P.window)) {
+    if constexpr (TREE) {
+      if (k0 + KW - 1 >= s0 || (P.window >= 0 && k0 < last - P.window)) {
+        const uint64_t seen = TreeNode(P.tree, tok0 + tq, tq, s0, P.window).seen(k0) >> (4 * h);
+#pragma unroll
+        for (int mk = 0; mk < MK; ++mk)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (!((seen >> (32 * mk + 8 * (e >> 2) + (e & 3))) & 1)) s[mk][e] = -INFINITY;
+      }
+    } else if (k0 + KW - 1 > p_first || (P.window >= 0 && k0 < last - P.window)) {
 #pragma unroll
       for (int mk = 0; mk < MK; ++mk)
 #pragma unroll
@@ -404,7 +413,8 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
     }
     for (uint32_t left = bad; __builtin_expect(left != 0, 0); left &= left - 1) {
       const int c = w0 + __builtin_ctz(left);
-      careful_pair<E, DP>(P, row, kvh, pair_at(c), s0 + pair_pos(c), lane, 0, D);
+      careful_pair<E, DP, 32, TREE>(P, row, kvh, pair_at(c), s0 + pair_pos(c), lane, 0, D,
+                                    tok0 + pair_pos(c), pair_pos(c));
     }
   } else {
     // Merge the four waves' (o, m, l) of the same 32 pairs; thread t then owns an eighth of the
@@ -476,7 +486,8 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
     }
     for (int x = wave; x < 32; x += kWaves) {
       if (__builtin_expect(s_bad[x] == 0, 1)) continue;
-      careful_pair<E, DP>(P, row, kvh, pair_at(x), s0 + pair_pos(x), lane, 0, D);
+      careful_pair<E, DP, 32, TREE>(P, row, kvh, pair_at(x), s0 + pair_pos(x), lane, 0, D,
+                                    tok0 + pair_pos(x), pair_pos(x));
     }
   }
 }
@@ -485,7 +496,7 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
 // a block, a wave per step j of them, eight ranges' loads in flight. What the blocks are, and whether any is
 // cut, the kernel before has left (each workgroup finding its block again took 10.4 us where none was cut:
 // 17 rows of up to 10 tokens, 32 / 8 heads).
-template <class E>
+template <class E, bool TREE>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(TiledParams P, int pairs) {
   const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
   const int j = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -549,8 +560,9 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(TiledParams P, in
     store4(static_cast<E *>(P.out) + pair_at(in_block) + d + 4 * h, y);
   for (uint32_t left = bad; __builtin_expect(left != 0, 0); left &= left - 1) {
     const int c = __builtin_ctz(left);
-    careful_pair<E, 256, 4>(P, blk.b, kvh, pair_at(32 * w + c), blk.s0 + __builtin_amdgcn_readlane(t, c),
-                            lane, d, min(d + 8, P.D));
+    const int t_c = __builtin_amdgcn_readlane(t, c);
+    careful_pair<E, 256, 4, TREE>(P, blk.b, kvh, pair_at(32 * w + c), blk.s0 + t_c, lane, d, min(d + 8, P.D),
+                                  int64_t(blk.tok0) + t_c, t_c);
   }
 }
 
@@ -609,6 +621,7 @@ TiledParams tiled_params(const PagedArgs &a, const PagedTiles &tiles) {
   P.window = int(a.window < 0 ? -1 : a.window);
   P.D = int(a.head_dim);
   P.scale_log2 = float(kLog2e / std::sqrt(double(a.head_dim)));
+  P.tree = a.tree;
   P.seqlens = a.seqlens;
   P.cu = a.cu;
   P.T_new = int(a.t_new);
@@ -628,8 +641,12 @@ int run(const TiledParams &P, const PagedArgs &a, const TiledPlan &t) {
   const int64_t blocks = std::max<int64_t>(t.bound * P.H_kv, P.tiles.slots);
   if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
   if (blocks == 0) return MCAMD_OK;
-  hipLaunchKernelGGL((paged_tiled_kernel<E, DP, KS>), dim3(unsigned(blocks)), dim3(kThreads), 0,
-                     a.stream, P);
+  if (a.tree.masks)
+    hipLaunchKernelGGL((paged_tiled_kernel<E, DP, KS, true>), dim3(unsigned(blocks)), dim3(kThreads), 0,
+                       a.stream, P);
+  else
+    hipLaunchKernelGGL((paged_tiled_kernel<E, DP, KS, false>), dim3(unsigned(blocks)), dim3(kThreads), 0,
+                       a.stream, P);
   const int st = launch_status("paged_tiled");
   if (st != MCAMD_OK || P.tiles.slots == 0) return st;
   return launch_paged_tiles_merge(a, P.tiles, t.pairs, t.bound);
@@ -661,10 +678,10 @@ int launch_paged_tiles_merge(const PagedArgs &a, const PagedTiles &tiles, int pa
   const int64_t blocks = std::min<int64_t>(bound * P.H_kv, tiles.slots) * tiles.groups * P.md;
   if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
   const dim3 grid{unsigned(blocks)}, threads{kThreads};
-  if (a.dtype == MCAMD_BF16)
-    hipLaunchKernelGGL(paged_merge_kernel<bf16>, grid, threads, 0, a.stream, P, pairs);
-  else
-    hipLaunchKernelGGL(paged_merge_kernel<float>, grid, threads, 0, a.stream, P, pairs);
+  const bool bf = a.dtype == MCAMD_BF16;
+  const auto kernel = a.tree.masks ? bf ? paged_merge_kernel<bf16, true> : paged_merge_kernel<float, true>
+                                   : bf ? paged_merge_kernel<bf16, false> : paged_merge_kernel<float, false>;
+  hipLaunchKernelGGL(kernel, grid, threads, 0, a.stream, P, pairs);
   return launch_status("paged_merge");
 }
 

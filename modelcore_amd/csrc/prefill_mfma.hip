@@ -164,8 +164,8 @@ typedef const __attribute__((address_space(4))) int32_t *scalar_ints;  // read o
 // SPLIT: a workgroup per key range of a block (prefill_split.h), which takes the chunk's own keys from
 // k_new and v_new where they are given (the merge appends them). VARLEN: sequences of their own
 // lengths, packed along the token axis. PAGED: keys and values in pages, rows of any lengths, blocks cut
-// where T has room.
-template <bool SPLIT, bool VARLEN, bool PAGED = false>
+// where T has room. TREE: a row's tokens are nodes of a drafted tree.
+template <bool SPLIT, bool VARLEN, bool PAGED = false, bool TREE = false>
 __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const SplitGeo *S,
                                                   const uint16_t *k_new, const uint16_t *v_new,
                                                   const PagedTiles *T = nullptr) {
@@ -259,7 +259,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   const int p_abs = s0 + pos;
   const int p_first = s0 + q0;
   const int p_last = s0 + q_end - 1;
-  int lo = P.window >= 0 ? max(0, p_first - P.window) : 0;
+  int lo = P.window >= 0 ? max(0, (TREE ? s0 - 1 : p_first) - P.window) : 0;
   int hi = p_last;
   const int seen_from = lo;  // PAGED: tiles begin before it, at a multiple of their keys
   if constexpr (PAGED) lo &= ~(KT - 1);
@@ -448,6 +448,17 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   };
   // Masks the keys the pair may not see (tiles that straddle the diagonal or the window edge).
   auto mask = [&](f32x16 (&s)[2], int k0) {
+    if constexpr (TREE) {
+      if (k0 + KT - 1 >= s0 || (P.window >= 0 && k0 < p_last - P.window)) {
+        const uint64_t seen = TreeNode(T->tree, tok0 + pos, pos, s0, P.window).seen(k0) >> (4 * h);
+#pragma unroll
+        for (int mk = 0; mk < 2; ++mk)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (!((seen >> (32 * mk + 8 * (e >> 2) + (e & 3))) & 1)) s[mk][e] = -INFINITY;
+      }
+      return;
+    }
     const bool need_mask = (k0 + KT - 1 > p_first) || (P.window >= 0 && k0 < p_last - P.window);
     if (need_mask) {
 #pragma unroll
@@ -753,12 +764,13 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
       for (int e = 0; e < 16; ++e) ok = ok && finite(o[md][e] * inv);
     const uint64_t bad64 = __builtin_amdgcn_ballot_w64(live && !ok);
     if (__builtin_expect(bad64 != 0, 0)) {
-      const CarefulParams C{P.q, P.k_cache, P.v_cache, T->kv, P.out, P.H_kv, P.window, D, P.scale_log2};
+      const CarefulParams C{P.q,  P.k_cache, P.v_cache,    T->kv, P.out, P.H_kv, P.window, D,
+                            P.scale_log2, T->tree};
       for (uint32_t left = uint32_t(bad64) | uint32_t(bad64 >> 32); left != 0; left &= left - 1) {
         const int pr2 = wave * 32 + __builtin_ctz(left), t = q0 + pr2 / P.G;
-        careful_pair<bf16, D, 8>(C, row, kvh,
-                                 ((tok0 + t) * P.H + int64_t(kvh) * P.G + (pr2 - pr2 / P.G * P.G)) * D,
-                                 s0 + t, lane, 0, D);
+        careful_pair<bf16, D, 8, TREE>(C, row, kvh,
+                                       ((tok0 + t) * P.H + int64_t(kvh) * P.G + (pr2 - pr2 / P.G * P.G)) * D,
+                                       s0 + t, lane, 0, D, tok0 + t, t);
       }
       if ((uint32_t(bad64 >> col) | uint32_t(bad64 >> (32 + col))) & 1u) return;
     }
@@ -801,6 +813,9 @@ __global__ __launch_bounds__(kThreads, 1) void prefill_mfma_varlen_kernel(MfmaPa
 }
 __global__ __launch_bounds__(kThreads, 1) void paged_mfma_kernel(MfmaParams P, PagedTiles T) {
   prefill_mfma_body<false, false, true>(P, nullptr, nullptr, nullptr, &T);
+}
+__global__ __launch_bounds__(kThreads, 1) void paged_tree_mfma_kernel(MfmaParams P, PagedTiles T) {
+  prefill_mfma_body<false, false, true, true>(P, nullptr, nullptr, nullptr, &T);
 }
 __global__ __launch_bounds__(kThreads, 1) void prefill_mfma_split_kernel(
     MfmaParams P, SplitGeo S, const uint16_t *k_new, const uint16_t *v_new) {
@@ -920,6 +935,7 @@ int launch_paged_mfma(const PagedArgs &a, int64_t skip) {
   P.scale_log2 = float(kLog2e / std::sqrt(double(D)));
   PagedTiles T{};
   T.kv = a.kv;
+  T.tree = a.tree;
   T.n_rows = int(a.n_rows);
   T.total = int(a.total);
   T.skip = int(skip);
@@ -933,7 +949,8 @@ int launch_paged_mfma(const PagedArgs &a, int64_t skip) {
   const int64_t blocks = std::max<int64_t>(bound * P.H_kv, T.slots);
   if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
   if (blocks == 0) return MCAMD_OK;
-  hipLaunchKernelGGL(paged_mfma_kernel, dim3(unsigned(blocks)), dim3(kThreads), 0, a.stream, P, T);
+  hipLaunchKernelGGL(a.tree.masks ? paged_tree_mfma_kernel : paged_mfma_kernel, dim3(unsigned(blocks)),
+                     dim3(kThreads), 0, a.stream, P, T);
   const int st = launch_status("paged_mfma");
   if (st != MCAMD_OK || T.slots == 0) return st;
   return launch_paged_tiles_merge(a, T, P.QT * P.G, bound);

@@ -320,23 +320,29 @@ def _paged_scratch_bytes(device_index, *sizes):
     return _ext.lib().mcamd_paged_scratch_bytes(*sizes)
 
 
-def _check_paged_positions(block_table, seqlens, lens, n_pages, page, window):
+@functools.lru_cache(maxsize=1024)
+def _tree_scratch_bytes(device_index, *sizes):
+    """mcamd_paged_tree_scratch_bytes, likewise."""
+    return _ext.lib().mcamd_paged_tree_scratch_bytes(*sizes)
+
+
+def _check_paged_positions(block_table, seqlens, lens, n_pages, page, window, what):
     """Checked mode over a paged cache: every position within its row's line of the table, every page
     that is read or written a page of the pool."""
     if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("flash_attn_paged_with_kvcache: checked mode reads the block table on the "
+        raise RuntimeError(f"{what}: checked mode reads the block table on the "
                            "host and cannot run under graph capture; call set_checked(False) first")
     table, room = block_table.tolist(), block_table.shape[1] * page
     for b, (s0, n) in enumerate(zip(seqlens.tolist(), lens)):
         if n == 0:
             continue
         if s0 < 0 or s0 + n > room:
-            raise IndexError(f"flash_attn_paged_with_kvcache: positions [{s0}, {s0 + n}) of row {b} "
+            raise IndexError(f"{what}: positions [{s0}, {s0 + n}) of row {b} "
                              f"fall outside the {room} of its line of the block table")
         first = max(0, s0 - window) if window >= 0 else 0
         for i in range(first // page, (s0 + n - 1) // page + 1):
             if not 0 <= table[b][i] < n_pages:
-                raise IndexError(f"flash_attn_paged_with_kvcache: page {table[b][i]} of row {b} is "
+                raise IndexError(f"{what}: page {table[b][i]} of row {b} is "
                                  f"not one of the pool's {n_pages}")
 
 
@@ -370,7 +376,38 @@ def flash_attn_paged_with_kvcache(q, k_pages, v_pages, k=None, v=None, *, block_
         NaN and appends nothing, and a query that sees a key in a page outside the pool is NaN; in
         checked mode (``set_checked``) such a call raises IndexError instead.
     """
-    what = "flash_attn_paged_with_kvcache"
+    return _paged_attention("flash_attn_paged_with_kvcache", q, k_pages, v_pages, k, v, None, block_table,
+                            cache_seqlens, cu_seqlens, max_seqlen, causal, window_size)
+
+
+def flash_attn_paged_tree_with_kvcache(q, k_pages, v_pages, k=None, v=None, *, tree_masks=None,
+                                       block_table=None, cache_seqlens=None, cu_seqlens=None,
+                                       max_seqlen=None, window_size=(-1, -1)):
+    """flash_attn_paged_with_kvcache for rows whose new tokens are nodes of a drafted tree, each of which
+    attends the row's tokens, its ancestors and itself. Extension with no counterpart in the reference.
+
+    Args:
+        q, k_pages, v_pages, k, v, block_table, cache_seqlens, cu_seqlens: as there; node i of row b is
+            its token i, written behind the row's tokens at cache_seqlens[b] + i.
+        tree_masks: (B, T_new, words), or, with cu_seqlens, (total, words) int64 (``paged_tree``): bit
+            j % 64 of a node's word j // 64, j up to its own index, says that node j is itself or one of
+            its ancestors. Words for every node of the longest row, at most 16.
+        window_size: (left, right); left = -1 means unlimited. A node stands at position cache_seqlens[b]
+            + depth, its bits less one: of its ancestors it attends the `left` nearest, of the row's
+            tokens those at most `left` positions before it.
+
+    Returns:
+        A tensor of q's shape and dtype, NaN where flash_attn_paged_with_kvcache's would be, zeros for a
+        node that attends nothing (no bits, and no tokens in its row).
+    """
+    return _paged_attention("flash_attn_paged_tree_with_kvcache", q, k_pages, v_pages, k, v,
+                            () if tree_masks is None else tree_masks, block_table, cache_seqlens,
+                            cu_seqlens, max_seqlen, True, window_size)
+
+
+def _paged_attention(what, q, k_pages, v_pages, k, v, masks, block_table, cache_seqlens, cu_seqlens,
+                     max_seqlen, causal, window_size):
+    """Both operators over pages; masks: the nodes' (with trees), or None."""
     _ext.require_rocm(q, what=what)  # the others are on its device, checked below
     packed = cu_seqlens is not None
     shape = q.shape
@@ -423,6 +460,14 @@ def flash_attn_paged_with_kvcache(q, k_pages, v_pages, k=None, v=None, *, block_
         raise ValueError(f"n_head {H} is not a multiple of n_kv_head {H_kv}")
     _ext.same_device(dev, k=k, v=v, block_table=block_table, cu_seqlens=cu_seqlens)
     seqlens = _check_seqlens(cache_seqlens, B, dev)
+    if masks is not None:
+        given = getattr(masks, "shape", ())
+        if len(given) != len(shape) - 1 or given[:-1] != shape[:-2] or masks.dtype != torch.int64 \
+                or not 1 <= given[-1] <= 16 or longest > 64 * given[-1]:
+            raise ValueError(f"tree_masks is required: {(*shape[:-2], 'words')} int64, words for "
+                             f"{longest} nodes, at most 16; got {tuple(given)}")
+        _ext.same_device(dev, tree_masks=masks)
+        masks = masks.contiguous()
     w = _window(window_size)
     if CHECK_POSITIONS and B > 0:
         lens = [longest] * B
@@ -433,23 +478,28 @@ def flash_attn_paged_with_kvcache(q, k_pages, v_pages, k=None, v=None, *, block_
                 raise IndexError(f"{what}: cu_seqlens must ascend from 0 to at most {total} in "
                                  f"steps of at most max_seqlen {longest}")
             lens = [y - x for x, y in zip(ends, ends[1:])]
-        _check_paged_positions(block_table, seqlens, lens, n_pages, page, w)
+        _check_paged_positions(block_table, seqlens, lens, n_pages, page, w, what)
     q = q.contiguous()
     if k is not None:
         k, v = k.contiguous(), v.contiguous()
     out = torch.empty_like(q)
     with _ext.on_device(dev):
-        nbytes = _paged_scratch_bytes(dev.index, B, total, longest, H, H_kv, D, max_pages, page, w,
-                                      code)
+        nbytes = (_paged_scratch_bytes if masks is None else _tree_scratch_bytes)(
+            dev.index, B, total, longest, H, H_kv, D, max_pages, page, w, code)
         # Scratch of the call's own: calls on several streams, and captured graphs, share nothing.
         ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-        st = _ext.lib().mcamd_flash_attn_paged_with_kvcache(
-            q.data_ptr(), k.data_ptr() if k is not None else None,
-            v.data_ptr() if v is not None else None, k_pages.data_ptr(), v_pages.data_ptr(),
-            block_table.data_ptr(), line, seqlens.data_ptr(),
-            cu_seqlens.data_ptr() if packed else None, out.data_ptr(), B, total, longest, H, H_kv, D,
-            n_pages, page, stride, max_pages, w, int(bool(causal)), code,
-            ws.data_ptr() if ws is not None else None, nbytes, _ext.stream_handle(dev))
+        operands = (q.data_ptr(), k.data_ptr() if k is not None else None,
+                    v.data_ptr() if v is not None else None, k_pages.data_ptr(), v_pages.data_ptr(),
+                    block_table.data_ptr(), line, seqlens.data_ptr(),
+                    cu_seqlens.data_ptr() if packed else None)
+        sizes = (out.data_ptr(), B, total, longest, H, H_kv, D, n_pages, page, stride, max_pages, w)
+        scratch = (code, ws.data_ptr() if ws is not None else None, nbytes, _ext.stream_handle(dev))
+        if masks is None:
+            st = _ext.lib().mcamd_flash_attn_paged_with_kvcache(*operands, *sizes, int(bool(causal)),
+                                                                *scratch)
+        else:
+            st = _ext.lib().mcamd_flash_attn_paged_tree_with_kvcache(
+                *operands, masks.data_ptr(), masks.shape[-1], *sizes, *scratch)
     _ext.check(st, what)
     return out
 
@@ -496,6 +546,7 @@ flash_attn = SimpleNamespace(
     flash_attn_with_kvcache=flash_attn_with_kvcache,
     flash_attn_varlen_with_kvcache=flash_attn_varlen_with_kvcache,
     flash_attn_paged_with_kvcache=flash_attn_paged_with_kvcache,
+    flash_attn_paged_tree_with_kvcache=flash_attn_paged_tree_with_kvcache,
     # Keyword arguments of flash_attn_with_kvcache beyond the reference's (callers check this
     # before passing them, so that an operator without them can stand in).
     EXTENSIONS=frozenset({"advance", "shared_prefix"}),

@@ -9,6 +9,10 @@ rows that have ended. Neither reads anything on the host, so both can sit in a c
 same inputs always give the same pages. ``modelcore_amd.cache.PagedKVCache`` keeps the tables and calls
 both.
 
+A row's new tokens may be a drafted tree instead of a sequence (``flash_attn_paged_tree_with_kvcache``):
+``paged_tree`` then says where its nodes stand and whom they see, and ``paged_keep`` makes the accepted
+ones the row's next tokens, in place, and gives back the pages that the others were in.
+
 There is no counterpart in the reference, whose cache reserves T_max positions for every row
 (modelcore/cache.py:22-23).
 """
@@ -20,7 +24,10 @@ import torch
 
 from modelcore_amd import _ext
 
-__all__ = ["PagedPlan", "paged_reserve", "paged_release", "check_page_size"]
+__all__ = ["PagedPlan", "TreePlan", "paged_reserve", "paged_release", "paged_tree", "paged_keep",
+           "check_page_size"]
+
+MAX_TREE_NODES = 1024  # of a row
 
 
 class PagedPlan(NamedTuple):
@@ -152,3 +159,130 @@ def paged_release(block_table, cache_seqlens, rows, free_pages, free_count, *, p
             rows.numel(), n, free_pages.data_ptr(), free_count.data_ptr(), max_pages,
             n_pages, page_size, _ext.stream_handle(dev))
     _ext.check(st, "paged_release")
+
+
+class TreePlan(NamedTuple):
+    """The nodes of a forward's drafted trees (``paged_tree``)."""
+    positions: torch.Tensor  # (total,) int32: the row's tokens + the node's depth, or -1
+    masks: torch.Tensor      # (total, words) int64: the node's ancestors and itself, 64 nodes a word
+
+
+def paged_tree(parents, cu_seqlens, cache_seqlens, *, max_seqlen) -> TreePlan:
+    """Positions and ancestors of drafted nodes. Node i of a row, i its index among the row's new tokens,
+    is a guess at what follows node parents[i], which comes before it (-1: what follows the row's tokens).
+
+    Args:
+        parents: (total,) int32, the rows' nodes one after another
+        cu_seqlens: (rows + 1,) int32 offsets of the rows (``PagedPlan.cu_seqlens``)
+        cache_seqlens: (rows,) int32, each row's tokens so far (read only)
+        max_seqlen: at least the nodes of the widest row (host int), at most 1024
+
+    Returns:
+        TreePlan, with ceil(max_seqlen / 64) words a node. A node whose chain of parents does not go down
+        to -1, one of a row of negative length or at a position past 31 bits, and one that is past its row's
+        last word or past the last row, has position -1 and no bits.
+    """
+    what = "paged_tree"
+    _ext.require_rocm(parents, what=what)
+    dev = parents.device
+    _ext.same_device(dev, cu_seqlens=cu_seqlens, cache_seqlens=cache_seqlens)
+    for name, t in (("parents", parents), ("cu_seqlens", cu_seqlens), ("cache_seqlens", cache_seqlens)):
+        if t.dtype != torch.int32 or t.dim() != 1:
+            raise ValueError(f"{name} must be one-dimensional int32; got {tuple(t.shape)} {t.dtype}")
+    n, total, max_seqlen = cache_seqlens.numel(), parents.numel(), int(max_seqlen)
+    if cu_seqlens.numel() != n + 1:
+        raise ValueError(f"cu_seqlens must be ({n + 1},) int32; got {tuple(cu_seqlens.shape)}")
+    if not 0 <= max_seqlen <= MAX_TREE_NODES:
+        raise ValueError(f"max_seqlen must be 0 to {MAX_TREE_NODES}; got {max_seqlen}")
+    words = max(1, -(-max_seqlen // 64))
+    parents, cu_seqlens, cache_seqlens = (t.contiguous() for t in (parents, cu_seqlens, cache_seqlens))
+    positions = torch.empty_like(parents)
+    masks = parents.new_empty((total, words), dtype=torch.int64)
+    with _ext.on_device(dev):
+        st = _ext.lib().mcamd_paged_tree(parents.data_ptr(), cu_seqlens.data_ptr(),
+                                         cache_seqlens.data_ptr(), positions.data_ptr(), masks.data_ptr(),
+                                         n, total, words, _ext.stream_handle(dev))
+    _ext.check(st, what)
+    return TreePlan(positions, masks)
+
+
+def _check_keep(block_table, cache_seqlens, new_lens, kept, counts, page_size, n_pages):
+    """Checked mode: every row's kept nodes are some of its own, ascending, and its pages the pool's."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("paged_keep: checked mode reads the block table on the host and cannot run under "
+                           "graph capture; call set_checked(False) first")
+    table, width = block_table.tolist(), block_table.shape[1]
+    rows = zip(cache_seqlens.tolist(), new_lens.tolist(), counts.tolist(), kept.tolist())
+    for b, (s, t, c, nodes) in enumerate(rows):
+        if not 0 <= c <= min(max(t, 0), kept.shape[1]):
+            raise IndexError(f"paged_keep: row {b} keeps {c} of its {t} nodes")
+        if c and not all(j <= i < t for j, i in enumerate(nodes[:c])) or \
+                any(x >= y for x, y in zip(nodes[:c], nodes[1:c])):
+            raise IndexError(f"paged_keep: row {b} keeps nodes {nodes[:c]} of {t}, which are not ascending "
+                             "nodes of it")
+        if s < 0 or t > 0 and s + t > width * page_size:
+            raise IndexError(f"paged_keep: positions [{s}, {s + t}) of row {b} fall outside the "
+                             f"{width * page_size} of its line of the block table")
+        for i in range(s // page_size, -(-(s + max(t, 0)) // page_size)):
+            if not 0 <= table[b][i] < n_pages:
+                raise IndexError(f"paged_keep: page {table[b][i]} of row {b} is not one of the pool's {n_pages}")
+
+
+def paged_keep(k_pages, v_pages, block_table, cache_seqlens, new_lens, kept, counts, free_pages, free_count):
+    """The rows keep the accepted ones of the nodes they were given pages for (``paged_reserve``): node
+    kept[b, j] becomes token cache_seqlens[b] + j of row b, its key and value moving there in every slot,
+    cache_seqlens goes up by counts, and pages that no token is left in go back onto the stack. All in
+    place, and without a host read.
+
+    Args:
+        k_pages, v_pages: pools (n_slots, n_pages, page_size, H_kv, D), or one slot's without the first
+            dim, bf16 or fp32
+        block_table, cache_seqlens, free_pages, free_count: as ``paged_reserve``
+        new_lens: (rows,) int32, each row's nodes, as they were reserved
+        kept: (rows, n) int32, the nodes to keep, ascending, as many as counts says (``verify_drafts``)
+        counts: (rows,) int32; 0 for a row that keeps nothing (its nodes' pages go back all the same)
+
+    A row that was refused its pages keeps nothing. A node that is not one of its row's, or stands before the
+    place it should move to, is not moved. The pages that a row's nodes lie in are its own alone. Checked mode
+    (``flash_attn.set_checked``) reads the tables back and raises where kept nodes are not ascending nodes of
+    their row, or a page is outside the pool.
+    """
+    what = "paged_keep"
+    n, max_pages, stride, n_pages, dev = _check_tables(block_table, cache_seqlens, free_pages, free_count,
+                                                       what)
+    _ext.require_rocm(k_pages, v_pages, what=what)
+    _ext.same_device(dev, k_pages=k_pages, v_pages=v_pages, new_lens=new_lens, kept=kept, counts=counts)
+    if k_pages.dim() == 4:
+        k_pages, v_pages = k_pages.unsqueeze(0), v_pages.unsqueeze(0)
+    if k_pages.dim() != 5 or k_pages.shape != v_pages.shape or k_pages.shape[1] != n_pages:
+        raise ValueError(f"k_pages/v_pages must both be (n_slots, {n_pages}, page_size, H_kv, D); got "
+                         f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    slots, _, page, heads, dim = k_pages.shape
+    page = check_page_size(page)
+    if k_pages.dtype != v_pages.dtype:
+        raise TypeError(f"v_pages is {v_pages.dtype}, k_pages is {k_pages.dtype}")
+    code = _ext.dtype_code(k_pages.dtype)
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        if slots and not t[0, 0].is_contiguous():
+            raise ValueError(f"each page of {name} must be contiguous; strides {t.stride()}")
+    if (n_pages > 1 and k_pages.stride(1) != v_pages.stride(1)) \
+            or (slots > 1 and k_pages.stride(0) != v_pages.stride(0)):
+        raise ValueError("k_pages and v_pages must have the same strides")
+    page_stride = k_pages.stride(1) if n_pages > 1 else page * heads * dim
+    slot_stride = k_pages.stride(0) if slots > 1 else n_pages * page_stride
+    for name, t in (("new_lens", new_lens), ("counts", counts)):
+        if t.dtype != torch.int32 or t.shape != (n,):
+            raise ValueError(f"{name} must be ({n},) int32; got {tuple(t.shape)} {t.dtype}")
+    if kept.dtype != torch.int32 or kept.dim() != 2 or kept.shape[0] != n:
+        raise ValueError(f"kept must be ({n}, nodes) int32; got {tuple(kept.shape)} {kept.dtype}")
+    new_lens, kept, counts = new_lens.contiguous(), kept.contiguous(), counts.contiguous()
+    from modelcore_amd.kernels import flash_attn
+    if flash_attn.CHECK_POSITIONS:
+        _check_keep(block_table, cache_seqlens, new_lens, kept, counts, page, n_pages)
+    with _ext.on_device(dev):
+        st = _ext.lib().mcamd_paged_keep(
+            k_pages.data_ptr(), v_pages.data_ptr(), slots, slot_stride, block_table.data_ptr(), stride,
+            cache_seqlens.data_ptr(), new_lens.data_ptr(), kept.data_ptr(), kept.shape[1],
+            counts.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), n, max_pages, n_pages, page,
+            page_stride, heads * dim, code, _ext.stream_handle(dev))
+    _ext.check(st, what)
