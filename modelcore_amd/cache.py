@@ -268,6 +268,14 @@ class PagedKVCache:
     host keeps its own account of lengths and free pages (``lengths``, ``pages_free``) and raises before
     a launch where the pool or a row's line of the table is too small, so nothing is read back.
 
+    A row's new tokens may also be a drafted tree, guesses at what follows it, of which the model's answer
+    decides how many stay (``modelcore_amd.sampling.verify_drafts``)::
+
+        step = cache.begin_tree([[-1, 0, 0, 1], [-1]])   # row 0: its last token, two guesses, one after the first
+        logits = model(ids, kv_cache=step)[0]            # of every node
+        done = verify_drafts(logits, ids[0], step.parents, step.cu_seqlens, numbers, max_seqlen=4)
+        cache.keep(step, done.kept, done.counts)         # the accepted nodes are the rows' tokens
+
     A step can be captured: ``begin(n)`` in the capture, with the same count for every row, then
     ``note_device_step(n)`` before each replay, which checks and moves the host's account. The model that
     runs the captured step bounds the replays' positions by its rotary tables (``PagedStep.bound_positions``).
@@ -339,9 +347,48 @@ class PagedKVCache:
         """Reserve the pages of each row's next tokens -- a count per row, or one for all -- and return
         the ``PagedStep`` to run the model with. The step's forward must run before the next begin
         or release: its pages are the rows' only then (``reset`` is the way out of one that failed)."""
+        return self._begin(self._lens(new_lens), None)
+
+    def begin_tree(self, parents):
+        """Reserve the pages of each row's drafted tree, parents[b][i] being the node that node i of row b
+        follows, one before it, or -1 for a root (no nodes: the row sits this step out); returns the
+        ``TreeStep`` to run the model with. Its nodes are the row's only until ``keep``, which must follow
+        the step's forward before the next begin or release."""
+        from modelcore_amd.kernels.paged import MAX_TREE_NODES
+        parents = [[int(p) for p in row] for row in parents]
+        if self.cache_seqlens.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a step of trees cannot be captured: what the rows keep of them is the host's "
+                               "to know before the next step")
+        for b, row in enumerate(parents):
+            assert len(row) <= MAX_TREE_NODES, f"row {b} has {len(row)} nodes, more than {MAX_TREE_NODES}"
+            assert all(-1 <= p < i for i, p in enumerate(row)), \
+                f"a node's parent is a node before it, or -1; row {b} has {row}"
+        return self._begin(self._lens([len(row) for row in parents]), parents)
+
+    def keep(self, step, kept, counts):
+        """Row b keeps nodes kept[b, :counts[b]] of its tree (ascending; ``verify_drafts`` gives both), which
+        become its next tokens, and gives back the pages of the others (``paged_keep``). Returns how many
+        each row keeps, as a list: the one host read of a step."""
+        from modelcore_amd.kernels.paged import paged_keep
+        assert isinstance(step, TreeStep) and step is self._open, "the trees are not those this cache has begun"
+        assert step._done, "the step's forward has not run"
+        paged_keep(self.k_pages, self.v_pages, self.block_table, self.cache_seqlens, step._counts, kept, counts,
+                   self.free_pages, self.free_count)
+        took = [max(0, min(c, n, kept.shape[1])) for c, n in zip(counts.tolist(), step.lens)]
+        self._open = None
+        for b, (t, c) in enumerate(zip(step.lens, took)):
+            n = self.lengths[b]
+            self.pages_free += self._pages(n + t) - self._pages(n + c)
+            self.lengths[b] = n + c
+        return took
+
+    def _check_closed(self):
+        assert not self._open, "the trees of the step before have not been kept" \
+            if isinstance(self._open, TreeStep) and self._open._done else "the step before has not run"
+
+    def _begin(self, lens, parents):
         from modelcore_amd.kernels.paged import paged_reserve
-        assert not self._open, "the step before has not run"
-        lens = self._lens(new_lens)
+        self._check_closed()
         dev = self.cache_seqlens.device
         capturing = dev.type == "cuda" and torch.cuda.is_current_stream_capturing()
         if capturing and len(set(lens)) > 1:
@@ -354,7 +401,8 @@ class PagedKVCache:
             counts = torch.tensor(lens, dtype=torch.int32, device=dev)
         plan = paged_reserve(self.block_table, self.cache_seqlens, counts, self.free_pages,
                              self.free_count, total=sum(lens), page_size=self.page_size)
-        step = PagedStep(self, lens, counts, plan, capturing)
+        step = PagedStep(self, lens, counts, plan, capturing) if parents is None \
+            else TreeStep(self, lens, counts, plan, parents)
         if not capturing:  # the host's account moves once the plan is under way
             self._open = step
             self.pages_free -= taken
@@ -362,7 +410,7 @@ class PagedKVCache:
 
     def note_device_step(self, new_lens):
         """The host's side of a captured begin + forward, before its replay: checked, then moved."""
-        assert not self._open, "the step before has not run"
+        self._check_closed()
         lens = self._lens(new_lens)
         taken = self._room(lens)
         lengths = [n + t for n, t in zip(self.lengths, lens)]
@@ -374,7 +422,7 @@ class PagedKVCache:
     def release(self, rows):
         """Rows that have ended give their pages back and are empty."""
         from modelcore_amd.kernels.paged import paged_release
-        assert not self._open, "the step before has not run"
+        self._check_closed()
         rows = [int(r) for r in rows]
         assert len(set(rows)) == len(rows), "rows must be distinct"
         assert all(0 <= r < self.batch_size for r in rows), \
@@ -454,3 +502,35 @@ class PagedStep:
         if not self._captured:
             self._done, c._open = True, None
             c.lengths = [n + t for n, t in zip(c.lengths, self.lens)]
+
+
+class TreeStep(PagedStep):
+    """One forward over a PagedKVCache whose rows' new tokens are nodes of drafted trees
+    (``PagedKVCache.begin_tree``). The logits are those of every node; the rows move on with
+    ``PagedKVCache.keep``."""
+
+    def __init__(self, cache, lens, counts, plan, parents):
+        from modelcore_amd.kernels.paged import paged_tree
+        super().__init__(cache, lens, counts, plan, False)
+        dev = cache.cache_seqlens.device
+        self.parents = torch.tensor([p for row in parents for p in row], dtype=torch.int32, device=dev)
+        self.tree = paged_tree(self.parents, plan.cu_seqlens, cache.cache_seqlens, max_seqlen=self.max_seqlen)
+        self.longest = 0
+        for n, row in zip(cache.lengths, parents):
+            depth = []
+            for p in row:
+                depth.append(depth[p] + 1 if p >= 0 else 1)
+            self.longest = max(self.longest, n + max(depth, default=0))
+
+    positions = property(lambda self: self.tree.positions)
+    masks = property(lambda self: self.tree.masks)
+
+    @property
+    def last(self):
+        raise TypeError("a drafted tree has no last token: its logits are those of every node (model(...))")
+
+    def advance(self, num_tokens):
+        """The forward has run; the rows move on by what they keep."""
+        assert num_tokens == self.total, "a paged forward covers every row's new tokens"
+        self.check_open()
+        self._done = True

@@ -7,6 +7,9 @@ prompts are prefilled together as one packed sequence (``PackedPrefill``: no pad
 written straight into its first sample row and copied into the others
 (``KVCache.fill_sample_rows``), the rows right-ragged; row ``p * num_samples + s`` is sample ``s``
 of prompt ``p``.
+
+``DraftedDecoder`` takes several tokens a step: guesses at what follows each row go through the model as a
+tree, over a paged cache, and as many stay as the model's own distribution accepts.
 """
 from __future__ import annotations
 
@@ -163,3 +166,96 @@ class CapturedStep:
         self.graph.replay()
         self.decoder.kv_cache._pos_uniform += 1
         return self.tokens
+
+
+def lookup_drafts(tokens, *, ngram=2, width=2, length=4):
+    """Guesses at what follows `tokens` from the text itself: what followed the last earlier occurrences of
+    its last `ngram` tokens, `width` of them at most and `length` tokens of each, as one tree. Returns
+    (tokens, parents) of the guesses, node 0 being the last of `tokens` and the guesses nodes 1, 2, .."""
+    end = tokens[-ngram:]
+    drafts, parents, children, found = [], [], {}, 0
+    for at in range(len(tokens) - ngram - 1, -1, -1):
+        if found == width:
+            break
+        if tokens[at:at + ngram] != end:
+            continue
+        found += 1
+        node = 0
+        for t in tokens[at + ngram:at + ngram + length]:
+            if (node, t) not in children:
+                drafts.append(t)
+                parents.append(node)
+                children[node, t] = len(drafts)
+            node = children[node, t]
+    return drafts, parents
+
+
+class DraftedDecoder:
+    """Decoding with drafted tokens: each step runs every row's last token and guesses at what follows it as
+    one tree, and the row moves on by all that the model accepts, at least one token.
+
+    drafter(tokens) gives a row's guesses as (tokens, parents), node 0 being its last token (see
+    ``lookup_drafts``). The tokens that come out are a draw from the model's own distribution at
+    `temperature` (0: its likeliest tokens), whatever the guesses were; they are keyed by `seed` and the
+    step, not by the row alone. ``tokens[b]`` is row b's prompt and what has been emitted."""
+
+    @torch.inference_mode()
+    def __init__(self, model, manager, prompts, *, max_tokens, drafter=lookup_drafts, temperature=0.0, seed=0,
+                 page_size=16, n_pages=None):
+        from modelcore_amd.sampling import verify_drafts
+        self.model, self.drafter, self.temperature, self._verify = model, drafter, float(temperature), verify_drafts
+        self.tokens = [list(p) for p in prompts]
+        lengths = [len(p) for p in self.tokens]
+        assert lengths and min(lengths) > 0, "empty prompt"
+        device = model.get_device()
+        self.cache = manager.new_paged_kv_cache(model, batch_size=len(lengths), seq_len=max(lengths) + max_tokens,
+                                                page_size=page_size, n_pages=n_pages, device=device)
+        self._rng = torch.Generator(device=device).manual_seed(seed)
+        self.running = [True] * len(lengths)
+        # The prompts, and the first token of each row from a tree of its root alone.
+        ids = torch.tensor([t for p in self.tokens for t in p], dtype=torch.long, device=device)[None]
+        logits = model.last_logits(ids, self.cache.begin(lengths), None)
+        n = len(lengths)
+        first = self._draw(logits, torch.zeros(n, dtype=torch.long, device=device),
+                           torch.full((n,), -1, dtype=torch.int32, device=device),
+                           torch.arange(n + 1, dtype=torch.int32, device=device), 1)
+        for row, t in zip(self.tokens, first.tokens.tolist()):
+            row.append(t[0])
+
+    def _draw(self, logits, ids, parents, cu_seqlens, longest):
+        numbers = torch.rand(len(ids), generator=self._rng, device=ids.device)
+        return self._verify(logits, ids, parents, cu_seqlens, numbers, temperature=self.temperature,
+                            max_seqlen=longest)
+
+    def finish(self, rows):
+        """Rows that have ended give their pages back and take no part in further steps."""
+        rows = [r for r in rows if self.running[r]]
+        for r in rows:
+            self.running[r] = False
+        self.cache.release(rows)
+
+    @torch.inference_mode()
+    def step(self):
+        """One forward over every running row's tree; returns the tokens each row has gained, [] for a row that
+        has ended."""
+        trees, ids = [], []
+        for b, row in enumerate(self.tokens):
+            drafts, parents = self.drafter(row) if self.running[b] else ([], [])
+            # As many nodes as the row's positions have room for; those left out come after those kept.
+            room = self.cache.max_seq_len - self.cache.lengths[b] - 1
+            assert not self.running[b] or room >= 0, \
+                f"Sequence length {len(row)} exceeds cache length {self.cache.max_seq_len}"
+            trees.append([-1, *parents[:room]] if self.running[b] else [])
+            ids += [row[-1], *drafts[:room]] if self.running[b] else []
+        gained = [[] for _ in self.tokens]
+        if not ids:
+            return gained
+        step = self.cache.begin_tree(trees)
+        ids = torch.tensor(ids, dtype=torch.long, device=self.model.get_device())
+        logits = self.model.forward(ids[None], kv_cache=step)[0]
+        done = self._draw(logits, ids, step.parents, step.cu_seqlens, step.max_seqlen)
+        took = self.cache.keep(step, done.kept, done.counts)
+        for b, (n, new) in enumerate(zip(took, done.tokens.tolist())):
+            gained[b] = new[:n]
+            self.tokens[b] += gained[b]
+        return gained

@@ -27,7 +27,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from modelcore_amd.cache import KVCache, PackedPrefill, PagedKVCache, PagedStep
+from modelcore_amd.cache import KVCache, PackedPrefill, PagedKVCache, PagedStep, TreeStep
 from modelcore_amd.runtime import Runtime
 
 TYPE_KEY = "#type"
@@ -412,7 +412,7 @@ class Attention(nn.Module):
         """The layer over a paged cache (x is (1, total, n_embd), the rows' new tokens one after
         another): a producer rotates, norms and scales q and k and writes k and v to their slots in one
         launch, a KV-sharing consumer transforms q only, then the operator attends through the block
-        table. With fuse_epilogue off, the reference's separate ops and an operator that appends."""
+        table (a TreeStep's, along each node's path). With fuse_epilogue off, the reference's separate ops and an operator that appends."""
         _, T, _ = x.size()
         q, k, v = self._project(x)
         k_pages, v_pages = step.get_slot_cache(self.kv_slot)
@@ -433,9 +433,14 @@ class Attention(nn.Module):
             q, kw = q.unflatten(0, rows), {n: t.unflatten(0, rows) for n, t in kw.items()}
         else:
             kw.update(cu_seqlens=step.cu_seqlens, max_seqlen=step.max_seqlen)
-        y = self.attention.flash_attn_paged_with_kvcache(
-            q, k_pages, v_pages, block_table=step.block_table, cache_seqlens=step.cache_seqlens,
-            causal=True, window_size=(self.window, 0), **kw).view(1, T, self.n_head, self.head_dim)
+        kw.update(block_table=step.block_table, cache_seqlens=step.cache_seqlens,
+                  window_size=(self.window, 0))
+        if isinstance(step, TreeStep):
+            masks = step.masks.unflatten(0, rows) if step.uniform else step.masks
+            y = self.attention.flash_attn_paged_tree_with_kvcache(q, k_pages, v_pages, tree_masks=masks, **kw)
+        else:
+            y = self.attention.flash_attn_paged_with_kvcache(q, k_pages, v_pages, causal=True, **kw)
+        y = y.view(1, T, self.n_head, self.head_dim)
         if "output_gate" in self.features:
             y = self.features["output_gate"](y, x)
         return self.c_proj(y.contiguous().view(1, T, self.n_head * self.head_dim))  # T may be 0
@@ -947,6 +952,11 @@ class ModelManager:
         from modelcore_amd.generate import Decoder
         return Decoder(model, self, tokens, num_samples=num_samples, max_tokens=max_tokens,
                        device=device)
+
+    def new_drafted_decoder(self, model, prompts, *, max_tokens, **kw):
+        """A DraftedDecoder: several tokens a step, drafted on the host and verified by the model."""
+        from modelcore_amd.generate import DraftedDecoder
+        return DraftedDecoder(model, self, prompts, max_tokens=max_tokens, **kw)
 
 
 def param_count(model) -> int:
