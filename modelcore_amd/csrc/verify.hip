@@ -13,10 +13,15 @@
 //
 // The draw is the smallest token whose running sum of weights passes u_0 times the whole (u_0 the root's number,
 // which no test uses). It falls between neighbours of a whole vocabulary, where 32-bit sums would move
-// it: weights and sums are in 64 bits.
+// it: weights and sums are in 64 bits, whose multiply-adds run as fast here as those of 32. A weight is
+// exp2 by its series to the tenth power, within 2^-40.
 //
-// A workgroup has a row. Its sixteen waves each sum a run of the vocabulary, the run in which the draw falls is
-// cut in sixteen again, until a wave's lanes hold a token each.
+// Two launches. The first reads every logit once, a workgroup kChunk of a node's, and leaves the largest, its
+// place and the sum of the chunk's weights against it: bound by HBM. The second has a workgroup a row: a node's
+// chunks are put together by a wave, the probabilities of all drafts fetched at once, and the walk then goes
+// through LDS, every wave by itself; the sum (p - a q)+ over the vocabulary is taken where a further child has
+// to be tried against it. The draw finds its chunk by the chunks' sums (of what is left of p and q, by a pass
+// over the row) and reads that one again.
 #include "kernels.h"
 
 #include <cmath>
@@ -27,6 +32,16 @@ namespace {
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxNodes = 1024;
+constexpr int kChunkThreads = 256;
+constexpr int kRestChunks = 64;  // whose sums of (p - a q)+ are kept
+constexpr int kChunk = 16 * kChunkThreads;  // logits
+static_assert(kChunk == 4 * kThreads, "the draw's threads have four each");
+
+struct Part {  // of a chunk
+  double sum;
+  float top;
+  int at;
+};
 
 struct VerifyParams {
   const float *logits, *probs;
@@ -36,9 +51,39 @@ struct VerifyParams {
   const float *numbers;
   int32_t *kept, *counts;
   int64_t *out;
-  int total, most, vocab;
-  double inv_temp;
+  Part *parts;  // [total][chunks]
+  int total, most, vocab, chunks;
+  double scale;  // log2(e) / temperature
   int greedy;
+};
+
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // at any float's address
+
+// 2^y for y <= 0, to 2^-40: 2^n by the exponent, 2^f, |f| <= 1/2, by the series of e^(f ln 2).
+__device__ __forceinline__ double exp2_64(double y) {
+  const double n = __builtin_rint(y), r = (y - n) * 0.69314718055994530942;
+  double p = 1.0 / 3628800;
+  p = fma(p, r, 1.0 / 362880);
+  p = fma(p, r, 1.0 / 40320);
+  p = fma(p, r, 1.0 / 5040);
+  p = fma(p, r, 1.0 / 720);
+  p = fma(p, r, 1.0 / 120);
+  p = fma(p, r, 1.0 / 24);
+  p = fma(p, r, 1.0 / 6);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return y > -1000.0 ? ldexp(p, int(n)) : 0.0;
+}
+
+// Logits as weights against the largest of them, which an infinite one makes 1 and all others 0. NaN has none.
+struct Weigher {
+  float top;
+  double scale;
+  __device__ __forceinline__ double operator()(float x) const {
+    const double w = exp2_64((double(x) - double(top)) * scale);
+    return x == top ? 1.0 : x > -INFINITY && top < INFINITY ? w : 0.0;
+  }
 };
 
 __device__ __forceinline__ double wave_sum64(double x) {
@@ -46,188 +91,379 @@ __device__ __forceinline__ double wave_sum64(double x) {
   for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
   return x;
 }
-
-// Sums over the waves' runs, in order: what comes before run w and all.
-struct Sums {
-  double part[kWaves];
-};
-__device__ __forceinline__ double block_sum(double x, Sums &s) {
-  x = wave_sum64(x);
-  __syncthreads();  // the sums before have been read
-  if ((threadIdx.x & 63) == 0) s.part[threadIdx.x >> 6] = x;
-  __syncthreads();
-  double all = 0;
+__device__ __forceinline__ double wave_upto64(double x, int lane) {
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) all += s.part[w];
-  return all;
+  for (int o = 1; o < 64; o <<= 1) {
+    const double y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+__device__ __forceinline__ int wave_min(int x) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x = min(x, __shfl_xor(x, o, 64));
+  return x;
 }
 
-// A node's logits as weights against the largest of them, which an infinite one makes 1 and all others 0. NaN has none.
-struct Weigher {
-  float top;
-  double inv_temp;
-  __device__ __forceinline__ double operator()(float x) const {
-    if (x == top) return 1.0;
-    if (!(x > -INFINITY) || top == INFINITY) return 0.0;
-    return exp((double(x) - double(top)) * inv_temp);
+__global__ __launch_bounds__(kChunkThreads) void verify_parts_kernel(VerifyParams P) {
+  constexpr int W = kChunkThreads / 64;
+  __shared__ float s_top[W];
+  __shared__ int s_at[W];
+  __shared__ double s_sum[W];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int node = blockIdx.x / P.chunks, chunk = blockIdx.x - node * P.chunks;
+  const float *row = P.logits + int64_t(node) * P.logits_stride;
+  const int i0 = chunk * kChunk + 4 * tid;
+  f32x4u x[4];
+  if (chunk * kChunk + kChunk <= P.vocab) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const f32x4u *>(row + i0 + 4 * kChunkThreads * j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = i0 + 4 * kChunkThreads * j + e;
+        const float y = row[min(i, P.vocab - 1)];
+        x[j][e] = i < P.vocab ? y : -INFINITY;
+      }
   }
-};
+  float top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = fmaxf(top, x[j][e]);
+  top = wave_max<64>(top);
+  if (lane == 0) s_top[wave] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < W; ++w) top = fmaxf(top, s_top[w]);
+  Part *const part = P.parts + int64_t(blockIdx.x);
+  if (P.greedy) {
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (x[j][e] == top) at = min(at, i0 + 4 * kChunkThreads * j + e);
+    at = wave_min(at);
+    if (lane == 0) s_at[wave] = at;
+    __syncthreads();
+    if (tid > 0) return;
+    for (int w = 0; w < W; ++w) at = min(at, s_at[w]);
+    part->top = top;
+    part->at = at;
+    return;
+  }
+  const Weigher weigh{top, P.scale};
+  double sum = 0;
+  if (top > -INFINITY) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum += weigh(x[j][e]);
+  }
+  sum = wave_sum64(sum);
+  if (lane == 0) s_sum[wave] = sum;
+  __syncthreads();
+  if (tid > 0) return;
+  for (int w = 1; w < W; ++w) sum += s_sum[w];
+  part->sum = sum;
+  part->top = top;
+}
 
 __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyParams P) {
-  __shared__ Sums s_sums;
-  __shared__ float s_top[kWaves];
-  __shared__ int s_best[kWaves];
-  __shared__ int s_gone[kMaxNodes];
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ double s_all[kMaxNodes], s_w[kMaxNodes];
+  __shared__ float s_top[kMaxNodes], s_q[kMaxNodes], s_u[kMaxNodes];
+  __shared__ int s_up[kMaxNodes], s_token[kMaxNodes], s_best[kMaxNodes];
+  __shared__ double s_sum[kWaves];
+  __shared__ double s_rest[kRestChunks][kWaves];
+  __shared__ int s_gone[kMaxNodes], s_chunk;
+  __shared__ double s_want;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int begin = max(P.cu[b], 0), n = min(max(min(P.cu[b + 1], P.total) - begin, 0), P.most);
   int32_t *const kept = P.kept + int64_t(b) * P.most;
   int64_t *const out = P.out + int64_t(b) * P.most;
   for (int j = tid; j < P.most; j += kThreads) kept[j] = -1, out[j] = -1;
-  __syncthreads();  // the padding is written before the tokens
   if (n == 0) {
     if (tid == 0) P.counts[b] = 0;
     return;
   }
-  const int V = P.vocab;
-  int node = 0, count = 1, n_gone = 0, best = 0;
-  const float *row = nullptr, *q_row = nullptr;
-  Weigher weigh{0.f, P.inv_temp};
-  double all = 0, less = 0, left = 0;  // less, left: a and Z, of guesses Z in units of the weights
+  const int V = P.vocab, C = P.chunks;
+  // Every node's draft and number, and its chunks put together.
+  int up = 0, token = -1;
+  if (tid < n) {
+    const int64_t t = P.tokens[begin + tid];
+    token = t >= 0 && t < V ? int(t) : -1;
+    up = tid == 0 ? -1 : P.parents[begin + tid];
+    s_up[tid] = up;
+    s_token[tid] = token;
+    s_u[tid] = P.numbers[begin + tid];
+  }
+  for (int i = wave; i < n; i += kWaves) {
+    const Part *part = P.parts + int64_t(begin + i) * C;
+    float top = -INFINITY;
+    for (int c = lane; c < C; c += 64) top = fmaxf(top, part[c].top);
+    top = wave_max<64>(top);
+    if (P.greedy) {
+      int best = 0x7fffffff;
+      for (int c = lane; c < C; c += 64)
+        if (part[c].top == top) best = min(best, part[c].at);
+      best = wave_min(best);
+      if (lane == 0) s_best[i] = best;
+    } else {
+      const Weigher weigh{top, P.scale};
+      double all = 0;
+      for (int c = lane; c < C; c += 64) all += part[c].sum * weigh(part[c].top);
+      all = wave_sum64(all);
+      if (lane == 0) s_all[i] = all;
+    }
+    if (lane == 0) s_top[i] = top;
+  }
+  __syncthreads();
+  if (!P.greedy && tid > 0 && tid < n) {
+    s_w[tid] = 0;
+    if (up >= 0 && up < tid && token >= 0) {
+      const float x = P.logits[int64_t(begin + up) * P.logits_stride + token];
+      if (P.probs) s_q[tid] = P.probs[int64_t(begin + up) * P.probs_stride + token];
+      s_w[tid] = Weigher{s_top[up], P.scale}(x);
+    }
+  }
+  __syncthreads();
 
-  // The node's largest logit, where it is, and the sum of its weights.
+  int node = 0, count = 1;
+  double less = 0, left = 0;  // a and Z, of guesses Z in units of the weights
+  bool summed = true;         // left is the sum for this a
+  const float *row = nullptr, *q_row = nullptr;
+  Weigher weigh{0.f, P.scale};
+  double one = 0;  // over the node's weights
   auto enter = [&]() {
     row = P.logits + int64_t(begin + node) * P.logits_stride;
     q_row = P.probs ? P.probs + int64_t(begin + node) * P.probs_stride : nullptr;
-    float top = -INFINITY;
-    best = 0x7fffffff;
-    for (int i = tid; i < V; i += kThreads) {
-      const float x = row[i];
-      if (x > top || (x == top && i < best)) top = x, best = i;
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const float t2 = __shfl_xor(top, o, 64);
-      const int b2 = __shfl_xor(best, o, 64);
-      if (t2 > top || (t2 == top && b2 < best)) top = t2, best = b2;
-    }
-    __syncthreads();  // of the node before
-    if (lane == 0) s_top[wave] = top, s_best[wave] = best;
-    __syncthreads();
-    for (int w = 0; w < kWaves; ++w)
-      if (s_top[w] > top || (s_top[w] == top && s_best[w] < best)) top = s_top[w], best = s_best[w];
-    weigh.top = top;
-    less = 0, n_gone = 0;
+    weigh.top = s_top[node];
+    less = 0;
+    summed = true;
     if (P.greedy) return;
-    double sum = 0;
-    if (top > -INFINITY)
-      for (int i = tid; i < V; i += kThreads) sum += weigh(row[i]);
-    all = block_sum(sum, s_sums);
-    left = q_row ? 1.0 : all;
+    one = 1.0 / s_all[node];
+    left = q_row ? 1.0 : s_all[node];
   };
-  // What is left of token i's probability (q) or weight (guesses).
-  auto remains = [&](int i) {
-    double w = weigh(row[i]);
-    if (q_row) return fmax(w / all - less * double(q_row[i]), 0.0);
-    for (int g = 0; g < n_gone; ++g) w = s_gone[g] == i ? 0.0 : w;
-    return w;
+  // Four logits from token i on, or draft probabilities; past the vocabulary what has no weight.
+  auto four = [&](const float *from, int i, float none) {
+    f32x4u x;
+    if (i + 4 <= V) {
+      x = *reinterpret_cast<const f32x4u *>(from + i);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = i + e < V ? from[i + e] : none;
+    }
+    return x;
+  };
+  // What is left of the probabilities of four tokens.
+  auto rest_of = [&](const f32x4u &x, const f32x4u &q, double (&w)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = fmax(weigh(x[e]) * one - less * double(q[e]), 0.0);
+    return (w[0] + w[1]) + (w[2] + w[3]);
+  };
+  // The sum of it over the vocabulary, by its chunks' sums, of which the first ones are kept.
+  auto rest_sum = [&]() {
+    constexpr int U = 4;  // chunks whose loads are under way at once
+    double sum = 0;
+    __syncthreads();  // s_rest and s_sum have been read
+    for (int c0 = 0; c0 < C; c0 += U) {
+      f32x4u x[U], q[U];
+#pragma unroll
+      for (int c = 0; c < U; ++c) {
+        x[c] = four(row, (c0 + c) * kChunk + 4 * tid, -INFINITY);
+        q[c] = four(q_row, (c0 + c) * kChunk + 4 * tid, 0.f);
+      }
+#pragma unroll
+      for (int c = 0; c < U; ++c) {
+        double w[4];
+        const double part = wave_sum64(rest_of(x[c], q[c], w));
+        sum += part;
+        if (lane == 0 && c0 + c < kRestChunks) s_rest[c0 + c][wave] = part;
+      }
+    }
+    if (lane == 0) s_sum[wave] = sum;
+    __syncthreads();
+    sum = 0;
+    for (int w = 0; w < kWaves; ++w) sum += s_sum[w];
+    return sum;
   };
 
+  // The walk, by every wave alike.
   enter();
-  for (int i = 1; i < n; ++i) {
-    if (P.parents[begin + i] != node) continue;
-    const int64_t x = P.tokens[begin + i];
-    if (x < 0 || x >= V || !(weigh.top > -INFINITY)) continue;
-    bool taken;
-    const double u = P.numbers[begin + i];
-    if (P.greedy) {
-      taken = int(x) == best;
-    } else {
-      const double w = remains(int(x));
-      taken = u * left * (q_row ? double(q_row[x]) : 1.0) < w;
-      if (!taken) {
+  for (;;) {
+    int found = -1;
+    for (int base = (node + 1) & ~63; base < n && found < 0 && weigh.top > -INFINITY; base += 64) {
+      const int mine = base + lane;
+      const bool kid = mine > node && mine < n && s_up[min(mine, n - 1)] == node && s_token[min(mine, n - 1)] >= 0;
+      for (uint64_t left_of = __builtin_amdgcn_ballot_w64(kid); left_of != 0 && found < 0; left_of &= left_of - 1) {
+        const int i = base + __builtin_ctzll(left_of), x = s_token[i];
+        if (P.greedy) {
+          if (x == s_best[node]) found = i;
+          continue;
+        }
+        const double u = s_u[i];
         if (q_row) {
-          less += left;
-          double sum = 0;
-          for (int j = tid; j < V; j += kThreads) sum += remains(j);
-          left = block_sum(sum, s_sums);
+          if (!summed) left = rest_sum(), summed = true;
+          const double q = s_q[i];
+          if (u * left * q < fmax(s_w[i] * one - less * q, 0.0)) {
+            found = i;
+          } else {
+            less += left;
+            summed = false;
+          }
         } else {
-          left -= w;
-          __syncthreads();
-          if (tid == 0) s_gone[n_gone] = int(x);
-          ++n_gone;
-          __syncthreads();
+          double w = s_w[i];
+          for (int j = node + 1; j < i; ++j)  // refused before
+            if (s_up[j] == node && s_token[j] == x) w = 0;
+          if (u * left < w)
+            found = i;
+          else
+            left -= w;
         }
       }
     }
-    if (!taken) continue;
-    if (tid == 0) kept[count] = i, out[count - 1] = x;
+    if (found < 0) break;
+    node = found;
+    if (tid == 0) kept[count] = node, out[count - 1] = s_token[node];
     ++count;
-    node = i;
     enter();
   }
   if (tid == 0) kept[0] = 0, P.counts[b] = count;
   if (P.greedy || !(weigh.top > -INFINITY)) {
-    if (tid == 0) out[count - 1] = best == 0x7fffffff ? 0 : best;
+    if (tid == 0) out[count - 1] = weigh.top > -INFINITY ? s_best[node] : 0;
     return;
   }
 
-  // The draw. lo .. hi: where it falls; want: how far into its weights.
-  bool plain = false;  // nothing is left but rounding: from all of them
-  auto weight = [&](int i) { return plain ? weigh(row[i]) : remains(i); };
-  int lo = 0, hi = V;
-  double want = 0;
-  for (bool first = true; hi - lo > 64; first = false) {
-    const int each = (hi - lo + kWaves - 1) / kWaves;
-    const int from = min(lo + wave * each, hi), to = min(from + each, hi);
-    auto sums = [&]() {
-      double sum = 0;
-      for (int i = from + lane; i < to; i += 64) sum += weight(i);
-      return block_sum(sum, s_sums);
-    };
-    double sum = sums();
-    if (first) {
-      if (!(sum > 0)) {
-        plain = true;
-        sum = sums();
+  // The draw: the chunk first. Its first wave finds it, from the sums of the chunks (the node's own, less the
+  // guesses that were refused there, or of what is left of p and q).
+  int n_gone = 0;  // distinct refused guesses
+  const Part *parts = P.parts + int64_t(begin + node) * C;
+  bool rest = q_row && less > 0;  // else all of p, or p without the refused
+  if (!q_row) {
+    for (int base = (node + 1) & ~63; base < n; base += 64) {
+      const int mine = base + lane;
+      bool kid = mine > node && mine < n && s_up[min(mine, n - 1)] == node && s_token[min(mine, n - 1)] >= 0;
+      for (int j = node + 1; kid && j < mine; ++j) kid = !(s_up[j] == node && s_token[j] == s_token[mine]);
+      const uint64_t kids = __builtin_amdgcn_ballot_w64(kid);
+      if (wave == 0 && kid) s_gone[n_gone + __builtin_popcountll(kids & ((uint64_t(1) << lane) - 1))] = mine;
+      n_gone += __builtin_popcountll(kids);
+    }
+  }
+  __syncthreads();  // s_gone is written
+  auto chunk_sum = [&](int c) {
+    if (c >= C) return 0.0;
+    const double all = parts[c].sum * weigh(parts[c].top);
+    double sum = all;
+    for (int g = 0; g < n_gone; ++g)
+      if (s_token[s_gone[g]] / kChunk == c) sum -= s_w[s_gone[g]];
+    return sum > all * 0x1p-45 ? sum : 0.0;  // else rounding is what is left
+  };
+  auto pick = [&](double whole, auto sum_of) {  // by the first wave: the chunk, and how far into it
+    double want = double(s_u[0]) * whole, before = 0, in_last = 0;
+    int last = 0;
+    for (int c0 = 0; c0 < C; c0 += 64) {
+      const double x = sum_of(c0 + lane), upto = before + wave_upto64(x, lane);
+      const uint64_t past = __builtin_amdgcn_ballot_w64(x > 0 && upto > want), any = __builtin_amdgcn_ballot_w64(x > 0);
+      const int l = past ? __builtin_ctzll(past) : any ? 63 - __builtin_clzll(any) : 0;
+      if (any) last = c0 + l, in_last = __shfl(upto - x, l, 64);
+      if (past) break;
+      before = __shfl(upto, 63, 64);
+    }
+    if (lane == 0) s_chunk = last, s_want = want - in_last;
+  };
+  double whole = 0;
+  if (rest) {
+    whole = rest_sum();
+    rest = whole > 0;
+  }
+  if (!rest) {
+    if (wave == 0) {
+      for (int round = 0; round < 2; ++round) {
+        whole = 0;
+        for (int c = lane; c < C; c += 64) whole += chunk_sum(c);
+        whole = wave_sum64(whole);
+        if (whole > 0 || n_gone == 0) break;
+        n_gone = 0;  // nothing is left but rounding: from all of them
       }
-      want = double(P.numbers[begin]) * sum;
+      pick(whole, chunk_sum);
+      if (lane == 0) s_sum[0] = n_gone;
     }
-    double upto = 0, before = 0;
-    int part = -1, last = 0;
-    for (int w = 0; w < kWaves; ++w) {
-      const double x = s_sums.part[w];
-      if (x > 0) last = w;
-      if (part < 0 && upto + x > want) part = w, before = upto;
-      upto += x;
+    __syncthreads();
+    n_gone = int(s_sum[0]);
+  } else if (C <= kRestChunks) {
+    if (wave == 0)
+      pick(whole, [&](int c) {
+        double sum = 0;
+        if (c < C)
+          for (int k = 0; k < kWaves; ++k) sum += s_rest[c][k];
+        return sum;
+      });
+    __syncthreads();
+  } else {
+    // More chunks than are kept: one after another, until the draw's is passed.
+    const double want = double(s_u[0]) * whole;
+    double before = 0, in_last = 0;
+    int last = 0;
+    for (int c = 0; c < C; ++c) {
+      double w[4];
+      const int i = c * kChunk + 4 * tid;
+      double sum = wave_sum64(rest_of(four(row, i, -INFINITY), four(q_row, i, 0.f), w));
+      __syncthreads();
+      if (lane == 0) s_sum[wave] = sum;
+      __syncthreads();
+      sum = 0;
+      for (int k = 0; k < kWaves; ++k) sum += s_sum[k];
+      if (sum > 0) last = c, in_last = before;
+      before += sum;
+      if (before > want) break;
     }
-    if (part < 0) {  // by rounding past them all: the last one that has any
-      part = last, before = 0;
-      for (int w = 0; w < last; ++w) before += s_sums.part[w];
-    }
-    want -= before;
-    lo = min(lo + part * each, hi);
-    hi = min(lo + each, hi);
+    __syncthreads();
+    if (tid == 0) s_chunk = last, s_want = want - in_last;
+    __syncthreads();
   }
-  if (wave > 0) return;
-  const int i = lo + lane;
-  double w = i < hi ? weight(i) : 0.0;
-  if (V <= 64) {
-    const double sum = wave_sum64(w);
-    if (!(sum > 0)) {
-      plain = true;
-      w = i < hi ? weight(i) : 0.0;
-    }
-    want = double(P.numbers[begin]) * wave_sum64(w);
-  }
-  double upto = w;
+
+  // Then the token, four of the chunk's a thread.
+  const int i0 = s_chunk * kChunk + 4 * tid;
+  double w[4];
+  const f32x4u x = four(row, i0, -INFINITY);
+  if (rest) {
+    rest_of(x, four(q_row, i0, 0.f), w);
+  } else {
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double y = __shfl_up(upto, o, 64);
-    if (lane >= o) upto += y;
+    for (int e = 0; e < 4; ++e) {
+      w[e] = weigh(x[e]);
+      for (int g = 0; g < n_gone; ++g)
+        if (s_token[s_gone[g]] == i0 + e) w[e] = 0;
+    }
   }
-  const uint64_t past = __builtin_amdgcn_ballot_w64(w > 0 && upto > want), any = __builtin_amdgcn_ballot_w64(w > 0);
-  const int l = past ? __builtin_ctzll(past) : any ? 63 - __builtin_clzll(any) : 0;
-  if (lane == 0) out[count - 1] = lo + l;
+  double upto = wave_upto64((w[0] + w[1]) + (w[2] + w[3]), lane);
+  __syncthreads();  // s_sum has been read
+  if (lane == 63) s_sum[wave] = upto;
+  __syncthreads();
+  upto -= (w[0] + w[1]) + (w[2] + w[3]);
+  for (int k = 0; k < wave; ++k) upto += s_sum[k];
+  const double want = s_want;
+  int at = 0x7fffffff, last = -1;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    upto += w[e];
+    if (w[e] > 0) {
+      last = i0 + e;
+      if (upto > want) at = min(at, i0 + e);
+    }
+  }
+  // The first past it, or by rounding none: the last that has any.
+  at = wave_min(at);
+  last = -wave_min(-last);
+  if (lane == 0) s_gone[wave] = at, s_gone[kWaves + wave] = last;
+  __syncthreads();
+  if (tid > 0) return;
+  for (int k = 0; k < kWaves; ++k) at = min(at, s_gone[k]), last = max(last, s_gone[kWaves + k]);
+  out[count - 1] = at != 0x7fffffff ? at : max(last, 0);
 }
 
 }  // namespace
@@ -236,8 +472,8 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyParams P) {
 using namespace mcamd;
 
 extern "C" size_t mcamd_verify_drafts_scratch_bytes(int64_t total, int64_t vocab) {
-  (void)total, (void)vocab;
-  return 0;
+  if (total <= 0 || vocab <= 0 || total >= 0x7fffffff || vocab > (int64_t(1) << 30)) return 0;
+  return size_t(total) * size_t((vocab + kChunk - 1) / kChunk) * sizeof(Part);
 }
 
 extern "C" int mcamd_verify_drafts(const float *logits, int64_t logits_stride, const float *draft_probs,
@@ -246,7 +482,6 @@ extern "C" int mcamd_verify_drafts(const float *logits, int64_t logits_stride, c
                                    int32_t *counts, int64_t *out_tokens, int64_t n_rows, int64_t total,
                                    int64_t max_seqlen, int64_t vocab, float temperature, void *scratch,
                                    size_t scratch_bytes, void *stream) {
-  (void)scratch, (void)scratch_bytes;
   if (n_rows < 0 || total < 0 || max_seqlen < 1 || vocab <= 0 || vocab > (int64_t(1) << 30))
     return fail(MCAMD_EINVAL, "verify_drafts: need n_rows, total >= 0, max_seqlen >= 1, 0 < vocab <= 2^30");
   if (max_seqlen > kMaxNodes) return fail(MCAMD_EUNSUPPORTED, "verify_drafts: more than 1024 nodes in a row");
@@ -262,6 +497,12 @@ extern "C" int mcamd_verify_drafts(const float *logits, int64_t logits_stride, c
   }
   if (!cu_seqlens || !kept || !counts || !out_tokens || (total > 0 && (!logits || !tokens || !parents || !numbers)))
     return fail(MCAMD_EINVAL, "verify_drafts: null pointer");
+  const int64_t chunks = (vocab + kChunk - 1) / kChunk;
+  if (total * chunks > 0x7fffffff / kChunkThreads)
+    return fail(MCAMD_EUNSUPPORTED, "verify_drafts: grid too large");
+  if (!aligned(scratch, 16)) return fail(MCAMD_EINVAL, "verify_drafts: scratch not 16-byte aligned");
+  if (total > 0 && (!scratch || scratch_bytes < mcamd_verify_drafts_scratch_bytes(total, vocab)))
+    return fail(MCAMD_EWORKSPACE, "verify_drafts: scratch smaller than mcamd_verify_drafts_scratch_bytes()");
   VerifyParams P;
   P.logits = logits;
   P.probs = temperature > 0.f ? draft_probs : nullptr;
@@ -278,7 +519,15 @@ extern "C" int mcamd_verify_drafts(const float *logits, int64_t logits_stride, c
   P.most = int(max_seqlen);
   P.vocab = int(vocab);
   P.greedy = temperature == 0.f;
-  P.inv_temp = P.greedy ? 1.0 : 1.0 / double(temperature);
+  P.scale = P.greedy ? 1.0 : 1.44269504088896340736 / double(temperature);
+  P.parts = static_cast<Part *>(scratch);
+  P.chunks = int(chunks);
+  if (total > 0) {
+    hipLaunchKernelGGL(verify_parts_kernel, dim3(unsigned(total * chunks)), dim3(kChunkThreads), 0,
+                       as_stream(stream), P);
+    const int st = launch_status("verify_drafts");
+    if (st != MCAMD_OK) return st;
+  }
   hipLaunchKernelGGL(verify_kernel, dim3(unsigned(n_rows)), dim3(kThreads), 0, as_stream(stream), P);
   return launch_status("verify_drafts");
 }

@@ -20,6 +20,7 @@ target's own distribution accepts, and the token after the last of those.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple
 
 import torch
@@ -67,6 +68,11 @@ class Verified(NamedTuple):
     kept: torch.Tensor    # (rows, max_seqlen) int32: the accepted nodes, the root first, then -1
     counts: torch.Tensor  # (rows,) int32: how many (0 for a row without nodes)
     tokens: torch.Tensor  # (rows, max_seqlen) int64: the tokens after the root, as many, then -1
+
+
+@functools.lru_cache(maxsize=1024)
+def _verify_scratch_bytes(total, vocab):
+    return _ext.lib().mcamd_verify_drafts_scratch_bytes(total, vocab)
 
 
 def verify_drafts(logits, tokens, parents, cu_seqlens, numbers, *, temperature=1.0, draft_probs=None,
@@ -130,11 +136,11 @@ def verify_drafts(logits, tokens, parents, cu_seqlens, numbers, *, temperature=1
     kept = parents.new_empty((n, max_seqlen))
     counts = parents.new_empty((n,))
     out = tokens.new_empty((n, max_seqlen))
-    lib = _ext.lib()
     with _ext.on_device(dev):
-        nbytes = lib.mcamd_verify_drafts_scratch_bytes(total, vocab)
+        nbytes = _verify_scratch_bytes(total, vocab)
+        # Scratch of the call's own: calls on several streams, and captured graphs, share nothing.
         ws = logits.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-        st = lib.mcamd_verify_drafts(
+        st = _ext.lib().mcamd_verify_drafts(
             logits.data_ptr(), max(logits.stride(0), vocab), probs.data_ptr() if probs is not None else None,
             max(probs.stride(0), vocab) if probs is not None else 0, tokens.data_ptr(), parents.data_ptr(),
             cu_seqlens.data_ptr(), numbers.data_ptr(), kept.data_ptr(), counts.data_ptr(), out.data_ptr(),

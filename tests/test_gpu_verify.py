@@ -261,3 +261,9 @@ def test_at_random(seed):
     check(*drafted(seed + 50, lens, rng.choice([rng.randrange(1, 300), rng.randrange(300, 9000)]),
                    rng.choice([0.0, 1.0, 0.37, 1.6]), drawn, rng.choice([0.5, 2.0, 5.0]), rng.choice([0.1, 1.0]),
                    rng.choice(["random", "chain", "star"])), least=0.8)
+
+
+def test_vocabularies_of_more_chunks_than_are_kept():
+    """Past 262144 tokens the remainder's sums by chunk are made again; past 64 chunks a lane has several."""
+    for drawn in (False, True):
+        check(*drafted(40, [2, 2, 3], 300001, 1.0, drawn=drawn, off=2.0), least=0.3)
