@@ -13,15 +13,17 @@
 //
 // The draw is the smallest token whose running sum of weights passes u_0 times the whole (u_0 the root's number,
 // which no test uses). It falls between neighbours of a whole vocabulary, where 32-bit sums would move
-// it: weights and sums are in 64 bits, whose multiply-adds run as fast here as those of 32. A weight is
-// exp2 by its series to the tenth power, within 2^-40.
+// it: weights and sums are in 64 bits, whose multiply-adds run as fast here as those of 32.
 //
 // Two launches. The first reads every logit once, a workgroup kChunk of a node's, and leaves the largest, its
-// place and the sum of the chunk's weights against it: bound by HBM. The second has a workgroup a row: a node's
-// chunks are put together by a wave, the probabilities of all drafts fetched at once, and the walk then goes
-// through LDS, every wave by itself; the sum (p - a q)+ over the vocabulary is taken where a further child has
-// to be tried against it. The draw finds its chunk by the chunks' sums (of what is left of p and q, by a pass
-// over the row) and reads that one again.
+// place and the sum of the chunk's weights against it: bound by HBM (32 trees of 32 nodes, vocabulary 32768: 134
+// MB in 28 us, 4.8 TB/s). The second has a workgroup a row: a node's chunks are put together by a few lanes and the
+// probabilities of all drafts fetched at once; its first wave then walks, out of registers and LDS, and finds the
+// draw's chunk by the chunks' sums, all waves make the sums (p - a q)+ where they are wanted (before a further
+// child is tried against them, and for the draw) and read that chunk again. Bound by latency: seven round trips,
+// 12 us for those trees, 16 with such a sum over a row (64 chains of four); with sixteen waves that all walk 19
+// and 21, since a SIMD's four wait for one another. Weights are made eight side by side or four: the ten
+// multiply-adds of one wait for each other.
 #include "kernels.h"
 
 #include <cmath>
@@ -29,18 +31,23 @@
 namespace mcamd {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxNodes = 1024;
 constexpr int kChunkThreads = 256;
-constexpr int kRestChunks = 64;  // whose sums of (p - a q)+ are kept
+constexpr int kRestChunks = 2048;  // whose sums of (p - a q)+ have room
+constexpr double kNothing = 1e-290;  // of a probability: above the least that exp2_64 makes
 constexpr int kChunk = 16 * kChunkThreads;  // logits
-static_assert(kChunk == 4 * kThreads, "the draw's threads have four each");
+static_assert(kChunk == 8 * kThreads, "the draw's threads have eight each");
 
 struct Part {  // of a chunk
   double sum;
   float top;
   int at;
+};
+
+struct Link {  // of a node: whom it follows, and its token or -1
+  int up, token;
 };
 
 struct VerifyParams {
@@ -59,46 +66,82 @@ struct VerifyParams {
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // at any float's address
 
-// 2^y for y <= 0, to 2^-40: 2^n by the exponent, 2^f, |f| <= 1/2, by the series of e^(f ln 2).
-__device__ __forceinline__ double exp2_64(double y) {
-  const double n = __builtin_rint(y), r = (y - n) * 0.69314718055994530942;
-  double p = 1.0 / 3628800;
-  p = fma(p, r, 1.0 / 362880);
-  p = fma(p, r, 1.0 / 40320);
-  p = fma(p, r, 1.0 / 5040);
-  p = fma(p, r, 1.0 / 720);
-  p = fma(p, r, 1.0 / 120);
-  p = fma(p, r, 1.0 / 24);
-  p = fma(p, r, 1.0 / 6);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  return y > -1000.0 ? ldexp(p, int(n)) : 0.0;
+// 2^y for y up to 0 (from -1020 on), to 2^-45: y + 1.5 2^52 has the nearest whole number in its low word, which
+// goes into the exponent, and 2^f, |f| <= 1/2, is the polynomial that meets it in the ten Chebyshev points of the
+// interval. Seventeen instructions a logit with the sum, four fewer than by the series, rint and ldexp.
+// N of them side by side: alone, each multiply-add would wait for the one before.
+template <int N>
+__device__ __forceinline__ void exp2_64(double (&y)[N]) {
+  constexpr double kWhole = 6755399441055744.0;
+  constexpr double kSeries[10] = {1.0000000000000135,    0.6931471805599462,     0.2402265069564034,
+                                  0.05550410866465167,   0.009618129193934313,   0.0013333558200794592,
+                                  0.0001540343375125101, 1.5252672924850737e-05, 1.325964524488711e-06,
+                                  1.0205905413765595e-07};
+  double f[N], p[N];
+  int whole[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const double z = fmax(y[i], -1020.0), t = z + kWhole;
+    f[i] = z - (t - kWhole);
+    whole[i] = __double2loint(t) << 20;
+    p[i] = kSeries[9];
+  }
+#pragma unroll
+  for (int k = 8; k >= 0; --k)
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = fma(p[i], f[i], kSeries[k]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) y[i] = __hiloint2double(__double2hiint(p[i]) + whole[i], __double2loint(p[i]));
 }
 
 // Logits as weights against the largest of them, which an infinite one makes 1 and all others 0. NaN has none.
 struct Weigher {
   float top;
-  double scale;
+  double scale, shift;
+  __device__ __forceinline__ Weigher(float t, double s) : top(t), scale(s), shift(-double(t) * s) {}
+  // Of a finite top, -inf being next to nothing.
+  template <int N>
+  __device__ __forceinline__ void finite(const float (&x)[N], double (&w)[N]) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = fma(double(x[i]), scale, shift);
+    exp2_64(w);
+  }
+  template <int N>
+  __device__ __forceinline__ void weigh(const float (&x)[N], double (&w)[N]) const {
+    finite(x, w);
+    const bool inf = top == INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = inf ? (x[i] == top ? 1.0 : 0.0) : x[i] > -INFINITY ? w[i] : 0.0;
+  }
   __device__ __forceinline__ double operator()(float x) const {
-    const double w = exp2_64((double(x) - double(top)) * scale);
-    return x == top ? 1.0 : x > -INFINITY && top < INFINITY ? w : 0.0;
+    const float x1[1] = {x};
+    double w[1];
+    weigh(x1, w);
+    return w[0];
   }
 };
 
-__device__ __forceinline__ double wave_sum64(double x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+// Inclusive sums over the wave, by moves between lanes on the VALU: sixteen waves' shuffles would wait for one another
+// at the LDS.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved64(double x) {
+  return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(x), CTRL, ROWS, 0xf, false),
+                          __builtin_amdgcn_update_dpp(0, __double2loint(x), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ double wave_upto64(double x) {
+  x += moved64<0x111, 0xf>(x);  // row_shr:1
+  x += moved64<0x112, 0xf>(x);  // row_shr:2
+  x += moved64<0x114, 0xf>(x);  // row_shr:4
+  x += moved64<0x118, 0xf>(x);  // row_shr:8
+  x += moved64<0x142, 0xa>(x);  // row_bcast:15
+  x += moved64<0x143, 0xc>(x);  // row_bcast:31
   return x;
 }
-__device__ __forceinline__ double wave_upto64(double x, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
-  }
-  return x;
+__device__ __forceinline__ double lane64(double x, int lane) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(x), lane),
+                          __builtin_amdgcn_readlane(__double2loint(x), lane));
 }
+__device__ __forceinline__ double wave_sum64(double x) { return lane64(wave_upto64(x), 63); }
 __device__ __forceinline__ int wave_min(int x) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) x = min(x, __shfl_xor(x, o, 64));
@@ -155,13 +198,21 @@ __global__ __launch_bounds__(kChunkThreads) void verify_parts_kernel(VerifyParam
     part->at = at;
     return;
   }
-  const Weigher weigh{top, P.scale};
+  const Weigher weigh(top, P.scale);
   double sum = 0;
-  if (top > -INFINITY) {
+  if (fabsf(top) < INFINITY) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float y[4] = {x[j][0], x[j][1], x[j][2], x[j][3]};
+      double w[4];
+      weigh.finite(y, w);
+      sum += (w[0] + w[1]) + (w[2] + w[3]);
+    }
+  } else if (top > 0) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum += weigh(x[j][e]);
+      for (int e = 0; e < 4; ++e) sum += x[j][e] == top ? 1.0 : 0.0;
   }
   sum = wave_sum64(sum);
   if (lane == 0) s_sum[wave] = sum;
@@ -173,13 +224,20 @@ __global__ __launch_bounds__(kChunkThreads) void verify_parts_kernel(VerifyParam
 }
 
 __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyParams P) {
-  __shared__ double s_all[kMaxNodes], s_w[kMaxNodes];
+  __shared__ double s_all[kMaxNodes], s_one[kMaxNodes], s_w[kMaxNodes];
   __shared__ float s_top[kMaxNodes], s_q[kMaxNodes], s_u[kMaxNodes];
-  __shared__ int s_up[kMaxNodes], s_token[kMaxNodes], s_best[kMaxNodes];
+  __shared__ int s_best[kMaxNodes];
+  __shared__ __attribute__((aligned(16))) Link s_link[kMaxNodes + 1];
+  __shared__ __attribute__((aligned(16))) int s_gone[kMaxNodes];  // the tokens of refused guesses, and their weights
+  __shared__ double s_gone_w[kMaxNodes];
+  __shared__ double s_rest[kRestChunks];  // sums of (p - a q)+, by runs of tokens
   __shared__ double s_sum[kWaves];
-  __shared__ double s_rest[kRestChunks][kWaves];
-  __shared__ int s_gone[kMaxNodes], s_chunk;
-  __shared__ double s_want;
+  __shared__ struct {  // the first wave's word to the others
+    int what, node, count, chunk, n_gone;
+    bool rest;
+    double less, want;
+  } s_say;
+  enum { kDone, kSum, kDraw };
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int begin = max(P.cu[b], 0), n = min(max(min(P.cu[b + 1], P.total) - begin, 0), P.most);
@@ -192,62 +250,79 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyParams P) {
   }
   const int V = P.vocab, C = P.chunks;
   // Every node's draft and number, and its chunks put together.
-  int up = 0, token = -1;
-  if (tid < n) {
-    const int64_t t = P.tokens[begin + tid];
-    token = t >= 0 && t < V ? int(t) : -1;
-    up = tid == 0 ? -1 : P.parents[begin + tid];
-    s_up[tid] = up;
-    s_token[tid] = token;
-    s_u[tid] = P.numbers[begin + tid];
-  }
-  for (int i = wave; i < n; i += kWaves) {
-    const Part *part = P.parts + int64_t(begin + i) * C;
+  auto link_of = [&](int i) {
+    Link x{-1, -1};
+    if (i < n) {
+      const int64_t t = P.tokens[begin + i];
+      const float u = P.numbers[begin + i];
+      if (i > 0) x.up = P.parents[begin + i];
+      if (x.up >= i) x.up = -1;
+      if (t >= 0 && t < V) x.token = int(t);
+      s_u[i] = u;
+    }
+    if (i <= n) s_link[i] = x;  // and one behind them that follows none
+    return x;
+  };
+  auto logit_of = [&](int i, const Link &x) {  // of the draft, behind its parent
+    if (P.greedy || x.up < 0 || x.token < 0) return -INFINITY;
+    if (P.probs) s_q[i] = P.probs[int64_t(begin + x.up) * P.probs_stride + x.token];
+    return P.logits[int64_t(begin + x.up) * P.logits_stride + x.token];
+  };
+  const Link own = link_of(tid);
+  for (int i = tid + kThreads; i <= n; i += kThreads) link_of(i);
+  const float own_logit = logit_of(tid, own);
+  int lanes = 1;  // of a node, as many as its chunks
+  while (lanes < C && lanes < 64) lanes *= 2;
+  for (int i0 = wave * (64 / lanes); i0 < n; i0 += kThreads / lanes) {
+    const int i = i0 + lane / lanes, first = lane & (lanes - 1);
+    const Part *part = P.parts + int64_t(begin + min(i, n - 1)) * C;
     float top = -INFINITY;
-    for (int c = lane; c < C; c += 64) top = fmaxf(top, part[c].top);
-    top = wave_max<64>(top);
+    for (int c = first; c < C; c += lanes) top = fmaxf(top, part[c].top);
+    for (int o = lanes >> 1; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
     if (P.greedy) {
       int best = 0x7fffffff;
-      for (int c = lane; c < C; c += 64)
+      for (int c = first; c < C; c += lanes)
         if (part[c].top == top) best = min(best, part[c].at);
-      best = wave_min(best);
-      if (lane == 0) s_best[i] = best;
+      for (int o = lanes >> 1; o > 0; o >>= 1) best = min(best, __shfl_xor(best, o, 64));
+      if (first == 0 && i < n) s_best[i] = best;
     } else {
-      const Weigher weigh{top, P.scale};
+      const Weigher weigh(top, P.scale);
       double all = 0;
-      for (int c = lane; c < C; c += 64) all += part[c].sum * weigh(part[c].top);
-      all = wave_sum64(all);
-      if (lane == 0) s_all[i] = all;
+      for (int c = first; c < C; c += lanes) all += part[c].sum * weigh(part[c].top);
+      for (int o = lanes >> 1; o > 0; o >>= 1) all += __shfl_xor(all, o, 64);
+      if (first == 0 && i < n) s_all[i] = all, s_one[i] = 1.0 / all;
     }
-    if (lane == 0) s_top[i] = top;
+    if (first == 0 && i < n) s_top[i] = top;
   }
   __syncthreads();
-  if (!P.greedy && tid > 0 && tid < n) {
-    s_w[tid] = 0;
-    if (up >= 0 && up < tid && token >= 0) {
-      const float x = P.logits[int64_t(begin + up) * P.logits_stride + token];
-      if (P.probs) s_q[tid] = P.probs[int64_t(begin + up) * P.probs_stride + token];
-      s_w[tid] = Weigher{s_top[up], P.scale}(x);
+  for (int i = tid; !P.greedy && i < n; i += kThreads) {
+    const Link x = i == tid ? own : s_link[i];
+    const float logit = i == tid ? own_logit : logit_of(i, x);
+    double w = logit > -INFINITY ? Weigher(s_top[x.up], P.scale)(logit) : 0.0;
+    // A guess that a sibling before it has made has nothing left.
+    if (!P.probs) {
+      int again = 0;
+      if (n <= 64) {
+        for (int j0 = 0; j0 < n; j0 += 8)
+#pragma unroll
+          for (int j = j0; j < j0 + 8; ++j)
+            again |= int(__builtin_amdgcn_readlane(x.up, j) == x.up) &
+                     int(__builtin_amdgcn_readlane(x.token, j) == x.token) & int(j < lane);
+      } else {
+        const int4 *links = reinterpret_cast<const int4 *>(s_link);  // two nodes each
+#pragma unroll 8
+        for (int j = 0; j < min((i | 63) + 1, n) >> 1; ++j) {
+          const int4 y = links[j];
+          again |= int(y.x == x.up) & int(y.y == x.token) & int(2 * j < i);
+          again |= int(y.z == x.up) & int(y.w == x.token) & int(2 * j + 1 < i);
+        }
+      }
+      w = again ? 0.0 : w;
     }
+    s_w[i] = w;
   }
   __syncthreads();
 
-  int node = 0, count = 1;
-  double less = 0, left = 0;  // a and Z, of guesses Z in units of the weights
-  bool summed = true;         // left is the sum for this a
-  const float *row = nullptr, *q_row = nullptr;
-  Weigher weigh{0.f, P.scale};
-  double one = 0;  // over the node's weights
-  auto enter = [&]() {
-    row = P.logits + int64_t(begin + node) * P.logits_stride;
-    q_row = P.probs ? P.probs + int64_t(begin + node) * P.probs_stride : nullptr;
-    weigh.top = s_top[node];
-    less = 0;
-    summed = true;
-    if (P.greedy) return;
-    one = 1.0 / s_all[node];
-    left = q_row ? 1.0 : s_all[node];
-  };
   // Four logits from token i on, or draft probabilities; past the vocabulary what has no weight.
   auto four = [&](const float *from, int i, float none) {
     f32x4u x;
@@ -259,211 +334,247 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyParams P) {
     }
     return x;
   };
-  // What is left of the probabilities of four tokens.
-  auto rest_of = [&](const f32x4u &x, const f32x4u &q, double (&w)[4]) {
+  // What is left of the probabilities of four tokens: p - a q, where more than next to nothing is.
+  auto rest_of = [&](const Weigher &weigh, double one, double less, const f32x4u &x, const f32x4u &q,
+                     double (&w)[4]) {
+    const float y[4] = {x[0], x[1], x[2], x[3]};
+    weigh.finite(y, w);
+    if (weigh.top == INFINITY)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = fmax(weigh(x[e]) * one - less * double(q[e]), 0.0);
+      for (int e = 0; e < 4; ++e) w[e] = y[e] == INFINITY ? 1.0 : 0.0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = fmax(fma(w[e], one, fma(-less, double(q[e]), -kNothing)), 0.0);
     return (w[0] + w[1]) + (w[2] + w[3]);
   };
-  // The sum of it over the vocabulary, by its chunks' sums, of which the first ones are kept.
-  auto rest_sum = [&]() {
-    constexpr int U = 4;  // chunks whose loads are under way at once
-    double sum = 0;
-    __syncthreads();  // s_rest and s_sum have been read
-    for (int c0 = 0; c0 < C; c0 += U) {
-      f32x4u x[U], q[U];
+  // A chunk is `runs` runs of tokens, so that all waves have some.
+  int runs = 1;
+  while (runs * 2 * C <= kWaves) runs *= 2;
+  // s_rest of a node, run by run: by all waves.
+  auto rest_sums = [&](int node, double less) {
+    constexpr int U = 8;  // loads of each under way at once
+    const float *row = P.logits + int64_t(begin + node) * P.logits_stride;
+    const float *q_row = P.probs + int64_t(begin + node) * P.probs_stride;
+    const Weigher weigh(s_top[node], P.scale);
+    const double one = s_one[node];
+    const int each = kChunk / runs;
+    for (int r = wave; r < C * runs; r += kWaves) {
+      double sum = 0;
+      for (int i0 = 0; i0 < each; i0 += 256 * U) {
+        f32x4u x[U], q[U];
 #pragma unroll
-      for (int c = 0; c < U; ++c) {
-        x[c] = four(row, (c0 + c) * kChunk + 4 * tid, -INFINITY);
-        q[c] = four(q_row, (c0 + c) * kChunk + 4 * tid, 0.f);
-      }
+        for (int u = 0; u < U; ++u) {
+          const int i = i0 + 256 * u < each ? r * each + i0 + 256 * u + 4 * lane : V;
+          x[u] = four(row, i, -INFINITY);
+          q[u] = four(q_row, i, 0.f);
+        }
 #pragma unroll
-      for (int c = 0; c < U; ++c) {
-        double w[4];
-        const double part = wave_sum64(rest_of(x[c], q[c], w));
-        sum += part;
-        if (lane == 0 && c0 + c < kRestChunks) s_rest[c0 + c][wave] = part;
+        for (int u = 0; u < U; ++u) {
+          double w[4];
+          sum += rest_of(weigh, one, less, x[u], q[u], w);
+        }
       }
+      sum = wave_sum64(sum);
+      if (lane == 0) s_rest[r] = sum;
     }
-    if (lane == 0) s_sum[wave] = sum;
-    __syncthreads();
-    sum = 0;
-    for (int w = 0; w < kWaves; ++w) sum += s_sum[w];
-    return sum;
   };
 
-  // The walk, by every wave alike.
-  enter();
-  for (;;) {
-    int found = -1;
-    for (int base = (node + 1) & ~63; base < n && found < 0 && weigh.top > -INFINITY; base += 64) {
-      const int mine = base + lane;
-      const bool kid = mine > node && mine < n && s_up[min(mine, n - 1)] == node && s_token[min(mine, n - 1)] >= 0;
-      for (uint64_t left_of = __builtin_amdgcn_ballot_w64(kid); left_of != 0 && found < 0; left_of &= left_of - 1) {
-        const int i = base + __builtin_ctzll(left_of), x = s_token[i];
-        if (P.greedy) {
-          if (x == s_best[node]) found = i;
-          continue;
-        }
-        const double u = s_u[i];
-        if (q_row) {
-          if (!summed) left = rest_sum(), summed = true;
-          const double q = s_q[i];
-          if (u * left * q < fmax(s_w[i] * one - less * q, 0.0)) {
-            found = i;
-          } else {
-            less += left;
-            summed = false;
-          }
+  // The walk, by the first wave. The others wait for it (and would only be in its way), but for the sums of what
+  // is left and the draw. The first 64 nodes are in registers, a node a lane.
+  int node = 0, count = 1, base = 0;
+  double less = 0, left = 0;  // a and Z, of guesses Z in units of the weights
+  bool summed = true;         // left is the sum for this a
+  uint64_t kids = 0;          // that are left to try, among nodes base ..
+  const double my_w = P.greedy ? 0.0 : s_w[min(lane, n - 1)];
+  const float my_u = s_u[min(lane, n - 1)], my_q = P.probs ? s_q[min(lane, n - 1)] : 1.f;
+  auto kids_of = [&](int base) {  // the node's children among 64, bit by bit
+    const Link x = base == 0 ? own : s_link[min(base + lane, n)];
+    return __builtin_amdgcn_ballot_w64(x.up == node && x.token >= 0 && base + lane < n);
+  };
+  auto uniform = [](bool x) { return __builtin_amdgcn_ballot_w64(x) != 0; };  // x is the same in all lanes
+  auto lane32 = [&](float x, int l) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), l)); };
+  auto enter = [&]() {
+    less = 0;
+    summed = true;
+    if (!P.greedy) left = P.probs ? 1.0 : s_all[node];
+    base = node & ~63;
+    kids = s_top[node] > -INFINITY ? kids_of(base) : 0;
+  };
+  auto walk = [&]() {  // false where a sum is wanted first
+    for (;;) {
+      if (kids == 0) {
+        if (base + 64 >= n || !(s_top[node] > -INFINITY)) return true;
+        base += 64;
+        kids = kids_of(base);
+        continue;
+      }
+      const int l = __builtin_ctzll(kids), i = base + l;
+      bool taken;
+      if (P.greedy) {
+        taken = uniform(s_link[i].token == s_best[node]);
+      } else {
+        const double u = base == 0 ? lane32(my_u, l) : s_u[i], w = base == 0 ? lane64(my_w, l) : s_w[i];
+        if (P.probs) {
+          if (!summed) return false;
+          const double q = base == 0 ? lane32(my_q, l) : s_q[i];
+          taken = uniform(u * left * q < fmax(w * s_one[node] - less * q, 0.0));
+          if (!taken) less += left, summed = false;
         } else {
-          double w = s_w[i];
-          for (int j = node + 1; j < i; ++j)  // refused before
-            if (s_up[j] == node && s_token[j] == x) w = 0;
-          if (u * left < w)
-            found = i;
-          else
-            left -= w;
+          taken = uniform(u * left < w);
+          if (!taken) left -= w;
         }
       }
+      kids &= kids - 1;
+      if (!taken) continue;
+      node = i;
+      if (lane == 0) kept[count] = node, out[count - 1] = s_link[node].token;
+      ++count;
+      enter();
     }
-    if (found < 0) break;
-    node = found;
-    if (tid == 0) kept[count] = node, out[count - 1] = s_token[node];
-    ++count;
-    enter();
-  }
-  if (tid == 0) kept[0] = 0, P.counts[b] = count;
-  if (P.greedy || !(weigh.top > -INFINITY)) {
-    if (tid == 0) out[count - 1] = weigh.top > -INFINITY ? s_best[node] : 0;
-    return;
-  }
-
-  // The draw: the chunk first. Its first wave finds it, from the sums of the chunks (the node's own, less the
-  // guesses that were refused there, or of what is left of p and q).
-  int n_gone = 0;  // distinct refused guesses
-  const Part *parts = P.parts + int64_t(begin + node) * C;
-  bool rest = q_row && less > 0;  // else all of p, or p without the refused
-  if (!q_row) {
-    for (int base = (node + 1) & ~63; base < n; base += 64) {
-      const int mine = base + lane;
-      bool kid = mine > node && mine < n && s_up[min(mine, n - 1)] == node && s_token[min(mine, n - 1)] >= 0;
-      for (int j = node + 1; kid && j < mine; ++j) kid = !(s_up[j] == node && s_token[j] == s_token[mine]);
-      const uint64_t kids = __builtin_amdgcn_ballot_w64(kid);
-      if (wave == 0 && kid) s_gone[n_gone + __builtin_popcountll(kids & ((uint64_t(1) << lane) - 1))] = mine;
-      n_gone += __builtin_popcountll(kids);
-    }
-  }
-  __syncthreads();  // s_gone is written
-  auto chunk_sum = [&](int c) {
-    if (c >= C) return 0.0;
-    const double all = parts[c].sum * weigh(parts[c].top);
-    double sum = all;
-    for (int g = 0; g < n_gone; ++g)
-      if (s_token[s_gone[g]] / kChunk == c) sum -= s_w[s_gone[g]];
-    return sum > all * 0x1p-45 ? sum : 0.0;  // else rounding is what is left
   };
-  auto pick = [&](double whole, auto sum_of) {  // by the first wave: the chunk, and how far into it
+
+  // The draw's chunk: by the first wave, from the sums of the chunks, of which it is the one in which want falls.
+  auto pick = [&](double whole, auto sum_of) {
     double want = double(s_u[0]) * whole, before = 0, in_last = 0;
     int last = 0;
     for (int c0 = 0; c0 < C; c0 += 64) {
-      const double x = sum_of(c0 + lane), upto = before + wave_upto64(x, lane);
+      const double x = sum_of(c0 + lane), upto = before + wave_upto64(x);
       const uint64_t past = __builtin_amdgcn_ballot_w64(x > 0 && upto > want), any = __builtin_amdgcn_ballot_w64(x > 0);
       const int l = past ? __builtin_ctzll(past) : any ? 63 - __builtin_clzll(any) : 0;
-      if (any) last = c0 + l, in_last = __shfl(upto - x, l, 64);
+      if (any) last = c0 + l, in_last = lane64(upto - x, l);
       if (past) break;
-      before = __shfl(upto, 63, 64);
+      before = lane64(upto, 63);
     }
-    if (lane == 0) s_chunk = last, s_want = want - in_last;
+    if (lane == 0) s_say.chunk = last, s_say.want = want - in_last;
   };
-  double whole = 0;
-  if (rest) {
-    whole = rest_sum();
-    rest = whole > 0;
-  }
-  if (!rest) {
-    if (wave == 0) {
-      for (int round = 0; round < 2; ++round) {
-        whole = 0;
-        for (int c = lane; c < C; c += 64) whole += chunk_sum(c);
-        whole = wave_sum64(whole);
-        if (whole > 0 || n_gone == 0) break;
-        n_gone = 0;  // nothing is left but rounding: from all of them
+  // Where nothing is left of p - a q, or there is no q: p without the guesses that were refused.
+  auto pick_guesses = [&]() {
+    int n_gone = 0;
+    for (int base = node & ~63; !P.probs && base < n; base += 64) {
+      const double w = base == 0 ? my_w : s_w[min(base + lane, n - 1)];
+      const bool kid = ((kids_of(base) >> lane) & 1) && w > 0;  // distinct
+      const uint64_t all = __builtin_amdgcn_ballot_w64(kid);
+      if (kid) {
+        const int at = n_gone + __builtin_popcountll(all & ((uint64_t(1) << lane) - 1));
+        s_gone[at] = s_link[base + lane].token;
+        s_gone_w[at] = w;
       }
-      pick(whole, chunk_sum);
-      if (lane == 0) s_sum[0] = n_gone;
+      n_gone += __builtin_popcountll(all);
     }
-    __syncthreads();
-    n_gone = int(s_sum[0]);
-  } else if (C <= kRestChunks) {
-    if (wave == 0)
-      pick(whole, [&](int c) {
-        double sum = 0;
-        if (c < C)
-          for (int k = 0; k < kWaves; ++k) sum += s_rest[c][k];
-        return sum;
-      });
-    __syncthreads();
-  } else {
-    // More chunks than are kept: one after another, until the draw's is passed.
-    const double want = double(s_u[0]) * whole;
-    double before = 0, in_last = 0;
-    int last = 0;
-    for (int c = 0; c < C; ++c) {
-      double w[4];
-      const int i = c * kChunk + 4 * tid;
-      double sum = wave_sum64(rest_of(four(row, i, -INFINITY), four(q_row, i, 0.f), w));
-      __syncthreads();
-      if (lane == 0) s_sum[wave] = sum;
-      __syncthreads();
-      sum = 0;
-      for (int k = 0; k < kWaves; ++k) sum += s_sum[k];
-      if (sum > 0) last = c, in_last = before;
-      before += sum;
-      if (before > want) break;
+    // All waves look through the list, four at a time.
+    if (lane < 4 && n_gone + lane < kMaxNodes) s_gone[n_gone + lane] = -1, s_gone_w[n_gone + lane] = 0;
+    __builtin_amdgcn_wave_barrier();
+    const Part *parts = P.parts + int64_t(begin + node) * C;
+    const Weigher weigh(s_top[node], P.scale);
+    auto chunk_sum = [&](int c) {
+      if (c >= C) return 0.0;
+      const double all = parts[c].sum * weigh(parts[c].top);
+      double sum = all;
+#pragma unroll 4
+      for (int g = 0; g < n_gone; ++g) sum -= s_gone[g] / kChunk == c ? s_gone_w[g] : 0.0;
+      return sum > all * 0x1p-40 ? sum : 0.0;  // else rounding is what is left
+    };
+    double mine = 0, whole = 0;  // mine: the last of this lane's chunks
+    for (int round = 0; round < 2; ++round) {
+      whole = 0;
+      for (int c = lane; c < C; c += 64) whole += mine = chunk_sum(c);
+      whole = wave_sum64(whole);
+      if (whole > 0 || n_gone == 0) break;
+      n_gone = 0;  // nothing is left but rounding: from all of them
     }
-    __syncthreads();
-    if (tid == 0) s_chunk = last, s_want = want - in_last;
-    __syncthreads();
-  }
+    pick(whole, [&](int c) { return C <= 64 ? mine : chunk_sum(c); });
+    if (lane == 0) s_say.n_gone = n_gone, s_say.rest = false;
+  };
 
-  // Then the token, four of the chunk's a thread.
-  const int i0 = s_chunk * kChunk + 4 * tid;
-  double w[4];
-  const f32x4u x = four(row, i0, -INFINITY);
-  if (rest) {
-    rest_of(x, four(q_row, i0, 0.f), w);
-  } else {
+  bool walked = false;
+  for (bool first = true;; first = false) {
+    if (wave == 0) {
+      if (first) {
+        enter();
+      } else {  // the sum is there
+        left = 0;
+        for (int r = lane; r < C * runs; r += 64) left += s_rest[r];
+        left = wave_sum64(left);
+        summed = true;
+      }
+      walked = walked || walk();
+      int what = kSum;
+      if (walked) {
+        const bool none = P.greedy || !(s_top[node] > -INFINITY);
+        if (none) {
+          if (lane == 0) out[count - 1] = s_top[node] > -INFINITY ? s_best[node] : 0;
+          what = kDone;
+        } else if (!P.probs || less == 0 || (summed && !(left > 0))) {
+          pick_guesses();
+          what = kDraw;
+        } else if (summed) {
+          pick(left, [&](int c) {
+            double sum = 0;
+            if (c < C)
+              for (int r = 0; r < runs; ++r) sum += s_rest[c * runs + r];
+            return sum;
+          });
+          if (lane == 0) s_say.n_gone = 0, s_say.rest = true;
+          what = kDraw;
+        }
+        if (what != kSum && lane == 0) kept[0] = 0, P.counts[b] = count;
+      }
+      if (lane == 0) s_say.what = what, s_say.node = node, s_say.count = count, s_say.less = less;
+    }
+    __syncthreads();
+    if (s_say.what != kSum) break;
+    rest_sums(s_say.node, s_say.less);
+    __syncthreads();
+  }
+  if (s_say.what == kDone) return;
+
+  // Then the token, eight of the chunk's a thread.
+  const int at = s_say.node, i0 = s_say.chunk * kChunk + 8 * tid;
+  const float *row = P.logits + int64_t(begin + at) * P.logits_stride;
+  const f32x4u x0 = four(row, i0, -INFINITY), x1 = four(row, i0 + 4, -INFINITY);
+  const Weigher weigh(s_top[at], P.scale);
+  double w[8];
+  if (s_say.rest) {
+    const float *q_row = P.probs + int64_t(begin + at) * P.probs_stride;
+    const f32x4u q0 = four(q_row, i0, 0.f), q1 = four(q_row, i0 + 4, 0.f);
+    double w0[4], w1[4];
+    rest_of(weigh, s_one[at], s_say.less, x0, q0, w0);
+    rest_of(weigh, s_one[at], s_say.less, x1, q1, w1);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      w[e] = weigh(x[e]);
-      for (int g = 0; g < n_gone; ++g)
-        if (s_token[s_gone[g]] == i0 + e) w[e] = 0;
+    for (int e = 0; e < 4; ++e) w[e] = w0[e], w[4 + e] = w1[e];
+  } else {
+    const float y[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+    weigh.weigh(y, w);
+    for (int g = 0; g < s_say.n_gone; g += 4) {
+      const int4 gone = *reinterpret_cast<const int4 *>(&s_gone[g]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int i = i0 + e;
+        w[e] = (int(gone.x == i) | int(gone.y == i) | int(gone.z == i) | int(gone.w == i)) ? 0.0 : w[e];
+      }
     }
   }
-  double upto = wave_upto64((w[0] + w[1]) + (w[2] + w[3]), lane);
-  __syncthreads();  // s_sum has been read
+  const double mine_all = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+  double upto = wave_upto64(mine_all);
   if (lane == 63) s_sum[wave] = upto;
   __syncthreads();
-  upto -= (w[0] + w[1]) + (w[2] + w[3]);
-  for (int k = 0; k < wave; ++k) upto += s_sum[k];
-  const double want = s_want;
-  int at = 0x7fffffff, last = -1;
+  // The first wave that passes it, or by rounding none: the last that has any.
+  const double want = s_say.want;
+  const double of_wave = lane < kWaves ? s_sum[lane] : 0.0, upto_wave = wave_upto64(of_wave);
+  const uint64_t past_waves = __builtin_amdgcn_ballot_w64(of_wave > 0 && upto_wave > want),
+                 any_waves = __builtin_amdgcn_ballot_w64(of_wave > 0);
+  if (wave != (past_waves ? __builtin_ctzll(past_waves) : any_waves ? 63 - __builtin_clzll(any_waves) : 0)) return;
+  upto += lane64(upto_wave - of_wave, wave) - mine_all;
+  uint32_t past = 0, any = 0;  // of this lane's eight
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < 8; ++e) {
     upto += w[e];
-    if (w[e] > 0) {
-      last = i0 + e;
-      if (upto > want) at = min(at, i0 + e);
-    }
+    any |= w[e] > 0 ? 1u << e : 0u;
+    past |= w[e] > 0 && upto > want ? 1u << e : 0u;
   }
-  // The first past it, or by rounding none: the last that has any.
-  at = wave_min(at);
-  last = -wave_min(-last);
-  if (lane == 0) s_gone[wave] = at, s_gone[kWaves + wave] = last;
-  __syncthreads();
-  if (tid > 0) return;
-  for (int k = 0; k < kWaves; ++k) at = min(at, s_gone[k]), last = max(last, s_gone[kWaves + k]);
-  out[count - 1] = at != 0x7fffffff ? at : max(last, 0);
+  const uint64_t pasts = __builtin_amdgcn_ballot_w64(past != 0), anys = __builtin_amdgcn_ballot_w64(any != 0);
+  const int l = pasts ? __builtin_ctzll(pasts) : anys ? 63 - __builtin_clzll(anys) : 0;
+  if (lane != l) return;
+  out[s_say.count - 1] = i0 + (past ? __builtin_ctz(past) : any ? 31 - __builtin_clz(any) : 0);
 }
 
 }  // namespace
@@ -498,6 +609,8 @@ extern "C" int mcamd_verify_drafts(const float *logits, int64_t logits_stride, c
   if (!cu_seqlens || !kept || !counts || !out_tokens || (total > 0 && (!logits || !tokens || !parents || !numbers)))
     return fail(MCAMD_EINVAL, "verify_drafts: null pointer");
   const int64_t chunks = (vocab + kChunk - 1) / kChunk;
+  if (draft_probs && temperature > 0.f && chunks > kRestChunks)
+    return fail(MCAMD_EUNSUPPORTED, "verify_drafts: with draft_probs a vocabulary of at most 2^23");
   if (total * chunks > 0x7fffffff / kChunkThreads)
     return fail(MCAMD_EUNSUPPORTED, "verify_drafts: grid too large");
   if (!aligned(scratch, 16)) return fail(MCAMD_EINVAL, "verify_drafts: scratch not 16-byte aligned");
