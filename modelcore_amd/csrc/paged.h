@@ -320,6 +320,7 @@ struct PagedTiles {
   Cut *cuts;        // [slots]: the blocks of a call that may be cut, by their number
   int *n_cuts;      // and how many
   TreeMasks tree;
+  int target;       // of trees (tree_ranges.h): workgroups that a call's ranges aim at
 
   // Ranges of a block of n tiles: what pays for their partials, by the cost rule of prefill_split.h, none
   // much shorter than what starting it takes.

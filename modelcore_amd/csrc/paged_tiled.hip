@@ -20,6 +20,7 @@
 #include "paged_careful.h"
 #include "prefill_order.h"
 #include "prefill_split.h"
+#include "tree_ranges.h"
 
 #include <algorithm>
 #include <cmath>
@@ -116,13 +117,21 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
   E *const sK = reinterpret_cast<E *>(s_raw);
   E *const sV = sK + KT * KSTR;
 
-  const int id = P.cu ? int(blockIdx.x) : dealt_block(int(blockIdx.x), int(gridDim.x), P.deal);
-  PagedBlock blk;
-  const bool found =
-      find_paged_block(P.cu, P.seqlens, P.tiles.n_rows, P.T_new, P.tiles.total, P.G, P.H_kv, G_::PAIRS,
-                       P.tiles.skip, P.tiles.slots, P.kv.max_pages << P.kv.shift, P.tiles.halve,
-                       id / P.H_kv, threadIdx.x & 63, blk);
-  if (id == 0 && threadIdx.x == 0) P.tiles.note_call(found, blk);
+  const int id = P.cu || TREE ? int(blockIdx.x) : dealt_block(int(blockIdx.x), int(gridDim.x), P.deal);
+  typename std::conditional<TREE, TreeRange, PagedBlock>::type blk;
+  bool found;
+  if constexpr (TREE) {
+    const TreeRanges ranges{P.cu, P.seqlens, P.tiles.n_rows, P.T_new, P.tiles.total, P.G, P.H_kv, G_::PAIRS,
+                            P.tiles.skip, P.kv.max_pages << P.kv.shift, P.window, KT,
+                            P.tiles.slots > 0 ? P.tiles.target : 0, P.tiles.min_tiles};
+    found = find_tree_range(ranges, id / P.H_kv, threadIdx.x & 63, blk);
+    if (id == 0 && threadIdx.x == 0 && P.tiles.slots > 0) *P.tiles.n_cuts = blk.n_blocks;
+  } else {
+    found = find_paged_block(P.cu, P.seqlens, P.tiles.n_rows, P.T_new, P.tiles.total, P.G, P.H_kv, G_::PAIRS,
+                             P.tiles.skip, P.tiles.slots, P.kv.max_pages << P.kv.shift, P.tiles.halve,
+                             id / P.H_kv, threadIdx.x & 63, blk);
+    if (id == 0 && threadIdx.x == 0) P.tiles.note_call(found, blk);
+  }
   if (!found) return;
   const int kvh = id % P.H_kv, part = blk.part, row = blk.b, T_b = blk.T, s0 = blk.s0;
   const int64_t tok0 = blk.tok0;
@@ -153,7 +162,8 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
   const int64_t at = pair_at(pr);
   E *out = static_cast<E *>(P.out) + at;
   if (!row_ok) {
-    if (blk.noted && part == 0 && tid == 0) P.tiles.note_block(id, blk, 1, P.H_kv);
+    if constexpr (!TREE)
+      if (blk.noted && part == 0 && tid == 0) P.tiles.note_block(id, blk, 1, P.H_kv);
     if (live && part == 0 && (KS == 1 || wave == 0))
       for (int d = h; d < D; d += 2) out[d] = from_f32<E>(NAN);
     return;
@@ -166,15 +176,27 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
   int n_tiles = (hi - lo) / KT + 1;
   bool whole = true;
   if (blk.noted) {  // this workgroup's range of the block's tiles
-    const int ranges = P.tiles.ranges_of(blk, n_tiles);
+    int ranges;
+    if constexpr (TREE)
+      ranges = min(blk.ranges, n_tiles);
+    else
+      ranges = P.tiles.ranges_of(blk, n_tiles);
     if (part >= ranges) return;
-    if (part == 0 && tid == 0) P.tiles.note_block(id, blk, ranges, P.H_kv);
+    if (part == 0 && tid == 0) {
+      if constexpr (TREE)
+        note_tree_range(P.tiles, blk, kvh, P.H_kv, ranges);
+      else
+        P.tiles.note_block(id, blk, ranges, P.H_kv);
+    }
     whole = ranges == 1;
     const int t0 = part * n_tiles / ranges, t1 = (part + 1) * n_tiles / ranges;
     hi = min(hi, lo + t1 * KT - 1);
     lo += t0 * KT;
     n_tiles = t1 - t0;
   }
+
+  int64_t slot = id;  // of this range's partials
+  if constexpr (TREE) slot = int64_t(blk.slot + part) * P.H_kv + kvh;
 
   // Q^T fragments, B[k = dim][n = pair]. bf16: dims 16 kd + 8h .. + 7 of step kd; fp32: dims
   // 8c + 4h .. + 3, one for each of four steps. Dims past the head_dim are zero.
@@ -378,7 +400,7 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
   if constexpr (KS == 1) {
     if (!whole) {
       if (!live) return;
-      const int64_t g = int64_t(id) * kWaves + wave;
+      const int64_t g = slot * kWaves + wave;
 #pragma unroll
       for (int md = 0; md < MD; ++md)
 #pragma unroll
@@ -466,7 +488,7 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
     const bool c_live = c < n;
     if (!whole) {
       if (!c_live) return;
-      const int64_t g = id;
+      const int64_t g = slot;
       const int x = tid & 7;
 #pragma unroll
       for (int i = 0; i < DT / 4; ++i)
@@ -510,11 +532,12 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(TiledParams P, in
   const int n_blocks = *P.tiles.n_cuts;
   const PagedTiles::Cut blk = P.tiles.cuts[id];
   const int ranges = blk.ranges;
-  if (d >= P.D || id >= n_blocks || ranges == 1) return;  // of one range: written by the block itself
+  if (d >= P.D || id >= (TREE ? n_blocks * P.H_kv : n_blocks) || ranges == 1) return;  // of one range: written by the block itself
   const int kvh = id % P.H_kv;
   const int64_t n_pairs = int64_t(blk.T) * P.G, p0 = int64_t(blk.qt) * pairs;
   const int n = int(min(int64_t(pairs), n_pairs - p0));
   const int in_block = 32 * w + col;
+  if (TREE && 32 * w >= n) return;  // no pair of the 32
   const bool live = in_block < n;
   const int t = live ? int((p0 + in_block) / P.G) : 0;
   auto pair_at = [&](int i) {
@@ -523,8 +546,13 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(TiledParams P, in
   };
 
   constexpr int U = 8;
-  const int64_t group = int64_t(id) * groups + w, step = int64_t(n_blocks) * groups;
-  const int64_t second = int64_t(blk.second) * groups + w;
+  int64_t group = int64_t(id) * groups + w, step = int64_t(n_blocks) * groups;
+  int64_t second = int64_t(blk.second) * groups + w;
+  if constexpr (TREE) {  // the ranges one after another, KV heads between them
+    group = second;
+    step = int64_t(P.H_kv) * groups;
+    second += step;
+  }
   float M = -INFINITY, L = 0.f;
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
   for (int r0 = 0; r0 < ranges; r0 += U) {
@@ -569,7 +597,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(TiledParams P, in
 // What a call runs: the waves over pairs (KS = 1) or keys (KS = 4), and room for the partials of cut
 // blocks.
 struct TiledPlan {
-  int ks, pairs, kt, slots, min_tiles;
+  int ks, pairs, kt, slots, min_tiles, target;
   int64_t bound;  // of blocks
   float tile_us;
 };
@@ -588,7 +616,11 @@ TiledPlan tiled_plan(const PagedArgs &a, int64_t skip) {
     // Measured time of a tile on a compute unit of its own, per head dim (prefill_tiled.hip).
     t.tile_us = float(a.head_dim) * (ks == 4 ? (bf ? 0.027f : 0.085f) : (bf ? 0.012f : 0.035f));
     t.min_tiles = std::max(1, int(kRangeUs / t.tile_us));
-    t.slots = paged_slots(a, t.bound, t.pairs, a.head_dim <= 128 ? 2 : 1, int64_t(t.min_tiles) * t.kt);
+    t.target = (a.head_dim <= 128 ? 2 : 1) * device_cus();
+    if (a.tree.masks)
+      t.slots = paged_keys(a) >= 2 * int64_t(t.min_tiles) * t.kt ? int(tree_slots(t.target, a.n_kv_head)) : 0;
+    else
+      t.slots = paged_slots(a, t.bound, t.pairs, a.head_dim <= 128 ? 2 : 1, int64_t(t.min_tiles) * t.kt);
     return t;
   };
   const TiledPlan whole = plan(1);
@@ -638,7 +670,8 @@ int run(const TiledParams &P, const PagedArgs &a, const TiledPlan &t) {
   using G_ = Geo<E, DP, KS>;
   if (t.pairs != G_::PAIRS || t.kt != G_::KT)
     return fail(MCAMD_EINVAL, "paged attention: plan and kernel disagree");
-  const int64_t blocks = std::max<int64_t>(t.bound * P.H_kv, P.tiles.slots);
+  const int64_t blocks = a.tree.masks && P.tiles.slots > 0 ? tree_blocks(t.bound, t.target, P.H_kv)
+                                                           : std::max<int64_t>(t.bound * P.H_kv, P.tiles.slots);
   if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
   if (blocks == 0) return MCAMD_OK;
   if (a.tree.masks)
@@ -674,8 +707,9 @@ int dispatch(const TiledParams &P, const PagedArgs &a, const TiledPlan &t) {
 
 int launch_paged_tiles_merge(const PagedArgs &a, const PagedTiles &tiles, int pairs, int64_t bound) {
   const TiledParams P = tiled_params(a, tiles);
-  // Of more blocks than slots none is cut.
-  const int64_t blocks = std::min<int64_t>(bound * P.H_kv, tiles.slots) * tiles.groups * P.md;
+  // Of more blocks than slots none is cut; of a tree's a cut one has two at least.
+  const int64_t cut = a.tree.masks ? tiles.slots / 2 : tiles.slots;
+  const int64_t blocks = std::min<int64_t>(bound * P.H_kv, cut) * tiles.groups * P.md;
   if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
   const dim3 grid{unsigned(blocks)}, threads{kThreads};
   const bool bf = a.dtype == MCAMD_BF16;
@@ -700,6 +734,7 @@ int launch_paged_tiled(const PagedArgs &a, int64_t skip) {
   T.kt = t.kt;
   T.groups = t.pairs / 32;
   T.min_tiles = t.min_tiles;
+  T.target = t.target;
   paged_tiles_buffers(a, T, t.slots, slot_floats(a, t.pairs), t.pairs * 2);
   T.ratio = t.tile_us * MCAMD_SPLIT_BYTES_PER_US / (float(slot_floats(a, t.pairs)) * 8.f);
   const TiledParams P = tiled_params(a, T);

@@ -69,6 +69,7 @@
 #include "paged_careful.h"
 #include "prefill_order.h"
 #include "prefill_split.h"
+#include "tree_ranges.h"
 
 #include <cmath>
 #include <type_traits>
@@ -192,8 +193,17 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   // rows[b]; a query tile past the sequence's end has nothing to do (a whole workgroup).
   int row = b, T_b = P.T_new, s0;
   int64_t tok0 = int64_t(b) * P.T_new;
-  PagedBlock blk;
-  if constexpr (PAGED) {
+  typename std::conditional<TREE, TreeRange, PagedBlock>::type blk;
+  if constexpr (TREE) {
+    const TreeRanges ranges{P.cu, P.seqlens, T->n_rows, P.T_new, T->total, P.G, P.H_kv, P.QT * P.G, T->skip,
+                            int(P.T_max), P.window, KT, T->slots > 0 ? T->target : 0, T->min_tiles};
+    const bool found = find_tree_range(ranges, int(blockIdx.x) / P.H_kv, lane, blk);
+    if (blockIdx.x == 0 && tid == 0 && T->slots > 0) *T->n_cuts = blk.n_blocks;
+    if (!found) return;
+    kvh = int(blockIdx.x) % P.H_kv;
+    part = blk.part;
+    b = row = blk.b, qt = blk.qt, tok0 = blk.tok0, T_b = blk.T, s0 = blk.s0;
+  } else if constexpr (PAGED) {
     const bool found = find_paged_block(P.cu, P.seqlens, T->n_rows, P.T_new, T->total, P.G, P.H_kv,
                                         P.QT * P.G, T->skip, T->slots, int(P.T_max), T->halve,
                                         int(blockIdx.x) / P.H_kv, lane, blk);
@@ -236,7 +246,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   const int head = live ? pr - (pr / P.G) * P.G : 0;
   uint16_t *out = P.out + ((tok0 + pos) * P.H + int64_t(kvh) * P.G + head) * D;
   if (!row_ok) {
-    if constexpr (PAGED)
+    if constexpr (PAGED && !TREE)
       if (blk.noted && part == 0 && tid == 0) T->note_block(int(blockIdx.x), blk, 1, P.H_kv);
     if (live && part == 0)
       for (int d = h * 64; d < h * 64 + 64; ++d) out[d] = 0x7fc0;
@@ -268,9 +278,18 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   if constexpr (PAGED) {
     if (blk.noted) {
       const int tiles = (hi - lo) / KT + 1;
-      const int ranges = T->ranges_of(blk, tiles);
+      int ranges;
+      if constexpr (TREE)
+        ranges = min(blk.ranges, tiles);
+      else
+        ranges = T->ranges_of(blk, tiles);
       if (part >= ranges) return;
-      if (part == 0 && tid == 0) T->note_block(int(blockIdx.x), blk, ranges, P.H_kv);
+      if (part == 0 && tid == 0) {
+        if constexpr (TREE)
+          note_tree_range(*T, blk, kvh, P.H_kv, ranges);
+        else
+          T->note_block(int(blockIdx.x), blk, ranges, P.H_kv);
+      }
       whole = ranges == 1;
       const int t0 = part * tiles / ranges, t1 = (part + 1) * tiles / ranges;
       hi = min(hi, lo + t1 * KT - 1);
@@ -747,7 +766,8 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   if constexpr (PAGED) {
     if (!whole) {
       if (!live) return;
-      const int64_t g = int64_t(blockIdx.x) * kWaves + wave;
+      int64_t g = int64_t(blockIdx.x) * kWaves + wave;
+      if constexpr (TREE) g = (int64_t(blk.slot + part) * P.H_kv + kvh) * kWaves + wave;
 #pragma unroll
       for (int md = 0; md < 4; ++md)
 #pragma unroll
@@ -908,7 +928,17 @@ constexpr int64_t kSlotFloats = int64_t(kPairs) * (D + 2);
 
 }  // namespace
 
+namespace {
+
+// Partials of a call over trees, whose ranges aim at a workgroup per compute unit; 0 where no row has keys for two.
+int64_t tree_mfma_slots(const PagedArgs &a) {
+  return paged_keys(a) >= 2 * kMinRangeKeys ? tree_slots(device_cus(), a.n_kv_head) : 0;
+}
+
+}  // namespace
+
 size_t paged_mfma_bytes(const PagedArgs &a, int64_t skip) {
+  if (a.tree.masks) return paged_tiles_bytes(tree_mfma_slots(a), kSlotFloats);
   const int64_t G = a.n_head / a.n_kv_head;
   const int64_t pairs = kPairs / G * G;
   return paged_tiles_bytes(paged_slots(a, paged_blocks_bound(a, pairs, skip), pairs, 1, kMinRangeKeys),
@@ -943,10 +973,13 @@ int launch_paged_mfma(const PagedArgs &a, int64_t skip) {
   T.groups = kWaves;
   const int64_t bound = paged_blocks_bound(a, P.QT * P.G, skip);
   T.min_tiles = kMinRangeKeys / KT;
-  paged_tiles_buffers(a, T, paged_slots(a, bound, P.QT * P.G, 1, kMinRangeKeys), kSlotFloats, kPairs * 2);
+  const int64_t slots = a.tree.masks ? tree_mfma_slots(a) : paged_slots(a, bound, P.QT * P.G, 1, kMinRangeKeys);
+  paged_tiles_buffers(a, T, slots, kSlotFloats, kPairs * 2);
+  T.target = device_cus();
   // A tile of 64 keys takes 256 pairs 1.4 us; a range's partials are written and read.
   T.ratio = 1.4f * MCAMD_SPLIT_BYTES_PER_US / (float(kSlotFloats) * 8.f);
-  const int64_t blocks = std::max<int64_t>(bound * P.H_kv, T.slots);
+  const int64_t blocks = a.tree.masks && T.slots > 0 ? tree_blocks(bound, T.target, P.H_kv)
+                                                     : std::max<int64_t>(bound * P.H_kv, T.slots);
   if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
   if (blocks == 0) return MCAMD_OK;
   hipLaunchKernelGGL(a.tree.masks ? paged_tree_mfma_kernel : paged_mfma_kernel, dim3(unsigned(blocks)),
