@@ -382,6 +382,9 @@ size_t paged_tiled_bytes(const PagedArgs &a, int64_t skip);
 bool paged_mfma_supported(const PagedArgs &a);
 int launch_paged_mfma(const PagedArgs &a, int64_t skip);
 size_t paged_mfma_bytes(const PagedArgs &a, int64_t skip);
+// Every row of a bf16 call over trees, which it appends too.
+int launch_tree_stream(const PagedArgs &a);
+size_t tree_stream_bytes(const PagedArgs &a);
 // The ranges of cut blocks (of `pairs` pairs) added up.
 int launch_paged_tiles_merge(const PagedArgs &a, const PagedTiles &t, int pairs, int64_t bound);
 

@@ -59,7 +59,13 @@ Kernels kernels_of(const PagedArgs &a) {
 // are all to be on the chip at once.
 constexpr int64_t kAppendWithin = 512;
 
+// Rows of a bf16 call over trees, of more pairs than the streaming kernel takes for one of them.
+bool trees_of_many(const PagedArgs &a) {
+  return a.tree.masks && a.dtype == MCAMD_BF16 && !(a.t_new == 1 || a.t_new * (a.n_head / a.n_kv_head) <= few_of(a));
+}
+
 int launch(PagedArgs a) {
+  if (trees_of_many(a)) return launch_tree_stream(a);
   const Kernels k = kernels_of(a);
   const bool within = k.stream && (!k.tiles || a.total <= kAppendWithin);
   if (a.k_new && !within) {
@@ -97,6 +103,7 @@ size_t scratch_bytes(int64_t n_rows, int64_t total, int64_t max_seqlen, int64_t 
   a.dtype = dtype;
   const uint64_t none = 0;
   if (tree) a.tree.masks = &none;
+  if (trees_of_many(a)) return tree_stream_bytes(a);
   // The sizes do not tell packed rows from uniform ones: room for both.
   const int32_t packed = 0;
   size_t most = 0;

@@ -1,0 +1,485 @@
+// Attention of drafted trees over a paged bf16 cache, for rows of more (node, head) pairs per KV head than a wave
+// holds: every key and value is read once for 128 pairs and put through the matrix cores for all of them.
+//
+// A workgroup of four waves has a key range of one block of 128 pairs of a KV head (tree_ranges.h), a wave 32
+// pairs of it. Its tiles of 32 keys are staged in LDS once for all four, straight from HBM (buffer loads to
+// LDS, whole rows of a page), in a ring of four: two waves load K, two V, each 16 keys, which share a
+// page, so that a load's page is one scalar; three tiles are under way while one is used, with a barrier a tile.
+// Products, layouts and numerics are those of the streaming kernel of few pairs (paged_stream.hip): scores and
+// sums in fp32, q as it is, weights as two bf16 terms, p = hi + lo, which keep them to 2^-17.
+//
+// Who sees whom: tree_bits.h, only in tiles that hold nodes or the window's edge. New nodes come from k_new and
+// v_new where given, and the block's last range puts them in their pages. A block of one range writes its
+// output; otherwise (o, m, l) go to scratch in fp32 and the merge launch adds the ranges up. Pairs that are not finite
+// are redone (paged_careful.h).
+#include "stream_tiles.h"
+#include "tree_ranges.h"
+
+namespace mcamd {
+namespace {
+
+constexpr int kBlock = 32 * kWaves;  // pairs
+constexpr int kRing = 4;             // tiles in LDS
+constexpr int kMinRangeTiles = 8;    // of a range, unless the row is shorter
+// Workgroups of a compute unit: as many as its LDS and registers hold.
+constexpr int tree_fill(int dp) { return dp <= 128 ? 2 : 1; }
+
+struct TreeParams : CarefulParams {
+  const void *k_new, *v_new;
+  const int32_t *seqlens, *cu;
+  int n_rows, t_new, total, H, G;
+  int target;     // workgroups a call aims at; 0: no row is cut
+  float *part_o;  // [slot][kBlock][D]
+  float *part_ml; // [slot][kBlock][2]
+  PagedTiles::Cut *cuts;
+  int *n_cuts;
+};
+
+template <int DP>
+__global__ __launch_bounds__(kThreads)
+    __attribute__((amdgpu_waves_per_eu(tree_fill(DP)))) void tree_stream_kernel(TreeParams P) {
+  using S_ = Shape<DP>;
+  constexpr int CPR = S_::CPR, RPI = S_::RPI, NV = S_::NV, KD = S_::KD, MD = S_::MD;
+  __shared__ __attribute__((aligned(1024))) uint16_t s_tiles[kRing][2][S_::TILE];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  TreeRange R;
+  const TreeRanges call{P.cu, P.seqlens, P.n_rows, P.t_new, P.total, P.G, P.H_kv, kBlock, 0,
+                        P.kv.max_pages << P.kv.shift, P.window, KT, P.target, kMinRangeTiles};
+  const bool found = find_tree_range(call, int(blockIdx.x) / P.H_kv, lane, R);
+  if (blockIdx.x == 0 && tid == 0 && P.target > 0) *P.n_cuts = R.n_blocks;
+  if (!found) return;
+  const int kvh = int(blockIdx.x) % P.H_kv, b = R.b, D = P.D;
+  const int h = lane >> 5, col = lane & 31;
+  const int pairs = R.T * P.G, p0 = R.qt * kBlock;
+  const int in_block = 32 * wave + col, pair = p0 + in_block;
+  const bool live = pair < pairs, busy = p0 + 32 * wave < pairs;  // this pair, any of the wave
+  const int t_q = live ? pair / P.G : 0;
+  const int64_t at = (int64_t(R.tok0 + t_q) * P.H + kvh * P.G + (live ? pair - t_q * P.G : 0)) * D;
+  uint16_t *out = static_cast<uint16_t *>(P.out) + at;
+  if (R.s0 < 0 || int64_t(R.s0) + R.T > int64_t(P.kv.max_pages) << P.kv.shift) {
+    if (live)
+      for (int d = 8 * h; d < D; d += 16)
+        *reinterpret_cast<uint4 *>(out + d) =
+            make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+    return;
+  }
+
+  const int t_last = min(p0 + kBlock - 1, pairs - 1) / P.G;
+  const int seen_from = P.window >= 0 ? max(0, R.s0 - 1 - P.window) : 0;  // keys any pair of the block sees
+  const int seen_to = R.s0 + t_last;
+  const int first_tile = seen_from / KT, n_tiles = seen_to / KT - first_tile + 1;
+  const int ranges = min(R.ranges, n_tiles);
+  if (R.part >= ranges) return;
+  if (R.noted && R.part == 0 && tid == 0)
+    P.cuts[int64_t(R.cut) * P.H_kv + kvh] =
+        PagedTiles::Cut{R.b, R.qt, R.tok0, R.T, R.s0, ranges, R.slot * P.H_kv + kvh, 0};
+  const int t0 = first_tile + int(int64_t(R.part) * n_tiles / ranges);
+  const int t1 = first_tile + int(int64_t(R.part + 1) * n_tiles / ranges);
+
+  const uint16_t *q = static_cast<const uint16_t *>(P.q) + at;
+  bf16x8 qf[KD];
+#pragma unroll
+  for (int kd = 0; kd < KD; ++kd) {
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (16 * kd + 8 * h < D) u = *reinterpret_cast<const uint4 *>(q + 16 * kd + 8 * h);
+    qf[kd] = __builtin_bit_cast(bf16x8, u);
+  }
+
+  // This wave's loads: 16 keys of K or V. Load i covers rows RPI i + lane / CPR; its lane's chunk goes to slot
+  // lane % CPR, wherever that is.
+  const bool is_v = wave >= 2;
+  const int half = wave & 1;
+  const int tok_bytes = P.H_kv * D * 2;
+  constexpr uint32_t kNowhere = 0x80000000u;
+  const int lr = lane / CPR, lc = lane % CPR;
+  uint32_t off[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int r = RPI * i + lr, c = lc ^ (is_v ? S_::v_swz(r) : S_::k_swz(r));
+    off[i] = 8 * c < D ? uint32_t(r * tok_bytes + 16 * c) : kNowhere;
+  }
+  const scalar_ints table = (scalar_ints)(P.kv.table + b * P.kv.table_stride);
+  const int64_t head_at = int64_t(kvh) * D * 2;
+  const uint32_t page_bytes = uint32_t(tok_bytes) << P.kv.shift;
+  const char *const pool = static_cast<const char *>(is_v ? P.v_pages : P.k_pages);
+  const char *const new_rows = static_cast<const char *>(is_v ? P.v_new : P.k_new);
+  const bool fresh = P.k_new != nullptr;
+  bool lost = false;
+  // The page of this wave's keys of a tile; one that no key needs is page 0.
+  auto page_of = [&](int tile) {
+    const int k = tile * KT + 16 * half;
+    return tile < t1 && k + 15 >= seen_from && k <= seen_to ? table[k >> P.kv.shift] : 0;
+  };
+  auto load_tile = [&](int tile, int id) {
+    const int k0 = tile * KT, k = k0 + 16 * half;
+    uint16_t *const to = s_tiles[tile % kRing][is_v] + half * NV * 512;
+    lost = lost || !P.kv.is_page(id);
+    if (fresh && k0 + KT > R.s0) {
+      // Nodes come from their own rows; past the last one it is read again.
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int r = 16 * half + RPI * i + lr, key = max(seen_from, min(k0 + r, seen_to));
+        const int c = min(lc ^ (is_v ? S_::v_swz(r) : S_::k_swz(r)), D / 8 - 1);
+        const char *from = key >= R.s0 ? new_rows + int64_t(R.tok0 + key - R.s0) * tok_bytes
+                                       : pool + 2 * P.kv.offset(id, P.kv.in_page(key), int64_t(P.H_kv) * D);
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void *)(from + head_at + 16 * c),
+            (__attribute__((address_space(3))) void *)(to + i * 512), 16, 0, 0);
+      }
+      return;
+    }
+    const bool edge = k0 < seen_from || k0 + KT - 1 > seen_to;
+    const char *base = pool + (P.kv.is_page(id) ? id : 0) * P.kv.page_stride * 2 + head_at;
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        (void *)base, 0, int(page_bytes - uint32_t(head_at)), 0x00020000);
+    const int in_page = P.kv.in_page(k) * tok_bytes;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      uint32_t o = off[i];
+      if (edge) {
+        const int key = k + RPI * i + lr;
+        o = key >= seen_from && key <= seen_to ? o : kNowhere;
+      }
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rsrc, (__attribute__((address_space(3))) void *)(to + i * 512), 16, int(o), in_page, 0, 0);
+    }
+  };
+
+  // LDS addresses of this lane's reads, in a tile.
+  uint32_t ka[KD], va[2 * MD];
+#pragma unroll
+  for (int kd = 0; kd < KD; ++kd)
+    ka[kd] = lds_addr(s_tiles[0][0]) + 2 * (col * DP + 8 * ((2 * kd + h) ^ S_::k_swz(col)));
+  const int tr_row = (lane & 15) >> 2, tr_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+  for (int md = 0; md < MD; ++md)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int r = 4 * h + tr_row + 8 * u, c = 32 * md + tr_col;
+      va[2 * md + u] = lds_addr(s_tiles[0][1]) + 2 * (r * DP + 8 * ((c >> 3) ^ S_::v_swz(r)) + (c & 7));
+    }
+
+  f32x16 o[MD];
+#pragma unroll
+  for (int md = 0; md < MD; ++md)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[md][e] = 0.f;
+  float m = -INFINITY, l = 0.f;
+
+  if (D < DP) {  // dims past the head's are zero, whether or not a load past a page's end writes
+    for (int i = tid; i < kRing * 2 * S_::TILE / 8; i += kThreads)
+      reinterpret_cast<uint4 *>(s_tiles)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+  }
+  int id[kRing - 1];
+#pragma unroll
+  for (int i = 0; i < kRing - 1; ++i) id[i] = page_of(t0 + i);
+  // The queries have arrived: a wait for them behind the loads to LDS would be one for those too.
+#pragma unroll
+  for (int kd = 0; kd < KD; ++kd) asm volatile("" : "+v"(qf[kd]));
+#pragma unroll
+  for (int i = 0; i < kRing - 1; ++i)
+    if (t0 + i < t1) load_tile(t0 + i, id[i]);
+  int next = page_of(t0 + kRing - 1);
+  for (int tile = t0; tile < t1; ++tile) {
+    const int k0 = tile * KT;
+    // This wave's loads of the tile have landed: those of the two after it may be under way.
+    if (tile + 2 < t1)
+      wait_loads<2 * NV>();
+    else if (tile + 1 < t1)
+      wait_loads<NV>();
+    else
+      wait_loads<0>();
+    // And everyone's; and everyone has read the tile before, whose place the next load takes.
+    __builtin_amdgcn_s_barrier();
+    if (tile + kRing - 1 < t1) load_tile(tile + kRing - 1, next);
+    next = page_of(tile + kRing);
+    if (!busy) continue;
+    const uint32_t in_ring = uint32_t(tile % kRing) * (2 * S_::TILE * 2);
+
+    f32x16 s;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = 0.f;
+    constexpr int KB = KD < 8 ? KD : 8;
+#pragma unroll
+    for (int k8 = 0; k8 < KD; k8 += KB) {
+      bf16x8 f[KB];
+      uint32_t a[KB];
+#pragma unroll
+      for (int i = 0; i < KB; ++i) a[i] = ka[k8 + i] + in_ring;
+      read_rows<KB>(f, a);
+#pragma unroll
+      for (int i = 0; i < KB; ++i)
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i], qf[k8 + i], s, 0, 0, 0);
+    }
+
+    // Keys the pair may not see.
+    if (k0 + KT - 1 >= R.s0 || (P.window >= 0 && k0 < R.s0 + t_last - P.window)) {
+      const uint64_t seen = TreeNode(P.tree, R.tok0 + t_q, t_q, R.s0, P.window).seen(k0) >> (4 * h);
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (!((seen >> (8 * (e >> 2) + (e & 3))) & 1)) s[e] = -INFINITY;
+    }
+    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int e = 0; e < 16; ++e) m4[e & 3] = fmaxf(m4[e & 3], s[e]);
+    const float mx = max_halves(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]))) * P.scale_log2;
+    if (__builtin_amdgcn_ballot_w64(mx > m) != 0) {
+      const float m_new = fmaxf(m, mx);
+      const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - m_new);
+      l *= alpha;
+#pragma unroll
+      for (int md = 0; md < MD; ++md)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[md][e] *= alpha;
+      m = m_new;
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+    float w[16], ts[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      w[e] = fast_exp2(fmaf(s[e], P.scale_log2, -ref));
+      ts[e & 3] += w[e];
+    }
+    l += (ts[0] + ts[1]) + (ts[2] + ts[3]);
+
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      f32x8 pv;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) pv[e] = w[8 * ks + e];
+      const bf16x8 hi8 = __builtin_convertvector(pv, bf16x8);
+      const bf16x8 lo8 = __builtin_convertvector(pv - __builtin_convertvector(hi8, f32x8), bf16x8);
+      constexpr int VB = 2 * MD < 8 ? 2 * MD : 8;
+#pragma unroll
+      for (int v8 = 0; v8 < 2 * MD; v8 += VB) {
+        bf16x4 f[VB];
+        uint32_t a[VB];
+#pragma unroll
+        for (int i = 0; i < VB; ++i) a[i] = va[v8 + i] + ks * 32 * DP + in_ring;
+        read_columns<VB>(f, a);
+#pragma unroll
+        for (int i = 0; i < VB / 2; ++i) {
+          const int md = v8 / 2 + i;
+          const bf16x8 x = __builtin_shufflevector(f[2 * i], f[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+          o[md] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, hi8, o[md], 0, 0, 0);
+          o[md] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, lo8, o[md], 0, 0, 0);
+        }
+      }
+    }
+  }
+  l = sum_halves(l);
+
+  // The new nodes into their pages, by the block's last range: in every block, so that a redo below finds
+  // them whichever other block has come how far; they write the same.
+  if (fresh && R.part == ranges - 1) {
+    const int units = D / 8;  // of 16 bytes, of K and of V
+    for (int i = tid; i < R.T * units; i += kThreads) {
+      const int t = i / units, u = i - t * units, key = R.s0 + t;
+      const int pid = P.kv.table[b * P.kv.table_stride + (key >> P.kv.shift)];
+      if (!P.kv.is_page(pid)) continue;
+      const int64_t from = int64_t(R.tok0 + t) * tok_bytes + head_at + 16 * u;
+      const int64_t to = 2 * P.kv.offset(pid, P.kv.in_page(key), int64_t(P.H_kv) * D) + head_at + 16 * u;
+      const uint4 x = *reinterpret_cast<const uint4 *>(static_cast<const char *>(P.k_new) + from);
+      const uint4 y = *reinterpret_cast<const uint4 *>(static_cast<const char *>(P.v_new) + from);
+      *reinterpret_cast<uint4 *>(static_cast<char *>(const_cast<void *>(P.k_pages)) + to) = x;
+      *reinterpret_cast<uint4 *>(static_cast<char *>(const_cast<void *>(P.v_pages)) + to) = y;
+    }
+  }
+  if (__syncthreads_or(lost)) l = NAN;  // and the nodes are in their pages
+
+  // o[md][4j + i] is dim 32 md + 8 j + 4 h + i of pair `col`.
+  if (ranges > 1) {
+    if (!live) return;
+    const int64_t slot = (int64_t(R.slot + R.part) * P.H_kv + kvh) * kBlock + in_block;
+    float *po = P.part_o + slot * D;
+#pragma unroll
+    for (int md = 0; md < MD; ++md)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (32 * md + 8 * j < D)
+          *reinterpret_cast<float4 *>(po + 32 * md + 8 * j + 4 * h) =
+              make_float4(o[md][4 * j], o[md][4 * j + 1], o[md][4 * j + 2], o[md][4 * j + 3]);
+    if (h == 0) *reinterpret_cast<float2 *>(P.part_ml + slot * 2) = make_float2(m, l);
+    return;
+  }
+  const float inv = 1.f / l;
+  bool ok = true;
+#pragma unroll
+  for (int md = 0; md < MD; ++md)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      o[md][e] *= inv;
+      ok = ok && (finite(o[md][e]) || 32 * md + 8 * (e >> 2) >= D);
+    }
+  const uint64_t bad64 = __builtin_amdgcn_ballot_w64(live && !ok);
+  const uint32_t bad = uint32_t(bad64) | uint32_t(bad64 >> 32);
+  if (live && !((bad >> col) & 1u)) {
+#pragma unroll
+    for (int md = 0; md < MD; ++md)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (32 * md + 8 * j >= D) continue;
+        const f32x4 x = {o[md][4 * j], o[md][4 * j + 1], o[md][4 * j + 2], o[md][4 * j + 3]};
+        *reinterpret_cast<uint2 *>(out + 32 * md + 8 * j + 4 * h) =
+            __builtin_bit_cast(uint2, __builtin_convertvector(x, bf16x4));
+      }
+  }
+  for (uint32_t left = bad; __builtin_expect(left != 0, 0); left &= left - 1) {
+    const int pr = p0 + 32 * wave + __builtin_ctz(left), t = pr / P.G;
+    careful_pair<bf16, DP, 8, true>(P, b, kvh, (int64_t(R.tok0 + t) * P.H + kvh * P.G + (pr - t * P.G)) * D,
+                                    R.s0 + t, lane, 0, D, R.tok0 + t, t);
+  }
+}
+
+// The ranges of cut blocks added up: a workgroup has two pairs (D up to 128; one of more) of a block and KV head, half
+// a wave a pair with four dims a lane, and its waves every fourth range each, eight of them under way.
+template <int DP>
+__global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeParams P) {
+  constexpr int LPP = DP <= 128 ? 32 : 64, N = 64 / LPP, U = 8;  // lanes of a pair, pairs of a wave
+  __shared__ f32x4 s_o[kWaves][64];
+  __shared__ float2 s_ml[kWaves][N];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int id = blockIdx.y;  // of the cut blocks, KV heads counted
+  if (id >= *P.n_cuts * P.H_kv) return;
+  const PagedTiles::Cut blk = P.cuts[id];
+  const int kvh = id % P.H_kv, n = min(kBlock, blk.T * P.G - blk.qt * kBlock), ranges = blk.ranges;
+  const int first = N * int(blockIdx.x);
+  if (ranges == 1 || first >= n) return;  // of one range: written by the block itself
+  const int in_block = first + lane / LPP, d = 4 * (lane % LPP);
+  const int64_t step = int64_t(P.H_kv) * kBlock, slot = int64_t(blk.second) * kBlock + min(in_block, n - 1);
+  float M = -INFINITY, L = 0.f;
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+  for (int r0 = wave; r0 < ranges; r0 += U * kWaves) {
+    float2 x[U];
+    f32x4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = slot + min(r0 + u * kWaves, ranges - 1) * step;
+      x[u] = *reinterpret_cast<const float2 *>(P.part_ml + at * 2);
+      v[u] = *reinterpret_cast<const f32x4 *>(P.part_o + at * P.D + min(d, P.D - 4));
+    }
+    float m_new = M;
+#pragma unroll
+    for (int u = 0; u < U; ++u) m_new = r0 + u * kWaves < ranges ? fmaxf(m_new, x[u].x) : m_new;
+    const float keep = M == -INFINITY ? 0.f : fast_exp2(M - m_new);
+    L *= M == -INFINITY ? 1.f : keep;  // 0 then, or a NaN that must stay
+    y *= keep;
+    M = m_new;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (r0 + u * kWaves >= ranges) break;
+      const float a = x[u].x == -INFINITY ? 0.f : fast_exp2(x[u].x - M);
+      L += x[u].y * (x[u].x == -INFINITY ? 1.f : a);
+      y += a * v[u];
+    }
+  }
+  s_o[wave][lane] = y;
+  if (lane % LPP == 0) s_ml[wave][lane / LPP] = make_float2(M, L);
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) M = fmaxf(M, s_ml[w][lane / LPP].x);
+  L = 0.f;
+  y = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float2 x = s_ml[w][lane / LPP];
+    const float a = x.x == -INFINITY ? 0.f : fast_exp2(x.x - M);
+    L += x.y * (x.x == -INFINITY ? 1.f : a);
+    y += a * s_o[w][lane];
+  }
+  y *= 1.f / L;
+  const bool there = in_block < n && d < P.D;
+  const bool ok = !there || (finite(y[0]) && finite(y[1]) && finite(y[2]) && finite(y[3]));
+  uint64_t bad = __builtin_amdgcn_ballot_w64(!ok);
+  auto pair_at = [&](int i, int &t) {
+    const int pr = blk.qt * kBlock + i;
+    t = pr / P.G;
+    return (int64_t(blk.tok0 + t) * P.H + int64_t(kvh) * P.G + (pr - t * P.G)) * P.D;
+  };
+  int t;
+  const int64_t at = pair_at(min(in_block, n - 1), t);
+  const bool redo = (bad >> (lane / LPP * LPP) & (N == 1 ? ~uint64_t(0) : 0xffffffffu)) != 0;
+  if (there && !redo)
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(P.out) + at + d) =
+        __builtin_bit_cast(uint2, __builtin_convertvector(y, bf16x4));
+  if (__builtin_expect(bad == 0, 1)) return;
+  for (int i = 0; i < N; ++i) {
+    if (!(bad >> (i * LPP) & (N == 1 ? ~uint64_t(0) : 0xffffffffu)) || first + i >= n) continue;
+    const int64_t to = pair_at(first + i, t);
+    careful_pair<bf16, DP, 8, true>(P, blk.b, kvh, to, blk.s0 + t, lane, 0, P.D, int64_t(blk.tok0) + t, t);
+  }
+}
+
+int64_t block_bound(const PagedArgs &a) { return paged_blocks_bound(a, kBlock, 0); }
+int64_t target_of(const PagedArgs &a) {
+  return paged_keys(a) >= 2 * kMinRangeTiles * KT ? int64_t(tree_fill(head_pad(a.head_dim))) * device_cus() : 0;
+}
+size_t bytes_of(const PagedArgs &a, int64_t target) {
+  return target == 0 ? 0 : paged_tiles_bytes(tree_slots(target, a.n_kv_head), kBlock * (a.head_dim + 2));
+}
+
+template <int DP>
+int run(const TreeParams &P, const PagedArgs &a) {
+  const int64_t bound = block_bound(a);
+  const int64_t blocks = P.target > 0 ? tree_blocks(bound, P.target, P.H_kv) : bound * P.H_kv;
+  if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
+  if (blocks == 0) return MCAMD_OK;
+  hipLaunchKernelGGL(tree_stream_kernel<DP>, dim3(unsigned(blocks)), dim3(kThreads), 0, a.stream, P);
+  const int st = launch_status("tree_stream");
+  if (st != MCAMD_OK || P.target == 0) return st;
+  // A cut block has two ranges at least.
+  const int64_t cut = std::min<int64_t>(bound * P.H_kv, tree_slots(P.target, P.H_kv) / 2);
+  const int64_t pairs = std::min<int64_t>(kBlock, a.t_new * P.G), each = DP <= 128 ? 2 : 1;
+  if (cut > 65535) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
+  hipLaunchKernelGGL(tree_merge_kernel<DP>, dim3(unsigned((pairs + each - 1) / each), unsigned(cut)), dim3(kThreads),
+                     0, a.stream, P);
+  return launch_status("tree_merge");
+}
+
+}  // namespace
+
+size_t tree_stream_bytes(const PagedArgs &a) { return bytes_of(a, target_of(a)); }
+
+int launch_tree_stream(const PagedArgs &a) {
+  TreeParams P{};
+  P.q = a.q;
+  P.k_pages = a.k_pages;
+  P.v_pages = a.v_pages;
+  P.kv = a.kv;
+  P.out = a.out;
+  P.H_kv = int(a.n_kv_head);
+  P.window = int(a.window < 0 ? -1 : a.window);
+  P.D = int(a.head_dim);
+  P.scale_log2 = float(kLog2e / std::sqrt(double(a.head_dim)));
+  P.tree = a.tree;
+  P.k_new = a.k_new;
+  P.v_new = a.v_new;
+  P.seqlens = a.seqlens;
+  P.cu = a.cu;
+  P.n_rows = int(a.n_rows);
+  P.t_new = int(a.t_new);
+  P.total = int(a.total);
+  P.H = int(a.n_head);
+  P.G = int(a.n_head / a.n_kv_head);
+  const int64_t target = target_of(a);
+  if (target > 0 && a.scratch && a.scratch_bytes >= bytes_of(a, target)) {
+    const int64_t slots = tree_slots(target, a.n_kv_head);
+    P.target = int(target);
+    P.part_o = static_cast<float *>(a.scratch);
+    P.part_ml = P.part_o + slots * kBlock * a.head_dim;
+    P.cuts = reinterpret_cast<PagedTiles::Cut *>(P.part_ml + slots * kBlock * 2);
+    P.n_cuts = reinterpret_cast<int *>(P.cuts + slots);
+  }
+  switch (head_pad(a.head_dim)) {
+    case 32: return run<32>(P, a);
+    case 64: return run<64>(P, a);
+    case 128: return run<128>(P, a);
+    default: return run<256>(P, a);
+  }
+}
+
+}  // namespace mcamd
