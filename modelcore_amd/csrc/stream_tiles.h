@@ -86,6 +86,61 @@ __device__ __forceinline__ void read_columns(bf16x4 (&f)[N], const uint32_t (&a)
                  : "memory");
 }
 
+// The same from an offset on, bytes that an instruction holds (below 65536).
+template <int OFF, int N>
+__device__ __forceinline__ void read_rows_at(bf16x8 (&f)[N], const uint32_t (&a)[N]) {
+  static_assert(N == 2 || N == 4 || N == 8, "");
+  static_assert(OFF < 65536, "");
+  if constexpr (N == 8)
+    asm volatile(
+        "ds_read_b128 %0, %8 offset:%16\n ds_read_b128 %1, %9 offset:%16\n ds_read_b128 %2, %10 offset:%16\n"
+        "ds_read_b128 %3, %11 offset:%16\n ds_read_b128 %4, %12 offset:%16\n ds_read_b128 %5, %13 offset:%16\n"
+        "ds_read_b128 %6, %14 offset:%16\n ds_read_b128 %7, %15 offset:%16\n s_waitcnt lgkmcnt(0)"
+        : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3]), "=&v"(f[4]), "=&v"(f[5]), "=&v"(f[6]),
+          "=&v"(f[7])
+        : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5]), "v"(a[6]), "v"(a[7]), "i"(OFF)
+        : "memory");
+  else if constexpr (N == 4)
+    asm volatile(
+        "ds_read_b128 %0, %4 offset:%8\n ds_read_b128 %1, %5 offset:%8\n ds_read_b128 %2, %6 offset:%8\n"
+        "ds_read_b128 %3, %7 offset:%8\n s_waitcnt lgkmcnt(0)"
+        : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3])
+        : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "i"(OFF)
+        : "memory");
+  else
+    asm volatile("ds_read_b128 %0, %2 offset:%4\n ds_read_b128 %1, %3 offset:%4\n s_waitcnt lgkmcnt(0)"
+                 : "=&v"(f[0]), "=&v"(f[1])
+                 : "v"(a[0]), "v"(a[1]), "i"(OFF)
+                 : "memory");
+}
+template <int OFF, int N>
+__device__ __forceinline__ void read_columns_at(bf16x4 (&f)[N], const uint32_t (&a)[N]) {
+  static_assert(N == 2 || N == 4 || N == 8, "");
+  static_assert(OFF < 65536, "");
+  if constexpr (N == 8)
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8 offset:%16\n ds_read_b64_tr_b16 %1, %9 offset:%16\n"
+        "ds_read_b64_tr_b16 %2, %10 offset:%16\n ds_read_b64_tr_b16 %3, %11 offset:%16\n"
+        "ds_read_b64_tr_b16 %4, %12 offset:%16\n ds_read_b64_tr_b16 %5, %13 offset:%16\n"
+        "ds_read_b64_tr_b16 %6, %14 offset:%16\n ds_read_b64_tr_b16 %7, %15 offset:%16\n s_waitcnt lgkmcnt(0)"
+        : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3]), "=&v"(f[4]), "=&v"(f[5]), "=&v"(f[6]),
+          "=&v"(f[7])
+        : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5]), "v"(a[6]), "v"(a[7]), "i"(OFF)
+        : "memory");
+  else if constexpr (N == 4)
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %4 offset:%8\n ds_read_b64_tr_b16 %1, %5 offset:%8\n"
+        "ds_read_b64_tr_b16 %2, %6 offset:%8\n ds_read_b64_tr_b16 %3, %7 offset:%8\n s_waitcnt lgkmcnt(0)"
+        : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3])
+        : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "i"(OFF)
+        : "memory");
+  else
+    asm volatile("ds_read_b64_tr_b16 %0, %2 offset:%4\n ds_read_b64_tr_b16 %1, %3 offset:%4\n s_waitcnt lgkmcnt(0)"
+                 : "=&v"(f[0]), "=&v"(f[1])
+                 : "v"(a[0]), "v"(a[1]), "i"(OFF)
+                 : "memory");
+}
+
 template <int N>
 __device__ __forceinline__ void wait_loads() {
   static_assert(N < 64, "");

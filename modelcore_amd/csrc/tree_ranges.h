@@ -16,6 +16,25 @@
 
 namespace mcamd {
 
+// Inclusive sum over the wave, by moves between lanes.
+__device__ __forceinline__ int wave_scan32(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);  // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);  // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);  // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return v;
+}
+// ceil(x / y) of x up to 2^26, y > 0: the quotient of floats is off by at most two.
+__device__ __forceinline__ int ceil_of(int x, int y) {
+  int q = int(float(x) * __builtin_amdgcn_rcpf(float(y)));
+  const int r = x - q * y;  // of -2 y to 3 y
+  q += (r > 0) + (r > y) + (r > 2 * y);
+  q -= (r <= -y) + (r <= -2 * y);
+  return q;
+}
+
 struct TreeRanges {
   const int32_t *cu, *seqlens;
   int n_rows, t_new, total, G, H_kv, pairs, skip, room, window, kt;
@@ -28,14 +47,14 @@ struct TreeRanges {
     Row r;
     row_tokens(cu, t_new, total, b, r.tok0, r.T);
     r.s0 = seqlens[b];
-    r.blocks = few_pairs(r.T, G, skip) ? 0 : int((uint32_t(r.T * G) + uint32_t(pairs) - 1) / uint32_t(pairs));
+    r.blocks = few_pairs(r.T, G, skip) ? 0 : ceil_of(r.T * G, pairs);
     const bool ok = r.s0 >= 0 && r.s0 <= room - r.T;
     const int lo = window >= 0 ? max(0, r.s0 - 1 - window) : 0;
-    r.tiles = ok ? int(uint32_t(r.s0 + r.T - 1 - lo) / uint32_t(kt)) + 1 : 1;
+    r.tiles = ok ? int((uint32_t(r.s0 + r.T - lo) + uint32_t(kt) - 1) / uint32_t(kt)) : 1;  // a shift
     return r;
   }
   static __device__ __forceinline__ int ranges_of(const Row &r, int len) {
-    return int((uint32_t(r.tiles) + uint32_t(len) - 1) / uint32_t(len));
+    return len >= r.tiles ? 1 : ceil_of(r.tiles, len);
   }
   static __device__ __forceinline__ int64_t wave_total64(int64_t x) {
 #pragma unroll
@@ -46,6 +65,24 @@ struct TreeRanges {
   // Tiles of a range, at most. first: row `lane`.
   __device__ __forceinline__ int len_of(int lane, const Row &first) const {
     if (target == 0) return 0x7fffffff;
+    const int slots = max(target / H_kv, 1);
+    if (n_rows <= 64) {
+      const int blocks = lane < n_rows ? first.blocks : 0, units = wave_total(blocks);
+      if (units <= slots && __builtin_amdgcn_ballot_w64(blocks > 0 && first.tiles > 1 << 14) == 0) {
+        const int work = wave_total(blocks * first.tiles);  // at most 1024 blocks of 2^14 tiles
+        int less = max(ceil_of(work, slots), min_tiles) - 1;  // has more ranges, or is too short
+        // work / len whole ranges and up to one more a block are no more than that.
+        int len = slots > units ? max(ceil_of(work, slots - units), min_tiles) : 1 << 14;
+        for (int step = 0; step < 8 && len - less > 1; ++step) {
+          const int mid = less + (len - less) / 2;
+          if (wave_total(blocks * ranges_of(first, mid)) <= slots)
+            len = mid;
+          else
+            less = mid;
+        }
+        return __builtin_amdgcn_readfirstlane(len);
+      }
+    }
     int64_t work = 0, units = 0;
     for (int b = lane; b < n_rows; b += 64) {
       const Row r = b == lane ? first : row_of(b);
@@ -54,21 +91,8 @@ struct TreeRanges {
     }
     work = wave_total64(work);
     units = wave_total64(units);
-    const int64_t slots = max(target / H_kv, 1);
     const int64_t most = units < slots / 2 ? slots - units : (slots + 1) / 2;
-    int len = int(max((work + most - 1) / most, int64_t(min_tiles)));  // has at most that many ranges
-    if (n_rows <= 64 && units <= slots) {
-      int less = int(max((work + slots - 1) / slots, int64_t(min_tiles))) - 1;  // has more, or is too short
-      const int blocks = lane < n_rows ? first.blocks : 0;
-      for (int step = 0; step < 8 && len - less > 1; ++step) {
-        const int mid = less + (len - less) / 2;
-        if (wave_total(blocks * ranges_of(first, mid)) <= slots)
-          len = mid;
-        else
-          less = mid;
-      }
-    }
-    return __builtin_amdgcn_readfirstlane(len);
+    return __builtin_amdgcn_readfirstlane(int(max((work + most - 1) / most, int64_t(min_tiles))));
   }
 };
 
@@ -91,7 +115,7 @@ __device__ __forceinline__ bool find_tree_range(const TreeRanges &c, int id, int
     const int blocks = b0 + lane < c.n_rows ? r.blocks : 0;
     const int ranges = c.target == 0 ? 1 : TreeRanges::ranges_of(r, len);
     const int n = ranges * blocks, n_cut = ranges > 1 ? n : 0, cuts = ranges > 1 ? blocks : 0;
-    const int upto = wave_upto(n, lane), cut_upto = wave_upto(n_cut, lane), cuts_upto = wave_upto(cuts, lane);
+    const int upto = wave_scan32(n), cut_upto = wave_scan32(n_cut), cuts_upto = wave_scan32(cuts);
     const uint64_t past = v.b < 0 ? __builtin_amdgcn_ballot_w64(upto > id) : 0;
     if (past != 0) {
       const int l = __builtin_ctzll(past);

@@ -15,12 +15,16 @@
 #include "stream_tiles.h"
 #include "tree_ranges.h"
 
+#include <type_traits>
+
 namespace mcamd {
 namespace {
 
 constexpr int kBlock = 32 * kWaves;  // pairs
 constexpr int kRing = 4;             // tiles in LDS
 constexpr int kMinRangeTiles = 8;    // of a range, unless the row is shorter
+constexpr float kTileSumLimit = 32768.f;  // 2^15: a lane's weights of one tile sum to at most this
+static_assert(kRing == 4, "the loop goes round the ring by name");
 // Workgroups of a compute unit: as many as its LDS and registers hold.
 constexpr int tree_fill(int dp) { return dp <= 128 ? 2 : 1; }
 
@@ -112,11 +116,12 @@ __global__ __launch_bounds__(kThreads)
     const int k = tile * KT + 16 * half;
     return tile < t1 && k + 15 >= seen_from && k <= seen_to ? table[k >> P.kv.shift] : 0;
   };
-  auto load_tile = [&](int tile, int id) {
+  // Into place `at` of the ring; past the range's end zeros, so that as many loads are under way in every turn.
+  auto load_tile = [&](int tile, int id, int at) {
     const int k0 = tile * KT, k = k0 + 16 * half;
-    uint16_t *const to = s_tiles[tile % kRing][is_v] + half * NV * 512;
+    uint16_t *const to = s_tiles[at][is_v] + half * NV * 512;
     lost = lost || !P.kv.is_page(id);
-    if (fresh && k0 + KT > R.s0) {
+    if (fresh && tile < t1 && k0 + KT > R.s0) {
       // Nodes come from their own rows; past the last one it is read again.
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -130,7 +135,7 @@ __global__ __launch_bounds__(kThreads)
       }
       return;
     }
-    const bool edge = k0 < seen_from || k0 + KT - 1 > seen_to;
+    const bool edge = k0 < seen_from || k0 + KT - 1 > seen_to || tile >= t1;
     const char *base = pool + (P.kv.is_page(id) ? id : 0) * P.kv.page_stride * 2 + head_at;
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
         (void *)base, 0, int(page_bytes - uint32_t(head_at)), 0x00020000);
@@ -140,7 +145,7 @@ __global__ __launch_bounds__(kThreads)
       uint32_t o = off[i];
       if (edge) {
         const int key = k + RPI * i + lr;
-        o = key >= seen_from && key <= seen_to ? o : kNowhere;
+        o = key >= seen_from && key <= seen_to && tile < t1 ? o : kNowhere;
       }
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           rsrc, (__attribute__((address_space(3))) void *)(to + i * 512), 16, int(o), in_page, 0, 0);
@@ -176,28 +181,27 @@ __global__ __launch_bounds__(kThreads)
   int id[kRing - 1];
 #pragma unroll
   for (int i = 0; i < kRing - 1; ++i) id[i] = page_of(t0 + i);
-  // The queries have arrived: a wait for them behind the loads to LDS would be one for those too.
+#pragma unroll
+  for (int i = 0; i < kRing - 1; ++i) load_tile(t0 + i, id[i], i);
+  int next = page_of(t0 + kRing - 1);
+  // The queries were asked for before these and are there with the first tile: waited for here, since in the loop
+  // the compiler would wait for the loads to LDS with them.
+  wait_loads<2 * NV>();
 #pragma unroll
   for (int kd = 0; kd < KD; ++kd) asm volatile("" : "+v"(qf[kd]));
-#pragma unroll
-  for (int i = 0; i < kRing - 1; ++i)
-    if (t0 + i < t1) load_tile(t0 + i, id[i]);
-  int next = page_of(t0 + kRing - 1);
-  for (int tile = t0; tile < t1; ++tile) {
+
+  // One tile, in place AT of the ring.
+  auto turn = [&](int tile, auto at_c) __attribute__((always_inline)) {
+    constexpr int AT = decltype(at_c)::value;
+    constexpr int kAt = AT * 2 * S_::TILE * 2, kOff = kAt < 49152 ? kAt : 0;  // bytes, of which an instruction's
     const int k0 = tile * KT;
-    // This wave's loads of the tile have landed: those of the two after it may be under way.
-    if (tile + 2 < t1)
-      wait_loads<2 * NV>();
-    else if (tile + 1 < t1)
-      wait_loads<NV>();
-    else
-      wait_loads<0>();
-    // And everyone's; and everyone has read the tile before, whose place the next load takes.
+    // This wave's loads of the tile have landed, those of the two after it may be under way; and everyone's; and
+    // everyone has read the tile before, whose place the next load takes.
+    wait_loads<2 * NV>();
     __builtin_amdgcn_s_barrier();
-    if (tile + kRing - 1 < t1) load_tile(tile + kRing - 1, next);
+    load_tile(tile + kRing - 1, next, (AT + kRing - 1) % kRing);
     next = page_of(tile + kRing);
-    if (!busy) continue;
-    const uint32_t in_ring = uint32_t(tile % kRing) * (2 * S_::TILE * 2);
+    if (!busy) return;
 
     f32x16 s;
 #pragma unroll
@@ -208,8 +212,8 @@ __global__ __launch_bounds__(kThreads)
       bf16x8 f[KB];
       uint32_t a[KB];
 #pragma unroll
-      for (int i = 0; i < KB; ++i) a[i] = ka[k8 + i] + in_ring;
-      read_rows<KB>(f, a);
+      for (int i = 0; i < KB; ++i) a[i] = ka[k8 + i] + (kAt - kOff);
+      read_rows_at<kOff, KB>(f, a);
 #pragma unroll
       for (int i = 0; i < KB; ++i)
         s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i], qf[k8 + i], s, 0, 0, 0);
@@ -222,11 +226,25 @@ __global__ __launch_bounds__(kThreads)
       for (int e = 0; e < 16; ++e)
         if (!((seen >> (8 * (e >> 2) + (e & 3))) & 1)) s[e] = -INFINITY;
     }
-    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    // Weights against the running maximum; the tile's own is taken, and the sums rescaled, only where a lane's
+    // weights sum past 2^15 or are not finite, or the pair has no maximum yet.
+    float w[16];
+    auto weigh = [&]() {
+      const float ref = m == -INFINITY ? 0.f : m;
+      float ts[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < 16; ++e) m4[e & 3] = fmaxf(m4[e & 3], s[e]);
-    const float mx = max_halves(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]))) * P.scale_log2;
-    if (__builtin_amdgcn_ballot_w64(mx > m) != 0) {
+      for (int e = 0; e < 16; ++e) {
+        w[e] = fast_exp2(fmaf(s[e], P.scale_log2, -ref));
+        ts[e & 3] += w[e];
+      }
+      return (ts[0] + ts[1]) + (ts[2] + ts[3]);
+    };
+    float tl = weigh();
+    if (__builtin_amdgcn_ballot_w64(!(tl <= kTileSumLimit) || m == -INFINITY) != 0) {
+      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int e = 0; e < 16; ++e) m4[e & 3] = fmaxf(m4[e & 3], s[e]);
+      const float mx = max_halves(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]))) * P.scale_log2;
       const float m_new = fmaxf(m, mx);
       const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - m_new);
       l *= alpha;
@@ -235,18 +253,12 @@ __global__ __launch_bounds__(kThreads)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[md][e] *= alpha;
       m = m_new;
+      tl = weigh();
     }
-    const float ref = m == -INFINITY ? 0.f : m;
-    float w[16], ts[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      w[e] = fast_exp2(fmaf(s[e], P.scale_log2, -ref));
-      ts[e & 3] += w[e];
-    }
-    l += (ts[0] + ts[1]) + (ts[2] + ts[3]);
+    l += tl;
 
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
+    auto add_values = [&](auto ks_c) __attribute__((always_inline)) {  // of 16 keys
+      constexpr int ks = decltype(ks_c)::value;
       f32x8 pv;
 #pragma unroll
       for (int e = 0; e < 8; ++e) pv[e] = w[8 * ks + e];
@@ -258,8 +270,8 @@ __global__ __launch_bounds__(kThreads)
         bf16x4 f[VB];
         uint32_t a[VB];
 #pragma unroll
-        for (int i = 0; i < VB; ++i) a[i] = va[v8 + i] + ks * 32 * DP + in_ring;
-        read_columns<VB>(f, a);
+        for (int i = 0; i < VB; ++i) a[i] = va[v8 + i] + (kAt - kOff);
+        read_columns_at<kOff + ks * 32 * DP, VB>(f, a);
 #pragma unroll
         for (int i = 0; i < VB / 2; ++i) {
           const int md = v8 / 2 + i;
@@ -268,8 +280,21 @@ __global__ __launch_bounds__(kThreads)
           o[md] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, lo8, o[md], 0, 0, 0);
         }
       }
-    }
+    };
+    add_values(std::integral_constant<int, 0>{});
+    add_values(std::integral_constant<int, 1>{});
+  };
+  for (int tile = t0;;) {
+    turn(tile, std::integral_constant<int, 0>{});
+    if (++tile >= t1) break;
+    turn(tile, std::integral_constant<int, 1>{});
+    if (++tile >= t1) break;
+    turn(tile, std::integral_constant<int, 2>{});
+    if (++tile >= t1) break;
+    turn(tile, std::integral_constant<int, 3>{});
+    if (++tile >= t1) break;
   }
+  wait_loads<0>();
   l = sum_halves(l);
 
   // The new nodes into their pages, by the block's last range: in every block, so that a redo below finds
