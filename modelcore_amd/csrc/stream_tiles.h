@@ -113,6 +113,28 @@ __device__ __forceinline__ void read_rows_at(bf16x8 (&f)[N], const uint32_t (&a)
                  : "v"(a[0]), "v"(a[1]), "i"(OFF)
                  : "memory");
 }
+// Four rows (or two) from each of two offsets on.
+template <int OFF, int OFF2, int N>
+__device__ __forceinline__ void read_rows_two(bf16x8 (&f)[N], bf16x8 (&g)[N], const uint32_t (&a)[N]) {
+  static_assert(N == 2 || N == 4, "");
+  static_assert(OFF2 < 65536, "");
+  if constexpr (N == 4)
+    asm volatile(
+        "ds_read_b128 %0, %8 offset:%12\n ds_read_b128 %4, %8 offset:%13\n"
+        "ds_read_b128 %1, %9 offset:%12\n ds_read_b128 %5, %9 offset:%13\n"
+        "ds_read_b128 %2, %10 offset:%12\n ds_read_b128 %6, %10 offset:%13\n"
+        "ds_read_b128 %3, %11 offset:%12\n ds_read_b128 %7, %11 offset:%13\n s_waitcnt lgkmcnt(0)"
+        : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3]), "=&v"(g[0]), "=&v"(g[1]), "=&v"(g[2]), "=&v"(g[3])
+        : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "i"(OFF), "i"(OFF2)
+        : "memory");
+  else
+    asm volatile(
+        "ds_read_b128 %0, %4 offset:%6\n ds_read_b128 %2, %4 offset:%7\n"
+        "ds_read_b128 %1, %5 offset:%6\n ds_read_b128 %3, %5 offset:%7\n s_waitcnt lgkmcnt(0)"
+        : "=&v"(f[0]), "=&v"(f[1]), "=&v"(g[0]), "=&v"(g[1])
+        : "v"(a[0]), "v"(a[1]), "i"(OFF), "i"(OFF2)
+        : "memory");
+}
 template <int OFF, int N>
 __device__ __forceinline__ void read_columns_at(bf16x4 (&f)[N], const uint32_t (&a)[N]) {
   static_assert(N == 2 || N == 4 || N == 8, "");

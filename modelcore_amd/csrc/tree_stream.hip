@@ -1,12 +1,18 @@
 // Attention of drafted trees over a paged bf16 cache, for rows of more (node, head) pairs per KV head than a wave
-// holds: every key and value is read once for 128 pairs and put through the matrix cores for all of them.
+// holds: every key and value is read once for 128 pairs (64) and put through the matrix cores for all of them.
 //
-// A workgroup of four waves has a key range of one block of 128 pairs of a KV head (tree_ranges.h), a wave 32
-// pairs of it. Its tiles of 32 keys are staged in LDS once for all four, straight from HBM (buffer loads to
-// LDS, whole rows of a page), in a ring of four: two waves load K, two V, each 16 keys, which share a
-// page, so that a load's page is one scalar; three tiles are under way while one is used, with a barrier a tile.
-// Products, layouts and numerics are those of the streaming kernel of few pairs (paged_stream.hip): scores and
-// sums in fp32, q as it is, weights as two bf16 terms, p = hi + lo, which keep them to 2^-17.
+// A workgroup of four waves has a key range of one block of pairs of a KV head (tree_ranges.h), a wave 32 of
+// its 128 pairs, or, where no row has more than 64 (WK = 2), 32 of 64 and half of each tile's keys. Tiles of 64
+// keys are staged in LDS once for all four, straight from HBM (buffer loads to LDS, whole rows of a page), one
+// tile while the one before is used: a wave loads 16 keys of K and of V, which share a page, so that a load's
+// page is one scalar. One barrier a tile; two workgroups a compute unit, of which one's products run under the
+// other's softmax.
+//   S^T (keys x pairs) = K . Q^T     v_mfma_f32_32x32x16_bf16, two independent sums of 32 keys
+//   O^T (D x pairs)   += V^T . P^T   V^T by LDS transpose reads
+// in the layouts of paged_stream.hip, a pair per lane. Scores, statistics and sums are fp32, q enters as it is,
+// the weights are rounded to bf16 once, as in the other kernels of many pairs (prefill_mfma.hip): the
+// outputs are 2.3e-3 of their norm off, of which their own rounding makes 1.7e-3. Weights in two terms, p = hi + lo,
+// are half again as many products: one row of 64 nodes after 16384 tokens 51.5 us for 44.5.
 //
 // Who sees whom: tree_bits.h, only in tiles that hold nodes or the window's edge. New nodes come from k_new and
 // v_new where given, and the block's last range puts them in their pages. A block of one range writes its
@@ -20,11 +26,10 @@
 namespace mcamd {
 namespace {
 
-constexpr int kBlock = 32 * kWaves;  // pairs
-constexpr int kRing = 4;             // tiles in LDS
-constexpr int kMinRangeTiles = 8;    // of a range, unless the row is shorter
+constexpr int kTile = 64;                 // keys
+constexpr int kMinRangeTiles = 4;         // of a range, unless the row is shorter
 constexpr float kTileSumLimit = 32768.f;  // 2^15: a lane's weights of one tile sum to at most this
-static_assert(kRing == 4, "the loop goes round the ring by name");
+constexpr int block_of(int wk) { return 32 * kWaves / wk; }  // pairs
 // Workgroups of a compute unit: as many as its LDS and registers hold.
 constexpr int tree_fill(int dp) { return dp <= 128 ? 2 : 1; }
 
@@ -33,37 +38,42 @@ struct TreeParams : CarefulParams {
   const int32_t *seqlens, *cu;
   int n_rows, t_new, total, H, G;
   int target;     // workgroups a call aims at; 0: no row is cut
-  float *part_o;  // [slot][kBlock][D]
-  float *part_ml; // [slot][kBlock][2]
+  float *part_o;   // [slot][pairs of a block][D]
+  float *part_ml;  // [slot][pairs of a block][2]
   PagedTiles::Cut *cuts;
   int *n_cuts;
 };
 
-template <int DP>
+template <int DP, int WK>
 __global__ __launch_bounds__(kThreads)
     __attribute__((amdgpu_waves_per_eu(tree_fill(DP)))) void tree_stream_kernel(TreeParams P) {
   using S_ = Shape<DP>;
   constexpr int CPR = S_::CPR, RPI = S_::RPI, NV = S_::NV, KD = S_::KD, MD = S_::MD;
-  __shared__ __attribute__((aligned(1024))) uint16_t s_tiles[kRing][2][S_::TILE];
+  constexpr int kBlock = block_of(WK), MK = 2 / WK;  // pairs of a block, 32 keys of a wave's tile
+  constexpr int HALF = S_::TILE;                     // elements of 32 keys
+  // Two tiles, K then V of each; at the end the sums of waves 2 and 3 (WK = 2).
+  __shared__ __attribute__((aligned(1024))) uint16_t s_tiles[2][2][2 * HALF];
+  __shared__ float s_ml[2][2][32];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   TreeRange R;
   const TreeRanges call{P.cu, P.seqlens, P.n_rows, P.t_new, P.total, P.G, P.H_kv, kBlock, 0,
-                        P.kv.max_pages << P.kv.shift, P.window, KT, P.target, kMinRangeTiles};
+                        P.kv.max_pages << P.kv.shift, P.window, kTile, P.target, kMinRangeTiles};
   const bool found = find_tree_range(call, int(blockIdx.x) / P.H_kv, lane, R);
   if (blockIdx.x == 0 && tid == 0 && P.target > 0) *P.n_cuts = R.n_blocks;
   if (!found) return;
   const int kvh = int(blockIdx.x) % P.H_kv, b = R.b, D = P.D;
   const int h = lane >> 5, col = lane & 31;
+  const int pg = WK == 1 ? wave : wave & 1, kg = WK == 1 ? 0 : wave >> 1;  // its 32 pairs, and half of the keys
   const int pairs = R.T * P.G, p0 = R.qt * kBlock;
-  const int in_block = 32 * wave + col, pair = p0 + in_block;
-  const bool live = pair < pairs, busy = p0 + 32 * wave < pairs;  // this pair, any of the wave
+  const int in_block = 32 * pg + col, pair = p0 + in_block;
+  const bool live = pair < pairs, busy = p0 + 32 * pg < pairs;  // this pair, any of the wave
   const int t_q = live ? pair / P.G : 0;
   const int64_t at = (int64_t(R.tok0 + t_q) * P.H + kvh * P.G + (live ? pair - t_q * P.G : 0)) * D;
   uint16_t *out = static_cast<uint16_t *>(P.out) + at;
   if (R.s0 < 0 || int64_t(R.s0) + R.T > int64_t(P.kv.max_pages) << P.kv.shift) {
-    if (live)
+    if (live && kg == 0)
       for (int d = 8 * h; d < D; d += 16)
         *reinterpret_cast<uint4 *>(out + d) =
             make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
@@ -73,7 +83,7 @@ __global__ __launch_bounds__(kThreads)
   const int t_last = min(p0 + kBlock - 1, pairs - 1) / P.G;
   const int seen_from = P.window >= 0 ? max(0, R.s0 - 1 - P.window) : 0;  // keys any pair of the block sees
   const int seen_to = R.s0 + t_last;
-  const int first_tile = seen_from / KT, n_tiles = seen_to / KT - first_tile + 1;
+  const int first_tile = seen_from / kTile, n_tiles = seen_to / kTile - first_tile + 1;
   const int ranges = min(R.ranges, n_tiles);
   if (R.part >= ranges) return;
   if (R.noted && R.part == 0 && tid == 0)
@@ -91,64 +101,73 @@ __global__ __launch_bounds__(kThreads)
     qf[kd] = __builtin_bit_cast(bf16x8, u);
   }
 
-  // This wave's loads: 16 keys of K or V. Load i covers rows RPI i + lane / CPR; its lane's chunk goes to slot
-  // lane % CPR, wherever that is.
-  const bool is_v = wave >= 2;
-  const int half = wave & 1;
+  // This wave's loads: keys 16 wave .. of a tile, K and V. Load i covers rows RPI i + lane / CPR; its lane's chunk
+  // goes to slot lane % CPR, wherever that is. (The swizzles of a row are those of the row modulo 16.)
   const int tok_bytes = P.H_kv * D * 2;
   constexpr uint32_t kNowhere = 0x80000000u;
   const int lr = lane / CPR, lc = lane % CPR;
-  uint32_t off[NV];
+  uint32_t off_k[NV], off_v[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int r = RPI * i + lr, c = lc ^ (is_v ? S_::v_swz(r) : S_::k_swz(r));
-    off[i] = 8 * c < D ? uint32_t(r * tok_bytes + 16 * c) : kNowhere;
+    const int r = RPI * i + lr, ck = lc ^ S_::k_swz(r), cv = lc ^ S_::v_swz(r);
+    off_k[i] = 8 * ck < D ? uint32_t(r * tok_bytes + 16 * ck) : kNowhere;
+    off_v[i] = 8 * cv < D ? uint32_t(r * tok_bytes + 16 * cv) : kNowhere;
   }
   const scalar_ints table = (scalar_ints)(P.kv.table + b * P.kv.table_stride);
   const int64_t head_at = int64_t(kvh) * D * 2;
   const uint32_t page_bytes = uint32_t(tok_bytes) << P.kv.shift;
-  const char *const pool = static_cast<const char *>(is_v ? P.v_pages : P.k_pages);
-  const char *const new_rows = static_cast<const char *>(is_v ? P.v_new : P.k_new);
   const bool fresh = P.k_new != nullptr;
   bool lost = false;
   // The page of this wave's keys of a tile; one that no key needs is page 0.
   auto page_of = [&](int tile) {
-    const int k = tile * KT + 16 * half;
+    const int k = tile * kTile + 16 * wave;
     return tile < t1 && k + 15 >= seen_from && k <= seen_to ? table[k >> P.kv.shift] : 0;
   };
-  // Into place `at` of the ring; past the range's end zeros, so that as many loads are under way in every turn.
+  // Into place `at`; past the range's end zeros, so that as many loads are under way in every turn.
   auto load_tile = [&](int tile, int id, int at) {
-    const int k0 = tile * KT, k = k0 + 16 * half;
-    uint16_t *const to = s_tiles[at][is_v] + half * NV * 512;
+    const int k0 = tile * kTile, k = k0 + 16 * wave;
+    uint16_t *const to_k = s_tiles[at][0] + wave * NV * 512, *const to_v = s_tiles[at][1] + wave * NV * 512;
     lost = lost || !P.kv.is_page(id);
-    if (fresh && tile < t1 && k0 + KT > R.s0) {
+    if (fresh && tile < t1 && k0 + kTile > R.s0) {
       // Nodes come from their own rows; past the last one it is read again.
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int r = 16 * half + RPI * i + lr, key = max(seen_from, min(k0 + r, seen_to));
-        const int c = min(lc ^ (is_v ? S_::v_swz(r) : S_::k_swz(r)), D / 8 - 1);
-        const char *from = key >= R.s0 ? new_rows + int64_t(R.tok0 + key - R.s0) * tok_bytes
-                                       : pool + 2 * P.kv.offset(id, P.kv.in_page(key), int64_t(P.H_kv) * D);
+        const int r = RPI * i + lr, key = max(seen_from, min(k + r, seen_to));
+        const bool node = key >= R.s0;
+        const int64_t from = (node ? int64_t(R.tok0 + key - R.s0) * tok_bytes
+                                   : 2 * P.kv.offset(id, P.kv.in_page(key), int64_t(P.H_kv) * D)) + head_at;
+        const int ck = min(lc ^ S_::k_swz(r), D / 8 - 1), cv = min(lc ^ S_::v_swz(r), D / 8 - 1);
         __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void *)(from + head_at + 16 * c),
-            (__attribute__((address_space(3))) void *)(to + i * 512), 16, 0, 0);
+            (const __attribute__((address_space(1))) void *)(static_cast<const char *>(node ? P.k_new : P.k_pages) +
+                                                             from + 16 * ck),
+            (__attribute__((address_space(3))) void *)(to_k + i * 512), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void *)(static_cast<const char *>(node ? P.v_new : P.v_pages) +
+                                                             from + 16 * cv),
+            (__attribute__((address_space(3))) void *)(to_v + i * 512), 16, 0, 0);
       }
       return;
     }
-    const bool edge = k0 < seen_from || k0 + KT - 1 > seen_to || tile >= t1;
-    const char *base = pool + (P.kv.is_page(id) ? id : 0) * P.kv.page_stride * 2 + head_at;
-    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
-        (void *)base, 0, int(page_bytes - uint32_t(head_at)), 0x00020000);
+    const bool edge = k0 < seen_from || k0 + kTile - 1 > seen_to || tile >= t1;
+    const int64_t base = (P.kv.is_page(id) ? id : 0) * P.kv.page_stride * 2 + head_at;
+    const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+        (void *)(static_cast<const char *>(P.k_pages) + base), 0, int(page_bytes - uint32_t(head_at)), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+        (void *)(static_cast<const char *>(P.v_pages) + base), 0, int(page_bytes - uint32_t(head_at)), 0x00020000);
     const int in_page = P.kv.in_page(k) * tok_bytes;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      uint32_t o = off[i];
+      uint32_t ok = off_k[i], ov = off_v[i];
       if (edge) {
         const int key = k + RPI * i + lr;
-        o = key >= seen_from && key <= seen_to && tile < t1 ? o : kNowhere;
+        const bool there = key >= seen_from && key <= seen_to && tile < t1;
+        ok = there ? ok : kNowhere;
+        ov = there ? ov : kNowhere;
       }
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rsrc, (__attribute__((address_space(3))) void *)(to + i * 512), 16, int(o), in_page, 0, 0);
+          rk, (__attribute__((address_space(3))) void *)(to_k + i * 512), 16, int(ok), in_page, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rv, (__attribute__((address_space(3))) void *)(to_v + i * 512), 16, int(ov), in_page, 0, 0);
     }
   };
 
@@ -156,14 +175,15 @@ __global__ __launch_bounds__(kThreads)
   uint32_t ka[KD], va[2 * MD];
 #pragma unroll
   for (int kd = 0; kd < KD; ++kd)
-    ka[kd] = lds_addr(s_tiles[0][0]) + 2 * (col * DP + 8 * ((2 * kd + h) ^ S_::k_swz(col)));
+    ka[kd] = lds_addr(s_tiles[0][0]) + 2 * (kg * HALF + col * DP + 8 * ((2 * kd + h) ^ S_::k_swz(col)));
   const int tr_row = (lane & 15) >> 2, tr_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
   for (int md = 0; md < MD; ++md)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int r = 4 * h + tr_row + 8 * u, c = 32 * md + tr_col;
-      va[2 * md + u] = lds_addr(s_tiles[0][1]) + 2 * (r * DP + 8 * ((c >> 3) ^ S_::v_swz(r)) + (c & 7));
+      va[2 * md + u] =
+          lds_addr(s_tiles[0][1]) + 2 * (kg * HALF + r * DP + 8 * ((c >> 3) ^ S_::v_swz(r)) + (c & 7));
     }
 
   f32x16 o[MD];
@@ -174,68 +194,85 @@ __global__ __launch_bounds__(kThreads)
   float m = -INFINITY, l = 0.f;
 
   if (D < DP) {  // dims past the head's are zero, whether or not a load past a page's end writes
-    for (int i = tid; i < kRing * 2 * S_::TILE / 8; i += kThreads)
+    for (int i = tid; i < 2 * 2 * 2 * HALF / 8; i += kThreads)
       reinterpret_cast<uint4 *>(s_tiles)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
   }
-  int id[kRing - 1];
-#pragma unroll
-  for (int i = 0; i < kRing - 1; ++i) id[i] = page_of(t0 + i);
-#pragma unroll
-  for (int i = 0; i < kRing - 1; ++i) load_tile(t0 + i, id[i], i);
-  int next = page_of(t0 + kRing - 1);
-  // The queries were asked for before these and are there with the first tile: waited for here, since in the loop
-  // the compiler would wait for the loads to LDS with them.
-  wait_loads<2 * NV>();
+  {
+    const int id = page_of(t0);
+    load_tile(t0, id, 0);
+  }
+  int next = page_of(t0 + 1);
+  // The queries were asked for before these: waited for here, since in the loop the compiler would wait for the
+  // loads to LDS with them.
+  wait_loads<0>();
 #pragma unroll
   for (int kd = 0; kd < KD; ++kd) asm volatile("" : "+v"(qf[kd]));
 
-  // One tile, in place AT of the ring.
+  // One tile, in place AT.
   auto turn = [&](int tile, auto at_c) __attribute__((always_inline)) {
     constexpr int AT = decltype(at_c)::value;
-    constexpr int kAt = AT * 2 * S_::TILE * 2, kOff = kAt < 49152 ? kAt : 0;  // bytes, of which an instruction's
-    const int k0 = tile * KT;
-    // This wave's loads of the tile have landed, those of the two after it may be under way; and everyone's; and
-    // everyone has read the tile before, whose place the next load takes.
-    wait_loads<2 * NV>();
+    constexpr int kAt = AT * 2 * 2 * HALF * 2, kOff = kAt < 40000 ? kAt : 0;  // bytes, of which an instruction's
+    const int k0 = tile * kTile + 32 * kg;  // of this wave
+    // This wave's loads of the tile have landed, and everyone's; and everyone has read the tile before, whose place
+    // the next load takes.
+    wait_loads<0>();
     __builtin_amdgcn_s_barrier();
-    load_tile(tile + kRing - 1, next, (AT + kRing - 1) % kRing);
-    next = page_of(tile + kRing);
+    load_tile(tile + 1, next, 1 - AT);
+    next = page_of(tile + 2);
     if (!busy) return;
 
-    f32x16 s;
+    f32x16 s[MK];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) s[e] = 0.f;
-    constexpr int KB = KD < 8 ? KD : 8;
+    for (int mk = 0; mk < MK; ++mk)
 #pragma unroll
-    for (int k8 = 0; k8 < KD; k8 += KB) {
-      bf16x8 f[KB];
+      for (int e = 0; e < 16; ++e) s[mk][e] = 0.f;
+    constexpr int KB = KD < 4 ? KD : 4;
+    auto scores = [&](auto k8_c) __attribute__((always_inline)) {
+      constexpr int k8 = decltype(k8_c)::value;
+      bf16x8 f[MK][KB];
       uint32_t a[KB];
 #pragma unroll
       for (int i = 0; i < KB; ++i) a[i] = ka[k8 + i] + (kAt - kOff);
-      read_rows_at<kOff, KB>(f, a);
+      if constexpr (MK == 2)
+        read_rows_two<kOff, kOff + 2 * HALF, KB>(f[0], f[MK - 1], a);
+      else
+        read_rows_at<kOff, KB>(f[0], a);
 #pragma unroll
       for (int i = 0; i < KB; ++i)
-        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i], qf[k8 + i], s, 0, 0, 0);
-    }
+#pragma unroll
+        for (int mk = 0; mk < MK; ++mk)
+          s[mk] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[mk][i], qf[k8 + i], s[mk], 0, 0, 0);
+    };
+    scores(std::integral_constant<int, 0>{});
+    if constexpr (KD > 4) scores(std::integral_constant<int, 4>{});
+    if constexpr (KD > 8) scores(std::integral_constant<int, 8>{});
+    if constexpr (KD > 12) scores(std::integral_constant<int, 12>{});
 
     // Keys the pair may not see.
-    if (k0 + KT - 1 >= R.s0 || (P.window >= 0 && k0 < R.s0 + t_last - P.window)) {
+    if (k0 + 32 * MK - 1 >= R.s0 || (P.window >= 0 && k0 < R.s0 + t_last - P.window)) {
       const uint64_t seen = TreeNode(P.tree, R.tok0 + t_q, t_q, R.s0, P.window).seen(k0) >> (4 * h);
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (!((seen >> (8 * (e >> 2) + (e & 3))) & 1)) s[e] = -INFINITY;
+      for (int mk = 0; mk < MK; ++mk)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (!((seen >> (32 * mk + 8 * (e >> 2) + (e & 3))) & 1)) s[mk][e] = -INFINITY;
     }
     // Weights against the running maximum; the tile's own is taken, and the sums rescaled, only where a lane's
     // weights sum past 2^15 or are not finite, or the pair has no maximum yet.
-    float w[16];
-    auto weigh = [&]() {
+    bf16x8 pk[2 * MK];
+    auto weigh = [&]() __attribute__((always_inline)) {
       const float ref = m == -INFINITY ? 0.f : m;
       float ts[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        w[e] = fast_exp2(fmaf(s[e], P.scale_log2, -ref));
-        ts[e & 3] += w[e];
+      for (int ks = 0; ks < 2 * MK; ++ks) {
+        f32x8 w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          w[e] = fast_exp2(fmaf(s[ks >> 1][8 * (ks & 1) + e], P.scale_log2, -ref));
+          ts[e & 3] += w[e];
+        }
+        pk[ks] = __builtin_convertvector(w, bf16x8);
       }
       return (ts[0] + ts[1]) + (ts[2] + ts[3]);
     };
@@ -243,7 +280,9 @@ __global__ __launch_bounds__(kThreads)
     if (__builtin_amdgcn_ballot_w64(!(tl <= kTileSumLimit) || m == -INFINITY) != 0) {
       float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int e = 0; e < 16; ++e) m4[e & 3] = fmaxf(m4[e & 3], s[e]);
+      for (int mk = 0; mk < MK; ++mk)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) m4[e & 3] = fmaxf(m4[e & 3], s[mk][e]);
       const float mx = max_halves(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]))) * P.scale_log2;
       const float m_new = fmaxf(m, mx);
       const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - m_new);
@@ -259,11 +298,6 @@ __global__ __launch_bounds__(kThreads)
 
     auto add_values = [&](auto ks_c) __attribute__((always_inline)) {  // of 16 keys
       constexpr int ks = decltype(ks_c)::value;
-      f32x8 pv;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) pv[e] = w[8 * ks + e];
-      const bf16x8 hi8 = __builtin_convertvector(pv, bf16x8);
-      const bf16x8 lo8 = __builtin_convertvector(pv - __builtin_convertvector(hi8, f32x8), bf16x8);
       constexpr int VB = 2 * MD < 8 ? 2 * MD : 8;
 #pragma unroll
       for (int v8 = 0; v8 < 2 * MD; v8 += VB) {
@@ -276,22 +310,21 @@ __global__ __launch_bounds__(kThreads)
         for (int i = 0; i < VB / 2; ++i) {
           const int md = v8 / 2 + i;
           const bf16x8 x = __builtin_shufflevector(f[2 * i], f[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
-          o[md] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, hi8, o[md], 0, 0, 0);
-          o[md] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, lo8, o[md], 0, 0, 0);
+          o[md] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, pk[ks], o[md], 0, 0, 0);
         }
       }
     };
     add_values(std::integral_constant<int, 0>{});
     add_values(std::integral_constant<int, 1>{});
+    if constexpr (MK == 2) {
+      add_values(std::integral_constant<int, 2>{});
+      add_values(std::integral_constant<int, 3>{});
+    }
   };
   for (int tile = t0;;) {
     turn(tile, std::integral_constant<int, 0>{});
     if (++tile >= t1) break;
     turn(tile, std::integral_constant<int, 1>{});
-    if (++tile >= t1) break;
-    turn(tile, std::integral_constant<int, 2>{});
-    if (++tile >= t1) break;
-    turn(tile, std::integral_constant<int, 3>{});
     if (++tile >= t1) break;
   }
   wait_loads<0>();
@@ -313,7 +346,36 @@ __global__ __launch_bounds__(kThreads)
       *reinterpret_cast<uint4 *>(static_cast<char *>(const_cast<void *>(P.v_pages)) + to) = y;
     }
   }
-  if (__syncthreads_or(lost)) l = NAN;  // and the nodes are in their pages
+  if (__syncthreads_or(lost)) l = NAN;  // and the nodes are in their pages, the tiles read
+
+  if constexpr (WK == 2) {  // waves 2 and 3 hand their sums to 0 and 1
+    static_assert(2 * 32 * DP * 4 <= int(sizeof(s_tiles)), "two waves' sums fit the tiles");
+    float *const so = reinterpret_cast<float *>(s_tiles) + pg * 32 * DP;
+    if (kg == 1) {
+#pragma unroll
+      for (int md = 0; md < MD; ++md)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<float4 *>(so + ((md * 4 + j) * 64 + lane) * 4) =
+              make_float4(o[md][4 * j], o[md][4 * j + 1], o[md][4 * j + 2], o[md][4 * j + 3]);
+      if (h == 0) s_ml[pg][0][col] = m, s_ml[pg][1][col] = l;
+    }
+    __syncthreads();
+    if (kg == 1) return;
+    const float m2 = s_ml[pg][0][col], M = fmaxf(m, m2);
+    const float a1 = m == -INFINITY ? 0.f : fast_exp2(m - M), a2 = m2 == -INFINITY ? 0.f : fast_exp2(m2 - M);
+    // Without a key l = 0; a NaN l must stay.
+    l = l * (m == -INFINITY ? 1.f : a1) + s_ml[pg][1][col] * (m2 == -INFINITY ? 1.f : a2);
+    m = M;
+#pragma unroll
+    for (int md = 0; md < MD; ++md)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 x = *reinterpret_cast<const f32x4 *>(so + ((md * 4 + j) * 64 + lane) * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[md][4 * j + i] = fmaf(x[i], a2, o[md][4 * j + i] * a1);
+      }
+  }
 
   // o[md][4j + i] is dim 32 md + 8 j + 4 h + i of pair `col`.
   if (ranges > 1) {
@@ -353,7 +415,7 @@ __global__ __launch_bounds__(kThreads)
       }
   }
   for (uint32_t left = bad; __builtin_expect(left != 0, 0); left &= left - 1) {
-    const int pr = p0 + 32 * wave + __builtin_ctz(left), t = pr / P.G;
+    const int pr = p0 + 32 * pg + __builtin_ctz(left), t = pr / P.G;
     careful_pair<bf16, DP, 8, true>(P, b, kvh, (int64_t(R.tok0 + t) * P.H + kvh * P.G + (pr - t * P.G)) * D,
                                     R.s0 + t, lane, 0, D, R.tok0 + t, t);
   }
@@ -361,8 +423,9 @@ __global__ __launch_bounds__(kThreads)
 
 // The ranges of cut blocks added up: a workgroup has two pairs (D up to 128; one of more) of a block and KV head, half
 // a wave a pair with four dims a lane, and its waves every fourth range each, eight of them under way.
-template <int DP>
+template <int DP, int WK>
 __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeParams P) {
+  constexpr int kBlock = block_of(WK);
   constexpr int LPP = DP <= 128 ? 32 : 64, N = 64 / LPP, U = 8;  // lanes of a pair, pairs of a wave
   __shared__ f32x4 s_o[kWaves][64];
   __shared__ float2 s_ml[kWaves][N];
@@ -439,30 +502,37 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeParams P) {
   }
 }
 
-int64_t block_bound(const PagedArgs &a) { return paged_blocks_bound(a, kBlock, 0); }
+// Half the keys a wave where no row has more pairs than two waves hold.
+int split_of(const PagedArgs &a) { return a.t_new * (a.n_head / a.n_kv_head) <= block_of(2) ? 2 : 1; }
 int64_t target_of(const PagedArgs &a) {
-  return paged_keys(a) >= 2 * kMinRangeTiles * KT ? int64_t(tree_fill(head_pad(a.head_dim))) * device_cus() : 0;
+  return paged_keys(a) >= 2 * kMinRangeTiles * kTile ? int64_t(tree_fill(head_pad(a.head_dim))) * device_cus() : 0;
 }
 size_t bytes_of(const PagedArgs &a, int64_t target) {
-  return target == 0 ? 0 : paged_tiles_bytes(tree_slots(target, a.n_kv_head), kBlock * (a.head_dim + 2));
+  return target == 0 ? 0
+                     : paged_tiles_bytes(tree_slots(target, a.n_kv_head), block_of(split_of(a)) * (a.head_dim + 2));
 }
 
-template <int DP>
-int run(const TreeParams &P, const PagedArgs &a) {
-  const int64_t bound = block_bound(a);
+template <int DP, int WK>
+int run_split(const TreeParams &P, const PagedArgs &a) {
+  constexpr int kBlock = block_of(WK);
+  const int64_t bound = paged_blocks_bound(a, kBlock, 0);
   const int64_t blocks = P.target > 0 ? tree_blocks(bound, P.target, P.H_kv) : bound * P.H_kv;
   if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
   if (blocks == 0) return MCAMD_OK;
-  hipLaunchKernelGGL(tree_stream_kernel<DP>, dim3(unsigned(blocks)), dim3(kThreads), 0, a.stream, P);
+  hipLaunchKernelGGL((tree_stream_kernel<DP, WK>), dim3(unsigned(blocks)), dim3(kThreads), 0, a.stream, P);
   const int st = launch_status("tree_stream");
   if (st != MCAMD_OK || P.target == 0) return st;
   // A cut block has two ranges at least.
   const int64_t cut = std::min<int64_t>(bound * P.H_kv, tree_slots(P.target, P.H_kv) / 2);
   const int64_t pairs = std::min<int64_t>(kBlock, a.t_new * P.G), each = DP <= 128 ? 2 : 1;
   if (cut > 65535) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
-  hipLaunchKernelGGL(tree_merge_kernel<DP>, dim3(unsigned((pairs + each - 1) / each), unsigned(cut)), dim3(kThreads),
-                     0, a.stream, P);
+  hipLaunchKernelGGL((tree_merge_kernel<DP, WK>), dim3(unsigned((pairs + each - 1) / each), unsigned(cut)),
+                     dim3(kThreads), 0, a.stream, P);
   return launch_status("tree_merge");
+}
+template <int DP>
+int run(const TreeParams &P, const PagedArgs &a) {
+  return split_of(a) == 2 ? run_split<DP, 2>(P, a) : run_split<DP, 1>(P, a);
 }
 
 }  // namespace
@@ -495,8 +565,9 @@ int launch_tree_stream(const PagedArgs &a) {
     const int64_t slots = tree_slots(target, a.n_kv_head);
     P.target = int(target);
     P.part_o = static_cast<float *>(a.scratch);
-    P.part_ml = P.part_o + slots * kBlock * a.head_dim;
-    P.cuts = reinterpret_cast<PagedTiles::Cut *>(P.part_ml + slots * kBlock * 2);
+    const int64_t pairs = slots * block_of(split_of(a));
+    P.part_ml = P.part_o + pairs * a.head_dim;
+    P.cuts = reinterpret_cast<PagedTiles::Cut *>(P.part_ml + pairs * 2);
     P.n_cuts = reinterpret_cast<int *>(P.cuts + slots);
   }
   switch (head_pad(a.head_dim)) {
