@@ -674,12 +674,10 @@ int run(const TiledParams &P, const PagedArgs &a, const TiledPlan &t) {
                                                            : std::max<int64_t>(t.bound * P.H_kv, P.tiles.slots);
   if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
   if (blocks == 0) return MCAMD_OK;
-  if (a.tree.masks)
-    hipLaunchKernelGGL((paged_tiled_kernel<E, DP, KS, true>), dim3(unsigned(blocks)), dim3(kThreads), 0,
-                       a.stream, P);
-  else
-    hipLaunchKernelGGL((paged_tiled_kernel<E, DP, KS, false>), dim3(unsigned(blocks)), dim3(kThreads), 0,
-                       a.stream, P);
+  auto kernel = paged_tiled_kernel<E, DP, KS, false>;
+  if constexpr (std::is_same<E, float>::value)  // trees in bf16: tree_stream.hip, paged_stream.hip
+    if (a.tree.masks) kernel = paged_tiled_kernel<E, DP, KS, true>;
+  hipLaunchKernelGGL(kernel, dim3(unsigned(blocks)), dim3(kThreads), 0, a.stream, P);
   const int st = launch_status("paged_tiled");
   if (st != MCAMD_OK || P.tiles.slots == 0) return st;
   return launch_paged_tiles_merge(a, P.tiles, t.pairs, t.bound);
@@ -712,9 +710,9 @@ int launch_paged_tiles_merge(const PagedArgs &a, const PagedTiles &tiles, int pa
   const int64_t blocks = std::min<int64_t>(bound * P.H_kv, cut) * tiles.groups * P.md;
   if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
   const dim3 grid{unsigned(blocks)}, threads{kThreads};
-  const bool bf = a.dtype == MCAMD_BF16;
-  const auto kernel = a.tree.masks ? bf ? paged_merge_kernel<bf16, true> : paged_merge_kernel<float, true>
-                                   : bf ? paged_merge_kernel<bf16, false> : paged_merge_kernel<float, false>;
+  const auto kernel = a.dtype == MCAMD_BF16 ? paged_merge_kernel<bf16, false>
+                      : a.tree.masks        ? paged_merge_kernel<float, true>
+                                            : paged_merge_kernel<float, false>;
   hipLaunchKernelGGL(kernel, grid, threads, 0, a.stream, P, pairs);
   return launch_status("paged_merge");
 }

@@ -69,7 +69,6 @@
 #include "paged_careful.h"
 #include "prefill_order.h"
 #include "prefill_split.h"
-#include "tree_ranges.h"
 
 #include <cmath>
 #include <type_traits>
@@ -165,8 +164,8 @@ typedef const __attribute__((address_space(4))) int32_t *scalar_ints;  // read o
 // SPLIT: a workgroup per key range of a block (prefill_split.h), which takes the chunk's own keys from
 // k_new and v_new where they are given (the merge appends them). VARLEN: sequences of their own
 // lengths, packed along the token axis. PAGED: keys and values in pages, rows of any lengths, blocks cut
-// where T has room. TREE: a row's tokens are nodes of a drafted tree.
-template <bool SPLIT, bool VARLEN, bool PAGED = false, bool TREE = false>
+// where T has room.
+template <bool SPLIT, bool VARLEN, bool PAGED = false>
 __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const SplitGeo *S,
                                                   const uint16_t *k_new, const uint16_t *v_new,
                                                   const PagedTiles *T = nullptr) {
@@ -193,17 +192,8 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   // rows[b]; a query tile past the sequence's end has nothing to do (a whole workgroup).
   int row = b, T_b = P.T_new, s0;
   int64_t tok0 = int64_t(b) * P.T_new;
-  typename std::conditional<TREE, TreeRange, PagedBlock>::type blk;
-  if constexpr (TREE) {
-    const TreeRanges ranges{P.cu, P.seqlens, T->n_rows, P.T_new, T->total, P.G, P.H_kv, P.QT * P.G, T->skip,
-                            int(P.T_max), P.window, KT, T->slots > 0 ? T->target : 0, T->min_tiles};
-    const bool found = find_tree_range(ranges, int(blockIdx.x) / P.H_kv, lane, blk);
-    if (blockIdx.x == 0 && tid == 0 && T->slots > 0) *T->n_cuts = blk.n_blocks;
-    if (!found) return;
-    kvh = int(blockIdx.x) % P.H_kv;
-    part = blk.part;
-    b = row = blk.b, qt = blk.qt, tok0 = blk.tok0, T_b = blk.T, s0 = blk.s0;
-  } else if constexpr (PAGED) {
+  PagedBlock blk;
+  if constexpr (PAGED) {
     const bool found = find_paged_block(P.cu, P.seqlens, T->n_rows, P.T_new, T->total, P.G, P.H_kv,
                                         P.QT * P.G, T->skip, T->slots, int(P.T_max), T->halve,
                                         int(blockIdx.x) / P.H_kv, lane, blk);
@@ -246,7 +236,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   const int head = live ? pr - (pr / P.G) * P.G : 0;
   uint16_t *out = P.out + ((tok0 + pos) * P.H + int64_t(kvh) * P.G + head) * D;
   if (!row_ok) {
-    if constexpr (PAGED && !TREE)
+    if constexpr (PAGED)
       if (blk.noted && part == 0 && tid == 0) T->note_block(int(blockIdx.x), blk, 1, P.H_kv);
     if (live && part == 0)
       for (int d = h * 64; d < h * 64 + 64; ++d) out[d] = 0x7fc0;
@@ -269,7 +259,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   const int p_abs = s0 + pos;
   const int p_first = s0 + q0;
   const int p_last = s0 + q_end - 1;
-  int lo = P.window >= 0 ? max(0, (TREE ? s0 - 1 : p_first) - P.window) : 0;
+  int lo = P.window >= 0 ? max(0, p_first - P.window) : 0;
   int hi = p_last;
   const int seen_from = lo;  // PAGED: tiles begin before it, at a multiple of their keys
   if constexpr (PAGED) lo &= ~(KT - 1);
@@ -278,18 +268,9 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   if constexpr (PAGED) {
     if (blk.noted) {
       const int tiles = (hi - lo) / KT + 1;
-      int ranges;
-      if constexpr (TREE)
-        ranges = min(blk.ranges, tiles);
-      else
-        ranges = T->ranges_of(blk, tiles);
+      const int ranges = T->ranges_of(blk, tiles);
       if (part >= ranges) return;
-      if (part == 0 && tid == 0) {
-        if constexpr (TREE)
-          note_tree_range(*T, blk, kvh, P.H_kv, ranges);
-        else
-          T->note_block(int(blockIdx.x), blk, ranges, P.H_kv);
-      }
+      if (part == 0 && tid == 0) T->note_block(int(blockIdx.x), blk, ranges, P.H_kv);
       whole = ranges == 1;
       const int t0 = part * tiles / ranges, t1 = (part + 1) * tiles / ranges;
       hi = min(hi, lo + t1 * KT - 1);
@@ -467,17 +448,6 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   };
   // Masks the keys the pair may not see (tiles that straddle the diagonal or the window edge).
   auto mask = [&](f32x16 (&s)[2], int k0) {
-    if constexpr (TREE) {
-      if (k0 + KT - 1 >= s0 || (P.window >= 0 && k0 < p_last - P.window)) {
-        const uint64_t seen = TreeNode(T->tree, tok0 + pos, pos, s0, P.window).seen(k0) >> (4 * h);
-#pragma unroll
-        for (int mk = 0; mk < 2; ++mk)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (!((seen >> (32 * mk + 8 * (e >> 2) + (e & 3))) & 1)) s[mk][e] = -INFINITY;
-      }
-      return;
-    }
     const bool need_mask = (k0 + KT - 1 > p_first) || (P.window >= 0 && k0 < p_last - P.window);
     if (need_mask) {
 #pragma unroll
@@ -766,8 +736,7 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
   if constexpr (PAGED) {
     if (!whole) {
       if (!live) return;
-      int64_t g = int64_t(blockIdx.x) * kWaves + wave;
-      if constexpr (TREE) g = (int64_t(blk.slot + part) * P.H_kv + kvh) * kWaves + wave;
+      const int64_t g = int64_t(blockIdx.x) * kWaves + wave;
 #pragma unroll
       for (int md = 0; md < 4; ++md)
 #pragma unroll
@@ -784,13 +753,12 @@ __device__ __forceinline__ void prefill_mfma_body(const MfmaParams &P, const Spl
       for (int e = 0; e < 16; ++e) ok = ok && finite(o[md][e] * inv);
     const uint64_t bad64 = __builtin_amdgcn_ballot_w64(live && !ok);
     if (__builtin_expect(bad64 != 0, 0)) {
-      const CarefulParams C{P.q,  P.k_cache, P.v_cache,    T->kv, P.out, P.H_kv, P.window, D,
-                            P.scale_log2, T->tree};
+      const CarefulParams C{P.q, P.k_cache, P.v_cache, T->kv, P.out, P.H_kv, P.window, D, P.scale_log2};
       for (uint32_t left = uint32_t(bad64) | uint32_t(bad64 >> 32); left != 0; left &= left - 1) {
         const int pr2 = wave * 32 + __builtin_ctz(left), t = q0 + pr2 / P.G;
-        careful_pair<bf16, D, 8, TREE>(C, row, kvh,
-                                       ((tok0 + t) * P.H + int64_t(kvh) * P.G + (pr2 - pr2 / P.G * P.G)) * D,
-                                       s0 + t, lane, 0, D, tok0 + t, t);
+        careful_pair<bf16, D, 8>(C, row, kvh,
+                                 ((tok0 + t) * P.H + int64_t(kvh) * P.G + (pr2 - pr2 / P.G * P.G)) * D,
+                                 s0 + t, lane, 0, D);
       }
       if ((uint32_t(bad64 >> col) | uint32_t(bad64 >> (32 + col))) & 1u) return;
     }
@@ -833,9 +801,6 @@ __global__ __launch_bounds__(kThreads, 1) void prefill_mfma_varlen_kernel(MfmaPa
 }
 __global__ __launch_bounds__(kThreads, 1) void paged_mfma_kernel(MfmaParams P, PagedTiles T) {
   prefill_mfma_body<false, false, true>(P, nullptr, nullptr, nullptr, &T);
-}
-__global__ __launch_bounds__(kThreads, 1) void paged_tree_mfma_kernel(MfmaParams P, PagedTiles T) {
-  prefill_mfma_body<false, false, true, true>(P, nullptr, nullptr, nullptr, &T);
 }
 __global__ __launch_bounds__(kThreads, 1) void prefill_mfma_split_kernel(
     MfmaParams P, SplitGeo S, const uint16_t *k_new, const uint16_t *v_new) {
@@ -928,17 +893,7 @@ constexpr int64_t kSlotFloats = int64_t(kPairs) * (D + 2);
 
 }  // namespace
 
-namespace {
-
-// Partials of a call over trees, whose ranges aim at a workgroup per compute unit; 0 where no row has keys for two.
-int64_t tree_mfma_slots(const PagedArgs &a) {
-  return paged_keys(a) >= 2 * kMinRangeKeys ? tree_slots(device_cus(), a.n_kv_head) : 0;
-}
-
-}  // namespace
-
 size_t paged_mfma_bytes(const PagedArgs &a, int64_t skip) {
-  if (a.tree.masks) return paged_tiles_bytes(tree_mfma_slots(a), kSlotFloats);
   const int64_t G = a.n_head / a.n_kv_head;
   const int64_t pairs = kPairs / G * G;
   return paged_tiles_bytes(paged_slots(a, paged_blocks_bound(a, pairs, skip), pairs, 1, kMinRangeKeys),
@@ -965,7 +920,6 @@ int launch_paged_mfma(const PagedArgs &a, int64_t skip) {
   P.scale_log2 = float(kLog2e / std::sqrt(double(D)));
   PagedTiles T{};
   T.kv = a.kv;
-  T.tree = a.tree;
   T.n_rows = int(a.n_rows);
   T.total = int(a.total);
   T.skip = int(skip);
@@ -973,17 +927,13 @@ int launch_paged_mfma(const PagedArgs &a, int64_t skip) {
   T.groups = kWaves;
   const int64_t bound = paged_blocks_bound(a, P.QT * P.G, skip);
   T.min_tiles = kMinRangeKeys / KT;
-  const int64_t slots = a.tree.masks ? tree_mfma_slots(a) : paged_slots(a, bound, P.QT * P.G, 1, kMinRangeKeys);
-  paged_tiles_buffers(a, T, slots, kSlotFloats, kPairs * 2);
-  T.target = device_cus();
+  paged_tiles_buffers(a, T, paged_slots(a, bound, P.QT * P.G, 1, kMinRangeKeys), kSlotFloats, kPairs * 2);
   // A tile of 64 keys takes 256 pairs 1.4 us; a range's partials are written and read.
   T.ratio = 1.4f * MCAMD_SPLIT_BYTES_PER_US / (float(kSlotFloats) * 8.f);
-  const int64_t blocks = a.tree.masks && T.slots > 0 ? tree_blocks(bound, T.target, P.H_kv)
-                                                     : std::max<int64_t>(bound * P.H_kv, T.slots);
+  const int64_t blocks = std::max<int64_t>(bound * P.H_kv, T.slots);
   if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
   if (blocks == 0) return MCAMD_OK;
-  hipLaunchKernelGGL(a.tree.masks ? paged_tree_mfma_kernel : paged_mfma_kernel, dim3(unsigned(blocks)),
-                     dim3(kThreads), 0, a.stream, P, T);
+  hipLaunchKernelGGL(paged_mfma_kernel, dim3(unsigned(blocks)), dim3(kThreads), 0, a.stream, P, T);
   const int st = launch_status("paged_mfma");
   if (st != MCAMD_OK || T.slots == 0) return st;
   return launch_paged_tiles_merge(a, T, P.QT * P.G, bound);

@@ -119,12 +119,12 @@ __global__ __launch_bounds__(kThreads)
   const bool fresh = P.k_new != nullptr;
   bool lost = false;
   // The page of this wave's keys of a tile; one that no key needs is page 0.
-  auto page_of = [&](int tile) {
+  auto page_of = [&](int tile) __attribute__((always_inline)) {
     const int k = tile * kTile + 16 * wave;
     return tile < t1 && k + 15 >= seen_from && k <= seen_to ? table[k >> P.kv.shift] : 0;
   };
   // Into place `at`; past the range's end zeros, so that as many loads are under way in every turn.
-  auto load_tile = [&](int tile, int id, int at) {
+  auto load_tile = [&](int tile, int id, int at) __attribute__((always_inline)) {
     const int k0 = tile * kTile, k = k0 + 16 * wave;
     uint16_t *const to_k = s_tiles[at][0] + wave * NV * 512, *const to_v = s_tiles[at][1] + wave * NV * 512;
     lost = lost || !P.kv.is_page(id);
@@ -296,23 +296,23 @@ __global__ __launch_bounds__(kThreads)
     }
     l += tl;
 
-    auto add_values = [&](auto ks_c) __attribute__((always_inline)) {  // of 16 keys
-      constexpr int ks = decltype(ks_c)::value;
-      constexpr int VB = 2 * MD < 8 ? 2 * MD : 8;
+    constexpr int VB = 2 * MD < 8 ? 2 * MD : 8;
+    auto add_dims = [&](auto ks_c, auto v8_c) __attribute__((always_inline)) {
+      constexpr int ks = decltype(ks_c)::value, v8 = decltype(v8_c)::value;
+      bf16x4 f[VB];
+      uint32_t a[VB];
 #pragma unroll
-      for (int v8 = 0; v8 < 2 * MD; v8 += VB) {
-        bf16x4 f[VB];
-        uint32_t a[VB];
+      for (int i = 0; i < VB; ++i) a[i] = va[v8 + i] + (kAt - kOff);
+      read_columns_at<kOff + ks * 32 * DP, VB>(f, a);
 #pragma unroll
-        for (int i = 0; i < VB; ++i) a[i] = va[v8 + i] + (kAt - kOff);
-        read_columns_at<kOff + ks * 32 * DP, VB>(f, a);
-#pragma unroll
-        for (int i = 0; i < VB / 2; ++i) {
-          const int md = v8 / 2 + i;
-          const bf16x8 x = __builtin_shufflevector(f[2 * i], f[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
-          o[md] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, pk[ks], o[md], 0, 0, 0);
-        }
+      for (int i = 0; i < VB / 2; ++i) {
+        const bf16x8 x = __builtin_shufflevector(f[2 * i], f[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+        o[v8 / 2 + i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, pk[ks], o[v8 / 2 + i], 0, 0, 0);
       }
+    };
+    auto add_values = [&](auto ks_c) __attribute__((always_inline)) {  // of 16 keys
+      add_dims(ks_c, std::integral_constant<int, 0>{});
+      if constexpr (2 * MD > 8) add_dims(ks_c, std::integral_constant<int, 8>{});
     };
     add_values(std::integral_constant<int, 0>{});
     add_values(std::integral_constant<int, 1>{});
