@@ -1,12 +1,11 @@
 // Attention of drafted trees over a paged bf16 cache, for rows of more (node, head) pairs per KV head than a wave
 // holds: every key and value is read once for 128 pairs (64) and put through the matrix cores for all of them.
 //
-// A workgroup of four waves has a key range of one block of pairs of a KV head (tree_ranges.h), a wave 32 of
-// its 128 pairs, or, where no row has more than 64 (WK = 2), 32 of 64 and half of each tile's keys. Tiles of 64
-// keys are staged in LDS once for all four, straight from HBM (buffer loads to LDS, whole rows of a page), one
-// tile while the one before is used: a wave loads 16 keys of K and of V, which share a page, so that a load's
-// page is one scalar. One barrier a tile; two workgroups a compute unit, of which one's products run under the
-// other's softmax.
+// A workgroup has a key range of one block of pairs of a KV head (tree_ranges.h): 128 pairs, or 64 where no row has
+// more. A wave holds 32 of them, and the waves share the keys of a tile, 16 of which each loads: straight from
+// HBM to LDS (buffer loads, whole rows of a page), K and V, one tile while the one before is used; the 16 share a
+// page, so that a load's page is one scalar. One barrier a tile. At the end the waves of the same pairs join their
+// sums in LDS.
 //   S^T (keys x pairs) = K . Q^T     v_mfma_f32_32x32x16_bf16, two independent sums of 32 keys
 //   O^T (D x pairs)   += V^T . P^T   V^T by LDS transpose reads
 // in the layouts of paged_stream.hip, a pair per lane. Scores, statistics and sums are fp32, q enters as it is,
@@ -26,12 +25,14 @@
 namespace mcamd {
 namespace {
 
-constexpr int kTile = 64;                 // keys
-constexpr int kMinRangeTiles = 4;         // of a range, unless the row is shorter
+constexpr int kMinRangeKeys = 256;        // of a range, unless the row is shorter
 constexpr float kTileSumLimit = 32768.f;  // 2^15: a lane's weights of one tile sum to at most this
-constexpr int block_of(int wk) { return 32 * kWaves / wk; }  // pairs
-// Workgroups of a compute unit: as many as its LDS and registers hold.
-constexpr int tree_fill(int dp) { return dp <= 128 ? 2 : 1; }
+// Waves of a workgroup, and how many of those a compute unit holds. Blocks of 128 pairs have eight waves, so that
+// half as many partials are written and merged (one row of 64 nodes after 16384 tokens, 32 / 8 heads of 128: 42.9 us
+// for 46.5); those of 64, of which HBM is the bound, four, so that one workgroup's loads run while the other begins or
+// ends (32 rows of 16 nodes, 16 / 4 heads: 77 us for 85).
+constexpr int waves_of(int dp, int pairs) { return dp <= 128 && pairs == 128 ? 8 : 4; }
+constexpr int tree_fill(int dp, int pairs) { return dp <= 128 ? 8 / waves_of(dp, pairs) : 1; }
 
 struct TreeParams : CarefulParams {
   const void *k_new, *v_new;
@@ -44,28 +45,28 @@ struct TreeParams : CarefulParams {
   int *n_cuts;
 };
 
-template <int DP, int WK>
-__global__ __launch_bounds__(kThreads)
-    __attribute__((amdgpu_waves_per_eu(tree_fill(DP)))) void tree_stream_kernel(TreeParams P) {
+template <int DP, int kBlock>
+__global__ __launch_bounds__(64 * waves_of(DP, kBlock))
+    __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 2 : 1))) void tree_stream_kernel(TreeParams P) {
   using S_ = Shape<DP>;
   constexpr int CPR = S_::CPR, RPI = S_::RPI, NV = S_::NV, KD = S_::KD, MD = S_::MD;
-  constexpr int kBlock = block_of(WK), MK = 2 / WK;  // pairs of a block, 32 keys of a wave's tile
-  constexpr int HALF = S_::TILE;                     // elements of 32 keys
-  // Two tiles, K then V of each; at the end the sums of waves 2 and 3 (WK = 2).
-  __shared__ __attribute__((aligned(1024))) uint16_t s_tiles[2][2][2 * HALF];
-  __shared__ float s_ml[2][2][32];
+  constexpr int W = waves_of(DP, kBlock), kTile = 16 * W, kThreads = 64 * W;
+  constexpr int WP = kBlock / 32, WK = W / WP, MK = kTile / (32 * WK);  // waves over pairs, keys; 32 keys of a wave
+  // K and V of two tiles; at the end the sums of the waves over other keys than the first.
+  __shared__ __attribute__((aligned(1024))) uint16_t s_tiles[2][2][kTile * DP];
+  __shared__ float s_ml[WK][WP][2][32];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   TreeRange R;
   const TreeRanges call{P.cu, P.seqlens, P.n_rows, P.t_new, P.total, P.G, P.H_kv, kBlock, 0,
-                        P.kv.max_pages << P.kv.shift, P.window, kTile, P.target, kMinRangeTiles};
+                        P.kv.max_pages << P.kv.shift, P.window, kTile, P.target, kMinRangeKeys / kTile};
   const bool found = find_tree_range(call, int(blockIdx.x) / P.H_kv, lane, R);
   if (blockIdx.x == 0 && tid == 0 && P.target > 0) *P.n_cuts = R.n_blocks;
   if (!found) return;
   const int kvh = int(blockIdx.x) % P.H_kv, b = R.b, D = P.D;
   const int h = lane >> 5, col = lane & 31;
-  const int pg = WK == 1 ? wave : wave & 1, kg = WK == 1 ? 0 : wave >> 1;  // its 32 pairs, and half of the keys
+  const int pg = wave % WP, kg = wave / WP;  // its 32 pairs, and its part of a tile's keys
   const int pairs = R.T * P.G, p0 = R.qt * kBlock;
   const int in_block = 32 * pg + col, pair = p0 + in_block;
   const bool live = pair < pairs, busy = p0 + 32 * pg < pairs;  // this pair, any of the wave
@@ -126,7 +127,7 @@ __global__ __launch_bounds__(kThreads)
   // Into place `at`; past the range's end zeros, so that as many loads are under way in every turn.
   auto load_tile = [&](int tile, int id, int at) __attribute__((always_inline)) {
     const int k0 = tile * kTile, k = k0 + 16 * wave;
-    uint16_t *const to_k = s_tiles[at][0] + wave * NV * 512, *const to_v = s_tiles[at][1] + wave * NV * 512;
+    uint16_t *const to_k = s_tiles[0][at] + wave * NV * 512, *const to_v = s_tiles[1][at] + wave * NV * 512;
     lost = lost || !P.kv.is_page(id);
     if (fresh && tile < t1 && k0 + kTile > R.s0) {
       // Nodes come from their own rows; past the last one it is read again.
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(kThreads)
   uint32_t ka[KD], va[2 * MD];
 #pragma unroll
   for (int kd = 0; kd < KD; ++kd)
-    ka[kd] = lds_addr(s_tiles[0][0]) + 2 * (kg * HALF + col * DP + 8 * ((2 * kd + h) ^ S_::k_swz(col)));
+    ka[kd] = lds_addr(s_tiles[0][0]) + 2 * (kg * 32 * MK * DP + col * DP + 8 * ((2 * kd + h) ^ S_::k_swz(col)));
   const int tr_row = (lane & 15) >> 2, tr_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
   for (int md = 0; md < MD; ++md)
@@ -183,7 +184,7 @@ __global__ __launch_bounds__(kThreads)
     for (int u = 0; u < 2; ++u) {
       const int r = 4 * h + tr_row + 8 * u, c = 32 * md + tr_col;
       va[2 * md + u] =
-          lds_addr(s_tiles[0][1]) + 2 * (kg * HALF + r * DP + 8 * ((c >> 3) ^ S_::v_swz(r)) + (c & 7));
+          lds_addr(s_tiles[1][0]) + 2 * (kg * 32 * MK * DP + r * DP + 8 * ((c >> 3) ^ S_::v_swz(r)) + (c & 7));
     }
 
   f32x16 o[MD];
@@ -194,7 +195,7 @@ __global__ __launch_bounds__(kThreads)
   float m = -INFINITY, l = 0.f;
 
   if (D < DP) {  // dims past the head's are zero, whether or not a load past a page's end writes
-    for (int i = tid; i < 2 * 2 * 2 * HALF / 8; i += kThreads)
+    for (int i = tid; i < 2 * 2 * kTile * DP / 8; i += kThreads)
       reinterpret_cast<uint4 *>(s_tiles)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
   }
@@ -212,8 +213,8 @@ __global__ __launch_bounds__(kThreads)
   // One tile, in place AT.
   auto turn = [&](int tile, auto at_c) __attribute__((always_inline)) {
     constexpr int AT = decltype(at_c)::value;
-    constexpr int kAt = AT * 2 * 2 * HALF * 2, kOff = kAt < 40000 ? kAt : 0;  // bytes, of which an instruction's
-    const int k0 = tile * kTile + 32 * kg;  // of this wave
+    constexpr int kOff = AT * kTile * DP * 2;  // bytes
+    const int k0 = tile * kTile + 32 * MK * kg;  // of this wave
     // This wave's loads of the tile have landed, and everyone's; and everyone has read the tile before, whose place
     // the next load takes.
     wait_loads<0>();
@@ -233,9 +234,9 @@ __global__ __launch_bounds__(kThreads)
       bf16x8 f[MK][KB];
       uint32_t a[KB];
 #pragma unroll
-      for (int i = 0; i < KB; ++i) a[i] = ka[k8 + i] + (kAt - kOff);
+      for (int i = 0; i < KB; ++i) a[i] = ka[k8 + i];
       if constexpr (MK == 2)
-        read_rows_two<kOff, kOff + 2 * HALF, KB>(f[0], f[MK - 1], a);
+        read_rows_two<kOff, kOff + 64 * DP, KB>(f[0], f[MK - 1], a);
       else
         read_rows_at<kOff, KB>(f[0], a);
 #pragma unroll
@@ -302,7 +303,7 @@ __global__ __launch_bounds__(kThreads)
       bf16x4 f[VB];
       uint32_t a[VB];
 #pragma unroll
-      for (int i = 0; i < VB; ++i) a[i] = va[v8 + i] + (kAt - kOff);
+      for (int i = 0; i < VB; ++i) a[i] = va[v8 + i];
       read_columns_at<kOff + ks * 32 * DP, VB>(f, a);
 #pragma unroll
       for (int i = 0; i < VB / 2; ++i) {
@@ -348,32 +349,40 @@ __global__ __launch_bounds__(kThreads)
   }
   if (__syncthreads_or(lost)) l = NAN;  // and the nodes are in their pages, the tiles read
 
-  if constexpr (WK == 2) {  // waves 2 and 3 hand their sums to 0 and 1
-    static_assert(2 * 32 * DP * 4 <= int(sizeof(s_tiles)), "two waves' sums fit the tiles");
-    float *const so = reinterpret_cast<float *>(s_tiles) + pg * 32 * DP;
-    if (kg == 1) {
+  if constexpr (WK > 1) {  // the first waves of each 32 pairs take the others' sums
+    static_assert((WK - 1) * WP * 32 * DP * 4 <= int(sizeof(s_tiles)), "they fit the tiles");
+    float *const so = reinterpret_cast<float *>(s_tiles) + pg * 32 * DP + 4 * lane;
+    if (kg > 0)
 #pragma unroll
       for (int md = 0; md < MD; ++md)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<float4 *>(so + ((md * 4 + j) * 64 + lane) * 4) =
+          *reinterpret_cast<float4 *>(so + (kg - 1) * WP * 32 * DP + (md * 4 + j) * 256) =
               make_float4(o[md][4 * j], o[md][4 * j + 1], o[md][4 * j + 2], o[md][4 * j + 3]);
-      if (h == 0) s_ml[pg][0][col] = m, s_ml[pg][1][col] = l;
-    }
+    if (h == 0) s_ml[kg][pg][0][col] = m, s_ml[kg][pg][1][col] = l;
     __syncthreads();
-    if (kg == 1) return;
-    const float m2 = s_ml[pg][0][col], M = fmaxf(m, m2);
-    const float a1 = m == -INFINITY ? 0.f : fast_exp2(m - M), a2 = m2 == -INFINITY ? 0.f : fast_exp2(m2 - M);
-    // Without a key l = 0; a NaN l must stay.
-    l = l * (m == -INFINITY ? 1.f : a1) + s_ml[pg][1][col] * (m2 == -INFINITY ? 1.f : a2);
-    m = M;
+    if (kg > 0) return;
+#pragma unroll
+    for (int w = 1; w < WK; ++w) m = fmaxf(m, s_ml[w][pg][0][col]);
+    l = 0.f;
+    float a[WK];
+#pragma unroll
+    for (int w = 0; w < WK; ++w) {
+      const float m_w = s_ml[w][pg][0][col];
+      a[w] = m_w == -INFINITY ? 0.f : fast_exp2(m_w - m);
+      l += s_ml[w][pg][1][col] * (m_w == -INFINITY ? 1.f : a[w]);  // 0 then, or a NaN that must stay
+    }
 #pragma unroll
     for (int md = 0; md < MD; ++md)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const f32x4 x = *reinterpret_cast<const f32x4 *>(so + ((md * 4 + j) * 64 + lane) * 4);
+        f32x4 y = {o[md][4 * j], o[md][4 * j + 1], o[md][4 * j + 2], o[md][4 * j + 3]};
+        y *= a[0];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[md][4 * j + i] = fmaf(x[i], a2, o[md][4 * j + i] * a1);
+        for (int w = 1; w < WK; ++w)
+          y += a[w] * *reinterpret_cast<const f32x4 *>(so + (w - 1) * WP * 32 * DP + (md * 4 + j) * 256);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[md][4 * j + i] = y[i];
       }
   }
 
@@ -423,9 +432,8 @@ __global__ __launch_bounds__(kThreads)
 
 // The ranges of cut blocks added up: a workgroup has two pairs (D up to 128; one of more) of a block and KV head, half
 // a wave a pair with four dims a lane, and its waves every fourth range each, eight of them under way.
-template <int DP, int WK>
+template <int DP, int kBlock>
 __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeParams P) {
-  constexpr int kBlock = block_of(WK);
   constexpr int LPP = DP <= 128 ? 32 : 64, N = 64 / LPP, U = 8;  // lanes of a pair, pairs of a wave
   __shared__ f32x4 s_o[kWaves][64];
   __shared__ float2 s_ml[kWaves][N];
@@ -502,37 +510,37 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeParams P) {
   }
 }
 
-// Half the keys a wave where no row has more pairs than two waves hold.
-int split_of(const PagedArgs &a) { return a.t_new * (a.n_head / a.n_kv_head) <= block_of(2) ? 2 : 1; }
+// Pairs of a block.
+int block_of(const PagedArgs &a) { return a.t_new * (a.n_head / a.n_kv_head) <= 64 ? 64 : 128; }
+// Workgroups that a call aims at: all that the chip holds at once.
 int64_t target_of(const PagedArgs &a) {
-  return paged_keys(a) >= 2 * kMinRangeTiles * kTile ? int64_t(tree_fill(head_pad(a.head_dim))) * device_cus() : 0;
+  return paged_keys(a) >= 2 * kMinRangeKeys ? int64_t(tree_fill(head_pad(a.head_dim), block_of(a))) * device_cus() : 0;
 }
 size_t bytes_of(const PagedArgs &a, int64_t target) {
-  return target == 0 ? 0
-                     : paged_tiles_bytes(tree_slots(target, a.n_kv_head), block_of(split_of(a)) * (a.head_dim + 2));
+  return target == 0 ? 0 : paged_tiles_bytes(tree_slots(target, a.n_kv_head), block_of(a) * (a.head_dim + 2));
 }
 
-template <int DP, int WK>
-int run_split(const TreeParams &P, const PagedArgs &a) {
-  constexpr int kBlock = block_of(WK);
+template <int DP, int kBlock>
+int run_block(const TreeParams &P, const PagedArgs &a) {
+  constexpr int threads = 64 * waves_of(DP, kBlock);
   const int64_t bound = paged_blocks_bound(a, kBlock, 0);
   const int64_t blocks = P.target > 0 ? tree_blocks(bound, P.target, P.H_kv) : bound * P.H_kv;
-  if (blocks > 0x7fffffff / kThreads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
+  if (blocks > 0x7fffffff / threads) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
   if (blocks == 0) return MCAMD_OK;
-  hipLaunchKernelGGL((tree_stream_kernel<DP, WK>), dim3(unsigned(blocks)), dim3(kThreads), 0, a.stream, P);
+  hipLaunchKernelGGL((tree_stream_kernel<DP, kBlock>), dim3(unsigned(blocks)), dim3(threads), 0, a.stream, P);
   const int st = launch_status("tree_stream");
   if (st != MCAMD_OK || P.target == 0) return st;
   // A cut block has two ranges at least.
   const int64_t cut = std::min<int64_t>(bound * P.H_kv, tree_slots(P.target, P.H_kv) / 2);
   const int64_t pairs = std::min<int64_t>(kBlock, a.t_new * P.G), each = DP <= 128 ? 2 : 1;
   if (cut > 65535) return fail(MCAMD_EUNSUPPORTED, "paged attention: grid too large");
-  hipLaunchKernelGGL((tree_merge_kernel<DP, WK>), dim3(unsigned((pairs + each - 1) / each), unsigned(cut)),
+  hipLaunchKernelGGL((tree_merge_kernel<DP, kBlock>), dim3(unsigned((pairs + each - 1) / each), unsigned(cut)),
                      dim3(kThreads), 0, a.stream, P);
   return launch_status("tree_merge");
 }
 template <int DP>
 int run(const TreeParams &P, const PagedArgs &a) {
-  return split_of(a) == 2 ? run_split<DP, 2>(P, a) : run_split<DP, 1>(P, a);
+  return block_of(a) == 64 ? run_block<DP, 64>(P, a) : run_block<DP, 128>(P, a);
 }
 
 }  // namespace
@@ -565,7 +573,7 @@ int launch_tree_stream(const PagedArgs &a) {
     const int64_t slots = tree_slots(target, a.n_kv_head);
     P.target = int(target);
     P.part_o = static_cast<float *>(a.scratch);
-    const int64_t pairs = slots * block_of(split_of(a));
+    const int64_t pairs = slots * block_of(a);
     P.part_ml = P.part_o + pairs * a.head_dim;
     P.cuts = reinterpret_cast<PagedTiles::Cut *>(P.part_ml + pairs * 2);
     P.n_cuts = reinterpret_cast<int *>(P.cuts + slots);
