@@ -67,7 +67,8 @@ bool trees_of_many(const PagedArgs &a) {
 int launch(PagedArgs a) {
   if (trees_of_many(a)) return launch_tree_stream(a);
   const Kernels k = kernels_of(a);
-  const bool within = k.stream && (!k.tiles || a.total <= kAppendWithin);
+  // Trees' kernels take nodes from their own rows.
+  const bool within = a.tree.masks || (k.stream && (!k.tiles || a.total <= kAppendWithin));
   if (a.k_new && !within) {
     hipLaunchKernelGGL(paged_append_kernel, dim3(unsigned(paged_append_blocks(a))), dim3(kAppendThreads), 0,
                        a.stream, paged_append(a, 0));

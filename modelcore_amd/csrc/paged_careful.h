@@ -18,6 +18,7 @@ struct CarefulParams {
   int H_kv, window, D;
   float scale_log2;
   TreeMasks tree;  // of calls over trees
+  const void *k_new, *v_new;  // theirs: the nodes, which need not be in their pages yet; or null
 };
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
@@ -36,27 +37,33 @@ __device__ void careful_pair(const CarefulParams &P, int row, int kvh, int64_t a
   const E *kc = static_cast<const E *>(P.k_pages) + int64_t(kvh) * D;
   const E *vc = static_cast<const E *>(P.v_pages) + int64_t(kvh) * D;
   const int32_t *pages = P.kv.table + row * P.kv.table_stride;
-  auto key_at = [&](int t) { return P.kv.offset(pages[t >> P.kv.shift], P.kv.in_page(t), tok); };
+  // Where key t has its key, from kc on, or its value, from vc on.
+  auto from = [&](const E *cache, const void *fresh, int t) {
+    if constexpr (TREE)
+      if (fresh && t >= p - node)
+        return static_cast<const E *>(fresh) + (token - p + t) * tok + int64_t(kvh) * D;
+    return cache + P.kv.offset(pages[t >> P.kv.shift], P.kv.in_page(t), tok);
+  };
   float o[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) o[i] = 0.f;
   float m = -INFINITY, l = 0.f;  // l: of this lane's keys
-  int from = key_lo(p, P.window);
+  int first = key_lo(p, P.window);
   TreeNode N_;  // TREE: node `node` of its row, token `token` of the call
   if constexpr (TREE) {
     N_ = TreeNode(P.tree, token, node, p - node, P.window);
-    from = N_.first();
+    first = N_.first();
   }
-  for (int t0 = from; t0 <= p; t0 += 64) {
+  for (int t0 = first; t0 <= p; t0 += 64) {
     const int t = min(t0 + lane, p);
-    const int64_t t_at = key_at(t);
+    const E *k_at = from(kc, P.k_new, t);
     float s = 0.f;
     constexpr int KU = DP / VEC < LOADS / 4 ? DP / VEC : LOADS / 4;
     for (int c0 = 0; c0 < D; c0 += KU * VEC) {
       uint4 y[KU];
 #pragma unroll
       for (int c = 0; c < KU; ++c)
-        y[c] = *reinterpret_cast<const uint4 *>(kc + t_at + min(c0 + c * VEC, D - VEC));
+        y[c] = *reinterpret_cast<const uint4 *>(k_at + min(c0 + c * VEC, D - VEC));
 #pragma unroll
       for (int c = 0; c < KU; ++c) {
         float x[VEC], z[VEC], dot = s;
@@ -89,7 +96,7 @@ __device__ void careful_pair(const CarefulParams &P, int row, int kvh, int64_t a
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < N; ++i)
-          v[u][i] = vc[key_at(min(t0 + k0 + u, p)) + max(d0, min(lane + 64 * i, d1 - 1))];
+          v[u][i] = from(vc, P.v_new, min(t0 + k0 + u, p))[max(d0, min(lane + 64 * i, d1 - 1))];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const float wk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), k0 + u));

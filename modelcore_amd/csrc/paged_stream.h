@@ -30,7 +30,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(4))) int32_t *scalar_ints;  // read only, by the scalar unit
 
 struct StreamParams : CarefulParams {
-  const void *k_new, *v_new;
   const int32_t *seqlens, *cu;
   float *part_o, *part_ml;  // [slot][pair_slots][DP], [slot][pair_slots][2]
   int2 *where;              // per row: its first range and the ranges of a block, for the merge

@@ -237,10 +237,17 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
       const int c = tid + kThreads * i;
       const int key = min(k0 + c / (DP / VEC), hi);
       const int d = (c % (DP / VEC)) * VEC;
-      const int64_t off = P.kv.offset(page[i], P.kv.in_page(key), tok) + min(d, D - VEC);
+      int64_t off = P.kv.offset(page[i], P.kv.in_page(key), tok) + min(d, D - VEC);
       lost = lost || !P.kv.is_page(page[i]);
-      kr[i] = *reinterpret_cast<const u32x4 *>(kbase + off);
-      vr[i] = *reinterpret_cast<const u32x4 *>(vbase + off);
+      const E *kf = kbase, *vf = vbase;
+      if constexpr (TREE)
+        if (P.k_new && key >= s0) {  // the nodes from their own rows
+          kf = static_cast<const E *>(P.k_new) + int64_t(kvh) * D;
+          vf = static_cast<const E *>(P.v_new) + int64_t(kvh) * D;
+          off = (tok0 + key - s0) * tok + min(d, D - VEC);
+        }
+      kr[i] = *reinterpret_cast<const u32x4 *>(kf + off);
+      vr[i] = *reinterpret_cast<const u32x4 *>(vf + off);
     }
   };
   auto store_tile = [&]() {
@@ -394,6 +401,23 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
                 vp[(32 * mk + 8 * (e >> 2) + (e & 3)) * VSTR + 32 * md], w[mk][e], o[md], 0, 0, 0);
     }
   }
+
+  // The nodes whose first pair the block has, into their pages: by its last range.
+  if constexpr (TREE)
+    if (P.k_new && hi == last) {
+      const int units = D / VEC, own = q0 + (r0 > 0), end = pair_pos(n - 1) + 1;
+      for (int i = tid; i < (end - own) * units; i += kThreads) {
+        const int t = own + i / units, key = s0 + t, d = VEC * (i % units);
+        const int id = pages[key >> P.kv.shift];
+        if (!P.kv.is_page(id)) continue;
+        const int64_t fresh = (tok0 + t) * tok + int64_t(kvh) * D + d;
+        const int64_t to = P.kv.offset(id, P.kv.in_page(key), tok) + int64_t(kvh) * D + d;
+        const u32x4 x = *reinterpret_cast<const u32x4 *>(static_cast<const E *>(P.k_new) + fresh);
+        const u32x4 y = *reinterpret_cast<const u32x4 *>(static_cast<const E *>(P.v_new) + fresh);
+        *reinterpret_cast<u32x4 *>(static_cast<E *>(const_cast<void *>(P.k_pages)) + to) = x;
+        *reinterpret_cast<u32x4 *>(static_cast<E *>(const_cast<void *>(P.v_pages)) + to) = y;
+      }
+    }
 
   l = sum_halves(l);
   if (__syncthreads_or(lost)) l = NAN;
@@ -654,6 +678,8 @@ TiledParams tiled_params(const PagedArgs &a, const PagedTiles &tiles) {
   P.D = int(a.head_dim);
   P.scale_log2 = float(kLog2e / std::sqrt(double(a.head_dim)));
   P.tree = a.tree;
+  P.k_new = a.tree.masks ? a.k_new : nullptr;  // of other calls they are in their pages
+  P.v_new = a.tree.masks ? a.v_new : nullptr;
   P.seqlens = a.seqlens;
   P.cu = a.cu;
   P.T_new = int(a.t_new);

@@ -14,7 +14,7 @@
 // are half again as many products: one row of 64 nodes after 16384 tokens 51.5 us for 44.5.
 //
 // Who sees whom: tree_bits.h, only in tiles that hold nodes or the window's edge. New nodes come from k_new and
-// v_new where given, and the block's last range puts them in their pages. A block of one range writes its
+// v_new where given, and a block's last range puts its own in their pages. A block of one range writes its
 // output; otherwise (o, m, l) go to scratch in fp32 and the merge launch adds the ranges up. Pairs that are not finite
 // are redone (paged_careful.h).
 #include "stream_tiles.h"
@@ -35,7 +35,6 @@ constexpr int waves_of(int dp, int pairs) { return dp <= 128 && pairs == 128 ? 8
 constexpr int tree_fill(int dp, int pairs) { return dp <= 128 ? 8 / waves_of(dp, pairs) : 1; }
 
 struct TreeParams : CarefulParams {
-  const void *k_new, *v_new;
   const int32_t *seqlens, *cu;
   int n_rows, t_new, total, H, G;
   int target;     // workgroups a call aims at; 0: no row is cut
@@ -331,12 +330,12 @@ __global__ __launch_bounds__(64 * waves_of(DP, kBlock))
   wait_loads<0>();
   l = sum_halves(l);
 
-  // The new nodes into their pages, by the block's last range: in every block, so that a redo below finds
-  // them whichever other block has come how far; they write the same.
+  // The nodes whose first pair the block has, into their pages: by its last range.
   if (fresh && R.part == ranges - 1) {
     const int units = D / 8;  // of 16 bytes, of K and of V
-    for (int i = tid; i < R.T * units; i += kThreads) {
-      const int t = i / units, u = i - t * units, key = R.s0 + t;
+    const int own = (p0 + P.G - 1) / P.G, end = min((p0 + kBlock + P.G - 1) / P.G, R.T);
+    for (int i = tid; i < (end - own) * units; i += kThreads) {
+      const int row = i / units, t = own + row, u = i - row * units, key = R.s0 + t;
       const int pid = P.kv.table[b * P.kv.table_stride + (key >> P.kv.shift)];
       if (!P.kv.is_page(pid)) continue;
       const int64_t from = int64_t(R.tok0 + t) * tok_bytes + head_at + 16 * u;
@@ -347,7 +346,7 @@ __global__ __launch_bounds__(64 * waves_of(DP, kBlock))
       *reinterpret_cast<uint4 *>(static_cast<char *>(const_cast<void *>(P.v_pages)) + to) = y;
     }
   }
-  if (__syncthreads_or(lost)) l = NAN;  // and the nodes are in their pages, the tiles read
+  if (__syncthreads_or(lost)) l = NAN;  // and the tiles are read
 
   if constexpr (WK > 1) {  // the first waves of each 32 pairs take the others' sums
     static_assert((WK - 1) * WP * 32 * DP * 4 <= int(sizeof(s_tiles)), "they fit the tiles");
