@@ -44,9 +44,9 @@ struct TreeParams : CarefulParams {
   int *n_cuts;
 };
 
+// A range of a block, of KV head kvh.
 template <int DP, int kBlock>
-__global__ __launch_bounds__(64 * waves_of(DP, kBlock))
-    __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 2 : 1))) void tree_stream_kernel(TreeParams P) {
+__device__ __forceinline__ void attend_range(const TreeParams &P, const TreeRange R, int kvh) {
   using S_ = Shape<DP>;
   constexpr int CPR = S_::CPR, RPI = S_::RPI, NV = S_::NV, KD = S_::KD, MD = S_::MD;
   constexpr int W = waves_of(DP, kBlock), kTile = 16 * W, kThreads = 64 * W;
@@ -57,13 +57,7 @@ __global__ __launch_bounds__(64 * waves_of(DP, kBlock))
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  TreeRange R;
-  const TreeRanges call{P.cu, P.seqlens, P.n_rows, P.t_new, P.total, P.G, P.H_kv, kBlock, 0,
-                        P.kv.max_pages << P.kv.shift, P.window, kTile, P.target, kMinRangeKeys / kTile};
-  const bool found = find_tree_range(call, int(blockIdx.x) / P.H_kv, lane, R);
-  if (blockIdx.x == 0 && tid == 0 && P.target > 0) *P.n_cuts = R.n_blocks;
-  if (!found) return;
-  const int kvh = int(blockIdx.x) % P.H_kv, b = R.b, D = P.D;
+  const int b = R.b, D = P.D;
   const int h = lane >> 5, col = lane & 31;
   const int pg = wave % WP, kg = wave / WP;  // its 32 pairs, and its part of a tile's keys
   const int pairs = R.T * P.G, p0 = R.qt * kBlock;
@@ -427,6 +421,23 @@ __global__ __launch_bounds__(64 * waves_of(DP, kBlock))
     careful_pair<bf16, DP, 8, true>(P, b, kvh, (int64_t(R.tok0 + t) * P.H + kvh * P.G + (pr - t * P.G)) * D,
                                     R.s0 + t, lane, 0, D, R.tok0 + t, t);
   }
+}
+
+template <int DP, int kBlock>
+__global__ __launch_bounds__(64 * waves_of(DP, kBlock))
+    __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 2 : 1))) void tree_stream_kernel(TreeParams P) {
+  constexpr int kTile = 16 * waves_of(DP, kBlock);
+  TreeRange R;
+  const TreeRanges call{P.cu, P.seqlens, P.n_rows, P.t_new, P.total, P.G, P.H_kv, kBlock, 0,
+                        P.kv.max_pages << P.kv.shift, P.window, kTile, P.target, kMinRangeKeys / kTile};
+  const bool found = find_tree_range(call, int(blockIdx.x) / P.H_kv, threadIdx.x & 63, R);
+  if (blockIdx.x == 0 && threadIdx.x == 0 && P.target > 0) *P.n_cuts = R.n_blocks;
+  if (!found) return;
+  // The arguments are read again, which takes fewer registers in the loop over the tiles than to keep them all (one
+  // row of 1024 nodes after 16384 tokens, 32 / 8 heads of 128: 308 us for 316).
+  auto args = (const __attribute__((address_space(4))) TreeParams *)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(args));
+  attend_range<DP, kBlock>(*(const TreeParams *)args, R, int(blockIdx.x) % P.H_kv);
 }
 
 // The ranges of cut blocks added up: a workgroup has two pairs (D up to 128; one of more) of a block and KV head, half
