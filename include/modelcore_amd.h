@@ -503,7 +503,8 @@ int mcamd_flash_attn_paged_tree_with_kvcache(
  * logits nothing is accepted and the last token is 0. A child with a token outside [0, vocab) is passed over.
  * kept (n_rows, max_seqlen) gets the accepted nodes, the root first, counts (n_rows) how many, out_tokens
  * (n_rows, max_seqlen) the tokens after the root: those of the accepted nodes, then the last one, so as many;
- * -1 past them. A row without nodes has counts 0. max_seqlen (at most 1024): nodes past it are left out.
+ * -1 past them. A row without nodes has counts 0. max_seqlen (at most 1024): nodes past it are left out. vocab is
+ * at most 2^30, with draft_probs 2^23 (MCAMD_EUNSUPPORTED; a remainder's sums by 4096 tokens are held at once).
  * scratch: mcamd_verify_drafts_scratch_bytes(), 16-byte aligned, the call's own until it ends on the stream.
  */
 size_t mcamd_verify_drafts_scratch_bytes(int64_t total, int64_t vocab);

@@ -91,7 +91,7 @@ def verify_drafts(logits, tokens, parents, cu_seqlens, numbers, *, temperature=1
         temperature: of the softmax; 0 takes the largest logits (the first of equal ones)
         draft_probs: (total, vocab) fp32, row i the distribution that the children of node i were drawn
             from, independently of one another (rows of nodes without children are not read); None where
-            the drafts are guesses
+            the drafts are guesses; a vocabulary of at most 2^23 tokens then
         max_seqlen: at least the nodes of the widest row (host int), at most 1024; a row's nodes past it
             are left out
 

@@ -264,6 +264,6 @@ def test_at_random(seed):
 
 
 def test_vocabularies_of_more_chunks_than_are_kept():
-    """Past 262144 tokens the remainder's sums by chunk are made again; past 64 chunks a lane has several."""
+    """Past 64 chunks of 4096 logits a lane has several of them."""
     for drawn in (False, True):
         check(*drafted(40, [2, 2, 3], 300001, 1.0, drawn=drawn, off=2.0), least=0.3)

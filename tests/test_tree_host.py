@@ -52,11 +52,15 @@ def test_attention_of_nothing_is_no_launch():
     assert attention(total=0, masks=None) == _ext.OK
 
 
-def test_scratch_is_that_of_sequences_but_for_single_fp32_nodes():
+def test_scratch():
+    """Of use where keys can be cut into ranges, and only there; rows of few pairs have that of sequences."""
     lib = _ext.lib()
-    for sizes in ((32, 512, 16, 16, 4, 128, 512, 16, -1, _ext.BF16), (1, 64, 64, 32, 8, 128, 300, 64, -1, _ext.BF16),
-                  (60, 300, 8, 32, 8, 128, 600, 16, 1024, _ext.BF16)):
-        assert lib.mcamd_paged_tree_scratch_bytes(*sizes) == lib.mcamd_paged_scratch_bytes(*sizes) > 0
+    few = (60, 300, 8, 32, 8, 128, 600, 16, 1024, _ext.BF16)
+    assert lib.mcamd_paged_tree_scratch_bytes(*few) == lib.mcamd_paged_scratch_bytes(*few) > 0
+    for D in (64, 96, 128, 256):
+        for T, dtype in ((16, _ext.BF16), (64, _ext.BF16), (16, _ext.F32)):
+            assert lib.mcamd_paged_tree_scratch_bytes(4, 4 * T, T, 16, 4, D, 512, 64, -1, dtype) > 0
+            assert lib.mcamd_paged_tree_scratch_bytes(4, 4 * T, T, 16, 4, D, 1, 16, -1, dtype) == 0
     assert lib.mcamd_paged_tree_scratch_bytes(0, 0, 0, 8, 2, 128, 8, 16, -1, _ext.BF16) == 0
 
 
@@ -102,10 +106,15 @@ def test_keep_refuses():
 
 def test_verify_refuses():
     lib = _ext.lib()
+    most = 1 << 23  # tokens of a vocabulary whose remainder is summed
 
-    def verify(logits=FAKE, ls=100, probs=None, ps=0, cu=FAKE, n_rows=2, total=5, longest=4, V=100, t=1.0):
+    def verify(logits=FAKE, ls=100, probs=None, ps=0, cu=FAKE, n_rows=2, total=5, longest=4, V=100, t=1.0, scratch=FAKE,
+               nbytes=1 << 40):
         return lib.mcamd_verify_drafts(logits, ls, probs, ps, FAKE, FAKE, cu, FAKE, FAKE, FAKE, FAKE, n_rows, total, longest,
-                                       V, t, FAKE, 1 << 40, None)
+                                       V, t, scratch, nbytes, None)
+
+    need = lib.mcamd_verify_drafts_scratch_bytes(5, 100)
+    assert need > 0 and lib.mcamd_verify_drafts_scratch_bytes(0, 100) == 0
 
     for kw, code, words in ((dict(n_rows=-1), _ext.EINVAL, b"n_rows"), (dict(total=-1), _ext.EINVAL, b"total"),
                             (dict(longest=0), _ext.EINVAL, b"max_seqlen"), (dict(longest=1025), _ext.EUNSUPPORTED, b"1024"),
@@ -113,7 +122,11 @@ def test_verify_refuses():
                             (dict(t=-1.0), _ext.EINVAL, b"temperature"), (dict(t=float("nan")), _ext.EINVAL, b"temperature"),
                             (dict(t=float("inf")), _ext.EINVAL, b"temperature"), (dict(ls=99), _ext.EINVAL, b"stride"),
                             (dict(probs=FAKE, ps=99), _ext.EINVAL, b"stride"), (dict(logits=None), _ext.EINVAL, b"null"),
-                            (dict(cu=None), _ext.EINVAL, b"null"), (dict(total=0x7fffffff), _ext.EUNSUPPORTED, b"31 bits")):
+                            (dict(cu=None), _ext.EINVAL, b"null"), (dict(total=0x7fffffff), _ext.EUNSUPPORTED, b"31 bits"),
+                            (dict(V=most + 1, ls=most + 1, probs=FAKE, ps=most + 1), _ext.EUNSUPPORTED, b"2^23"),
+                            (dict(V=1 << 30, ls=1 << 30, total=1 << 10), _ext.EUNSUPPORTED, b"grid"),
+                            (dict(scratch=FAKE + 8), _ext.EINVAL, b"aligned"), (dict(scratch=None), _ext.EWORKSPACE, b"scratch"),
+                            (dict(nbytes=need - 1), _ext.EWORKSPACE, b"scratch")):
         refused(verify(**kw), code, words)
     assert verify(n_rows=0) == _ext.OK
 
