@@ -111,6 +111,8 @@ __device__ __forceinline__ void attend_range(const TreeParams &P, const TreeRang
   const int64_t head_at = int64_t(kvh) * D * 2;
   const uint32_t page_bytes = uint32_t(tok_bytes) << P.kv.shift;
   const bool fresh = P.k_new != nullptr;
+  const char *const k_pool = static_cast<const char *>(P.k_pages), *const v_pool = static_cast<const char *>(P.v_pages);
+  const int64_t k_step = static_cast<const char *>(P.k_new) - k_pool, v_step = static_cast<const char *>(P.v_new) - v_pool;
   bool lost = false;
   // The page of this wave's keys of a tile; one that no key needs is page 0.
   auto page_of = [&](int tile) __attribute__((always_inline)) {
@@ -132,12 +134,10 @@ __device__ __forceinline__ void attend_range(const TreeParams &P, const TreeRang
                                    : 2 * P.kv.offset(id, P.kv.in_page(key), int64_t(P.H_kv) * D)) + head_at;
         const int ck = min(lc ^ S_::k_swz(r), D / 8 - 1), cv = min(lc ^ S_::v_swz(r), D / 8 - 1);
         __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void *)(static_cast<const char *>(node ? P.k_new : P.k_pages) +
-                                                             from + 16 * ck),
+            (const __attribute__((address_space(1))) void *)(k_pool + from + (node ? k_step : 0) + 16 * ck),
             (__attribute__((address_space(3))) void *)(to_k + i * 512), 16, 0, 0);
         __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void *)(static_cast<const char *>(node ? P.v_new : P.v_pages) +
-                                                             from + 16 * cv),
+            (const __attribute__((address_space(1))) void *)(v_pool + from + (node ? v_step : 0) + 16 * cv),
             (__attribute__((address_space(3))) void *)(to_v + i * 512), 16, 0, 0);
       }
       return;
@@ -145,9 +145,9 @@ __device__ __forceinline__ void attend_range(const TreeParams &P, const TreeRang
     const bool edge = k0 < seen_from || k0 + kTile - 1 > seen_to || tile >= t1;
     const int64_t base = (P.kv.is_page(id) ? id : 0) * P.kv.page_stride * 2 + head_at;
     const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
-        (void *)(static_cast<const char *>(P.k_pages) + base), 0, int(page_bytes - uint32_t(head_at)), 0x00020000);
+        (void *)(k_pool + base), 0, int(page_bytes - uint32_t(head_at)), 0x00020000);
     const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
-        (void *)(static_cast<const char *>(P.v_pages) + base), 0, int(page_bytes - uint32_t(head_at)), 0x00020000);
+        (void *)(v_pool + base), 0, int(page_bytes - uint32_t(head_at)), 0x00020000);
     const int in_page = P.kv.in_page(k) * tok_bytes;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
