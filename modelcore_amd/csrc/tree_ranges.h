@@ -1,13 +1,15 @@
-// How a call over drafted trees is dealt to the workgroups of the tiled kernels: each takes a key range of one
-// block of a row's (node, head) pairs.
+// How a call over drafted trees is dealt to the workgroups of tree_stream.hip and paged_tiled.hip: each takes a key
+// range of one block of a row's (node, head) pairs.
 //
 // A row's nodes all see its tokens, so its blocks have the same tiles, and rows differ in how many. All ranges are
 // to be on the chip at once, none longer than it must be: `len`, the most tiles of a range, is the least for
 // which there are no more ranges than `target` workgroups (a KV head each), found by bisection over the sum of the
-// rows' ceil(tiles / len). With more blocks than half of that many, or more rows than a wave has lanes, it
-// is the work over what is left, which is at most twice that. Every wave does this sum by itself, 64
-// rows at a time. 32 rows of 16 nodes after 512 to 8191 tokens, 16 / 4 heads of 128: 88 us for 113 with two
-// ranges of every row.
+// rows' ceil(tiles / len). With more blocks than that, or more rows than a wave has lanes, it is the work over what
+// is left, which is at most twice that. Every wave does this sum by itself, 64 rows at a time. 32 rows of 16 nodes
+// after 512 to 8191 tokens, 16 / 4 heads of 128, on the kernel of 256 pairs: 104 us, 133 by the rule for sequences
+// (paged.h), which cuts by what each row has to give. Equal shares of all rows' tiles, of which a workgroup may have
+// the end of one block and the beginning of another, took 8 us for each such change and gave nothing: 77 us for
+// 76 in tree_stream.hip.
 #pragma once
 
 #include "paged.h"
