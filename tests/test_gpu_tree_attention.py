@@ -6,6 +6,7 @@ import torch
 
 import _tree
 from _paged import Pool
+from modelcore_amd import _ext
 from modelcore_amd.kernels import flash_attn as fa
 from modelcore_amd.kernels.flash_attn import flash_attn
 
@@ -340,3 +341,71 @@ def test_at_random(seed):
     pos = [rng.choice([0, rng.randrange(40), rng.randrange(700)]) for _ in range(rows)]
     Call(pos, trees(rng, sizes), H, H_kv, D, rng.choice([16, 32, 128]), rng.choice([BF, BF, F32]),
          rng.choice([-1, -1, rng.randrange(60)]), seed=seed, pad=rng.choice([0, 2])).check()
+
+
+@pytest.mark.parametrize("rows,T,H,H_kv,D,page,dtype", [
+    (70, 20, 8, 2, 64, 16, BF), (150, 9, 8, 1, 128, 32, BF), (70, 9, 4, 2, 64, 16, F32),  # more rows than a wave has lanes
+    (24, 40, 64, 32, 32, 16, BF), (9, 70, 64, 32, 64, 64, BF),  # more blocks than a KV head has workgroups
+    (2, 40, 600, 600, 8, 16, BF), (2, 3, 520, 520, 8, 16, F32)])  # more KV heads than workgroups that fill the chip
+def test_many_rows_blocks_and_heads(rows, T, H, H_kv, D, page, dtype):
+    rng = random.Random(rows)
+    sizes = [rng.choice([T, rng.randrange(1, T + 1)]) for _ in range(rows)]
+    pos = [rng.choice([0, rng.randrange(30), rng.randrange(500 if rows < 30 and H_kv < 100 else 120)]) for _ in range(rows)]
+    Call(pos, trees(rng, sizes), H, H_kv, D, page, dtype, max_pages=2048 // page).check()
+
+
+@pytest.mark.parametrize("window", [-1, 0, 7, 63, 64, 200, 900])
+@pytest.mark.parametrize("T,H,H_kv,D,dtype", [(60, 8, 2, 128, BF), (60, 4, 2, 256, BF), (30, 8, 4, 96, BF), (60, 4, 2, 64, F32)])
+def test_windows_of_wide_trees_over_ranges(T, H, H_kv, D, dtype, window):
+    """Windows that begin in any range of a cut row, and before the first key of a tile."""
+    rng = random.Random(window)
+    chain = [list(range(i + 1)) for i in range(T)]
+    bits = [chain, *trees(rng, [T, T // 2]), chain]
+    Call([0, 255, 1000, 1290], bits, H, H_kv, D, 64, dtype, window, max_pages=64).check()
+
+
+@pytest.mark.parametrize("T,H,H_kv,D,dtype", [(3, 8, 2, 128, BF), (16, 16, 4, 128, BF), (40, 16, 4, 64, BF), (20, 4, 4, 64, F32)])
+def test_without_scratch(T, H, H_kv, D, dtype):
+    """No scratch, or too little of it, cuts no row; the outputs are of the same kind."""
+    rng = random.Random(T)
+    call = Call([900, 100], trees(rng, [T, T]), H, H_kv, D, 16, dtype, max_pages=128)
+    lib, code = _ext.lib(), _ext.dtype_code(dtype)
+    table, pos = call.pool.table.to(DEV), i32(call.pos)
+    q, k, v = (t.to(DEV) for t in (call.q, call.k, call.v))
+    need = lib.mcamd_paged_tree_scratch_bytes(2, 2 * T, T, H, H_kv, D, 128, 16, -1, code)
+    assert need > 0
+    for nbytes in (0, need - 1):
+        kg, vg = call.place_new()
+        y = torch.full_like(q, NAN)
+        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=DEV)
+        st = lib.mcamd_flash_attn_paged_tree_with_kvcache(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), kg.data_ptr(), vg.data_ptr(), table.data_ptr(), 128, pos.data_ptr(), None,
+            call.masks.data_ptr(), call.masks.shape[-1], y.data_ptr(), 2, 2 * T, T, H, H_kv, D, call.pool.n_pages, 16,
+            16 * H_kv * D, 128, -1, code, ws.data_ptr() if nbytes else None, nbytes, _ext.stream_handle(y.device))
+        _ext.check(st, "tree attention")
+        torch.cuda.synchronize()
+        call.check(y.cpu())
+        assert same_bits(kg, call.pool.k) and same_bits(vg, call.pool.v)
+
+
+def test_two_streams_at_once():
+    """Calls that run beside each other on two streams have their own scratch."""
+    rng = random.Random(12)
+    calls = [Call([2500, 700], trees(rng, [16, 16]), 16, 4, 128, 16, BF, seed=s) for s in range(2)]
+    ready = []
+    for c in calls:
+        kg, vg = c.place_new()
+        ready.append((c.q.to(DEV).view(2, 16, 16, 128), kg, vg, dict(
+            k=c.k.to(DEV).view(2, 16, 4, 128), v=c.v.to(DEV).view(2, 16, 4, 128), tree_masks=c.masks.view(2, 16, 1),
+            block_table=c.pool.table.to(DEV), cache_seqlens=i32(c.pos))))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    out = [[], []]
+    for _ in range(10):
+        for i, (q, kg, vg, kw) in enumerate(ready):
+            with torch.cuda.stream(streams[i]):
+                out[i].append(op(q, kg, vg, **kw))
+    torch.cuda.synchronize()
+    for c, ys in zip(calls, out):
+        c.check(ys[0].view(-1, 16, 128).cpu())
+        assert all(same_bits(y, ys[0]) for y in ys)
