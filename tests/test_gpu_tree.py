@@ -50,6 +50,20 @@ def test_plan_of_chains_that_do_not_go_down():
     check_plan([-1, 0, -1, 0, 1], [2, 3], [-4, 2 ** 31 - 2], 3)
 
 
+@pytest.mark.parametrize("seed", range(4))
+def test_wide_plans_of_chains_that_do_not_go_down(seed):
+    """The same among hundreds of nodes, near and far from those that climb through them."""
+    rng = random.Random(seed)
+    lens, parents = [300, 1, 1000, 130], []
+    for n in lens:
+        row = [i - 1 if rng.random() < 0.8 else rng.randrange(max(0, i - 90), i) if i else -1 for i in range(n)]
+        for _ in range(n // 100):
+            i = rng.randrange(n)
+            row[i] = rng.choice([i, i + 1, n, -2, 2 ** 31 - 1, -2 ** 31])
+        parents += row
+    check_plan(parents, lens, [rng.randrange(5000) for _ in lens], 1000, pad=70)
+
+
 def test_plan_positions_past_31_bits_are_none():
     got = paged_tree(i32([-1, 0, 1]), i32([0, 3]), i32([2 ** 31 - 2]), max_seqlen=3)
     assert got.positions.tolist() == [2 ** 31 - 2, 2 ** 31 - 1, -1]
