@@ -640,7 +640,10 @@ TiledPlan tiled_plan(const PagedArgs &a, int64_t skip) {
     // Measured time of a tile on a compute unit of its own, per head dim (prefill_tiled.hip).
     t.tile_us = float(a.head_dim) * (ks == 4 ? (bf ? 0.027f : 0.085f) : (bf ? 0.012f : 0.035f));
     t.min_tiles = std::max(1, int(kRangeUs / t.tile_us));
-    t.target = (a.head_dim <= 128 ? 2 : 1) * device_cus();
+    // Trees: workgroups of four waves on the keys, and those of wide heads, one a compute unit, with two of which the
+    // ranges are shorter than it takes to begin one (one row of 5 nodes after 4000 tokens, 12 heads of 64: 19.7 us for
+    // 26.0; two rows of 256 after 4000, 12 / 4 heads of 128: 146 and 159; eight rows of 256 in 64 dims 335 for 244).
+    t.target = (ks == 1 && a.head_dim <= 64 ? 2 : 1) * device_cus();
     if (a.tree.masks)
       t.slots = paged_keys(a) >= 2 * int64_t(t.min_tiles) * t.kt ? int(tree_slots(t.target, a.n_kv_head)) : 0;
     else
@@ -657,6 +660,10 @@ TiledPlan tiled_plan(const PagedArgs &a, int64_t skip) {
   // 512, 12 heads of 64 in fp32 (24 us by that count, in a table of 576) 22.6 and 33.1; two prompts of 830, 12 / 4 heads of 128 in fp32 (71) 93 and 86; two chunks of 512
   // after 2000, 12 heads of 64 in bf16 (55) 37 and 33.
   const TiledPlan four = plan(4);
+  // Trees of at most 64 pairs always take it: most waves of a block of 128 pairs would have none, however many blocks
+  // there are. 64 rows of 2 nodes after 1000 to 3000 tokens, 8 heads of 64: 191 us for 410; 20 rows of 60 after 300
+  // to 1000, 12 heads of 64: 75 and 87; 30 rows of 50, 8 heads of 128: 119 and 148.
+  if (a.tree.masks && a.t_new * (a.n_head / a.n_kv_head) <= 64) return four;
   const bool fills = whole.bound * a.n_kv_head >= device_cus();
   const bool few = a.t_new * (a.n_head / a.n_kv_head) <= 64;
   const bool brief = float(paged_keys(a)) / float(four.kt) * four.tile_us <= kShortUs;
