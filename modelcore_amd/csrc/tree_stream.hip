@@ -350,84 +350,90 @@ __device__ __forceinline__ void attend_range(const TreeParams &P, const TreeRang
   }
   if (__syncthreads_or(lost)) l = NAN;  // and the tiles are read
 
-  if constexpr (WK > 1) {  // the first waves of each 32 pairs take the others' sums
-    static_assert((WK - 1) * WP * 32 * DP * 4 <= int(sizeof(s_tiles)), "they fit the tiles");
-    float *const so = reinterpret_cast<float *>(s_tiles) + pg * 32 * DP + 4 * lane;
-    if (kg > 0)
+  // The two waves of the same pairs add their sums up, each half of the dims: o[0 .. OWN) from dim d0 on. (32 dims
+  // are one piece: the first wave has it.)
+  constexpr bool HALVES = WK == 2 && MD > 1;
+  constexpr int OWN = HALVES ? MD / 2 : MD;
+  static_assert(WK <= 2 && MD <= 2 * OWN, "two waves");
+  const int d0 = HALVES ? 32 * OWN * kg : 0;
+  if constexpr (WK == 2) {
+    static_assert(kBlock * DP * 4 <= int(sizeof(s_tiles)), "they fit the tiles");
+    constexpr int GIVEN = HALVES ? OWN : 0;  // the first piece for the other
+    if (HALVES && kg == 1)
 #pragma unroll
-      for (int md = 0; md < MD; ++md)
+      for (int md = 0; md < OWN; ++md) {
+        const f32x16 x = o[md];
+        o[md] = o[MD - OWN + md];
+        o[MD - OWN + md] = x;
+      }
+    // [32 pairs][whose half][piece][8 dims][lane][4]
+    float *const so = reinterpret_cast<float *>(s_tiles) + pg * 32 * DP + 4 * lane;
+    if (HALVES || kg == 1)
+#pragma unroll
+      for (int i = 0; i < OWN; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<float4 *>(so + (kg - 1) * WP * 32 * DP + (md * 4 + j) * 256) =
-              make_float4(o[md][4 * j], o[md][4 * j + 1], o[md][4 * j + 2], o[md][4 * j + 3]);
+          *reinterpret_cast<float4 *>(so + ((HALVES ? 1 - kg : 0) * OWN + i) * 1024 + j * 256) =
+              make_float4(o[GIVEN + i][4 * j], o[GIVEN + i][4 * j + 1], o[GIVEN + i][4 * j + 2], o[GIVEN + i][4 * j + 3]);
     if (h == 0) s_ml[kg][pg][0][col] = m, s_ml[kg][pg][1][col] = l;
     __syncthreads();
-    if (kg > 0) return;
+    if (!HALVES && kg == 1) return;
+    const float m2 = s_ml[1 - kg][pg][0][col], l2 = s_ml[1 - kg][pg][1][col], both = fmaxf(m, m2);
+    const float a1 = m == -INFINITY ? 0.f : fast_exp2(m - both), a2 = m2 == -INFINITY ? 0.f : fast_exp2(m2 - both);
+    // Without a key l = 0; a NaN l must stay.
+    l = l * (m == -INFINITY ? 1.f : a1) + l2 * (m2 == -INFINITY ? 1.f : a2);
+    m = both;
 #pragma unroll
-    for (int w = 1; w < WK; ++w) m = fmaxf(m, s_ml[w][pg][0][col]);
-    l = 0.f;
-    float a[WK];
-#pragma unroll
-    for (int w = 0; w < WK; ++w) {
-      const float m_w = s_ml[w][pg][0][col];
-      a[w] = m_w == -INFINITY ? 0.f : fast_exp2(m_w - m);
-      l += s_ml[w][pg][1][col] * (m_w == -INFINITY ? 1.f : a[w]);  // 0 then, or a NaN that must stay
-    }
-#pragma unroll
-    for (int md = 0; md < MD; ++md)
+    for (int i = 0; i < OWN; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        f32x4 y = {o[md][4 * j], o[md][4 * j + 1], o[md][4 * j + 2], o[md][4 * j + 3]};
-        y *= a[0];
+        const f32x4 x = *reinterpret_cast<const f32x4 *>(so + ((HALVES ? kg : 0) * OWN + i) * 1024 + j * 256);
 #pragma unroll
-        for (int w = 1; w < WK; ++w)
-          y += a[w] * *reinterpret_cast<const f32x4 *>(so + (w - 1) * WP * 32 * DP + (md * 4 + j) * 256);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[md][4 * j + i] = y[i];
+        for (int e = 0; e < 4; ++e) o[i][4 * j + e] = fmaf(x[e], a2, o[i][4 * j + e] * a1);
       }
   }
 
-  // o[md][4j + i] is dim 32 md + 8 j + 4 h + i of pair `col`.
+  // o[i][4j + e] is dim d0 + 32 i + 8 j + 4 h + e of pair `col`.
   if (ranges > 1) {
     if (!live) return;
     const int64_t slot = (int64_t(R.slot + R.part) * P.H_kv + kvh) * kBlock + in_block;
-    float *po = P.part_o + slot * D;
+    float *po = P.part_o + slot * D + d0;
 #pragma unroll
-    for (int md = 0; md < MD; ++md)
+    for (int i = 0; i < OWN; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (32 * md + 8 * j < D)
-          *reinterpret_cast<float4 *>(po + 32 * md + 8 * j + 4 * h) =
-              make_float4(o[md][4 * j], o[md][4 * j + 1], o[md][4 * j + 2], o[md][4 * j + 3]);
-    if (h == 0) *reinterpret_cast<float2 *>(P.part_ml + slot * 2) = make_float2(m, l);
+        if (d0 + 32 * i + 8 * j < D)
+          *reinterpret_cast<float4 *>(po + 32 * i + 8 * j + 4 * h) =
+              make_float4(o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]);
+    if (h == 0 && kg == 0) *reinterpret_cast<float2 *>(P.part_ml + slot * 2) = make_float2(m, l);
     return;
   }
   const float inv = 1.f / l;
   bool ok = true;
 #pragma unroll
-  for (int md = 0; md < MD; ++md)
+  for (int i = 0; i < OWN; ++i)
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      o[md][e] *= inv;
-      ok = ok && (finite(o[md][e]) || 32 * md + 8 * (e >> 2) >= D);
+      o[i][e] *= inv;
+      ok = ok && (finite(o[i][e]) || d0 + 32 * i + 8 * (e >> 2) >= D);
     }
   const uint64_t bad64 = __builtin_amdgcn_ballot_w64(live && !ok);
   const uint32_t bad = uint32_t(bad64) | uint32_t(bad64 >> 32);
   if (live && !((bad >> col) & 1u)) {
 #pragma unroll
-    for (int md = 0; md < MD; ++md)
+    for (int i = 0; i < OWN; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (32 * md + 8 * j >= D) continue;
-        const f32x4 x = {o[md][4 * j], o[md][4 * j + 1], o[md][4 * j + 2], o[md][4 * j + 3]};
-        *reinterpret_cast<uint2 *>(out + 32 * md + 8 * j + 4 * h) =
+        if (d0 + 32 * i + 8 * j >= D) continue;
+        const f32x4 x = {o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
+        *reinterpret_cast<uint2 *>(out + d0 + 32 * i + 8 * j + 4 * h) =
             __builtin_bit_cast(uint2, __builtin_convertvector(x, bf16x4));
       }
   }
   for (uint32_t left = bad; __builtin_expect(left != 0, 0); left &= left - 1) {
     const int pr = p0 + 32 * pg + __builtin_ctz(left), t = pr / P.G;
     careful_pair<bf16, DP, 8, true>(P, b, kvh, (int64_t(R.tok0 + t) * P.H + kvh * P.G + (pr - t * P.G)) * D,
-                                    R.s0 + t, lane, 0, D, R.tok0 + t, t);
+                                    R.s0 + t, lane, d0, min(d0 + 32 * OWN, D), R.tok0 + t, t);
   }
 }
 
