@@ -13,7 +13,7 @@
 // outputs are 2.3e-3 of their norm off, of which their own rounding makes 1.7e-3. Weights in two terms, p = hi + lo,
 // are half again as many products: one row of 64 nodes after 16384 tokens 51.5 us for 44.5.
 //
-// One row of 64 nodes after 16384 tokens, 32 / 8 heads of 128: 32 us and 6 for the merge; of 1024 nodes 304 us, 904
+// One row of 64 nodes after 16384 tokens, 32 / 8 heads of 128: 32 us and 6 for the merge; of 1024 nodes 298 us, 923
 // TFLOP/s. 32 rows of 16 nodes after 512 to 8191, 16 / 4 heads: 67 us and 8 (4.2 TB/s). A tile of 128 keys takes eight
 // waves of 128 pairs 2.4 us, which is what its LDS reads, its products and its softmax take one after another
 // (0.85 us each at their full rates): the waves of a workgroup pass through them together. Reads ahead of the products
