@@ -463,8 +463,12 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeParams P) {
   __shared__ float2 s_ml[kWaves][N];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int id = blockIdx.y;  // of the cut blocks, KV heads counted
-  if (id >= *P.n_cuts * P.H_kv) return;
-  const PagedTiles::Cut blk = P.cuts[id];
+  // Both asked for at once; a record past the last cut block is not used.
+  const scalar_ints record = (scalar_ints)(P.cuts + id);
+  const PagedTiles::Cut blk{record[0], record[1], record[2], record[3], record[4], record[5], record[6], 0};
+  const int n_cuts = *(scalar_ints)P.n_cuts;
+  asm volatile("" ::"s"(blk.ranges), "s"(n_cuts));
+  if (id >= n_cuts * P.H_kv) return;
   const int kvh = id % P.H_kv, n = min(kBlock, blk.T * P.G - blk.qt * kBlock), ranges = blk.ranges;
   const int first = N * int(blockIdx.x);
   if (ranges == 1 || first >= n) return;  // of one range: written by the block itself
