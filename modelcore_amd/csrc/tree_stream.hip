@@ -13,13 +13,13 @@
 // outputs are 2.3e-3 of their norm off, of which their own rounding makes 1.7e-3. Weights in two terms, p = hi + lo,
 // are half again as many products: one row of 64 nodes after 16384 tokens 51.5 us for 44.5.
 //
-// One row of 64 nodes after 16384 tokens, 32 / 8 heads of 128: 32 us and 6 for the merge; of 1024 nodes 298 us, 923
+// One row of 64 nodes after 16384 tokens, 32 / 8 heads of 128: 32 us and 5 for the merge; of 1024 nodes 298 us, 923
 // TFLOP/s. 32 rows of 16 nodes after 512 to 8191, 16 / 4 heads: 67 us and 8 (4.2 TB/s). A tile of 128 keys takes eight
 // waves of 128 pairs 2.4 us, which is what its LDS reads, its products and its softmax take one after another
 // (0.85 us each at their full rates): the waves of a workgroup pass through them together. Reads ahead of the products
-// and waves' priorities changed nothing. Of the rest, finding the range takes 3 us, queries, pages and the first tile 4,
-// the sums' way out 3. Blocks of 64 pairs run at 6.2 TB/s while they read; the longest range ends 15 us
-// after the median one.
+// and waves' priorities changed nothing. Of the rest, finding the range takes 1.7 us, queries, pages and the first tile
+// 3.7, the sums' way out 3. Blocks of 64 pairs run at 6.2 TB/s while they read; the longest range ends 9 us after the
+// median one.
 //
 // Who sees whom: tree_bits.h, only in tiles that hold nodes or the window's edge. New nodes come from k_new and
 // v_new where given, and a block's last range puts its own in their pages. A block of one range writes its
