@@ -45,7 +45,7 @@ constexpr int tree_fill(int dp, int pairs) { return dp <= 128 ? 8 / waves_of(dp,
 struct TreeParams : CarefulParams {
   const int32_t *seqlens, *cu;
   int n_rows, t_new, total, H, G;
-  int target;     // workgroups a call aims at; 0: no row is cut
+  int target;      // workgroups a call aims at; 0: no row is cut
   float *part_o;   // [slot][pairs of a block][D]
   float *part_ml;  // [slot][pairs of a block][2]
   PagedTiles::Cut *cuts;
@@ -59,7 +59,7 @@ __device__ __forceinline__ void attend_range(const TreeParams &P, const TreeRang
   constexpr int CPR = S_::CPR, RPI = S_::RPI, NV = S_::NV, KD = S_::KD, MD = S_::MD;
   constexpr int W = waves_of(DP, kBlock), kTile = 16 * W, kThreads = 64 * W;
   constexpr int WP = kBlock / 32, WK = W / WP, MK = kTile / (32 * WK);  // waves over pairs, keys; 32 keys of a wave
-  // K and V of two tiles; at the end the sums of the waves over other keys than the first.
+  // K and V of two tiles; at the end the halves of their sums that waves of the same pairs hand each other.
   __shared__ __attribute__((aligned(1024))) uint16_t s_tiles[2][2][kTile * DP];
   __shared__ float s_ml[WK][WP][2][32];
 

@@ -252,24 +252,25 @@ def paged_keep(k_pages, v_pages, block_table, cache_seqlens, new_lens, kept, cou
                                                        what)
     _ext.require_rocm(k_pages, v_pages, what=what)
     _ext.same_device(dev, k_pages=k_pages, v_pages=v_pages, new_lens=new_lens, kept=kept, counts=counts)
-    if k_pages.dim() == 4:
-        k_pages, v_pages = k_pages.unsqueeze(0), v_pages.unsqueeze(0)
-    if k_pages.dim() != 5 or k_pages.shape != v_pages.shape or k_pages.shape[1] != n_pages:
+    shape, at, v_at = k_pages.shape, k_pages.stride(), v_pages.stride()
+    if len(shape) not in (4, 5) or v_pages.shape != shape or shape[-4] != n_pages:
         raise ValueError(f"k_pages/v_pages must both be (n_slots, {n_pages}, page_size, H_kv, D); got "
-                         f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
-    slots, _, page, heads, dim = k_pages.shape
+                         f"{tuple(shape)} and {tuple(v_pages.shape)}")
+    page, heads, dim = shape[-3:]
+    slots = shape[0] if len(shape) == 5 else 1
     page = check_page_size(page)
     if k_pages.dtype != v_pages.dtype:
         raise TypeError(f"v_pages is {v_pages.dtype}, k_pages is {k_pages.dtype}")
     code = _ext.dtype_code(k_pages.dtype)
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if slots and not t[0, 0].is_contiguous():
-            raise ValueError(f"each page of {name} must be contiguous; strides {t.stride()}")
-    if (n_pages > 1 and k_pages.stride(1) != v_pages.stride(1)) \
-            or (slots > 1 and k_pages.stride(0) != v_pages.stride(0)):
+    packed = (heads * dim, dim, 1)
+    for name, steps in (("k_pages", at), ("v_pages", v_at)):
+        if steps[-3:] != packed and any(size != 1 and step != want for size, step, want in
+                                        zip((page, heads, dim), steps[-3:], packed)):
+            raise ValueError(f"each page of {name} must be contiguous; strides {steps}")
+    if (n_pages > 1 and at[-4] != v_at[-4]) or (slots > 1 and at[0] != v_at[0]):
         raise ValueError("k_pages and v_pages must have the same strides")
-    page_stride = k_pages.stride(1) if n_pages > 1 else page * heads * dim
-    slot_stride = k_pages.stride(0) if slots > 1 else n_pages * page_stride
+    page_stride = at[-4] if n_pages > 1 else page * heads * dim
+    slot_stride = at[0] if slots > 1 else n_pages * page_stride
     for name, t in (("new_lens", new_lens), ("counts", counts)):
         if t.dtype != torch.int32 or t.shape != (n,):
             raise ValueError(f"{name} must be ({n},) int32; got {tuple(t.shape)} {t.dtype}")
