@@ -121,7 +121,7 @@ struct Weigher {
   }
 };
 
-// Inclusive sums over the wave, by moves between lanes on the VALU: sixteen waves' shuffles would wait for one another
+// Inclusive sums over the wave, by moves between lanes on the VALU: the waves' shuffles would wait for one another
 // at the LDS.
 template <int CTRL, int ROWS>
 __device__ __forceinline__ double moved64(double x) {

@@ -412,7 +412,8 @@ class Attention(nn.Module):
         """The layer over a paged cache (x is (1, total, n_embd), the rows' new tokens one after
         another): a producer rotates, norms and scales q and k and writes k and v to their slots in one
         launch, a KV-sharing consumer transforms q only, then the operator attends through the block
-        table (a TreeStep's, along each node's path). With fuse_epilogue off, the reference's separate ops and an operator that appends."""
+        table (a TreeStep's, along each node's path). With fuse_epilogue off, the reference's separate ops and
+        an operator that appends."""
         _, T, _ = x.size()
         q, k, v = self._project(x)
         k_pages, v_pages = step.get_slot_cache(self.kv_slot)

@@ -187,6 +187,31 @@ def test_keep_one_slot_and_no_rows():
     paged_keep(k, v, table[:0], held[:0], i32([]), i32([]).view(0, 2), i32([]), free, count)
 
 
+def test_keep_refuses_what_it_cannot_follow():
+    pool = torch.zeros(2, 6, 16, 2, 8, dtype=torch.bfloat16, device=DEV)
+    good = dict(k_pages=pool, v_pages=pool.clone(), block_table=i32([[1, -1]]), cache_seqlens=i32([4]), new_lens=i32([3]),
+                kept=i32([[0, 2]]), counts=i32([2]), free_pages=i32([0, 2, 3, 4, 5, -1]), free_count=i32([5]))
+    heads_first = pool.transpose(2, 3).contiguous().transpose(2, 3)
+    apart = torch.zeros(2, 12, 16, 2, 8, dtype=torch.bfloat16, device=DEV)[:, ::2]
+    for kw, error, words in (
+            (dict(k_pages=heads_first), ValueError, "each page of k_pages must be contiguous"),
+            (dict(v_pages=pool[..., ::2].repeat_interleave(1, -1)), ValueError, "must both be"),
+            (dict(k_pages=pool[..., ::2], v_pages=pool[..., ::2]), ValueError, "contiguous"),
+            (dict(v_pages=apart), ValueError, "same strides"), (dict(v_pages=pool.float()), TypeError, "v_pages is"),
+            (dict(k_pages=pool[:, :5], v_pages=pool[:, :5]), ValueError, "must both be"),
+            (dict(k_pages=pool[0, 0], v_pages=pool[0, 0]), ValueError, "must both be"),
+            (dict(k_pages=pool.half(), v_pages=pool.half()), TypeError, "bfloat16 or float32"),
+            (dict(counts=i32([2, 1])), ValueError, "counts must be"), (dict(new_lens=i32([3]).long()), ValueError, "new_lens"),
+            (dict(kept=i32([0, 2])), ValueError, "kept must be"), (dict(kept=i32([[0], [1]])), ValueError, "kept must be"),
+            (dict(free_count=i32([5, 5])), ValueError, "free_count"), (dict(block_table=i32([1, -1])), ValueError, "block_table"),
+            (dict(kept=torch.zeros(1, 2, dtype=torch.int32)), ValueError, "kept is on cpu")):
+        with pytest.raises(error, match=words):
+            paged_keep(**{**good, **kw})
+    assert good["cache_seqlens"].tolist() == [4] and good["free_count"].tolist() == [5]
+    paged_keep(**good)
+    assert good["cache_seqlens"].tolist() == [6]
+
+
 def test_reserve_tree_and_keep_in_a_captured_graph():
     """The bookkeeping of a step of trees replayed, lengths moving on from replay to replay, against the same
     steps without a graph."""
