@@ -6,8 +6,8 @@
 // nodes of its bits, with a window only those at most `window` positions before it: of the tokens the last
 // ones, of its bits the window + 1 highest, since an ancestor's index and its depth rise together.
 //
-// The bits are read from memory where they are needed, which is in tiles that hold nodes or the window's
-// edge: a handful of a row's tiles, and no registers in the others.
+// The word with a node's own bit is kept, the others are read from memory where they are needed, which is in
+// tiles that hold nodes or the window's edge: a handful of a row's tiles.
 #pragma once
 
 #include "common.h"
@@ -23,20 +23,32 @@ struct TreeMasks {
 
 struct TreeNode {
   const uint64_t *line;
+  uint64_t mine;  // the word with the node's own bit, less the bits past it
   int words, node, s0, window, pos;
 
+  // That word as it stands, to be asked for early.
+  static __device__ __forceinline__ uint64_t own_word(const TreeMasks &m, int64_t token, int node) {
+    return node >> 6 < m.words ? m.masks[token * m.words + (node >> 6)] : 0;
+  }
   __device__ __forceinline__ TreeNode() {}
   __device__ __forceinline__ TreeNode(const TreeMasks &m, int64_t token, int node_, int s0_, int window_)
-      : line(m.masks + token * m.words), words(m.words), node(node_), s0(s0_), window(window_) {
-    int n = 0;
-    for (int k = 0; k <= node >> 6; ++k) n += __popcll(word(k));
+      : TreeNode(m, token, node_, s0_, window_, own_word(m, token, node_)) {}
+  __device__ __forceinline__ TreeNode(const TreeMasks &m, int64_t token, int node_, int s0_, int window_, uint64_t own)
+      : line(m.masks + token * m.words),
+        mine(own & ~uint64_t(0) >> (63 - (node_ & 63))),
+        words(m.words),
+        node(node_),
+        s0(s0_),
+        window(window_) {
+    int n = __popcll(mine);
+    for (int k = 0; k < node >> 6; ++k) n += __popcll(word(k));
     pos = s0 + n - 1;
   }
   // Word k, less the bits past the node's own.
   __device__ __forceinline__ uint64_t word(int k) const {
     const int own = node >> 6;
     if (k < 0 || k > own || k >= words) return 0;
-    return line[k] & (k < own ? ~uint64_t(0) : ~uint64_t(0) >> (63 - (node & 63)));
+    return k == own ? mine : line[k];
   }
   // The first key that may be seen.
   __device__ __forceinline__ int first() const { return window >= 0 ? max(0, min(s0, pos - window)) : 0; }

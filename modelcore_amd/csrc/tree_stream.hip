@@ -13,7 +13,7 @@
 // outputs are 2.3e-3 of their norm off, of which their own rounding makes 1.7e-3. Weights in two terms, p = hi + lo,
 // are half again as many products: one row of 64 nodes after 16384 tokens 51.5 us for 44.5.
 //
-// One row of 64 nodes after 16384 tokens, 32 / 8 heads of 128: 32 us and 5 for the merge; of 1024 nodes 298 us, 923
+// One row of 64 nodes after 16384 tokens, 32 / 8 heads of 128: 32 us and 5 for the merge; of 1024 nodes 290 us, 949
 // TFLOP/s. 32 rows of 16 nodes after 512 to 8191, 16 / 4 heads: 67 us and 8 (4.2 TB/s). A tile of 128 keys takes eight
 // waves of 128 pairs 2.4 us, which is what its LDS reads, its products and its softmax take one after another
 // (0.85 us each at their full rates): the waves of a workgroup pass through them together. Reads ahead of the products
@@ -102,6 +102,8 @@ __device__ __forceinline__ void attend_range(const TreeParams &P, const TreeRang
     if (16 * kd + 8 * h < D) u = *reinterpret_cast<const uint4 *>(q + 16 * kd + 8 * h);
     qf[kd] = __builtin_bit_cast(bf16x8, u);
   }
+
+  const uint64_t own_word = TreeNode::own_word(P.tree, R.tok0 + t_q, t_q);
 
   // This wave's loads: keys 16 wave .. of a tile, K and V. Load i covers rows RPI i + lane / CPR; its lane's chunk
   // goes to slot lane % CPR, wherever that is. (The swizzles of a row are those of the row modulo 16.)
@@ -210,6 +212,7 @@ __device__ __forceinline__ void attend_range(const TreeParams &P, const TreeRang
   wait_loads<0>();
 #pragma unroll
   for (int kd = 0; kd < KD; ++kd) asm volatile("" : "+v"(qf[kd]));
+  const TreeNode node(P.tree, R.tok0 + t_q, t_q, R.s0, P.window, own_word);
 
   // One tile, in place AT.
   auto turn = [&](int tile, auto at_c) __attribute__((always_inline)) {
@@ -253,7 +256,7 @@ __device__ __forceinline__ void attend_range(const TreeParams &P, const TreeRang
 
     // Keys the pair may not see.
     if (k0 + 32 * MK - 1 >= R.s0 || (P.window >= 0 && k0 < R.s0 + t_last - P.window)) {
-      const uint64_t seen = TreeNode(P.tree, R.tok0 + t_q, t_q, R.s0, P.window).seen(k0) >> (4 * h);
+      const uint64_t seen = node.seen(k0) >> (4 * h);
 #pragma unroll
       for (int mk = 0; mk < MK; ++mk)
 #pragma unroll
