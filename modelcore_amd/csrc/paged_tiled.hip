@@ -20,6 +20,7 @@
 #include "paged_careful.h"
 #include "prefill_order.h"
 #include "prefill_split.h"
+#include "range_tiles.h"
 #include "tree_ranges.h"
 
 #include <algorithm>
@@ -189,7 +190,7 @@ __global__ __launch_bounds__(kThreads) void paged_tiled_kernel(TiledParams P) {
         P.tiles.note_block(id, blk, ranges, P.H_kv);
     }
     whole = ranges == 1;
-    const int t0 = part * n_tiles / ranges, t1 = (part + 1) * n_tiles / ranges;
+    const int t0 = range_tile(part, n_tiles, ranges), t1 = range_tile(part + 1, n_tiles, ranges);
     hi = min(hi, lo + t1 * KT - 1);
     lo += t0 * KT;
     n_tiles = t1 - t0;

@@ -25,6 +25,7 @@
 // v_new where given, and a block's last range puts its own in their pages. A block of one range writes its
 // output; otherwise (o, m, l) go to scratch in fp32 and the merge launch adds the ranges up. Pairs that are not finite
 // are redone (paged_careful.h).
+#include "range_tiles.h"
 #include "stream_tiles.h"
 #include "tree_ranges.h"
 
@@ -91,8 +92,8 @@ __device__ __forceinline__ void attend_range(const TreeParams &P, const TreeRang
   if (R.noted && R.part == 0 && tid == 0)
     P.cuts[int64_t(R.cut) * P.H_kv + kvh] =
         PagedTiles::Cut{R.b, R.qt, R.tok0, R.T, R.s0, ranges, R.slot * P.H_kv + kvh, 0};
-  const int t0 = first_tile + int(int64_t(R.part) * n_tiles / ranges);
-  const int t1 = first_tile + int(int64_t(R.part + 1) * n_tiles / ranges);
+  const int t0 = first_tile + range_tile(R.part, n_tiles, ranges);
+  const int t1 = first_tile + range_tile(R.part + 1, n_tiles, ranges);
 
   const uint16_t *q = static_cast<const uint16_t *>(P.q) + at;
   bf16x8 qf[KD];
