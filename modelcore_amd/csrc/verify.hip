@@ -68,7 +68,7 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // at any
 
 // 2^y for y up to 0 (from -1020 on), to 2^-45: y + 1.5 2^52 has the nearest whole number in its low word, which
 // goes into the exponent, and 2^f, |f| <= 1/2, is the polynomial that meets it in the ten Chebyshev points of the
-// interval. Seventeen instructions a logit with the sum, four fewer than by the series, rint and ldexp.
+// interval. Eighteen instructions a logit with the sum, four fewer than by the series, rint and ldexp.
 // N of them side by side: alone, each multiply-add would wait for the one before.
 template <int N>
 __device__ __forceinline__ void exp2_64(double (&y)[N]) {
@@ -95,15 +95,18 @@ __device__ __forceinline__ void exp2_64(double (&y)[N]) {
 }
 
 // Logits as weights against the largest of them, which an infinite one makes 1 and all others 0. NaN has none.
+// The largest is taken off before the scale is put on, so that its own weight is 1 and no exponent is above 0: one
+// multiply-add with -top * scale would leave that product's rounding, which passes 1 from |top| / temperature = 6e15
+// on.
 struct Weigher {
   float top;
-  double scale, shift;
-  __device__ __forceinline__ Weigher(float t, double s) : top(t), scale(s), shift(-double(t) * s) {}
+  double scale;
+  __device__ __forceinline__ Weigher(float t, double s) : top(t), scale(s) {}
   // Of a finite top, -inf being next to nothing.
   template <int N>
   __device__ __forceinline__ void finite(const float (&x)[N], double (&w)[N]) const {
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = fma(double(x[i]), scale, shift);
+    for (int i = 0; i < N; ++i) w[i] = (double(x[i]) - double(top)) * scale;
     exp2_64(w);
   }
   template <int N>
