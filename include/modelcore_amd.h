@@ -499,12 +499,13 @@ int mcamd_flash_attn_paged_tree_with_kvcache(
  *  - temperature 0: x is accepted if it is the first of the largest logits (draft_probs is not read).
  * Where none is, the row's last token is the first whose running sum of what is left, max(p - a q, 0) or p
  * without the refused, passes numbers[node 0] times the whole (of p, where nothing is left). Probabilities and
- * sums are in 64 bits. A NaN logit and -inf are probability 0, +inf logits share it all; of a node with no other
- * logits nothing is accepted and the last token is 0. A child with a token outside [0, vocab) is passed over.
- * kept (n_rows, max_seqlen) gets the accepted nodes, the root first, counts (n_rows) how many, out_tokens
- * (n_rows, max_seqlen) the tokens after the root: those of the accepted nodes, then the last one, so as many;
- * -1 past them. A row without nodes has counts 0. max_seqlen (at most 1024): nodes past it are left out. vocab is
- * at most 2^30, with draft_probs 2^23 (MCAMD_EUNSUPPORTED; a remainder's sums by 4096 tokens are held at once).
+ * sums are in 64 bits; one up to 1e-290 of the largest is 0. A NaN logit and -inf are probability 0, +inf logits
+ * share it all; of a node with no other logits nothing is accepted and the last token is 0. A child with a token
+ * outside [0, vocab) is passed over. kept (n_rows, max_seqlen) gets the accepted nodes, the root first, counts
+ * (n_rows) how many, out_tokens (n_rows, max_seqlen) the tokens after the root: those of the accepted nodes, then
+ * the last one, so as many; -1 past them. A row without nodes has counts 0. max_seqlen (at most 1024): nodes past
+ * it are left out. vocab is at most 2^30, with draft_probs 2^23 (MCAMD_EUNSUPPORTED; a remainder's sums by 4096
+ * tokens are held at once).
  * scratch: mcamd_verify_drafts_scratch_bytes(), 16-byte aligned, the call's own until it ends on the stream.
  */
 size_t mcamd_verify_drafts_scratch_bytes(int64_t total, int64_t vocab);

@@ -36,7 +36,7 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kMaxNodes = 1024;
 constexpr int kChunkThreads = 256;
 constexpr int kRestChunks = 2048;  // whose sums of (p - a q)+ have room
-constexpr double kNothing = 1e-290;  // of a probability: above the least that exp2_64 makes
+constexpr double kNothing = 1e-290;  // a weight up to that counts as 0; above the least that exp2_64 makes, 2^-1020
 constexpr int kChunk = 16 * kChunkThreads;  // logits
 static_assert(kChunk == 8 * kThreads, "the draw's threads have eight each");
 
@@ -102,7 +102,8 @@ struct Weigher {
   float top;
   double scale;
   __device__ __forceinline__ Weigher(float t, double s) : top(t), scale(s) {}
-  // Of a finite top, -inf being next to nothing.
+  // Of a finite top, those so far below it that they are 0 in 64 bits being next to nothing: for sums, in which the
+  // largest is.
   template <int N>
   __device__ __forceinline__ void finite(const float (&x)[N], double (&w)[N]) const {
 #pragma unroll
@@ -114,7 +115,7 @@ struct Weigher {
     finite(x, w);
     const bool inf = top == INFINITY;
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = inf ? (x[i] == top ? 1.0 : 0.0) : x[i] > -INFINITY ? w[i] : 0.0;
+    for (int i = 0; i < N; ++i) w[i] = inf ? (x[i] == top ? 1.0 : 0.0) : w[i] > kNothing ? w[i] : 0.0;
   }
   __device__ __forceinline__ double operator()(float x) const {
     const float x1[1] = {x};

@@ -98,9 +98,10 @@ def verify_drafts(logits, tokens, parents, cu_seqlens, numbers, *, temperature=1
     At a node the children are tried in the order of their indices. Drawn from q, x is accepted if number * Z *
     q(x) < max(p(x) - a q(x), 0), where a = 0 and Z = 1, and after each that is refused a + Z and sum(max(p -
     a q, 0)). A guess is accepted if number * Z < p(x), Z being 1 less the p of those refused before it. The
-    last token is drawn from what is left of p. Probabilities are in 64 bits. -inf and NaN logits are
-    probability 0 (so a caller's top_k is a mask of -inf); of a node with no others nothing is accepted and
-    the last token is 0. A child whose token is outside the vocabulary is passed over.
+    last token is drawn from what is left of p. Probabilities are in 64 bits; one up to 1e-290 of the largest is 0.
+    -inf and NaN logits are probability 0 (so a caller's top_k is a mask of -inf, or of the type's lowest value); of
+    a node with no others nothing is accepted and the last token is 0. A child whose token is outside the
+    vocabulary is passed over.
     """
     what = "verify_drafts"
     _ext.require_rocm(logits, what=what)

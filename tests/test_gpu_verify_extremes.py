@@ -81,3 +81,19 @@ def test_rows_of_the_lowest_and_largest_values(V, drawn):
     logits[:, V // 3] = LARGEST
     tokens, parents, _, numbers, probs = trees(8, lens, V, logits, drawn)
     check(logits, tokens, parents, lens, numbers, 1.0, probs)
+
+
+@pytest.mark.parametrize("drawn", [False, True])
+@pytest.mark.parametrize("V", [50, 9000])
+@pytest.mark.parametrize("far", [LOWEST, -1e30, -1e5, -900.0])
+def test_a_number_of_zero_takes_nothing_that_has_no_probability(far, V, drawn):
+    """exp of a finite logit so far below the largest is 0 in 64 bits: such a token is neither accepted nor drawn."""
+    g = torch.Generator().manual_seed(9)
+    lens = [5, 1, 4, 6]
+    logits = torch.randn(sum(lens), V, generator=g)
+    logits[:, :V // 2] = far
+    logits[1::3, :V - 3] = far
+    tokens, parents, _, _, probs = trees(10, lens, V, logits, drawn)
+    tokens[2::2] %= V // 2
+    for u in (0.0, 2.0 ** -24):
+        check(logits, tokens, parents, lens, torch.full((sum(lens),), u), 1.0, probs, least=1.0 if u == 0 else 0.5)
