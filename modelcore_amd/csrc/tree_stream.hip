@@ -9,9 +9,10 @@
 //   S^T (keys x pairs) = K . Q^T     v_mfma_f32_32x32x16_bf16, two independent sums of 32 keys
 //   O^T (D x pairs)   += V^T . P^T   V^T by LDS transpose reads
 // in the layouts of paged_stream.hip, a pair per lane. Scores, statistics and sums are fp32, q enters as it is,
-// the weights are rounded to bf16 once, as in the other kernels of many pairs (prefill_mfma.hip): the
-// outputs are 2.3e-3 of their norm off, of which their own rounding makes 1.7e-3. Weights in two terms, p = hi + lo,
-// are half again as many products: one row of 64 nodes after 16384 tokens 51.5 us for 44.5.
+// the weights as two bf16 terms, p = hi + lo, which keep them to 2^-17, as in paged_stream.hip and the tiled kernel: a
+// row is as exact beside wide trees as alone, and as a tree as a sequence. With hi alone the outputs were 2.3e-3 of
+// their norm off instead of the 1.7e-3 of their own rounding, for a third fewer products: one row of 64 nodes after
+// 16384 tokens, 32 / 8 heads of 128, 35.2 us for 42.1; 32 rows of 16 nodes, 16 / 4 heads, bound by HBM, 73.8 for 74.2.
 //
 // One row of 64 nodes after 16384 tokens, 32 / 8 heads of 128: 32 us and 5 for the merge; of 1024 nodes 290 us, 949
 // TFLOP/s. 32 rows of 16 nodes after 512 to 8191, 16 / 4 heads: 67 us and 8 (4.2 TB/s). A tile of 128 keys takes eight
@@ -266,7 +267,7 @@ __device__ __forceinline__ void attend_range(const TreeParams &P, const TreeRang
     }
     // Weights against the running maximum; the tile's own is taken, and the sums rescaled, only where a lane's
     // weights sum past 2^15 or are not finite, or the pair has no maximum yet.
-    bf16x8 pk[2 * MK];
+    bf16x8 pk[2 * MK], pl[2 * MK];  // their two terms
     auto weigh = [&]() __attribute__((always_inline)) {
       const float ref = m == -INFINITY ? 0.f : m;
       float ts[4] = {0.f, 0.f, 0.f, 0.f};
@@ -279,6 +280,7 @@ __device__ __forceinline__ void attend_range(const TreeParams &P, const TreeRang
           ts[e & 3] += w[e];
         }
         pk[ks] = __builtin_convertvector(w, bf16x8);
+        pl[ks] = __builtin_convertvector(w - __builtin_convertvector(pk[ks], f32x8), bf16x8);
       }
       return (ts[0] + ts[1]) + (ts[2] + ts[3]);
     };
@@ -314,6 +316,7 @@ __device__ __forceinline__ void attend_range(const TreeParams &P, const TreeRang
       for (int i = 0; i < VB / 2; ++i) {
         const bf16x8 x = __builtin_shufflevector(f[2 * i], f[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
         o[v8 / 2 + i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, pk[ks], o[v8 / 2 + i], 0, 0, 0);
+        o[v8 / 2 + i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, pl[ks], o[v8 / 2 + i], 0, 0, 0);
       }
     };
     auto add_values = [&](auto ks_c) __attribute__((always_inline)) {  // of 16 keys
