@@ -220,8 +220,8 @@ def _check_keep(block_table, cache_seqlens, new_lens, kept, counts, page_size, n
                 any(x >= y for x, y in zip(nodes[:c], nodes[1:c])):
             raise IndexError(f"paged_keep: row {b} keeps nodes {nodes[:c]} of {t}, which are not ascending "
                              "nodes of it")
-        if s < 0 or t > 0 and s + t > width * page_size:
-            raise IndexError(f"paged_keep: positions [{s}, {s + t}) of row {b} fall outside the "
+        if s < 0 or s + max(t, 0) > width * page_size:
+            raise IndexError(f"paged_keep: positions [{s}, {s + max(t, 0)}) of row {b} fall outside the "
                              f"{width * page_size} of its line of the block table")
         for i in range(s // page_size, -(-(s + max(t, 0)) // page_size)):
             if not 0 <= table[b][i] < n_pages:
