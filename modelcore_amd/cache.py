@@ -401,11 +401,13 @@ class PagedKVCache:
             counts = torch.tensor(lens, dtype=torch.int32, device=dev)
         plan = paged_reserve(self.block_table, self.cache_seqlens, counts, self.free_pages,
                              self.free_count, total=sum(lens), page_size=self.page_size)
+        if not capturing:  # the host's account moves once the plan is under way, whatever becomes of the step
+            self._open = plan
+            self.pages_free -= taken
         step = PagedStep(self, lens, counts, plan, capturing) if parents is None \
             else TreeStep(self, lens, counts, plan, parents)
-        if not capturing:  # the host's account moves once the plan is under way
+        if not capturing:
             self._open = step
-            self.pages_free -= taken
         return step
 
     def note_device_step(self, new_lens):
