@@ -195,7 +195,8 @@ class DraftedDecoder:
     one tree, and the row moves on by all that the model accepts, at least one token.
 
     drafter(tokens) gives a row's guesses as (tokens, parents), node 0 being its last token (see
-    ``lookup_drafts``). The tokens that come out are a draw from the model's own distribution at
+    ``lookup_drafts``); where a row's positions, a tree (1024 nodes) or the free pages have no room for all of
+    them, the first are taken. The tokens that come out are a draw from the model's own distribution at
     `temperature` (0: its likeliest tokens), whatever the guesses were; they are keyed by `seed` and the
     step, not by the row alone. ``tokens[b]`` is row b's prompt and what has been emitted."""
 
@@ -234,19 +235,39 @@ class DraftedDecoder:
             self.running[r] = False
         self.cache.release(rows)
 
+    def _guesses(self, wanted):
+        """The most guesses that each row may have for all trees to fit the free pages, wanted[b] being row b's own;
+        0 where the rows' last tokens alone take them all."""
+        c = self.cache
+
+        def fits(most):
+            return sum(c._pages(c.lengths[b] + 1 + min(n, most)) - c._pages(c.lengths[b])
+                       for b, n in wanted.items()) <= c.pages_free
+
+        most = max(wanted.values(), default=0)
+        while most > 0 and not fits(most):
+            most -= 1
+        return most
+
     @torch.inference_mode()
     def step(self):
         """One forward over every running row's tree; returns the tokens each row has gained, [] for a row that
         has ended."""
-        trees, ids = [], []
+        from modelcore_amd.kernels.paged import MAX_TREE_NODES
+        rows = {}  # of those running: their guesses, as many as positions and a tree have room for
         for b, row in enumerate(self.tokens):
-            drafts, parents = self.drafter(row) if self.running[b] else ([], [])
-            # As many nodes as the row's positions have room for; those left out come after those kept.
+            if not self.running[b]:
+                continue
             room = self.cache.max_seq_len - self.cache.lengths[b] - 1
-            assert not self.running[b] or room >= 0, \
-                f"Sequence length {len(row)} exceeds cache length {self.cache.max_seq_len}"
-            trees.append([-1, *parents[:room]] if self.running[b] else [])
-            ids += [row[-1], *drafts[:room]] if self.running[b] else []
+            assert room >= 0, f"Sequence length {len(row)} exceeds cache length {self.cache.max_seq_len}"
+            room = min(room, MAX_TREE_NODES - 1)
+            drafts, parents = self.drafter(row)
+            rows[b] = drafts[:room], parents[:room]
+        most = self._guesses({b: len(parents) for b, (_, parents) in rows.items()})
+        trees, ids = [[] for _ in self.tokens], []
+        for b, (drafts, parents) in rows.items():  # the nodes left out come after those kept
+            trees[b] = [-1, *parents[:most]]
+            ids += [self.tokens[b][-1], *drafts[:most]]
         gained = [[] for _ in self.tokens]
         if not ids:
             return gained
