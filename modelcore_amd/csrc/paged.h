@@ -319,7 +319,6 @@ struct PagedTiles {
   };
   Cut *cuts;        // [slots]: the blocks of a call that may be cut, by their number
   int *n_cuts;      // and how many
-  TreeMasks tree;
   int target;       // of trees (tree_ranges.h): workgroups that a call's ranges aim at
 
   // Ranges of a block of n tiles: what pays for their partials, by the cost rule of prefill_split.h, none
@@ -339,10 +338,13 @@ struct PagedTiles {
   }
 };
 
-// Keys of a block, at most: by the width of the table's lines, since the rows' lengths are the device's.
+// Keys of a block, at most: by the width of the table's lines, since the rows' lengths are the device's. Behind a
+// window they are the window's and the block's own tokens, of trees all nodes of the row: one row of 600 nodes after
+// 2000 tokens, 4 heads of 128 in bf16, window 100, 27 us in ranges, 37 without; where the blocks fill the chip anyhow,
+// 1024 nodes of 32 / 8 heads, 61 and 57.
 inline int64_t paged_keys(const PagedArgs &a) {
-  const int64_t room = int64_t(a.kv.max_pages) << a.kv.shift;
-  return a.window < 0 ? room : std::min<int64_t>(room, a.window + 256 + 64);
+  const int64_t room = int64_t(a.kv.max_pages) << a.kv.shift, own = a.tree.masks ? a.t_new + 1 : 0;
+  return a.window < 0 ? room : std::min(room, a.window + std::max<int64_t>(own, 256 + 64));
 }
 
 // Room for the partials of `per_cu` workgroups per compute unit, where a call of at most `blocks` blocks can

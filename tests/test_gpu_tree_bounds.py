@@ -1,10 +1,13 @@
-"""Attention of drafted trees over the longest rows that its header allows, on the GPU."""
+"""Attention of drafted trees over the longest rows and of the widest trees, on the GPU."""
+import random
+
 import pytest
 import torch
 
 import _tree
 from _paged_blocks import close
 from modelcore_amd.kernels.flash_attn import flash_attn
+from test_gpu_tree_attention import Call
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -36,3 +39,14 @@ def test_one_key_among_hundreds_of_millions(dtype, T, D, n, where):
     # The others weigh at most 2^30 exp(-199); a weight and the sum are each rounded, and so is the mean.
     want = v[pool - 1, at % page, 0].double().cpu().expand(1, T, 1, D)
     close(y, want, torch.finfo(dtype).eps * want.abs() + 2.0 ** -24)
+
+
+@pytest.mark.parametrize("window", [0, 5, 100, 190])
+@pytest.mark.parametrize("T,H,H_kv,D,dtype", [(1024, 2, 1, 64, BF), (400, 4, 1, 128, BF), (500, 2, 2, 32, F32), (330, 4, 1, 128, F32)])
+def test_wide_trees_behind_narrow_windows(T, H, H_kv, D, dtype, window):
+    """Keys cut into ranges of which most lie among the nodes: a chain, whose nodes see those just before them, and a
+    tree, whose nodes see some far before them."""
+    rng = random.Random(T)
+    near = [max(-1, i - rng.choice([1, 1, 2])) for i in range(T)]
+    far = [-1] + [rng.randrange(i) for i in range(1, T)]
+    Call([700, 60], [_tree.ancestors(near), _tree.ancestors(far)], H, H_kv, D, 64, dtype, window, max_pages=64).check()
