@@ -207,7 +207,9 @@ extern "C" int mcamd_paged_keep(void *k_pages, void *v_pages, int64_t n_slots, i
       max_pages > kMax31 / page_size || row_elems > kMax31 / page_size)
     return fail(MCAMD_EUNSUPPORTED, "paged_keep: more than 65535 rows or 32767 slots, or sizes beyond 31 bits");
   const int64_t elem = dtype == MCAMD_F32 ? 4 : 2;
-  if (page_stride < page_size * row_elems || (n_slots > 1 && slot_stride < (n_pages - 1) * page_stride + page_size * row_elems))
+  const int64_t page_elems = page_size * row_elems;
+  if (page_stride < page_elems ||  // the pages before a slot's last one: by a quotient, which stays within 64 bits
+      (n_slots > 1 && (slot_stride < page_elems || (slot_stride - page_elems) / page_stride < n_pages - 1)))
     return fail(MCAMD_EINVAL, "paged_keep: page_stride or slot_stride smaller than what it steps over");
   if (n_rows == 0) {
     clear_error();
