@@ -4,7 +4,7 @@ import random
 import pytest
 import torch
 
-from test_gpu_verify import check
+from test_gpu_verify import check, drafted
 
 pytestmark = pytest.mark.gpu
 LOWEST, LARGEST = torch.finfo(torch.float32).min, torch.finfo(torch.float32).max
@@ -97,3 +97,10 @@ def test_a_number_of_zero_takes_nothing_that_has_no_probability(far, V, drawn):
     tokens[2::2] %= V // 2
     for u in (0.0, 2.0 ** -24):
         check(logits, tokens, parents, lens, torch.full((sum(lens),), u), 1.0, probs, least=1.0 if u == 0 else 0.5)
+
+
+@pytest.mark.parametrize("V,lens", [(400, [130, 200, 90, 300]), (5000, [100, 70])])
+@pytest.mark.parametrize("seed", range(3))
+def test_wide_stars_of_drawn_drafts(seed, V, lens):
+    """Up to hundreds of children of one node, most of them refused: a remainder's sum after each."""
+    check(*drafted(seed, lens, V, 1.0, drawn=True, tree="star", off=3.0, spread=3.0), least=1.0)
