@@ -14,11 +14,12 @@
 // their norm off instead of the 1.7e-3 of their own rounding, for a third fewer products: one row of 64 nodes after
 // 16384 tokens, 32 / 8 heads of 128, 35.2 us for 42.1; 32 rows of 16 nodes, 16 / 4 heads, bound by HBM, 73.8 for 74.2.
 //
-// One row of 64 nodes after 16384 tokens, 32 / 8 heads of 128: 32 us and 5 for the merge; of 1024 nodes 290 us, 949
-// TFLOP/s. 32 rows of 16 nodes after 512 to 8191, 16 / 4 heads: 67 us and 8 (4.2 TB/s). A tile of 128 keys takes eight
-// waves of 128 pairs 2.4 us, which is what its LDS reads, its products and its softmax take one after another
-// (0.85 us each at their full rates): the waves of a workgroup pass through them together. Reads ahead of the products
-// and waves' priorities changed nothing. Of the rest, finding the range takes 1.7 us, queries, pages and the first tile
+// One row of 64 nodes after 16384 tokens, 32 / 8 heads of 128: 36 us and 5.5 for the merge; of 1024 nodes 394 us, 698
+// TFLOP/s of the formula's products and half as many again for the second term: 1047. 32 rows of 16 nodes after 512 to
+// 8191, 16 / 4 heads: 66 us and 8.5 (4.2 TB/s). A tile of 128 keys takes eight waves of 128 pairs 3.1 us, which is what
+// its LDS reads, its products and its softmax take one after another (0.85, 1.3 and 0.9 us at their full rates): the
+// waves of a workgroup pass through them together. Reads ahead of the products and waves' priorities changed nothing
+// when the weights had one term (2.4 us). Of the rest, finding the range takes 1.7 us, queries, pages and the first tile
 // 3.7, the sums' way out 3. Blocks of 64 pairs run at 6.2 TB/s while they read; the longest range ends 9 us after the
 // median one.
 //
@@ -38,9 +39,10 @@ namespace {
 constexpr int kMinRangeKeys = 256;        // of a range, unless the row is shorter
 constexpr float kTileSumLimit = 32768.f;  // 2^15: a lane's weights of one tile sum to at most this
 // Waves of a workgroup, and how many of those a compute unit holds. Blocks of 128 pairs have eight waves, so that
-// half as many partials are written and merged (one row of 64 nodes after 16384 tokens, 32 / 8 heads of 128: 42.9 us
-// for 46.5); those of 64, of which HBM is the bound, four, so that one workgroup's loads run while the other begins or
-// ends (32 rows of 16 nodes, 16 / 4 heads: 77 us for 85).
+// half as many partials are written and merged (one row of 64 nodes after 16384 tokens, 32 / 8 heads of 128: 41.0 us
+// for 44.3; of 1024 nodes 394 for 418; eight rows of 256 nodes, which are many blocks, in 64 dims 147 for 141); those of
+// 64, of which HBM is the bound, four, so that one workgroup's loads run while the other begins or ends (32 rows of 16
+// nodes, 16 / 4 heads: 77 us for 85 with one-term weights).
 constexpr int waves_of(int dp, int pairs) { return dp <= 128 && pairs == 128 ? 8 : 4; }
 constexpr int tree_fill(int dp, int pairs) { return dp <= 128 ? 8 / waves_of(dp, pairs) : 1; }
 
@@ -454,11 +456,7 @@ __global__ __launch_bounds__(64 * waves_of(DP, kBlock))
   const bool found = find_tree_range(call, int(blockIdx.x) / P.H_kv, threadIdx.x & 63, R);
   if (blockIdx.x == 0 && threadIdx.x == 0 && P.target > 0) *P.n_cuts = R.n_blocks;
   if (!found) return;
-  // The arguments are read again, which takes fewer registers in the loop over the tiles than to keep them all (one
-  // row of 1024 nodes after 16384 tokens, 32 / 8 heads of 128: 308 us for 316).
-  auto args = (const __attribute__((address_space(4))) TreeParams *)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(args));
-  attend_range<DP, kBlock>(*(const TreeParams *)args, R, int(blockIdx.x) % P.H_kv);
+  attend_range<DP, kBlock>(P, R, int(blockIdx.x) % P.H_kv);
 }
 
 // The ranges of cut blocks added up: a workgroup has two pairs (D up to 128; one of more) of a block and KV head, half
