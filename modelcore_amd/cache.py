@@ -368,7 +368,7 @@ class PagedKVCache:
     def keep(self, step, kept, counts):
         """Row b keeps nodes kept[b, :counts[b]] of its tree (ascending; ``verify_drafts`` gives both), which
         become its next tokens, and gives back the pages of the others (``paged_keep``). Returns how many
-        each row keeps, as a list: the one host read of a step."""
+        each row keeps, as a list, for which it reads `counts` on the host."""
         from modelcore_amd.kernels.paged import paged_keep
         assert isinstance(step, TreeStep) and step is self._open, "the trees are not those this cache has begun"
         assert step._done, "the step's forward has not run"

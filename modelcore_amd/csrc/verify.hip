@@ -17,7 +17,7 @@
 //
 // Two launches. The first reads every logit once, a workgroup kChunk of a node's, and leaves the largest, its
 // place and the sum of the chunk's weights against it: bound by HBM (32 trees of 32 nodes, vocabulary 32768: 134
-// MB in 28 us, 4.8 TB/s). The second has a workgroup a row: a node's chunks are put together by a few lanes and the
+// MB in 29 to 32 us, 4.2 to 4.6 TB/s). The second has a workgroup a row: a node's chunks are put together by a few lanes and the
 // probabilities of all drafts fetched at once; its first wave then walks, out of registers and LDS, and finds the
 // draw's chunk by the chunks' sums, all waves make the sums (p - a q)+ where they are wanted (before a further
 // child is tried against them, and for the draw) and read that chunk again. Bound by latency: seven round trips,
