@@ -15,15 +15,15 @@
 // which no test uses). It falls between neighbours of a whole vocabulary, where 32-bit sums would move
 // it: weights and sums are in 64 bits, whose multiply-adds run as fast here as those of 32.
 //
-// Two launches. The first reads every logit once, a workgroup kChunk of a node's, and leaves the largest, its
-// place and the sum of the chunk's weights against it: bound by HBM (32 trees of 32 nodes, vocabulary 32768: 134
-// MB in 29 to 32 us, 4.2 to 4.6 TB/s). The second has a workgroup a row: a node's chunks are put together by a few lanes and the
-// probabilities of all drafts fetched at once; its first wave then walks, out of registers and LDS, and finds the
-// draw's chunk by the chunks' sums, all waves make the sums (p - a q)+ where they are wanted (before a further
-// child is tried against them, and for the draw) and read that chunk again. Bound by latency: seven round trips,
-// 12 us for those trees, 16 with such a sum over a row (64 chains of four); with sixteen waves that all walk 19
-// and 21, since a SIMD's four wait for one another. Weights are made eight side by side or four: the ten
-// multiply-adds of one wait for each other.
+// Two launches. The first reads every logit once, a workgroup kChunk of a node's, and leaves the largest, its place
+// and the sum of the chunk's weights against it: bound by HBM (32 trees of 32 nodes, vocabulary 32768: 134 MB in 29
+// to 32 us, 4.2 to 4.6 TB/s). The second has a workgroup a row: a node's chunks are put together by a few lanes and
+// the probabilities of all drafts fetched at once; its first wave then walks, out of registers and LDS, and finds
+// the draw's chunk by the chunks' sums, all waves make the sums (p - a q)+ where they are wanted (before a further
+// child is tried against them, and for the draw) and read that chunk again. Bound by latency: seven round trips, 12
+// us for those trees, 16 with such a sum over a row (64 chains of four); with sixteen waves that all walk 19 and 21,
+// since a SIMD's four wait for one another. Weights are made eight side by side or four: the ten multiply-adds of
+// one wait for each other.
 #include "kernels.h"
 
 #include <cmath>
